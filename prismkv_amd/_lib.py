@@ -13,6 +13,7 @@ from pathlib import Path
 DEFAULT_LIBRARY = Path(__file__).resolve().with_name("libprismkv_hip.so")
 
 _U64, _I32, _I64, _SZ = ctypes.c_uint64, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_F64 = ctypes.c_double
 
 # name -> (argument types without the trailing stream, has_stream, restype)
 SIGNATURES = {
@@ -65,6 +66,12 @@ SIGNATURES = {
     "prismkv_attend_f32": ([_U64] * 7 + [_I32, _I32, _I32, _I64, _I64, _I64, _I32, _SZ], True, _I32),
     "prismkv_union_n": ([_U64] * 6 + [_I32, _I32, _I64, _I64, _I32, _SZ], True, _I32),
     "prismkv_select_cap_n": ([_U64] * 5 + [_I32, _I32, _I64, _I64, _I32], True, _I32),
+    # the paged cache
+    "prismkv_paged_append": ([_U64] * 15 + [_I64] * 5 + [_I32] * 5 + [_I64] * 4 + [_I32], True, _I32),
+    "prismkv_paged_attend_work_bytes": ([_I32] * 4 + [_I64, _I32], False, _SZ),
+    "prismkv_paged_attend": ([_U64] * 11 + [_I32] * 6 + [_I64] * 4 + [_F64, _I32, _SZ], True, _I32),
+    "prismkv_paged_evict_work_bytes": ([_I32, _I32, _I64], False, _SZ),
+    "prismkv_paged_evict": ([_U64] * 14 + [_I32] * 8 + [_I64] * 4 + [_I32, _SZ], True, _I32),
     # error handling of the bounded inter-workgroup waits
     "prismkv_set_spin_limit": ([_I32], False, _I32),
     "prismkv_get_spin_limit": ([], False, _I32),

@@ -1,0 +1,387 @@
+"""Keys and values of several sequences in pages, for dense decoding beside
+the routed one: `PagedCache.append` writes new rows, `attend` runs one new
+query token of every sequence over its pages, and `evict` bounds a cache by
+accumulated attention weight.  No counterpart in the reference.
+
+Any head layout with head_dim 64, 128 or 256 (NotImplementedError otherwise),
+bf16, fp16 or fp32.  As for `Native8B`: validation happens on the host before
+anything is enqueued (ValueError), calls go to the current stream of the
+cache's device, never synchronise and can be captured into a HIP graph after
+one eager call has made their workspaces; lengths and page table are read on
+the device.  An instance's buffers are shared state: one instance per stream,
+and graphs captured from it are replayed on one stream.  A slot below a
+sequence's length that has no page is reported at the next call
+(RuntimeError); the results since then are invalid.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+HEAD_DIMS = (64, 128, 256)
+ERR_PAGES = 4
+_SCORED = ("seen", "scores", "positions")
+
+
+def _check(cond, what):
+    if not cond:
+        raise ValueError(what)
+
+
+def _i32(x, shape, device, what):
+    _check(isinstance(x, torch.Tensor) and x.dtype == torch.int32 and tuple(x.shape) == shape and x.is_contiguous()
+           and x.device == device, f"{what} must be a contiguous int32 {list(shape)} on the cache's device")
+    return x
+
+
+class PagedCache:
+    """A cache of `sequences` sequences in `pages` pages of `page_size` slots;
+    a sequence takes at most `max_pages` of them.
+
+    Tensors: k, v [pages, kv_heads, page_size, head_dim]; table i32
+    [sequences, max_pages] (-1: no page); lengths i32 [sequences]; and, if
+    `scored`, seen i32 [sequences] (tokens appended so far), scores f32 and
+    positions i32 [sequences, kv_heads, max_pages * page_size] (each slot's
+    accumulated attention weight and its token's number), which eviction goes
+    by.  Slots at and behind a length hold nothing of meaning.
+
+    `reserve` and `release` hand out pages on the host; calls that take `into`
+    (a `fork`) write their results there and leave this cache's own lengths,
+    scores and positions, so that a step can be taken back."""
+
+    def __init__(self, sequences, pages, max_pages, *, page_size=64, kv_heads=8, head_dim=128, dtype=torch.bfloat16,
+                 scored=False, device="cuda", library=None):
+        for value, what in ((sequences, "sequences"), (pages, "pages"), (max_pages, "max_pages"),
+                            (page_size, "page_size"), (kv_heads, "kv_heads")):
+            _check(int(value) >= 1, f"{what} must be positive")
+        device = torch.device(device)
+        _check(device.type == "cuda", "native backend requires a device tensor")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        _native_types(int(head_dim), dtype)
+        shape = (int(pages), int(kv_heads), int(page_size), int(head_dim))
+        slots = int(max_pages) * int(page_size)
+        _check_slots(int(sequences), slots)
+        k = torch.zeros(shape, dtype=dtype, device=device)
+        v = torch.zeros(shape, dtype=dtype, device=device)
+        table = torch.full((int(sequences), int(max_pages)), -1, dtype=torch.int32, device=device)
+        lengths = torch.zeros(int(sequences), dtype=torch.int32, device=device)
+        meta = {}
+        if scored:
+            meta = dict(seen=torch.zeros_like(lengths),
+                        scores=torch.zeros(int(sequences), int(kv_heads), slots, device=device),
+                        positions=torch.zeros(int(sequences), int(kv_heads), slots, dtype=torch.int32, device=device))
+        self._setup(k, v, table, lengths, library=library, **meta)
+        self._free = list(range(int(pages)))[::-1]
+        self._pages = [[] for _ in range(int(sequences))]
+
+    @classmethod
+    def from_tensors(cls, k, v, table, lengths, *, seen=None, scores=None, positions=None, library=None):
+        """A cache over the caller's own tensors (pages of any strides of
+        16-byte multiples, the same for k and v), whose page table the caller
+        keeps: `reserve` and `release` are not offered.  seen, scores and
+        positions are given all or none."""
+        obj = cls.__new__(cls)
+        obj._setup(k, v, table, lengths, seen=seen, scores=scores, positions=positions, library=library)
+        return obj
+
+    def _setup(self, k, v, table, lengths, *, seen=None, scores=None, positions=None, library=None, err=None):
+        _check(isinstance(k, torch.Tensor) and k.device.type == "cuda", "native backend requires a device tensor")
+        _check(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device,
+               "K and V pages [pages, kv_heads, page_size, head_dim] of one type required")
+        pages, kv_heads, page_size, head_dim = k.shape
+        _native_types(head_dim, k.dtype)
+        _check(min(k.shape) >= 1, "K and V pages [pages, kv_heads, page_size, head_dim] of one type required")
+        es = k.element_size()
+        _check(k.stride() == v.stride() and k.stride(3) == 1, "K and V pages of equal strides and contiguous rows required")
+        _check(not any(s * es % 16 for s in k.stride()[:3]) and not (k.data_ptr() | v.data_ptr()) % 16,
+               "K/V rows must be 16-byte aligned")
+        _check(k.stride(2) >= head_dim and (pages == 1 or k.stride(0) >= head_dim) and
+               (kv_heads == 1 or k.stride(1) >= head_dim), "K/V rows must not overlap")
+        _check(table.dim() == 2 and min(table.shape) >= 1, "an int32 page table [sequences, max_pages] required")
+        sequences, max_pages = table.shape
+        slots = max_pages * page_size
+        _check_slots(sequences, slots)
+        _i32(table, (sequences, max_pages), k.device, "table")
+        _i32(lengths, (sequences,), k.device, "lengths")
+        given = [x is not None for x in (seen, scores, positions)]
+        _check(all(given) or not any(given), "seen, scores and positions are given together")
+        if all(given):
+            shape = (sequences, kv_heads, slots)
+            _i32(seen, (sequences,), k.device, "seen")
+            _i32(positions, shape, k.device, "positions")
+            _check(isinstance(scores, torch.Tensor) and scores.dtype == torch.float32 and tuple(scores.shape) == shape
+                   and scores.is_contiguous() and scores.device == k.device,
+                   f"scores must be a contiguous float32 {list(shape)} on the cache's device")
+        self.lib = _lib.load(library)
+        if self.lib.missing:
+            raise RuntimeError(f"{self.lib.path.name} lacks entry points {self.lib.missing}; rebuild it")
+        self.k, self.v, self.table, self.lengths = k, v, table, lengths
+        self.seen, self.scores, self.positions = seen, scores, positions
+        self.device = k.device
+        self._shape = (sequences, kv_heads, head_dim, page_size, max_pages)
+        self._cache_args = (kv_heads, head_dim, page_size, max_pages, pages, *k.stride()[:3])
+        self._dtype = DTYPES[k.dtype]
+        self._free = self._pages = None
+        self._attend_work, self._evict_work = {}, None
+        if err is None:
+            with torch.cuda.device(self.device):
+                # the error word, with the address of a host-mapped one that the next call reads
+                host = torch.zeros(4, dtype=torch.int32, pin_memory=True)
+                address = self.lib.query("prismkv_mapped_pointer", host.data_ptr())
+                if not address:
+                    raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")
+                err = torch.zeros(2, dtype=torch.int64, device=self.device)
+                err[1] = address
+            err = (err, host)
+        self._err = err
+
+    # ------------------------------------------------------------ pages
+
+    @property
+    def scored(self):
+        return self.scores is not None
+
+    @property
+    def slots(self):
+        """Slots of one sequence's table."""
+        return self._shape[3] * self._shape[4]
+
+    def fork(self):
+        """A cache over the same pages and page table with copies of this
+        one's lengths, scores and positions: the `into` of a step that may be
+        taken back.  (Rows that `evict` moved stay moved.)"""
+        obj = PagedCache.__new__(PagedCache)
+        meta = {name: getattr(self, name).clone() for name in _SCORED} if self.scored else {}
+        obj._setup(self.k, self.v, self.table, self.lengths.clone(), library=self.lib.path, err=self._err, **meta)
+        return obj
+
+    def reserve(self, tokens):
+        """Makes room for `tokens` slots in every sequence (an int, or one per
+        sequence), from the free pages; RuntimeError when they run out, and
+        nothing is then reserved.  Pages are kept until `release`."""
+        self._owns_pages()
+        sequences, _, _, page_size, max_pages = self._shape
+        tokens = [int(tokens)] * sequences if isinstance(tokens, int) else [int(t) for t in tokens]
+        _check(len(tokens) == sequences, "one token count per sequence required")
+        _check(all(0 <= t <= self.slots for t in tokens), f"token counts must be in [0, {self.slots}]")
+        more = [max(0, -(-t // page_size) - len(held)) for t, held in zip(tokens, self._pages)]
+        if sum(more) > len(self._free):
+            raise RuntimeError(f"{sum(more)} pages wanted, {len(self._free)} free")
+        if not any(more):
+            return
+        for held, count in zip(self._pages, more):
+            held.extend(self._free.pop() for _ in range(count))
+        self._write_table()
+
+    def release(self, sequence, tokens=0):
+        """Gives back the pages of a sequence behind its first `tokens` slots;
+        the caller sees to it that its length (and that of forks) is no larger."""
+        self._owns_pages()
+        _check(0 <= int(sequence) < self._shape[0] and int(tokens) >= 0, "no such sequence or slot")
+        held, page_size = self._pages[int(sequence)], self._shape[3]
+        keep = -(-int(tokens) // page_size)
+        if keep < len(held):
+            self._free.extend(reversed(held[keep:]))
+            del held[keep:]
+            self._write_table()
+
+    def _owns_pages(self):
+        if self._pages is None:
+            raise RuntimeError("the page table of this cache is kept by the caller (or the cache it was forked from)")
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("pages cannot be handed out inside a capture")
+
+    def _write_table(self):
+        max_pages = self._shape[4]
+        rows = torch.tensor([held + [-1] * (max_pages - len(held)) for held in self._pages], dtype=torch.int32)
+        self.table.copy_(rows)
+
+    # ------------------------------------------------------------ calls
+
+    def check_errors(self):
+        """RuntimeError if an earlier launch found a slot below a sequence's
+        length without a page: the results since the last check are invalid.
+        Reads a host-mapped word (no synchronisation, launches that have not
+        run yet are not seen) and clears it."""
+        err, host = self._err
+        if int(host[0]):
+            with torch.cuda.device(self.device):
+                torch.cuda.synchronize()
+                err[:1].zero_()
+                host.zero_()
+                torch.cuda.synchronize()
+            raise RuntimeError("paged cache: a slot below a sequence's length has no page; the results of the launches "
+                               "since the last check are invalid")
+
+    def _call(self, name, *args):
+        if torch.cuda.current_device() == self.device.index:
+            self.lib.call(name, *args, stream=torch.cuda.current_stream().cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                self.lib.call(name, *args, stream=torch.cuda.current_stream().cuda_stream)
+
+    def _into(self, into):
+        if into is None or into is self:
+            return self
+        _check(isinstance(into, PagedCache) and into.k.data_ptr() == self.k.data_ptr() and
+               into.table.data_ptr() == self.table.data_ptr() and into._shape == self._shape and
+               into._cache_args == self._cache_args and into.scored == self.scored,
+               "into must be a fork of this cache")
+        return into
+
+    def _workspace(self, nbytes, zero):
+        """A new workspace (zeroed up to `zero` bytes); never inside a capture,
+        whose memory would not outlive the graph and whose fill would not have run."""
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call of a kind makes its workspace: run it once before the capture")
+            work = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=self.device)
+            work[:zero].zero_()
+            return work
+
+    def append(self, k, v, offsets=None, *, into=None):
+        """Writes new rows behind every sequence's: k and v [rows, kv_heads,
+        head_dim] of the cache's type, one row per sequence, or with `offsets`
+        (i32 [sequences + 1], ascending from 0) rows offsets[b] .. offsets[b +
+        1] for sequence b.  Advances the lengths; of a scored cache also the
+        tokens seen, the rows starting with score 0.  The slots need pages
+        (`reserve`); a row without one is dropped and reported."""
+        to = self if into is None else self._into(into)
+        sequences, kv_heads, head_dim, _, _ = self._shape
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != kv_heads or k.shape[2] != head_dim:
+            raise ValueError(f"K and V rows [rows, {kv_heads}, {head_dim}] required")
+        if not (k.dtype == v.dtype == self.k.dtype and k.device == v.device == self.device):
+            raise ValueError("K and V rows of the cache's type on its device required")
+        rows, es = k.shape[0], k.element_size()
+        if rows and (k.stride(2) != 1 or v.stride(2) != 1):
+            raise ValueError("contiguous head dimension required")
+        strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+        if (strides[0] * es | strides[1] * es | strides[2] * es | strides[3] * es | k.data_ptr() | v.data_ptr()) % 16:
+            raise ValueError("K/V rows must be 16-byte aligned")
+        if offsets is not None:
+            _i32(offsets, (sequences + 1,), self.device, "offsets")
+        elif rows != sequences:
+            raise ValueError("one row per sequence, or offsets, required")
+        self.check_errors()
+        self._call("prismkv_paged_append", k.data_ptr(), v.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
+                   self.table.data_ptr(), 0 if offsets is None else offsets.data_ptr(), self.lengths.data_ptr(),
+                   to.lengths.data_ptr(), *self._scored_pointers(to), self._err[0].data_ptr(), rows, *strides,
+                   sequences, *self._cache_args, self._dtype)
+
+    def _scored_pointers(self, to):
+        if not self.scored:
+            return (0,) * 6
+        return (self.seen.data_ptr(), to.seen.data_ptr(), self.scores.data_ptr(), to.scores.data_ptr(),
+                self.positions.data_ptr(), to.positions.data_ptr())
+
+    def attend(self, q, *, scale=None, accumulate=False, lse=None, into=None):
+        """Softmax attention of q [sequences, heads, head_dim] (heads a
+        multiple of the cache's kv_heads; consecutive heads share a KV head)
+        over each sequence's slots, scaled by `scale` (default 1 /
+        sqrt(head_dim)); the output has q's shape and type, 0 for an empty
+        sequence.  `accumulate` adds to every slot's score its weight, summed
+        over the heads that share it.  `lse`, an f32 [sequences, heads] tensor,
+        receives the logarithm of each softmax's sum (-inf for an empty one)."""
+        return self._attend(q, self.lengths, scale, accumulate, lse, self if into is None else self._into(into))
+
+    def _check_q(self, q, scale, accumulate, lse):
+        """The query heads per KV head, and the scale."""
+        sequences, kv_heads, head_dim, _, _ = self._shape
+        if (q.dim() != 3 or q.shape[0] != sequences or q.shape[2] != head_dim or q.shape[1] < 1 or q.shape[1] % kv_heads
+                or not q.is_contiguous()):
+            raise ValueError(f"contiguous Q[{sequences}, a multiple of {kv_heads} heads, {head_dim}] required")
+        if q.dtype != self.k.dtype or q.device != self.device:
+            raise ValueError("Q of the cache's type on its device required")
+        if q.data_ptr() % 16:
+            raise ValueError("Q rows must be 16-byte aligned")
+        group = q.shape[1] // kv_heads
+        if group > 1024:
+            raise NotImplementedError("at most 1024 query heads per KV head")
+        if accumulate and self.scores is None:
+            raise ValueError("accumulate needs a scored cache")
+        scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+        if not math.isfinite(scale):
+            raise ValueError("a finite scale required")
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()
+                                or lse.device != self.device):
+            raise ValueError("lse must be a contiguous float32 [sequences, heads] on the cache's device")
+        return group, scale
+
+    def _attend(self, q, lengths, scale, accumulate, lse, to):
+        group, scale = self._check_q(q, scale, accumulate, lse)
+        self.check_errors()
+        sequences, kv_heads, head_dim, _, _ = self._shape
+        accumulate = bool(accumulate)
+        work = self._attend_work.get((group, accumulate))
+        if work is None:
+            # (the leading counters are zeroed; the kernels leave them so)
+            nbytes = self.lib.query("prismkv_paged_attend_work_bytes", sequences, kv_heads, group, head_dim, self.slots,
+                                    int(accumulate))
+            work = self._attend_work[(group, accumulate)] = self._workspace(
+                nbytes, 4 * sequences * kv_heads * ((group + 15) // 16))
+        out = torch.empty_like(q)
+        scores = (self.scores.data_ptr(), to.scores.data_ptr()) if accumulate else (0, 0)
+        self._call("prismkv_paged_attend", q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
+                   lengths.data_ptr(), *scores, 0 if lse is None else lse.data_ptr(), work.data_ptr(),
+                   self._err[0].data_ptr(), out.data_ptr(), sequences, kv_heads, group, head_dim, *self._cache_args[2:],
+                   scale, self._dtype, work.numel())
+        return out
+
+    def __call__(self, q, k, v, *, scale=None, accumulate=False, lse=None, into=None):
+        """A decode step: `append` one row of k and v [sequences, kv_heads,
+        head_dim] to every sequence, then `attend`.  With `into` both results
+        go there, the new rows into the shared pages behind this cache's
+        lengths."""
+        to = self if into is None else self._into(into)
+        self._check_q(q, scale, accumulate, lse)  # nothing is appended for a query that is refused
+        self.append(k, v, into=into)
+        return self._attend(q, to.lengths, scale, accumulate, lse, to)
+
+    def evict(self, keep, *, recent=0, sinks=0, into=None):
+        """Cuts every sequence longer than `keep` slots (an int, or i32
+        [sequences]) to them, per KV head: the `recent` newest tokens and the
+        first `sinks` ones stay before all others, then the slots of the
+        highest scores (NaN above all numbers), the lower slot on ties.  The
+        fewest rows move: a slot that stays and lies behind the budget goes
+        into one that became free, in ascending order, with its score and
+        position; the order of the slots is not that of the tokens afterwards.
+        The pages stay reserved (`release`)."""
+        to = self if into is None else self._into(into)
+        _check(self.scored, "evict needs a scored cache")
+        sequences, kv_heads, _, _, _ = self._shape
+        keeps = 0
+        if isinstance(keep, torch.Tensor):
+            keeps, keep = _i32(keep, (sequences,), self.device, "keep").data_ptr(), 0
+        keep, recent, sinks = int(keep), int(recent), int(sinks)
+        _check(min(keep, recent, sinks) >= 0 and max(keep, recent, sinks) < 2 ** 31,
+               "keep, recent and sinks must be in [0, 2^31)")
+        self.check_errors()
+        if self._evict_work is None:
+            self._evict_work = self._workspace(
+                self.lib.query("prismkv_paged_evict_work_bytes", sequences, kv_heads, self.slots), 0)
+        self._call("prismkv_paged_evict", self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
+                   self.lengths.data_ptr(), to.lengths.data_ptr(), *self._scored_pointers(to), keeps,
+                   self._evict_work.data_ptr(), self._err[0].data_ptr(), keep, recent, sinks, sequences,
+                   *self._cache_args, self._dtype, self._evict_work.numel())
+
+    def buffer_bytes(self):
+        """Live tensors held here, by name (a fork's pages are its origin's)."""
+        held = {name: x for name, x in vars(self).items() if isinstance(x, torch.Tensor)}
+        held.update((f"attend_work{key}", x) for key, x in self._attend_work.items())
+        return {name: x.numel() * x.element_size() for name, x in held.items()}
+
+
+def _native_types(head_dim, dtype):
+    if head_dim not in HEAD_DIMS or dtype not in DTYPES:
+        raise NotImplementedError("the paged cache holds bf16, fp16 or fp32 rows of head_dim 64, 128 or 256")
+
+
+def _check_slots(sequences, slots):
+    if slots > 1 << 30 or sequences * slots >= 1 << 31 or sequences > 65535:
+        raise NotImplementedError("at most 2^30 slots per sequence, 2^31 in all and 65535 sequences")
