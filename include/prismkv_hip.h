@@ -453,7 +453,8 @@ int prismkv_paged_append(uint64_t k, uint64_t v, uint64_t k_pages, uint64_t v_pa
  * of the softmax's sum, -infinity for an empty one.  Scores, sums and products
  * are accumulated in fp32.  With scores (not 0): scores_out[t] = scores[t] +
  * slot t's weights summed over the group's heads, for t < lengths[b]. */
-size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh);
+size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh,
+                                       int dtype);
 int prismkv_paged_attend(uint64_t q, uint64_t k, uint64_t v, uint64_t table, uint64_t lengths, uint64_t scores,
                          uint64_t scores_out, uint64_t lse, uint64_t paged_work, uint64_t err, uint64_t out, int sequences,
                          int kv_heads, int group, int head_dim, int page_size, int max_pages, int64_t pages,

@@ -68,7 +68,7 @@ SIGNATURES = {
     "prismkv_select_cap_n": ([_U64] * 5 + [_I32, _I32, _I64, _I64, _I32], True, _I32),
     # the paged cache
     "prismkv_paged_append": ([_U64] * 15 + [_I64] * 5 + [_I32] * 5 + [_I64] * 4 + [_I32], True, _I32),
-    "prismkv_paged_attend_work_bytes": ([_I32] * 4 + [_I64, _I32], False, _SZ),
+    "prismkv_paged_attend_work_bytes": ([_I32] * 4 + [_I64, _I32, _I32], False, _SZ),
     "prismkv_paged_attend": ([_U64] * 11 + [_I32] * 6 + [_I64] * 4 + [_F64, _I32, _SZ], True, _I32),
     "prismkv_paged_evict_work_bytes": ([_I32, _I32, _I64], False, _SZ),
     "prismkv_paged_evict": ([_U64] * 14 + [_I32] * 8 + [_I64] * 4 + [_I32, _SZ], True, _I32),

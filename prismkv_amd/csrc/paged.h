@@ -7,13 +7,16 @@ namespace prismkv {
 namespace {
 
 constexpr int kPT = 256;  // threads of the paged kernels but the selection
-constexpr int kPWaves = kPT / 64;
 constexpr unsigned kErrPages = 4u;  // error word: a slot within a sequence's length has no page of the cache
 
 // Element types of the C ABI (`dtype`).
 constexpr int kBf16 = 0, kFp16 = 1, kFp32 = 2;
 template <int DT>
 constexpr int kElem = DT == kFp32 ? 4 : 2;
+// P is held times 2^kBias: fp16 probabilities from 2^-29 of the maximum up stay
+// normal numbers (bf16 and fp32 have the exponents for them).
+template <int DT>
+constexpr int kBias = DT == kFp16 ? 15 : 0;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -27,10 +30,17 @@ struct PageDiv {
   __device__ __forceinline__ int of(int t) const { return (int)(((unsigned long long)(unsigned)t * mul) >> shift); }
 };
 
-// Chunks that the attention aims at: two workgroups of 4 waves on each of the
-// 256 CUs.  The grid has room for one more per (sequence, head tile), so that
-// rounding up never runs out of it.
-constexpr int kLogUnits = 9;
+// Workgroups that the attention's rows are dealt to: one on each of the 256 CUs,
+// of 8 waves (two a SIMD, each with a tile in flight), or of 4 where a tile of
+// head_dim 256 takes the registers of two.  Two workgroups of 4 waves read as fast,
+// but leave twice the partial states to join (64K: 54.0 us against 47.8).
+constexpr int kUnits = 256;
+template <int D>
+constexpr int kAWaves = D == 256 ? 4 : 8;
+constexpr int kQuantum = 32;  // tokens that are dealt at a time
+// Quanta of a workgroup at least: a tile (32 tokens, fp32 16) for each wave.
+template <int DT, int D>
+constexpr int kLeast = DT == kFp32 ? kAWaves<D> / 2 : kAWaves<D>;
 
 struct PagedAttend {
   const void *q, *k, *v;
@@ -38,62 +48,124 @@ struct PagedAttend {
   const float* scores;  // weigh: the scores read and written, or null
   float *scores_out, *lse_out;
   void* out;
-  float *logits, *lse_work, *state;  // workspace: weigh's scores in the exp2 domain and their log-sums; chunk states
-  unsigned *counters, *err;
+  float *logits, *lse_work, *state;  // workspace: unscaled scores and log-sums (to be weighed), partial states
+  unsigned *counters, *err;          // counters: null where a second launch joins the states
   int64_t head_bytes, logit_stride, slots;
-  unsigned page_units, slot_units, state_stride;  // 16-byte units; floats per chunk state
+  unsigned page_units, slot_units, state_stride;  // 16-byte units; floats per partial state
   PageDiv div;
   int sequences, kv_heads, group, tiles, page_size, max_pages, pages;
   float scale;  // log2(e) times the caller's
 };
 
+// 16 bytes that another workgroup wrote through (agent scope, as ld_dev).
+__device__ __forceinline__ float4 ld_dev4(__amdgpu_buffer_rsrc_t r, unsigned byte_offset) {
+  const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, byte_offset, 0, 16);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
 __device__ __forceinline__ int clamp_length(const PagedAttend& a, int n) { return min(max(n, 0), (int)a.slots); }
 
-// A workgroup's share: chunk `chunk` of `chunks` of sequence b's n tokens, `per`
-// tokens each (a multiple of 32), for head tile hh; b < 0: none.
-struct PagedUnit {
-  int b, hh, n, chunk, chunks, per;
+// Quanta of a pair of n tokens: whole workgroups' worths (so that short pairs are
+// not cut for their neighbours' sake), one for an empty sequence's output.
+template <int kL>
+__device__ __host__ __forceinline__ int quanta_of(int n) {
+  return n > 0 ? (n + kL * kQuantum - 1) / (kL * kQuantum) * kL : kL;
+}
+
+// How the quanta of all pairs (sequence, head tile), pair after pair, are dealt:
+// evenly to kUnits workgroups, or kLeast each while there are fewer.  The shares
+// differ by one quantum at most, and no CU gets a second workgroup after its
+// first (65792 tokens of 8 heads: 66 us with 514 workgroups for 512 places, 54
+// with 512).
+template <int kL>
+struct PagedDeal {
+  int total;
+  __device__ __forceinline__ int begin(int unit) const {
+    if (total <= kUnits * kL) return min(unit * kL, total);
+    return (int)((unsigned long long)unit * (unsigned)total / kUnits);
+  }
+  // the workgroup whose share holds quantum x
+  __device__ __forceinline__ int unit_of(int x) const {
+    if (total <= kUnits * kL) return x / kL;
+    int u = min((int)((float)(x + 1) * kUnits / (float)total), kUnits - 1);  // off by one at most
+    while (begin(u) > x) --u;
+    while (begin(u + 1) <= x) ++u;
+    return u;
+  }
 };
 
-// Every wave finds its workgroup's share by itself (uniform; one load of the
-// lengths and a lane scan for up to 64 sequences): chunks of about
-// total / 2^kLogUnits tokens, so a long sequence among short ones is spread
-// over as many workgroups as its share of the work.
-__device__ __forceinline__ PagedUnit find_unit(const PagedAttend& a, int unit) {
+// A pair's quanta [from, from + quanta) lie in the shares of `chunks` workgroups
+// from `unit` on.  A workgroup has at most two partial states: slot 2 unit of the
+// pair that its first quantum lies in, slot 2 unit + 1 of the one that its share
+// ends in; so the pair's state 0 lies `odd` slots behind slot 2 unit, state c 2c.
+struct PagedParts {
+  int unit, chunks, odd;
+  template <int kL>
+  __device__ __forceinline__ PagedParts(const PagedDeal<kL>& deal, int from, int quanta)
+      : unit(deal.unit_of(from)), chunks(deal.unit_of(from + quanta - 1) - unit + 1), odd(deal.begin(unit) != from) {}
+};
+
+// A workgroup's share: quanta [at, end), of which the first is `first` of pair
+// (b, hh) with n tokens.
+template <int kL>
+struct PagedSpan {
+  PagedDeal<kL> deal;
+  int at, end, b, hh, n, first;
+};
+
+// Calls f(i, n, c) for the lengths n and quanta c of 64 sequences from i on at a
+// time (a lane each, 0 past the last), until it returns true.
+template <int kL, typename F>
+__device__ __forceinline__ void each_64(const PagedAttend& a, F f) {
   const int lane = threadIdx.x & 63;
-  const int heads = a.kv_heads * a.tiles;
-  int first = 0;  // the lengths of the first 64 sequences
-  unsigned long long total = 0;
-  for (int i0 = 0; i0 < a.sequences; i0 += 64) {
-    const int n = i0 + lane < a.sequences ? clamp_length(a, a.lengths[i0 + lane]) : 0;
-    if (i0 == 0) first = n;
-    total += (unsigned)wave_sum_i(n);
+  for (int i = 0; i < a.sequences; i += 64) {
+    const bool in = i + lane < a.sequences;
+    const int n = in ? clamp_length(a, a.lengths[i + lane]) : 0;
+    if (f(i, n, in ? quanta_of<kL>(n) : 0)) return;
   }
-  const unsigned chunk = max((unsigned)((total * heads + (1u << kLogUnits) - 1) >> kLogUnits), 32u * kPWaves);
-  PagedUnit u;
-  u.b = -1;
-  const int at = unit / heads;
-  u.hh = unit - at * heads;
+}
+
+// Every wave finds its workgroup's share by itself (uniform; one load of the
+// lengths and a lane scan for up to 64 sequences), so that a long sequence among
+// short ones is spread over as many workgroups as its share of the rows.
+template <int kL>
+__device__ __forceinline__ PagedSpan<kL> find_span(const PagedAttend& a, int unit) {
+  const int heads = a.kv_heads * a.tiles;
+  PagedSpan<kL> u;
+  u.deal.total = 0;
+  each_64<kL>(a, [&](int, int, int c) {
+    u.deal.total += wave_sum_i(c);
+    return false;
+  });
+  u.deal.total *= heads;
+  u.at = u.deal.begin(unit);
+  u.end = u.deal.begin(unit + 1);
+  if (u.at >= u.end) return u;
+  const int to = u.at / heads;  // (a sequence's quanta begin at a multiple of heads)
   int base = 0;
-  for (int i0 = 0; i0 < a.sequences; i0 += 64) {
-    int n = first;
-    if (i0) n = i0 + lane < a.sequences ? clamp_length(a, a.lengths[i0 + lane]) : 0;
-    const int c = i0 + lane < a.sequences ? max((int)(((unsigned)n + chunk - 1) / chunk), 1) : 0;
+  each_64<kL>(a, [&](int i, int n, int c) {
     const int incl = (int)wave_incl_scan((unsigned)c);
     const int sum = __builtin_amdgcn_readlane(incl, 63);
-    if (at - base < sum) {
-      const int l = __ffsll((unsigned long long)__ballot(incl > at - base)) - 1;
-      u.b = i0 + l;
-      u.n = __builtin_amdgcn_readlane(n, l);
-      u.chunks = __builtin_amdgcn_readlane(c, l);
-      u.chunk = at - base - (__builtin_amdgcn_readlane(incl, l) - u.chunks);
-      u.per = (u.n + u.chunks - 1) / u.chunks;
-      u.per = (u.per + 31) & ~31;
-      return u;
+    if (to - base >= sum) {
+      base += sum;
+      return false;
     }
-    base += sum;
-  }
+    const int l = __ffsll((unsigned long long)__ballot(incl > to - base)) - 1;
+    const int own = __builtin_amdgcn_readlane(c, l);
+    const int in = u.at - (base + __builtin_amdgcn_readlane(incl, l) - own) * heads;  // within the sequence
+    u.b = i + l;
+    u.n = __builtin_amdgcn_readlane(n, l);
+    u.hh = in / own;
+    u.first = in - u.hh * own;
+    return true;
+  });
   return u;
+}
+
+// log2 of a softmax's sum from its maximum and the sum held times 2^kBias.
+template <int DT>
+__device__ __forceinline__ float log_sum(float M, float den) {
+  return den == 0.f ? -INFINITY : M + log2f(den) - kBias<DT>;
 }
 
 // Writes output element i (query head i / D of the tile, dim i % D) from the
@@ -106,7 +178,7 @@ __device__ __forceinline__ void finish(const PagedAttend& a, size_t head0, int i
   else if constexpr (DT == kFp16) reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)y;
   else reinterpret_cast<float*>(a.out)[at] = y;
   if (i % D == 0) {
-    const float l2 = den == 0.f ? -INFINITY : M + log2f(den) - (DT == kFp16 ? 15.f : 0.f);
+    const float l2 = log_sum<DT>(M, den);
     if (a.lse_out) a.lse_out[head0 + i / D] = l2 * 0.693147180559945309f;
     if (a.lse_work) a.lse_work[head0 + i / D] = l2;
   }

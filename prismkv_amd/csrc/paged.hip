@@ -19,38 +19,31 @@ namespace {
 // (2 bytes x 2 head_dim per 4 group head_dim flops), so the kernel is bound by
 // the reads.  One pass with the running maximum and sum (flash form).
 //
-// Split: the tokens of all sequences and KV heads are cut into about kUnits
-// equal chunks on the device (the lengths live there), a workgroup of 4 waves
-// per chunk, each wave on its own 32-token (fp32: 16) tiles: no barrier and no
-// LDS until the waves' states meet.  The last workgroup of a (sequence, head)
-// to arrive joins the chunks' states in chunk order, so the result does not
-// depend on the order of arrival.
+// Split: the tokens of all pairs of a sequence and a KV head (with more than 16
+// query heads a tile of them) are dealt evenly to the workgroups, on the device,
+// where the lengths are; a workgroup's share may end one pair and begin others.
+// Each of its waves takes every 8th 32-token tile (fp32: 16 tokens) by itself: no
+// barrier and no LDS until the waves' states meet at a pair's end.  A pair of
+// several workgroups is joined from their states in the order of its tokens, by
+// the last to arrive or by a second launch, so the result does not depend on the
+// order of arrival.
+//
+// Measured (MI355X, launches after one another in a graph): 65792 tokens, 8 x 4
+// heads, bf16, 47.8 us = 5.6 TB/s; 32 sequences of 6.4K tokens 136 us = 6.2 TB/s
+// (a plain read of as much memory reaches 6.9); 16 x 8192 of head_dim 256 in fp32
+// 93 us = 5.8; of head_dim 64 50 us = 5.3; 75 tokens 6.7 us.  About 6 us of a call
+// are the launch and the chain lengths -> page -> rows, 4 more the join.
 
-// Wave's running state of 16 heads (columns j) over head_dim D.
-template <int DT, int D>
-struct Acc;
-template <int D>
-struct Acc<kFp32, D> {
-  f32x4 hi[D / 16];
-};
-// 16-bit types: P is a head and a remainder of the type (two products, about
-// twice the type's significant bits), accumulated apart: a remainder of zero
-// times an infinite V is NaN, which the join drops when the head's sum has the
-// infinity.
-template <int D>
-struct Acc<kBf16, D> {
-  f32x4 hi[D / 16], lo[D / 16];
-};
-template <int D>
-struct Acc<kFp16, D> {
-  f32x4 hi[D / 16], lo[D / 16];
-};
-
+// 16-bit types: P is a head and a remainder of the type (two products into one
+// accumulator: about twice the type's significant bits).  The head is taken from
+// slightly below p, so that both are positive wherever p is and an infinite V
+// is not multiplied by a remainder of 0.
 // The tile of one step as loaded.  16-bit (32 tokens, two 16-token blocks):
 // lane (j, q) holds row j of each block at dims 32c + 8q .. +8 (K, the A operand
-// of the 16x16x32 product) and rows 4q + t at dims (D/16) j .. + D/16 (V): D/16
-// column blocks n map dim (D/16) j + n to column j, so that a load covers whole
-// rows and the pairs of rows are joined per dim with one byte permutation.
+// of the 16x16x32 product) and of rows 4q + t (V) 16 bytes out of every 256 (8 of
+// head_dim 64's 128), so that the 16 lanes of a load cover whole rows.  Column
+// block n of the output takes element n of a lane, dim(n, j); the rows' pairs are
+// joined per dim with one byte permutation.
 // fp32 (16 tokens): K dims 16c + 4q .. +4 (four 16x16x4 products per load), V
 // the same with float columns.
 template <int DT, int D>
@@ -59,6 +52,9 @@ struct Tile {
   static constexpr int kTokens = 16 * kBlocks;
   static constexpr int kKLoads = D * kElem<DT> / 64;        // 16-byte loads of a K row per lane
   static constexpr int kVWords = D * kElem<DT> / 64;        // 32-bit words of a V row per lane
+  static constexpr int kVStep = kVWords < 4 ? 4 * kVWords : 16;  // bytes of a piece
+  static constexpr int kRun = kVStep / kElem<DT>;           // elements of a piece
+  static __device__ __forceinline__ int dim(int n, int j) { return n / kRun * (16 * kRun) + j * kRun + n % kRun; }
   uint4 k[kBlocks][kKLoads];
   unsigned v[kBlocks][4][kVWords];
 };
@@ -73,7 +69,25 @@ __device__ __forceinline__ void load_words(unsigned (&dst)[W], const char* p) {
   } else {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      const uint4 x = load_nt16(p + 4 * i);
+      const uint4 x = load_nt16(p + 64 * i);
+      dst[i] = x.x;
+      dst[i + 1] = x.y;
+      dst[i + 2] = x.z;
+      dst[i + 3] = x.w;
+    }
+  }
+}
+
+template <int W>
+__device__ __forceinline__ void load_words_buf(unsigned (&dst)[W], __amdgpu_buffer_rsrc_t r, unsigned byte_offset) {
+  if constexpr (W == 2) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, byte_offset, 0, 2);
+    dst[0] = x[0];
+    dst[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const uint4 x = load_nt16_buf(r, byte_offset + 64 * i);
       dst[i] = x.x;
       dst[i + 1] = x.y;
       dst[i + 2] = x.z;
@@ -101,129 +115,331 @@ __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
 template <int DT>
 __device__ __forceinline__ void split16(float p, unsigned& hi, unsigned& lo) {
   if constexpr (DT == kBf16) {
-    const unsigned u = __float_as_uint(p);
+    const unsigned u = __float_as_uint(p * (1.f - 0x1p-9f)) & 0xffff0000u;
     hi = u >> 16;
-    lo = f32_to_bf16(p - __uint_as_float(u & 0xffff0000u));
+    lo = f32_to_bf16(p - __uint_as_float(u));
   } else {
-    const _Float16 h = (_Float16)p;
+    const _Float16 h = (_Float16)(p * (1.f - 0x1p-10f));
     const _Float16 l = (_Float16)(p - (float)h);
     hi = __builtin_bit_cast(unsigned short, h);
     lo = __builtin_bit_cast(unsigned short, l);
   }
 }
 
-// P is held times 2^kBias: fp16 probabilities from 2^-29 of the maximum up stay
-// normal numbers (bf16 and fp32 have the exponents for them).
-template <int DT>
-constexpr int kBias = DT == kFp16 ? 15 : 0;
-
 template <int N, int DT, int D>
-__device__ __forceinline__ void pv_columns(Acc<DT, D>& acc, const Tile<DT, D>& t, u32x4 ph, u32x4 pl) {
+__device__ __forceinline__ void pv_columns(f32x4 (&acc)[D / 16], const Tile<DT, D>& t, u32x4 ph, u32x4 pl) {
   if constexpr (N < D / 16) {
     const u32x4 vb = {pair16<N>(t.v[0][0], t.v[0][1]), pair16<N>(t.v[0][2], t.v[0][3]),
                       pair16<N>(t.v[1][0], t.v[1][1]), pair16<N>(t.v[1][2], t.v[1][3])};
-    acc.hi[N] = mfma32<DT>(ph, vb, acc.hi[N]);
-    acc.lo[N] = mfma32<DT>(pl, vb, acc.lo[N]);
-    pv_columns<N + 1>(acc, t, ph, pl);
+    acc[N] = mfma32<DT>(ph, vb, acc[N]);
+    acc[N] = mfma32<DT>(pl, vb, acc[N]);
+    pv_columns<N + 1, DT, D>(acc, t, ph, pl);
   }
 }
 
+// 2^(scale s - m): one rounding of the difference, however large the two are.  m
+// is finite or +infinity (no_less): where no score is above -infinity, 0 serves.
+__device__ __forceinline__ float weight(float s, float scale, float m) {
+  return __builtin_amdgcn_exp2f(fmaf(s, scale, -m));
+}
+__device__ __forceinline__ float no_less(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Factor of a state with maximum m under the joint maximum M >= m (no state: 0).
+__device__ __forceinline__ float rescale(float m, float M) {
+  return m == -INFINITY ? 0.f : m == M ? 1.f : exp2f(m - M);
+}
+
+// The joint maximum and sum of a pair's head g over its states, and the states'
+// factors in wt[c * stride] (LDS); by one wave.
+__device__ __forceinline__ float2 join_sums(const float* base, const PagedParts& parts, unsigned state_stride, int g,
+                                            float* wt, int stride) {
+  const int lane = threadIdx.x & 63;
+  float M = -INFINITY, den = 0.f;
+  for (int c0 = 0; c0 < parts.chunks; c0 += 64) {
+    const int c = c0 + lane;
+    const bool in = c < parts.chunks;
+    const float2 mz = ld_dev2(base + (in && c ? 2 * c : parts.odd) * state_stride + 2 * g);
+    const float m = in ? mz.x : -INFINITY;
+    const float nM = fmaxf(M, wave_max(m));
+    den = den * rescale(M, nM) + wave_sum(in ? rescale(m, nM) * mz.y : 0.f);
+    M = nM;
+    if (in && wt) wt[c * stride] = m;
+  }
+  if (wt)
+    for (int c = lane; c < parts.chunks; c += 64) wt[c * stride] = rescale(wt[c * stride], M);
+  return make_float2(M, den);
+}
+
+// Joins columns [col0, col0 + columns) (4 floats each of the [rows][D] output) of a
+// pair's states, by a workgroup of kThreads: the maxima and sums a wave per head,
+// while the first states' loads are in flight, then a thread per column and share
+// of the states, the shares added in LDS.
+template <int DT, int D, int kThreads>
+__device__ __forceinline__ void join_states(const PagedAttend& a, size_t head0, int rows, const PagedParts& parts, int col0,
+                                            int columns, float* lds) {
+  const int tid = threadIdx.x, w = tid >> 6;
+  float4* part = reinterpret_cast<float4*>(lds);  // [threads]
+  float* top = lds + 4 * kThreads;                // [16] joint maxima, [16] sums
+  float* wt = top + 32;                           // [chunks][rows] factors
+  const float* base = a.state + (size_t)2 * parts.unit * a.state_stride;
+  const __amdgpu_buffer_rsrc_t r = raw_buffer(base, 2 * parts.chunks * (int)a.state_stride * 4);
+  const int chunks = parts.chunks;
+  const int shares = max(kThreads / columns, 1), share = tid / columns;  // (columns > threads: in turns)
+  constexpr int kU = 8;
+  float4 x[kU];
+  auto load = [&](int c0, int col) {
+#pragma unroll
+    for (int e = 0; e < kU; ++e) {
+      const int c = min(c0 + e * shares, chunks - 1);
+      x[e] = ld_dev4(r, ((unsigned)(c ? 2 * c : parts.odd) * a.state_stride + 2 * rows + 4 * col) * 4);
+    }
+  };
+  int col = col0 + tid - share * columns;
+  load(share, col);
+  const int head = 4 * col0 / D, heads = (4 * (col0 + columns) - 1) / D + 1;  // of these columns
+  for (int i = head + w; i < heads; i += kThreads / 64) {
+    const float2 mz = join_sums(base, parts, a.state_stride, i, wt + i, rows);
+    if ((tid & 63) == 0) {
+      top[i] = mz.x;
+      top[16 + i] = mz.y;
+    }
+  }
+  __syncthreads();
+  while (true) {
+    const int g = 4 * col / D;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = share; share < shares && c0 < chunks;) {
+#pragma unroll
+      for (int e = 0; e < kU; ++e) {
+        const int c = c0 + e * shares;
+        if (c < chunks) {
+          const float f = wt[c * rows + g];
+          sum.x = fmaf(f, x[e].x, sum.x);
+          sum.y = fmaf(f, x[e].y, sum.y);
+          sum.z = fmaf(f, x[e].z, sum.z);
+          sum.w = fmaf(f, x[e].w, sum.w);
+        }
+      }
+      c0 += kU * shares;
+      if (c0 < chunks) load(c0, col);
+    }
+    if (shares > 1) {  // (then all columns are in this turn)
+      part[tid] = sum;
+      __syncthreads();
+      for (int k = 1; share == 0 && k < shares; ++k) {
+        const float4 y = part[tid + k * columns];
+        sum.x += y.x;
+        sum.y += y.y;
+        sum.z += y.z;
+        sum.w += y.w;
+      }
+    }
+    if (share == 0) {
+      finish<DT, D>(a, head0, 4 * col, top[g], top[16 + g], sum.x);
+      finish<DT, D>(a, head0, 4 * col + 1, top[g], top[16 + g], sum.y);
+      finish<DT, D>(a, head0, 4 * col + 2, top[g], top[16 + g], sum.z);
+      finish<DT, D>(a, head0, 4 * col + 3, top[g], top[16 + g], sum.w);
+    }
+    col += kThreads;
+    if (shares > 1 || col >= col0 + columns) return;
+    load(share, col);
+  }
+}
+
+// Where a wave's tiles lie.  `ask` looks up the pages of the tile at t0, `move`
+// makes it the tile that is loaded.
+template <int DT, int D, bool kAligned>
+struct Rows;
+
+// Pages of whole 16-token blocks: a block's page is the same for all lanes, so it
+// is looked up through the scalar cache, beside the vector loads' order, and read
+// through a buffer resource of its own that ends with the last token: rows past
+// the end come back as zeros, a block past the end is not read at all, and a lane
+// has one fixed offset per row.
 template <int DT, int D>
-__global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void paged_attend_kernel(PagedAttend a) {
+struct Rows<DT, D, true> {
   typedef Tile<DT, D> T;
-  constexpr int kQRegs = T::kKLoads;
-  extern __shared__ float lds[];
+  const PagedAttend& a;
+  const char *k, *v;
+  const int32_t* tab;
+  unsigned k_lane, v_lane[4];
+  int end;
+  int token[T::kBlocks], page[T::kBlocks];
+  __amdgpu_buffer_rsrc_t kr[T::kBlocks], vr[T::kBlocks];
+  bool bad = false;
+  __device__ __forceinline__ Rows(const PagedAttend& a, int b, int h, int end) : a(a), end(end) {
+    const unsigned lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4, slot = a.slot_units << 4;
+    k = reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes;
+    v = reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes;
+    tab = a.table + (size_t)b * a.max_pages;
+    k_lane = j * slot + 16 * q;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v_lane[r] = (4 * q + r) * slot + j * T::kVStep;
+  }
+  __device__ __forceinline__ void ask(int t0) {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) {
+      token[i] = t0 + 16 * i;
+      typedef const __attribute__((address_space(4))) int32_t* Uniform;
+      page[i] = *(Uniform)(uint64_t)(tab + __builtin_amdgcn_readfirstlane(a.div.of(min(token[i], end - 1))));
+    }
+  }
+  __device__ __forceinline__ void move() {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) {
+      const int rows = min(end - token[i], 16);
+      bad |= rows > 0 && (unsigned)page[i] >= (unsigned)a.pages;
+      const unsigned from = (unsigned)page[i] < (unsigned)a.pages ? (unsigned)page[i] : 0u;
+      const size_t at = ((size_t)from * a.page_units +
+                         (unsigned)(token[i] - a.div.of(token[i]) * a.page_size) * a.slot_units) << 4;
+      const int bytes = rows > 0 ? (int)((rows - 1) * (a.slot_units << 4)) + D * kElem<DT> : 0;
+      kr[i] = raw_buffer(k + at, bytes);
+      vr[i] = raw_buffer(v + at, bytes);
+    }
+  }
+  __device__ __forceinline__ void load_k(T& t) const {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+      for (int c = 0; c < T::kKLoads; ++c) t.k[i][c] = load_nt16_buf(kr[i], k_lane + 64 * c);
+  }
+  __device__ __forceinline__ void load_v(T& t) const {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_words_buf(t.v[i][r], vr[i], v_lane[r]);
+  }
+};
+
+// Any page size: each lane looks up the rows that it loads keys of, and takes the
+// values' rows from the lanes that have them.  Tokens past the end repeat the last.
+template <int DT, int D>
+struct Rows<DT, D, false> {
+  typedef Tile<DT, D> T;
+  const PagedAttend& a;
+  const char *k, *v;
+  const int32_t* tab;
+  int end, token[T::kBlocks], page[T::kBlocks];
+  unsigned row[T::kBlocks];  // 16-byte units
+  bool bad = false;
+  __device__ __forceinline__ Rows(const PagedAttend& a, int b, int h, int end) : a(a), end(end) {
+    const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+    k = reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes + 16 * q;
+    v = reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes + j * T::kVStep;
+    tab = a.table + (size_t)b * a.max_pages;
+  }
+  __device__ __forceinline__ void ask(int t0) {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) {
+      token[i] = min(t0 + 16 * i + (int)(threadIdx.x & 15), end - 1);
+      page[i] = tab[a.div.of(token[i])];
+    }
+  }
+  __device__ __forceinline__ void move() {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i) {
+      if ((unsigned)page[i] >= (unsigned)a.pages) {
+        bad = true;
+        page[i] = 0;
+      }
+      row[i] = (unsigned)page[i] * a.page_units +
+               (unsigned)(token[i] - a.div.of(token[i]) * a.page_size) * a.slot_units;
+    }
+  }
+  __device__ __forceinline__ void load_k(T& t) const {
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+      for (int c = 0; c < T::kKLoads; ++c) t.k[i][c] = load_nt16(k + ((size_t)row[i] << 4) + 64 * c);
+  }
+  __device__ __forceinline__ void load_v(T& t) const {
+    const int q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_words(t.v[i][r], v + ((size_t)(unsigned)__shfl((int)row[i], 4 * q + r) << 4));
+  }
+};
+
+// `count` quanta of one pair from its quantum u.first on: this workgroup's state
+// of them, and the pair's output if it is the only or the last to come.
+template <int DT, int D, bool kAligned>
+__device__ __forceinline__ void attend_segment(const PagedAttend& a, const PagedSpan<kLeast<DT, D>>& u, int quanta, int count, float* lds) {
+  typedef Tile<DT, D> T;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const PagedUnit u = find_unit(a, blockIdx.x);
-  if (u.b < 0) return;
   const int h = u.hh / a.tiles, g0 = 16 * (u.hh - h * a.tiles);
   const int rows = min(a.group - g0, 16);  // query heads of this tile
-  const int start = min(u.chunk * u.per, u.n), end = min(start + u.per, u.n);
+  const int start = min(u.first * kQuantum, u.n), end = min(start + count * kQuantum, u.n);
 
   // Q^T: column j is head j (zero past the tile's heads)
-  u32x4 qop[kQRegs];
+  u32x4 qop[T::kKLoads];
   {
     const char* qp = reinterpret_cast<const char*>(a.q) +
                      (((size_t)u.b * a.kv_heads + h) * a.group + g0 + min(j, rows - 1)) * (D * kElem<DT>) + 16 * q;
 #pragma unroll
-    for (int c = 0; c < kQRegs; ++c) {
+    for (int c = 0; c < T::kKLoads; ++c) {
       const uint4 x = *reinterpret_cast<const uint4*>(qp + 64 * c);
       qop[c] = j < rows ? u32x4{x.x, x.y, x.z, x.w} : u32x4{0u, 0u, 0u, 0u};
     }
   }
-  Acc<DT, D> acc;
+  f32x4 acc[D / 16];
 #pragma unroll
-  for (int n = 0; n < D / 16; ++n) {
-    acc.hi[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if constexpr (DT != kFp32) acc.lo[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int n = 0; n < D / 16; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, z = 0.f;  // head j's running maximum (exp2 domain), this lane's share of its sum
 
-  const char* kh = reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes + 16 * q;
-  const char* vh = reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes + j * (D * kElem<DT> / 16);
-  const int32_t* tab = a.table + (size_t)u.b * a.max_pages;
   float* logits = a.logits ? a.logits + (((size_t)u.b * a.kv_heads + h) * a.group + g0 + j) * a.logit_stride : nullptr;
-  bool bad = false;
-  // row offset (16-byte units) of token t, the last token's past the end
-  auto row_of = [&](int t) -> unsigned {
-    t = min(t, end - 1);
-    const int p = a.div.of(t);
-    int page = tab[p];
-    if ((unsigned)page >= (unsigned)a.pages) {
-      bad = true;
-      page = 0;
-    }
-    return (unsigned)page * a.page_units + (unsigned)(t - p * a.page_size) * a.slot_units;
-  };
+  Rows<DT, D, kAligned> rows_of(a, u.b, h, end);
 
+  // Loads run ahead without registers of their own: the next tile's keys are
+  // requested as soon as this one's are used up by the scores, its values after
+  // the products with this one's, and the pages of the tile after that in
+  // between (memory answers in order: whatever is waited for was asked first).
+  constexpr int kStep = kAWaves<D> * T::kTokens;
   int t0 = start + T::kTokens * w;
-  unsigned row[T::kBlocks];
+  T t;
   if (t0 < end) {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) row[i] = row_of(t0 + 16 * i + j);
+    rows_of.ask(t0);
+    rows_of.move();
+    rows_of.load_k(t);
+    rows_of.ask(t0 + kStep);
+    rows_of.load_v(t);
   }
-  while (t0 < end) {
-    T t;
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int c = 0; c < T::kKLoads; ++c) t.k[i][c] = load_nt16(kh + ((size_t)row[i] << 4) + 64 * c);
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) load_words(t.v[i][r], vh + ((size_t)(unsigned)__shfl((int)row[i], 4 * q + r) << 4));
-    const int next = t0 + kPWaves * T::kTokens;
-    if (next < end) {
-#pragma unroll
-      for (int i = 0; i < T::kBlocks; ++i) row[i] = row_of(next + 16 * i + j);
-    }
-
+  // (the loads of the tile behind the last are issued too: on every path as many
+  // are in flight, so that the compiler's wait counts are exact)
+  for (; t0 < end; t0 += kStep) {
     // scores: lane (j, q) gets tokens 16i + 4q + r of head j
     float s[T::kBlocks][4];
     float bm = -INFINITY;
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i) {
-      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+      f32x4 d = {0.f, 0.f, 0.f, 0.f}, d2 = d;  // (fp32: two shorter chains, whose rounding errors are smaller)
 #pragma unroll
       for (int c = 0; c < T::kKLoads; ++c) {
         const u32x4 kw = {t.k[i][c].x, t.k[i][c].y, t.k[i][c].z, t.k[i][c].w};
+        const u32x4 qw = qop[c];
         if constexpr (DT == kFp32) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qop[c][e]), d, 0, 0, 0);
+          for (int e = 0; e < 4; e += 2) {
+            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), d, 0, 0, 0);
+            d2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e + 1]), __uint_as_float(qw[e + 1]), d2, 0, 0,
+                                                      0);
+          }
         } else {
-          d = mfma32<DT>(kw, qop[c], d);
+          d = mfma32<DT>(kw, qw, d);
         }
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        s[i][r] = t0 + 16 * i + 4 * q + r < end ? d[r] * a.scale : -INFINITY;
-        bm = fmaxf(bm, s[i][r]);
+        s[i][r] = DT == kFp32 ? d[r] + d2[r] : d[r];
+        bm = fmaxf(bm, t0 + 16 * i + 4 * q + r < end ? s[i][r] * a.scale : -INFINITY);
       }
       if (logits && j < rows)
         *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
     }
+    rows_of.move();
+    rows_of.load_k(t);
+    rows_of.ask(t0 + 2 * kStep);
     bm = fmaxf(bm, xor16(bm));
     bm = fmaxf(bm, xor32(bm));
     if (__ballot(bm > m)) {
@@ -235,21 +451,21 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void paged_attend_kernel(Pag
       for (int r = 0; r < 4; ++r) {
         const float ah = __shfl(alpha, 4 * q + r);
 #pragma unroll
-        for (int n = 0; n < D / 16; ++n) {
-          acc.hi[n][r] *= ah;
-          if constexpr (DT != kFp32) acc.lo[n][r] *= ah;
-        }
+        for (int n = 0; n < D / 16; ++n) acc[n][r] *= ah;
       }
     }
+    const float top = no_less(m);
     float p[T::kBlocks][4];
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[i][r] = s[i][r] == -INFINITY ? 0.f : ldexpf(exp2f(s[i][r] - m), kBias<DT>);
+        p[i][r] = weight(s[i][r], a.scale, top);
+        if (t0 + 16 * i + 4 * q + r >= end) p[i][r] = 0.f;
+        if constexpr (kBias<DT> != 0) p[i][r] = ldexpf(p[i][r], kBias<DT>);
         z += p[i][r];
       }
-    if (t0 + T::kTokens > end) {  // rows past the end repeat the last one: 0 times its infinity must not be added
+    if (!kAligned && t0 + T::kTokens > end) {  // rows past the end repeat the last one: 0 times its infinity must not be added
 #pragma unroll
       for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
@@ -264,7 +480,7 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void paged_attend_kernel(Pag
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int n = 0; n < D / 16; ++n)
-          acc.hi[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][r], __uint_as_float(t.v[0][r][n]), acc.hi[n], 0, 0, 0);
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][r], __uint_as_float(t.v[0][r][n]), acc[n], 0, 0, 0);
     } else {
       unsigned hi[8], lo[8];
 #pragma unroll
@@ -273,16 +489,16 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void paged_attend_kernel(Pag
         for (int r = 0; r < 4; ++r) split16<DT>(p[i][r], hi[4 * i + r], lo[4 * i + r]);
       const u32x4 ph = {hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16};
       const u32x4 pl = {lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
-      pv_columns<0>(acc, t, ph, pl);
+      pv_columns<0, DT, D>(acc, t, ph, pl);
     }
-    t0 = next;
+    rows_of.load_v(t);
   }
-  if (__ballot(bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
+  if (__ballot(rows_of.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
 
   // the waves' states meet in LDS
-  float* sm = lds;                 // [waves][16] maxima
-  float* sz = sm + 16 * kPWaves;   // [waves][16] sums
-  float* sacc = sz + 16 * kPWaves; // [waves][rows][D]
+  float* sm = lds;  // [waves][16] maxima
+  float* sz = sm + 16 * kAWaves<D>;   // [waves][16] sums
+  float* sacc = sz + 16 * kAWaves<D>; // [waves][rows][D]
   z += xor16(z);
   z += xor32(z);
   if (lane < 16) {
@@ -292,88 +508,103 @@ __global__ __launch_bounds__(kPT, D == 256 ? 1 : 2) void paged_attend_kernel(Pag
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (4 * q + r < rows) {
-      float* dst = sacc + ((size_t)w * rows + 4 * q + r) * D + j * (D / 16);
+      float* dst = sacc + ((size_t)w * rows + 4 * q + r) * D;
 #pragma unroll
-      for (int n = 0; n < D / 16; n += 4) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = acc.hi[n + e][r];
-          if constexpr (DT != kFp32) {
-            const float rest = acc.lo[n + e][r];
-            if (isfinite(rest)) x[e] += rest;
-          }
-        }
-        *reinterpret_cast<float4*>(dst + n) = make_float4(x[0], x[1], x[2], x[3]);
-      }
+      for (int n = 0; n < D / 16; n += 4)  // (a piece is 4 or 8 elements)
+        *reinterpret_cast<float4*>(dst + T::dim(n, j)) = make_float4(acc[n][r], acc[n + 1][r], acc[n + 2][r], acc[n + 3][r]);
     }
   __syncthreads();
   const size_t head0 = ((size_t)u.b * a.kv_heads + h) * a.group + g0;  // this tile's first query head
-  float* state = a.state + (size_t)blockIdx.x * a.state_stride;        // [rows]{max, sum} then [rows][D]
-  for (int i = tid; i < rows * D; i += kPT) {
+  const int pair0 = u.at - u.first, unit = (int)blockIdx.x;
+  const bool whole = count == quanta;
+  float* state = a.state + (size_t)(2 * unit + (u.at != u.deal.begin(unit))) * a.state_stride;  // {max, sum}[rows], [rows][D]
+  for (int i = 2 * tid; i < rows * D; i += 128 * kAWaves<D>) {
     const int g = i / D;
     float M = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kPWaves; ++k) M = fmaxf(M, sm[16 * k + g]);
-    float den = 0.f, x = 0.f;
+    for (int k = 0; k < kAWaves<D>; ++k) M = fmaxf(M, sm[16 * k + g]);
+    float den = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int k = 0; k < kPWaves; ++k) {
-      const float wt = exp2_or_zero(sm[16 * k + g] == M ? (M == -INFINITY ? -INFINITY : 0.f) : sm[16 * k + g] - M);
+    for (int k = 0; k < kAWaves<D>; ++k) {
+      const float wt = rescale(sm[16 * k + g], M);
+      const float2 v = *reinterpret_cast<const float2*>(sacc + (size_t)k * rows * D + i);
       den = fmaf(wt, sz[16 * k + g], den);
-      x = fmaf(wt, sacc[((size_t)k * rows) * D + i], x);
+      x = fmaf(wt, v.x, x);
+      y = fmaf(wt, v.y, y);
     }
-    if (u.chunks == 1) {
+    if (whole) {
       finish<DT, D>(a, head0, i, M, den, x);
+      finish<DT, D>(a, head0, i + 1, M, den, y);
     } else {
       if (i % D == 0) st_dev2(state + 2 * g, M, den);
-      st_dev(state + 2 * rows + i, x);
+      st_dev2(state + 2 * rows + i, x, y);
     }
   }
-  if (u.chunks == 1) return;
+  if (whole || !a.counters) return;
 
-  // the last workgroup of this (sequence, head tile) joins the chunks
+  // the last workgroup of the pair joins the states
+  const PagedParts parts(u.deal, pair0, quanta);
   int* last = reinterpret_cast<int*>(lds);
   drain();
   __syncthreads();
   unsigned* counter = a.counters + (size_t)u.b * a.kv_heads * a.tiles + u.hh;
-  if (tid == 0) *last = inc_dev(counter) == (unsigned)(u.chunks - 1);
+  if (tid == 0) *last = inc_dev(counter) == (unsigned)(parts.chunks - 1);
   __syncthreads();
   const int is_last = *last;
   __syncthreads();
   if (!is_last) return;
   if (tid == 0) st_dev(counter, 0u);
-  const size_t step = (size_t)a.kv_heads * a.tiles * a.state_stride;  // between a sequence's chunks
-  const float* st0 = state - (size_t)u.chunk * step;
-  for (int i = tid; i < rows * D; i += kPT) {
-    const int g = i / D;
-    float M = -INFINITY, den = 0.f, x = 0.f;
-    for (int c0 = 0; c0 < u.chunks; c0 += 8) {
-      float2 mz[8];
-      float xv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float* st = st0 + (size_t)min(c0 + e, u.chunks - 1) * step;
-        mz[e] = ld_dev2(st + 2 * g);
-        xv[e] = ld_dev(st + 2 * rows + i);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (c0 + e >= u.chunks) break;
-        const float nM = fmaxf(M, mz[e].x);
-        const float old = M == nM ? 1.f : exp2_or_zero(M - nM);
-        const float wt = mz[e].x == nM ? (nM == -INFINITY ? 0.f : 1.f) : exp2_or_zero(mz[e].x - nM);
-        den = fmaf(wt, mz[e].y, den * old);
-        x = fmaf(wt, xv[e], x * old);
-        M = nM;
-      }
+  join_states<DT, D, 64 * kAWaves<D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
+}
+
+template <int DT, int D, bool kAligned>
+__global__ __launch_bounds__(64 * kAWaves<D>, kAWaves<D> / 4) void paged_attend_kernel(PagedAttend a) {
+  extern __shared__ float lds[];
+  PagedSpan<kLeast<DT, D>> u = find_span<kLeast<DT, D>>(a, blockIdx.x);
+  while (u.at < u.end) {  // the pairs that this workgroup's share lies in
+    const int quanta = quanta_of<kLeast<DT, D>>(u.n);
+    const int count = min(quanta - u.first, u.end - u.at);
+    attend_segment<DT, D, kAligned>(a, u, quanta, count, lds);
+    u.at += count;
+    u.first = 0;
+    if (++u.hh == a.kv_heads * a.tiles) {
+      u.hh = 0;
+      u.n = ++u.b < a.sequences ? clamp_length(a, a.lengths[u.b]) : 0;
     }
-    finish<DT, D>(a, head0, i, M, den, x);
+    __syncthreads();  // the next pair's states go where these were
   }
 }
 
-// scores_out[t] = scores[t] + sum over the group's heads of e^(s_t - lse): one
-// thread per slot, bound by the scores it reads (4 bytes per query head) and
-// the two score arrays.
+// Joins in a launch of their own: the states of a pair that are many and wide, over
+// several workgroups, kJoinColumns columns each.
+constexpr int kJoinColumns = 16;
+
+template <int DT, int D>
+__global__ __launch_bounds__(kPT) void paged_join_kernel(PagedAttend a) {
+  extern __shared__ float lds[];
+  const int b = blockIdx.z, lane = threadIdx.x & 63;
+  const int h = blockIdx.y / a.tiles, tile = blockIdx.y - h * a.tiles;
+  const int rows = min(a.group - 16 * tile, 16), col0 = blockIdx.x * kJoinColumns;
+  if (col0 >= rows * D / 4) return;
+  constexpr int kL = kLeast<DT, D>;
+  PagedDeal<kL> deal{0};
+  int from = 0, n = 0;  // quanta before sequence b, its length
+  each_64<kL>(a, [&](int i, int len, int c) {
+    deal.total += wave_sum_i(c);
+    from += wave_sum_i(i + lane < b ? c : 0);
+    if (i <= b && b < i + 64) n = __builtin_amdgcn_readlane(len, b - i);
+    return false;
+  });
+  deal.total *= a.kv_heads * a.tiles;
+  const int quanta = quanta_of<kL>(n);
+  const PagedParts parts(deal, from * a.kv_heads * a.tiles + (int)blockIdx.y * quanta, quanta);
+  if (parts.chunks == 1) return;  // its workgroup has finished it
+  join_states<DT, D, kPT>(a, ((size_t)b * a.kv_heads + h) * a.group + 16 * tile, rows, parts, col0, kJoinColumns, lds);
+}
+
+// scores_out[t] = scores[t] + sum over the group's heads of e^(s_t - lse): a
+// thread per slot; bound by the scores that it reads (4 bytes per query head and
+// slot) and the two score arrays.
 __global__ __launch_bounds__(kPT) void paged_weigh_kernel(PagedAttend a) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int n = clamp_length(a, a.lengths[b]);
@@ -382,10 +613,7 @@ __global__ __launch_bounds__(kPT) void paged_weigh_kernel(PagedAttend a) {
   const size_t at = ((size_t)b * a.kv_heads + h) * a.slots;
   for (int t = blockIdx.x * kPT + threadIdx.x; t < n; t += gridDim.x * kPT) {
     float sum = 0.f;
-    for (int g = 0; g < a.group; ++g) {
-      const float l = lse[g], s = logits[(size_t)g * a.logit_stride + t];
-      sum += s == -INFINITY ? 0.f : exp2f(s - l);
-    }
+    for (int g = 0; g < a.group; ++g) sum += weight(logits[(size_t)g * a.logit_stride + t], a.scale, no_less(lse[g]));
     a.scores_out[at + t] = a.scores[at + t] + sum;
   }
 }
@@ -661,37 +889,58 @@ bool bad_cache(int sequences, int kv_heads, int head_dim, int page_size, int max
 struct WorkLayout {
   size_t lse, state, logits, bytes;  // counters first
   unsigned state_stride;
-  int64_t logit_stride, units;
+  int64_t logit_stride, quanta, units;
 };
 
-WorkLayout attend_layout(int sequences, int kv_heads, int group, int head_dim, int64_t slots, bool weigh) {
+WorkLayout attend_layout(int sequences, int kv_heads, int group, int head_dim, int64_t slots, bool weigh, int dtype) {
   WorkLayout w;
   const int64_t tiles = (group + 15) / 16, heads = (int64_t)kv_heads * tiles;
-  // no sequence has more chunks than its longest table allows
-  const int64_t most = sequences * heads * ((slots + 32 * kPWaves - 1) / (32 * kPWaves));
-  w.units = (int64_t)sequences * heads + (1 << kLogUnits);
-  if (most < w.units) w.units = most;
+  const int least = (dtype == kFp32 ? 1 : 2) * (head_dim == 256 ? kAWaves<256> : kAWaves<128>) / 2;
+  const int64_t workgroups = sequences * heads * ((slots + least * kQuantum - 1) / (least * kQuantum));  // of full tables
+  w.quanta = workgroups * least;
+  w.units = workgroups < kUnits ? workgroups : kUnits;
   w.state_stride = (unsigned)((group < 16 ? group : 16) * (head_dim + 2));
   w.logit_stride = (slots + 31) & ~31ll;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   w.lse = up((size_t)sequences * heads * sizeof(unsigned));
   w.state = w.lse + up((size_t)sequences * kv_heads * group * sizeof(float));
-  w.logits = w.state + up((size_t)w.units * w.state_stride * sizeof(float));
+  w.logits = w.state + up((size_t)2 * w.units * w.state_stride * sizeof(float));
   w.bytes = w.logits + (weigh ? (size_t)sequences * kv_heads * group * w.logit_stride * sizeof(float) : 0);
   return w;
 }
 
-template <int DT, int D>
-int launch_attend(const PagedAttend& a, int64_t units, hipStream_t stream) {
-  const int rows = a.group < 16 ? a.group : 16;
-  const int lds = (32 * kPWaves + kPWaves * rows * D) * (int)sizeof(float);
+template <int DT, int D, bool kAligned>
+int launch_attend_rows(const PagedAttend& a, int64_t units, int lds, hipStream_t stream) {
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attend_kernel<DT, D>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             (32 * kPWaves + kPWaves * 16 * D) * (int)sizeof(float));
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attend_kernel<DT, D, kAligned>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL((paged_attend_kernel<DT, D>), dim3((unsigned)units), dim3(kPT), lds, stream, a);
+  hipLaunchKernelGGL((paged_attend_kernel<DT, D, kAligned>), dim3((unsigned)units), dim3(64 * kAWaves<D>), lds, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <int DT, int D>
+int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
+  const int rows = a.group < 16 ? a.group : 16;
+  const int64_t longest = a.slots / (kLeast<DT, D> * kQuantum) + 2;
+  const int64_t most = kUnits / (a.kv_heads * a.tiles) + 2;  // (a sequence's pairs are alike)
+  const int chunks = (int)(longest < most ? longest : most);  // of one pair at most
+    // Where a pair's states may be many and wide a second launch joins them: 65536
+  // tokens of one KV head and 16 query heads (264K floats) 20.0 us, 47.5 by the last
+  // workgroup; of 8 KV heads and 4 (17K) 48.2 against 47.8.
+  const bool apart = (int64_t)chunks * rows * D > 49152;
+  const int merge = 32 * kAWaves<D> + kAWaves<D> * rows * D, sums = 32 + chunks * rows;
+  const int join = apart ? 0 : 256 * kAWaves<D> + sums;
+  const int lds = (merge > join ? merge : join) * (int)sizeof(float);
+  if (apart) a.counters = nullptr;
+  // a lane's offset within a block is 32 bits
+  const bool aligned = a.page_size % 16 == 0 && a.slot_units < (1u << 23);
+  const int rc = aligned ? launch_attend_rows<DT, D, true>(a, units, lds, stream)
+                         : launch_attend_rows<DT, D, false>(a, units, lds, stream);
+  if (rc || !apart) return rc;
+  hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3((rows * D / 4 + kJoinColumns - 1) / kJoinColumns,
+                     a.kv_heads * a.tiles, a.sequences), dim3(kPT), (4 * kPT + sums) * (int)sizeof(float), stream, a);
   return (int)hipGetLastError();
 }
 
@@ -706,9 +955,10 @@ int launch_attend_dim(const PagedAttend& a, int head_dim, int64_t units, hipStre
 
 extern "C" {
 
-size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh) {
-  if (sequences < 1 || kv_heads < 1 || group < 1 || head_dim < 1 || slots < 1) return 0;
-  return attend_layout(sequences, kv_heads, group, head_dim, slots, weigh != 0).bytes;
+size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh,
+                                       int dtype) {
+  if (dtype < kBf16 || dtype > kFp32 || sequences < 1 || kv_heads < 1 || group < 1 || head_dim < 1 || slots < 1) return 0;
+  return attend_layout(sequences, kv_heads, group, head_dim, slots, weigh != 0, dtype).bytes;
 }
 
 int prismkv_paged_attend(uint64_t q, uint64_t k, uint64_t v, uint64_t table, uint64_t lengths, uint64_t scores,
@@ -723,8 +973,8 @@ int prismkv_paged_attend(uint64_t q, uint64_t k, uint64_t v, uint64_t table, uin
   if (!q || !k || !v || !table || !lengths || !paged_work || !err || !out || !scores != !scores_out) return kBadSize;
   if ((q | k | v | paged_work) & 15 || (table | lengths | scores | scores_out | lse) & 3 || err & 7) return kBadSize;
   const int64_t slots = (int64_t)page_size * max_pages;
-  const WorkLayout w = attend_layout(sequences, kv_heads, group, head_dim, slots, scores != 0);
-  if (work_bytes < w.bytes || w.units > INT32_MAX) return kBadSize;
+  const WorkLayout w = attend_layout(sequences, kv_heads, group, head_dim, slots, scores != 0, dtype);
+  if (work_bytes < w.bytes || w.quanta > INT32_MAX) return kBadSize;  // (quanta are counted in 32 bits)
   const int es = element_bytes(dtype);
   PagedAttend a{};
   a.q = reinterpret_cast<const void*>(q);

@@ -322,7 +322,7 @@ class PagedCache:
         if work is None:
             # (the leading counters are zeroed; the kernels leave them so)
             nbytes = self.lib.query("prismkv_paged_attend_work_bytes", sequences, kv_heads, group, head_dim, self.slots,
-                                    int(accumulate))
+                                    int(accumulate), self._dtype)
             work = self._attend_work[(group, accumulate)] = self._workspace(
                 nbytes, 4 * sequences * kv_heads * ((group + 15) // 16))
         out = torch.empty_like(q)

@@ -79,12 +79,13 @@ def test_refused_arguments(lib):  # noqa: F811
 
 
 def test_workspace_sizes(lib):  # noqa: F811
-    need = lib.query("prismkv_paged_attend_work_bytes", 3, 8, 4, 128, 160, 1)
+    need = lib.query("prismkv_paged_attend_work_bytes", 3, 8, 4, 128, 160, 1, 0)
     # the weighed logits of every query head and slot, at least
-    assert need >= 3 * 32 * 160 * 4 + lib.query("prismkv_paged_attend_work_bytes", 3, 8, 4, 128, 160, 0)
+    assert need >= 3 * 32 * 160 * 4 + lib.query("prismkv_paged_attend_work_bytes", 3, 8, 4, 128, 160, 0, 0)
     assert attend(lib, work=need - 1) == -1
     assert attend(lib, work=need) not in (0, -1, -2)  # past every host check, refused by the runtime (no device)
-    for bad in ((0, 8, 4, 128, 160, 0), (3, 0, 4, 128, 160, 0), (3, 8, 0, 128, 160, 0), (3, 8, 4, 128, 0, 0)):
+    for bad in ((0, 8, 4, 128, 160, 0, 0), (3, 0, 4, 128, 160, 0, 0), (3, 8, 0, 128, 160, 0, 0), (3, 8, 4, 128, 0, 0, 0),
+                (3, 8, 4, 128, 160, 0, 3)):
         assert lib.query("prismkv_paged_attend_work_bytes", *bad) == 0
     need = lib.query("prismkv_paged_evict_work_bytes", 3, 8, 160)
     assert need >= 24 * 160 * 4
