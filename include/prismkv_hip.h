@@ -428,10 +428,10 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  * slot below a length has no page (a row to append to it is dropped; attention
  * reads page 0 in its place; a move is left out), and at byte offset 8 the
  * optional host word's address, as in a workspace.  `paged_work` is scratch, of
- * the matching *_work_bytes for the call's own sizes; of prismkv_paged_attend's
- * the leading counters (sequences * kv_heads * ceil(group / 16) words) must be
- * zero before its first use and are left so, and calls sharing it must not
- * overlap. */
+ * the matching *_work_bytes for the call's own sizes; its
+ * leading counters (prismkv_paged_attend: sequences * kv_heads * ceil(group / 16)
+ * words, prismkv_paged_evict: sequences) must be zero before its first use and
+ * are left so; calls sharing it must not overlap. */
 
 /* Row i of sequence b's new rows (rows offsets[b] .. offsets[b + 1] of k and v
  * [rows][kv_heads][head_dim]; offsets i32 [sequences + 1] ascending from 0, or

@@ -194,7 +194,7 @@ struct PagedAppend {
   int64_t rows, k_row, k_head, v_row, v_head;  // bytes
   int64_t page_bytes, head_bytes, slot_bytes;
   PageDiv div;
-  int sequences, kv_heads, row_bytes, page_size, max_pages, pages, slots;
+  int sequences, kv_heads, log_pieces, page_size, max_pages, pages, slots;  // log_pieces: 16-byte pieces of a row
 };
 
 struct PagedEvict {
@@ -204,11 +204,11 @@ struct PagedEvict {
   int32_t *lengths_out, *seen_out, *positions_out;
   float* scores_out;
   int32_t *count, *src, *dst;  // workspace: moves per (sequence, KV head)
-  unsigned* err;
+  unsigned *counters, *tables, *err;
+  int64_t table_words;  // of a row
   int64_t page_bytes, head_bytes, slot_bytes, moves;
   PageDiv div;
-  int sequences, kv_heads, row_bytes, page_size, max_pages, pages, slots, keep, recent, sinks;
-  bool guard;  // some positions are protected
+  int sequences, kv_heads, log_pieces, page_size, max_pages, pages, slots, keep, recent, sinks, part, most_parts;
 };
 
 }  // namespace

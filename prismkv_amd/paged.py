@@ -15,6 +15,7 @@ sequence's length that has no page is reported at the next call
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -25,6 +26,12 @@ DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 HEAD_DIMS = (64, 128, 256)
 ERR_PAGES = 4
 _SCORED = ("seen", "scores", "positions")
+
+
+# The current stream's handle; building a torch.cuda.Stream for it takes 2.7 us of a
+# call's 13.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _check(cond, what):
@@ -137,7 +144,7 @@ class PagedCache:
                     raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")
                 err = torch.zeros(2, dtype=torch.int64, device=self.device)
                 err[1] = address
-            err = (err, host)
+            err = (err, host, ctypes.c_int32.from_address(host.data_ptr()))
         self._err = err
 
     # ------------------------------------------------------------ pages
@@ -209,8 +216,8 @@ class PagedCache:
         length without a page: the results since the last check are invalid.
         Reads a host-mapped word (no synchronisation, launches that have not
         run yet are not seen) and clears it."""
-        err, host = self._err
-        if int(host[0]):
+        err, host, word = self._err  # (word: host's first element, read without a tensor operation)
+        if word.value:
             with torch.cuda.device(self.device):
                 torch.cuda.synchronize()
                 err[:1].zero_()
@@ -220,19 +227,21 @@ class PagedCache:
                                "since the last check are invalid")
 
     def _call(self, name, *args):
-        if torch.cuda.current_device() == self.device.index:
-            self.lib.call(name, *args, stream=torch.cuda.current_stream().cuda_stream)
+        index = self.device.index
+        if torch.cuda.current_device() == index:
+            self.lib.call(name, *args, stream=_raw_stream(index))
         else:
-            with torch.cuda.device(self.device):
-                self.lib.call(name, *args, stream=torch.cuda.current_stream().cuda_stream)
+            with torch.cuda.device(index):
+                self.lib.call(name, *args, stream=_raw_stream(index))
 
     def _into(self, into):
         if into is None or into is self:
             return self
-        _check(isinstance(into, PagedCache) and into.k.data_ptr() == self.k.data_ptr() and
-               into.table.data_ptr() == self.table.data_ptr() and into._shape == self._shape and
-               into._cache_args == self._cache_args and into.scored == self.scored,
-               "into must be a fork of this cache")
+        if not (isinstance(into, PagedCache) and into.k.data_ptr() == self.k.data_ptr()
+                and into.v.data_ptr() == self.v.data_ptr() and into.table.data_ptr() == self.table.data_ptr()
+                and into._cache_args == self._cache_args and into._shape == self._shape
+                and (into.scores is None) == (self.scores is None)):
+            raise ValueError("into must be a fork of this cache")
         return into
 
     def _workspace(self, nbytes, zero):
@@ -254,25 +263,27 @@ class PagedCache:
         (`reserve`); a row without one is dropped and reported."""
         to = self if into is None else self._into(into)
         sequences, kv_heads, head_dim, _, _ = self._shape
-        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != kv_heads or k.shape[2] != head_dim:
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        if len(shape) != 3 or v.shape != shape or shape[1] != kv_heads or shape[2] != head_dim:
             raise ValueError(f"K and V rows [rows, {kv_heads}, {head_dim}] required")
-        if not (k.dtype == v.dtype == self.k.dtype and k.device == v.device == self.device):
+        dtype, device = self.k.dtype, self.device
+        if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
             raise ValueError("K and V rows of the cache's type on its device required")
-        rows, es = k.shape[0], k.element_size()
-        if rows and (k.stride(2) != 1 or v.stride(2) != 1):
+        rows, es = shape[0], k.element_size()
+        if rows and (ks[2] != 1 or vs[2] != 1):
             raise ValueError("contiguous head dimension required")
-        strides = (k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-        if (strides[0] * es | strides[1] * es | strides[2] * es | strides[3] * es | k.data_ptr() | v.data_ptr()) % 16:
+        kp, vp = k.data_ptr(), v.data_ptr()
+        if ((ks[0] | ks[1] | vs[0] | vs[1]) * es | kp | vp) % 16:
             raise ValueError("K/V rows must be 16-byte aligned")
         if offsets is not None:
             _i32(offsets, (sequences + 1,), self.device, "offsets")
         elif rows != sequences:
             raise ValueError("one row per sequence, or offsets, required")
         self.check_errors()
-        self._call("prismkv_paged_append", k.data_ptr(), v.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
-                   self.table.data_ptr(), 0 if offsets is None else offsets.data_ptr(), self.lengths.data_ptr(),
-                   to.lengths.data_ptr(), *self._scored_pointers(to), self._err[0].data_ptr(), rows, *strides,
-                   sequences, *self._cache_args, self._dtype)
+        self._call("prismkv_paged_append", kp, vp, self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
+                   0 if offsets is None else offsets.data_ptr(), self.lengths.data_ptr(), to.lengths.data_ptr(),
+                   *self._scored_pointers(to), self._err[0].data_ptr(), rows, ks[0], ks[1], vs[0], vs[1], sequences,
+                   *self._cache_args, self._dtype)
 
     def _scored_pointers(self, to):
         if not self.scored:
@@ -293,14 +304,15 @@ class PagedCache:
     def _check_q(self, q, scale, accumulate, lse):
         """The query heads per KV head, and the scale."""
         sequences, kv_heads, head_dim, _, _ = self._shape
-        if (q.dim() != 3 or q.shape[0] != sequences or q.shape[2] != head_dim or q.shape[1] < 1 or q.shape[1] % kv_heads
+        shape = q.shape
+        if (len(shape) != 3 or shape[0] != sequences or shape[2] != head_dim or shape[1] < 1 or shape[1] % kv_heads
                 or not q.is_contiguous()):
             raise ValueError(f"contiguous Q[{sequences}, a multiple of {kv_heads} heads, {head_dim}] required")
         if q.dtype != self.k.dtype or q.device != self.device:
             raise ValueError("Q of the cache's type on its device required")
         if q.data_ptr() % 16:
             raise ValueError("Q rows must be 16-byte aligned")
-        group = q.shape[1] // kv_heads
+        group = shape[1] // kv_heads
         if group > 1024:
             raise NotImplementedError("at most 1024 query heads per KV head")
         if accumulate and self.scores is None:
@@ -364,7 +376,7 @@ class PagedCache:
         self.check_errors()
         if self._evict_work is None:
             self._evict_work = self._workspace(
-                self.lib.query("prismkv_paged_evict_work_bytes", sequences, kv_heads, self.slots), 0)
+                self.lib.query("prismkv_paged_evict_work_bytes", sequences, kv_heads, self.slots), 4 * sequences)
         self._call("prismkv_paged_evict", self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
                    self.lengths.data_ptr(), to.lengths.data_ptr(), *self._scored_pointers(to), keeps,
                    self._evict_work.data_ptr(), self._err[0].data_ptr(), keep, recent, sinks, sequences,

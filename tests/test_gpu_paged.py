@@ -326,11 +326,47 @@ def test_evict_scores(values):
     check_evict(host, [n, n - 1], [keep, keep], cache, cache, 20, 0)
 
 
-@pytest.mark.parametrize("n,keep", [(70001, 30000), (70001, 69990), (70001, 5)])
-def test_evict_long(n, keep):
-    cache, host = make([n], 1, 64, 256, FP16, scored=True)
-    cache.evict(keep, recent=3, sinks=2)
-    check_evict(host, [n], [keep], cache, cache, 3, 2)
+@pytest.mark.parametrize("lengths,keep,ties", [([70001], 30000, False), ([70001], 69990, False), ([70001], 5, True),
+                                               ([16385, 9000, 0, 20000], 9000, True), ([40000, 300], 16384, True),
+                                               ([16384, 16383], 8191, True), ([24576], 8192, False),
+                                               ([20000] + [50] * 40, 700, False)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_evict_long(lengths, keep, ties, apart):
+    """Rows of several parts, and of one at its largest, with and without ties over their ends."""
+    cache, host = make(lengths, 2, 64, 256, FP16, scored=True)
+    if ties:
+        host["scores"].mul_(16).floor_()
+        cache.scores.copy_(host["scores"])
+    into = cache.fork() if apart else cache
+    cache.evict(keep, recent=3, sinks=2, into=into)
+    check_evict(host, lengths, [keep] * len(lengths), cache, into, 3, 2)
+
+
+def test_evict_longest():
+    """Parts of more than one pass over their workgroup's registers (past 2^20
+    slots), the result checked by torch's stable sort."""
+    n, keep, page = 1300003, 600000, 4096
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    pages = -(-n // page)
+    k = torch.randn(pages, 1, page, 64, generator=gen, device="cuda").half()
+    scores = torch.randint(0, 100000, (1, 1, pages * page), generator=gen, device="cuda").float()
+    positions = torch.arange(pages * page, device="cuda").int().view(1, 1, -1).contiguous()
+    table = torch.randperm(pages, generator=gen, device="cuda").int()[None]
+    i32 = lambda x: torch.tensor([x], dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = PagedCache.from_tensors(k, k.clone(), table, i32(n), seen=i32(n), scores=scores, positions=positions)
+    before, flat = scores.clone(), k[table[0].long()].view(-1, 64).clone()
+    cache.evict(keep, recent=10)
+    rank = before[0, 0, :n].clone()
+    rank[-10:] = math.inf
+    kept = torch.zeros(n, dtype=torch.bool, device="cuda")
+    kept[torch.sort(rank, descending=True, stable=True).indices[:keep]] = True
+    slot = torch.arange(keep, device="cuda")
+    slot[~kept[:keep]] = kept[keep:].nonzero()[:, 0] + keep
+    assert int(cache.lengths) == keep
+    assert torch.equal(cache.positions[0, 0, :keep], slot.int())
+    assert torch.equal(cache.scores[0, 0, :keep], before[0, 0, slot])
+    for x in (cache.k, cache.v):
+        assert torch.equal(bits(x[table[0].long()].view(-1, 64)[:keep]), bits(flat[slot]))
 
 
 def test_run_of_operators():

@@ -62,7 +62,7 @@ def test_refused_pointers(lib):  # noqa: F811
     for i in range(14):
         if i != 11:
             assert evict(lib, _without(good, i)) == -1, i
-    assert evict(lib, _without(good, 12, 18)) == -1 and evict(lib, _without(good, 13, 20)) == -1
+    assert evict(lib, _without(good, 12, 24)) == -1 and evict(lib, _without(good, 13, 20)) == -1
 
 
 def test_refused_arguments(lib):  # noqa: F811
