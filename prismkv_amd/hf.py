@@ -19,6 +19,17 @@ KV heads x 4 query heads, head_dim 128, bf16 activations, 16 selected buckets
 `Native8B.unique_cap`; mode "all_read" (the dense control) runs the model's
 own attention over the whole cache.
 
+Mode "evict" (no reference counterpart) is the other control of the routed
+decode's cost: per layer a `PagedCache` of at most `cache_budget` slots and the
+`evict_every` latest tokens.  The prompt's keys and values are weighed by its
+last `observe` queries and cut to the budget; every decode step then appends
+its token, attends to what is held and adds the step's weights to the scores,
+and a cache that has grown by `evict_every` tokens is cut again: the
+`cache_recent` newest and `cache_sinks` first tokens stay, then the highest
+scores.  Any number of KV and query heads with head_dim 64, 128 or 256;
+encoders are not used.  (The model's own cache object still grows; it is not
+read.)
+
 Records keep the reference's per-(layer, group) fields, including the
 `detailed_records` ones (old_unique, old_raw, generated_indexed_unique,
 generated_indexed_raw, initial_history, hf_reference.py:216-231); they are
@@ -43,6 +54,7 @@ from dataclasses import dataclass
 import torch
 
 from .native8b import DIM, FEATURES, GROUPS, HEADS, MAX_BLOCK, Native8B
+from .paged import DTYPES, HEAD_DIMS, PagedCache
 from .weights import Encoder, layer_tables  # noqa: F401  (Encoder re-exported: reference name)
 
 BACKEND = "prismkv_native"
@@ -184,14 +196,17 @@ class _Records:
         self.pending.append(entry)
 
     def dense(self, layer, prefix, total):
-        n = torch.full((GROUPS,), prefix)
+        self.bounded(layer, prefix, total, prefix, GROUPS)
+
+    def bounded(self, layer, prefix, total, held, groups):
+        n = torch.full((groups,), held)
         self.pending.append(dict(layer=layer, history=prefix, total=total, prefix=prefix, unique=n, raw=n,
-                                 buckets=torch.zeros(GROUPS, dtype=torch.long), old_unique=n, old_raw=n))
+                                 buckets=torch.zeros(groups, dtype=torch.long), old_unique=n, old_raw=n))
 
     def read(self):
         for e in self.pending:
             cols = {key: e[key].tolist() for key in ("unique", "raw", "buckets", "old_unique", "old_raw") if key in e}
-            for g in range(GROUPS):
+            for g in range(len(cols["unique"])):
                 rec = dict(layer=e["layer"], group=g, history=e["history"], unique=cols["unique"][g],
                            raw=cols["raw"][g], buckets=cols["buckets"][g], tail=e["total"] - e["history"],
                            routing_policy=self.mode)
@@ -205,16 +220,75 @@ class _Records:
         return self.done
 
 
+PAGE = 64  # slots of a page of mode "evict"
+
+
+class _BoundedLayer:
+    """One layer's cache of mode "evict": the held keys and values of its
+    prefix, built at its first decode step, and how many a sequence holds (the
+    host knows: every step adds one, a cut leaves the budget)."""
+
+    def __init__(self, session, K, V, prefix, observed):
+        kv_heads, head_dim = K.shape[0], K.shape[2]
+        self.session, self.held, self.total = session, prefix, prefix
+        most = max(min(prefix, session.cache_budget), 1) + session.evict_every + 1
+        pages = -(-max(prefix, most) // PAGE)
+        cache = PagedCache(1, pages, pages, page_size=PAGE, kv_heads=kv_heads, head_dim=head_dim, dtype=K.dtype,
+                           scored=True, device=K.device, library=session.library)
+        cache.reserve(prefix)
+        ends = torch.tensor([0, prefix], dtype=torch.int32, device=K.device)
+        cache.append(K[:, :prefix].transpose(0, 1), V[:, :prefix].transpose(0, 1), ends)
+        if observed is not None and prefix > session.cache_budget:
+            # the prompt's last queries, each over the tokens up to its own
+            queries = observed.transpose(0, 1).contiguous()
+            for i in range(len(queries)):
+                cache.lengths.fill_(prefix - len(queries) + 1 + i)
+                cache.attend(queries[i:i + 1], accumulate=True)
+        self.cache = cache
+        if prefix > session.cache_budget:
+            self._cut()
+        self.bound = -(-(session.cache_budget + session.evict_every) // PAGE)
+        if pages > self.bound:
+            cache.release(0, self.held)
+            self.cache = cache.resized(self.bound, self.bound)
+
+    def check_errors(self):
+        self.cache.check_errors()
+
+    def _cut(self):
+        s = self.session
+        self.cache.evict(s.cache_budget, recent=s.cache_recent, sinks=s.cache_sinks)
+        self.held = s.cache_budget
+
+    def step(self, q, k, v):
+        """Appends the token's k and v [kv_heads, head_dim] and attends with q [1, heads, head_dim]."""
+        if self.held >= self.session.cache_budget + self.session.evict_every:
+            self._cut()
+        needed = -(-(self.held + 1) // PAGE)
+        if needed > self.cache.table.shape[1]:  # (after a prompt shorter than the budget)
+            pages = min(2 * needed, self.bound)
+            self.cache = self.cache.resized(pages, pages)
+        self.cache.reserve(self.held + 1)
+        out = self.cache(q, k[None], v[None], accumulate=True)
+        self.held += 1
+        return out
+
+
 class HFNative:
     """Stateful all-group adapter; one session per model, one request at a
     time.  `capacity_step` is the token granularity by which a layer's index
-    capacity grows as the request gets longer."""
+    capacity grows as the request gets longer; the `cache_*` arguments,
+    `evict_every` and `observe` are mode "evict"'s."""
 
     def __init__(self, model, encoders, *, mode="sparse", router="moments", selected_buckets=16, unique_cap=None,
-                 update_interval=4096, detailed_records=False, capacity_step=8192, library=None):
+                 update_interval=4096, detailed_records=False, capacity_step=8192, library=None,
+                 cache_budget=4096, cache_recent=512, cache_sinks=4, evict_every=64, observe=32):
         # the reference's policy checks (hf_reference.py:77-84), then the native limits
-        if mode not in ("sparse", "all_read"):
-            raise ValueError("mode must be sparse or all_read")
+        if mode not in ("sparse", "all_read", "evict"):
+            raise ValueError("mode must be sparse, all_read or evict")
+        if mode == "evict" and (cache_budget < 1 or evict_every < 1 or min(cache_recent, cache_sinks, observe) < 0
+                                or cache_recent + cache_sinks > cache_budget):
+            raise ValueError("a positive cache budget that holds the recent and first tokens required")
         if router not in ("moments", "q_activation") or selected_buckets <= 0:
             raise ValueError("unsupported router/bucket count")
         if unique_cap is not None and not 0 <= unique_cap <= 1:
@@ -227,13 +301,17 @@ class HFNative:
             raise NotImplementedError(f"the native update indexes blocks of at most {MAX_BLOCK} keys")
         hooked = _find_attention(model)
         wanted = {(layer, g) for layer, h in hooked.items() for g in range(h.config.num_key_value_heads)}
-        if not hooked or set(encoders) != wanted:
+        if mode == "evict" and not encoders and hooked:
+            encoders = {}  # not used
+        elif not hooked or set(encoders) != wanted:
             raise ValueError(f"provide exactly all standard-attention KV encoders; missing={wanted - set(encoders)}, "
                              f"extra={set(encoders) - wanted}")
         self.model, self.encoders = model, encoders
         self.mode, self.router = mode, router
         self.selected_buckets, self.unique_cap = selected_buckets, unique_cap
         self.update_interval, self.force_prefill = update_interval, False
+        self.cache_budget, self.cache_recent, self.cache_sinks = int(cache_budget), int(cache_recent), int(cache_sinks)
+        self.evict_every, self.observe = int(evict_every), int(observe)
         self.detailed_records = detailed_records
         self.capacity_step, self.library = int(capacity_step), library
         self._hooked = hooked
@@ -253,6 +331,7 @@ class HFNative:
         if getattr(self, "_static", None) is not None:  # the finished request's steps join its records
             self._static.flush_records()
         self.prefix_lengths, self.ops = {}, {}
+        self._observed = {}  # layer -> the last queries of its prompt [heads, up to `observe`, head_dim] (mode "evict")
         self._log = _Records(self.mode, self.detailed_records)
 
     @contextmanager
@@ -271,6 +350,7 @@ class HFNative:
                 del h.module._prismkv_session
             h.config._attn_implementation = h.implementation
         self.ops.clear()
+        self._observed.clear()
 
     def generate(self, *args, **kwargs):
         """Reset for a new model.generate call/cache."""
@@ -339,11 +419,19 @@ class HFNative:
             # a new prefix: forget the layer's index, run the model's attention
             self.prefix_lengths[layer] = total
             self.ops.pop(layer, None)
+            if self.mode == "evict" and self.observe:
+                before = self._observed.get(layer) if total > steps else None
+                last = q[0, :, -self.observe:]
+                if before is not None and steps < self.observe:
+                    last = torch.cat((before, last), dim=1)[:, -self.observe:]
+                self._observed[layer] = last.clone()
             if attention_mask is None and 1 < steps < total:
                 # a cached chunk: query i sits at position total - steps + i
                 blocked = torch.ones(steps, total, dtype=torch.bool, device=q.device).triu_(total - steps + 1)
                 attention_mask = _additive_mask(blocked, q.dtype)
             return self.original[layer](module, q, k, v, attention_mask, **kwargs)
+        if self.mode == "evict":
+            return self._forward_bounded(layer, q, k[0], v[0], total)
         _, queries = _native_geometry(q, k)
         prefix = self.prefix_lengths[layer]
         if self.mode == "all_read":
@@ -357,6 +445,25 @@ class HFNative:
         out = op(q[0, :, 0].reshape(GROUPS, HEADS, DIM).contiguous(), K, V)
         self._log.sparse(layer, op, total, prefix)
         return out.reshape(1, 1, queries, q.shape[-1]), None
+
+    def _forward_bounded(self, layer, q, K, V, total):
+        """A decode step of mode "evict"."""
+        if q.shape[1] % K.shape[0]:
+            raise ValueError("Q heads must form equal-sized KV groups")
+        if q.shape[-1] not in HEAD_DIMS or q.dtype not in DTYPES or q.device.type != "cuda":
+            raise NotImplementedError("the paged cache holds bf16, fp16 or fp32 rows of head_dim 64, 128 or 256 on the "
+                                      "device")
+        if K.stride(-1) != 1 or V.stride(-1) != 1:
+            K, V = K.contiguous(), V.contiguous()
+        prefix, op = self.prefix_lengths[layer], self.ops.get(layer)
+        if total != (prefix if op is None else op.total) + 1:
+            raise RuntimeError("decode steps follow the prompt and each other one by one")
+        if op is None:
+            op = self.ops[layer] = _BoundedLayer(self, K, V, prefix, self._observed.pop(layer, None))
+        op.total = total
+        out = op.step(q[:, :, 0].contiguous(), K[:, -1], V[:, -1])
+        self._log.bounded(layer, prefix, total, op.held, K.shape[0])
+        return out.reshape(1, 1, q.shape[1], q.shape[-1]), None
 
     def _forward_static(self, module, q, k, v, attention_mask, **kwargs):
         """forward() over a StaticCache: K/V are the whole preallocated buffers

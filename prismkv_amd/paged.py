@@ -197,6 +197,30 @@ class PagedCache:
             del held[keep:]
             self._write_table()
 
+    def resized(self, pages, max_pages):
+        """A new cache of `pages` pages, at most `max_pages` to a sequence, with
+        this one's contents: per sequence its first max_pages pages, which the
+        caller knows to hold its length, their scores and positions.  (A cut
+        cache in the table of its longest prompt would keep that prompt's memory,
+        and its cuts the cost of that many slots.)"""
+        self._owns_pages()
+        sequences, kv_heads, head_dim, page_size, _ = self._shape
+        counts = [min(len(held), int(max_pages)) for held in self._pages]
+        _check(sum(counts) <= int(pages), "the sequences' pages do not fit")
+        new = PagedCache(sequences, pages, max_pages, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim,
+                         dtype=self.k.dtype, scored=self.scored, device=self.device, library=self.lib.path)
+        new.reserve([count * page_size for count in counts])
+        for held, own, count in zip(self._pages, new._pages, counts):
+            new.k[own] = self.k[held[:count]]
+            new.v[own] = self.v[held[:count]]
+        new.lengths.copy_(self.lengths)
+        if self.scored:
+            slots = min(new.slots, self.slots)
+            new.seen.copy_(self.seen)
+            new.scores[:, :, :slots] = self.scores[:, :, :slots]
+            new.positions[:, :, :slots] = self.positions[:, :, :slots]
+        return new
+
     def _owns_pages(self):
         if self._pages is None:
             raise RuntimeError("the page table of this cache is kept by the caller (or the cache it was forked from)")

@@ -137,3 +137,38 @@ def test_definition_of_evict():
         assert len(stay) == m
         if not any(positions[t] >= 35 or positions[t] < 2 for t in range(n)) and left and stay:
             assert min(scores[t] for t in stay) >= max(scores[t] for t in left)
+
+
+def test_evict_session_on_host():
+    """Mode "evict" without encoders: its checks, and the prefill through the model's own attention."""
+    from prismkv_amd.hf import DecodeGraph, HFNative
+    from tests.test_hf_host import encoders, tiny_qwen3
+    model = tiny_qwen3()
+    for bad in (dict(cache_budget=0), dict(evict_every=0), dict(cache_recent=-1), dict(observe=-1),
+                dict(cache_budget=10, cache_recent=8, cache_sinks=3)):
+        with pytest.raises(ValueError, match="cache budget"):
+            HFNative(model, {}, mode="evict", **bad)
+    with pytest.raises(ValueError, match="sparse, all_read or evict"):
+        HFNative(model, encoders(1), mode="dense")
+    with pytest.raises(ValueError, match="missing"):
+        HFNative(model, {}, mode="all_read")
+    ids = torch.randint(0, 128, (1, 12))
+    with torch.no_grad():
+        dense = model(ids).logits
+    session = HFNative(model, {}, mode="evict", observe=5)
+    with pytest.raises(NotImplementedError, match="sparse mode"):
+        DecodeGraph(session, None)
+    with torch.no_grad():
+        assert torch.equal(model(ids).logits, dense)
+    assert session._observed[0].shape == (32, 5, 128)
+    # chunks: the last queries of the whole prompt
+    from transformers import DynamicCache
+    whole = session._observed[0]
+    cache = DynamicCache(config=model.config)
+    session.begin_request()
+    with torch.no_grad(), session.prefill():
+        for lo, hi in ((0, 8), (8, 11), (11, 12)):
+            model(ids[:, lo:hi], past_key_values=cache, use_cache=True)
+    assert torch.allclose(session._observed[0], whole, atol=1e-5)
+    session.close()
+    assert model.config._attn_implementation == "sdpa" and not session._observed
