@@ -409,11 +409,12 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
 /* ---- the paged cache ------------------------------------------------------
  * No reference counterpart: keys and values of several sequences in pages,
  * dense attention of one new token of each, and a bounded cache that evicts by
- * accumulated attention weight.
- *   k_pages, v_pages  [pages][kv_heads][page_size][head_dim] of one type
- *            (`dtype` 0 bf16, 1 fp16, 2 fp32; -2 for another), head_dim 64, 128
- *            or 256, the same strides (in elements, 16-byte multiples, rows
- *            contiguous) for both, all rows within 2^36 bytes of the base;
+ * accumulated attention weight.  A cache is described by a host structure, read
+ * during the call only (device pointers as elsewhere; strides in elements):
+ *   k, v     [pages][kv_heads][page_size][head_dim] of one type (`dtype` 0 bf16,
+ *            1 fp16, 2 fp32; -2 for another), head_dim 64, 128 or 256, the same
+ *            strides for both, of 16-byte multiples with contiguous rows, all
+ *            rows of a head within 2^36 bytes;
  *   table    i32 [sequences][max_pages]: the page of slots [i page_size,
  *            (i + 1) page_size) of a sequence; an entry outside [0, pages) is no
  *            page.  slots = max_pages * page_size <= 2^30, sequences * slots <
@@ -421,45 +422,47 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *   lengths  i32 [sequences], read as clamped to [0, slots];
  *   seen     i32 [sequences]: tokens appended so far;
  *   scores   f32, positions i32 [sequences][kv_heads][slots]: each slot's
- *            accumulated weight and the number of its token.
- * Where `x_out` accompanies `x`, results go to x_out, which may be x itself or
- * not overlap it.  A page that belongs to several tables may be read, not
- * written.  `err` is 16 bytes, 8-byte aligned: the error word, set to 4 when a
- * slot below a length has no page (a row to append to it is dropped; attention
- * reads page 0 in its place; a move is left out), and at byte offset 8 the
- * optional host word's address, as in a workspace.  `paged_work` is scratch, of
- * the matching *_work_bytes for the call's own sizes; its
- * leading counters (prismkv_paged_attend: sequences * kv_heads * ceil(group / 16)
- * words, prismkv_paged_evict: sequences) must be zero before its first use and
- * are left so; calls sharing it must not overlap. */
+ *            accumulated weight and the number of its token (these three are 0
+ *            where nothing is scored);
+ *   err      16 bytes, 8-byte aligned: the error word, set to 4 when a slot
+ *            below a length has no page (a row to append to it is dropped;
+ *            attention reads page 0 in its place; a move is left out), and at
+ *            byte offset 8 the optional host word's address, as in a workspace.
+ * Results go to a second cache `into` over the same pages and table: the first
+ * itself, or one whose lengths, seen, scores and positions do not overlap the
+ * first's.  A page that belongs to several tables may be read, not written.
+ * `paged_work` is scratch, 16-byte aligned, of the matching *_work_bytes for the
+ * call's own sizes; its leading counters (prismkv_paged_attend: sequences *
+ * kv_heads * ceil(group / 16) words, prismkv_paged_evict: sequences) must be zero
+ * before its first use and are left so; calls sharing it must not overlap. */
+typedef struct prismkv_paged_cache {
+  uint64_t k, v, table, lengths, seen, scores, positions, err;
+  int64_t pages, page_stride, head_stride, slot_stride;
+  int32_t sequences, kv_heads, head_dim, page_size, max_pages, dtype;
+} prismkv_paged_cache;
 
 /* Row i of sequence b's new rows (rows offsets[b] .. offsets[b + 1] of k and v
  * [rows][kv_heads][head_dim]; offsets i32 [sequences + 1] ascending from 0, or
- * 0: one row each) goes to slot lengths[b] + i; lengths_out[b] = lengths[b] +
- * their number, and, where positions is not 0, the slot's score becomes 0 and
- * its position seen[b] + i in both score and position arrays, and seen_out[b] =
- * seen[b] + their number.  Strides of k and v rows and heads in elements,
- * 16-byte multiples. */
-int prismkv_paged_append(uint64_t k, uint64_t v, uint64_t k_pages, uint64_t v_pages, uint64_t table, uint64_t offsets,
-                         uint64_t lengths, uint64_t lengths_out, uint64_t seen, uint64_t seen_out, uint64_t scores,
-                         uint64_t scores_out, uint64_t positions, uint64_t positions_out, uint64_t err, int64_t rows,
-                         int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
-                         int sequences, int kv_heads, int head_dim, int page_size, int max_pages, int64_t pages,
-                         int64_t page_stride, int64_t head_stride, int64_t slot_stride, int dtype, uint64_t stream);
+ * 0: one row each) goes to slot lengths[b] + i; into's lengths[b] = lengths[b] +
+ * their number, and of a scored cache the slot's score becomes 0 and its position
+ * seen[b] + i in both caches, and into's seen[b] = seen[b] + their number.
+ * Strides of k and v rows and heads in elements, 16-byte multiples. */
+int prismkv_paged_append(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t k, uint64_t v,
+                         uint64_t offsets, int64_t rows, int64_t k_row_stride, int64_t k_head_stride,
+                         int64_t v_row_stride, int64_t v_head_stride, uint64_t stream);
 
 /* q [sequences][kv_heads * group][head_dim] -> out of the same shape and type:
  * softmax(scale q.k) v over each sequence's slots [0, lengths[b]), 0 where there
  * is none; lse f32 [sequences][kv_heads * group] (or 0) <- the natural logarithm
  * of the softmax's sum, -infinity for an empty one.  Scores, sums and products
- * are accumulated in fp32.  With scores (not 0): scores_out[t] = scores[t] +
- * slot t's weights summed over the group's heads, for t < lengths[b]. */
+ * are accumulated in fp32.  flags & 1: into's scores[t] = scores[t] + slot t's
+ * weights summed over the group's heads, for t < lengths[b].  flags & 2: the
+ * lengths are into's (an append that went there is attended to). */
 size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh,
                                        int dtype);
-int prismkv_paged_attend(uint64_t q, uint64_t k, uint64_t v, uint64_t table, uint64_t lengths, uint64_t scores,
-                         uint64_t scores_out, uint64_t lse, uint64_t paged_work, uint64_t err, uint64_t out, int sequences,
-                         int kv_heads, int group, int head_dim, int page_size, int max_pages, int64_t pages,
-                         int64_t page_stride, int64_t head_stride, int64_t slot_stride, double scale, int dtype,
-                         size_t work_bytes, uint64_t stream);
+int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t q, uint64_t lse,
+                         uint64_t paged_work, uint64_t out, int group, int flags, double scale, size_t work_bytes,
+                         uint64_t stream);
 
 /* Cuts every sequence to min(lengths[b], keep) slots (keeps i32 [sequences] in
  * place of `keep`, which is 0 then), per KV head: the slots that stay are the
@@ -468,12 +471,8 @@ int prismkv_paged_attend(uint64_t q, uint64_t k, uint64_t v, uint64_t table, uin
  * ascending.  The i-th staying slot at or behind the new length moves, with its
  * K and V rows, score and position, into the i-th leaving slot before it. */
 size_t prismkv_paged_evict_work_bytes(int sequences, int kv_heads, int64_t slots);
-int prismkv_paged_evict(uint64_t k_pages, uint64_t v_pages, uint64_t table, uint64_t lengths, uint64_t lengths_out,
-                        uint64_t seen, uint64_t seen_out, uint64_t scores, uint64_t scores_out, uint64_t positions,
-                        uint64_t positions_out, uint64_t keeps, uint64_t paged_work, uint64_t err, int keep, int recent,
-                        int sinks, int sequences, int kv_heads, int head_dim, int page_size, int max_pages, int64_t pages,
-                        int64_t page_stride, int64_t head_stride, int64_t slot_stride, int dtype, size_t work_bytes,
-                        uint64_t stream);
+int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t keeps,
+                        uint64_t paged_work, int keep, int recent, int sinks, size_t work_bytes, uint64_t stream);
 
 #ifdef __cplusplus
 }

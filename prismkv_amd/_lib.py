@@ -13,7 +13,7 @@ from pathlib import Path
 DEFAULT_LIBRARY = Path(__file__).resolve().with_name("libprismkv_hip.so")
 
 _U64, _I32, _I64, _SZ = ctypes.c_uint64, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
-_F64 = ctypes.c_double
+_F64, _PTR = ctypes.c_double, ctypes.c_void_p
 
 # name -> (argument types without the trailing stream, has_stream, restype)
 SIGNATURES = {
@@ -67,11 +67,11 @@ SIGNATURES = {
     "prismkv_union_n": ([_U64] * 6 + [_I32, _I32, _I64, _I64, _I32, _SZ], True, _I32),
     "prismkv_select_cap_n": ([_U64] * 5 + [_I32, _I32, _I64, _I64, _I32], True, _I32),
     # the paged cache
-    "prismkv_paged_append": ([_U64] * 15 + [_I64] * 5 + [_I32] * 5 + [_I64] * 4 + [_I32], True, _I32),
+    "prismkv_paged_append": ([_PTR] * 2 + [_U64] * 3 + [_I64] * 5, True, _I32),
     "prismkv_paged_attend_work_bytes": ([_I32] * 4 + [_I64, _I32, _I32], False, _SZ),
-    "prismkv_paged_attend": ([_U64] * 11 + [_I32] * 6 + [_I64] * 4 + [_F64, _I32, _SZ], True, _I32),
+    "prismkv_paged_attend": ([_PTR] * 2 + [_U64] * 4 + [_I32, _I32, _F64, _SZ], True, _I32),
     "prismkv_paged_evict_work_bytes": ([_I32, _I32, _I64], False, _SZ),
-    "prismkv_paged_evict": ([_U64] * 14 + [_I32] * 8 + [_I64] * 4 + [_I32, _SZ], True, _I32),
+    "prismkv_paged_evict": ([_PTR] * 2 + [_U64] * 2 + [_I32] * 3 + [_SZ], True, _I32),
     # error handling of the bounded inter-workgroup waits
     "prismkv_set_spin_limit": ([_I32], False, _I32),
     "prismkv_get_spin_limit": ([], False, _I32),
@@ -80,6 +80,13 @@ SIGNATURES = {
     "prismkv_scratch_bytes": ([], False, _SZ),
     "prismkv_decode_noalloc": ([_U64] * 13 + [_I32] * 4 + [_I64] * 4, True, _I32),
 }
+
+class PagedCacheDesc(ctypes.Structure):
+    """prismkv_paged_cache of include/prismkv_hip.h."""
+    _fields_ = [(name, _U64) for name in ("k", "v", "table", "lengths", "seen", "scores", "positions", "err")] + \
+               [(name, _I64) for name in ("pages", "page_stride", "head_stride", "slot_stride")] + \
+               [(name, _I32) for name in ("sequences", "kv_heads", "head_dim", "page_size", "max_pages", "dtype")]
+
 
 _loaded: dict[str, "Library"] = {}
 

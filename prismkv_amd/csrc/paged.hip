@@ -9,6 +9,8 @@
 // through.
 #include "paged.h"
 
+#include "prismkv_hip.h"
+
 namespace prismkv {
 namespace {
 
@@ -1292,25 +1294,38 @@ PageDiv page_div(int page_size) {
 
 int element_bytes(int dtype) { return dtype == kFp32 ? 4 : 2; }
 
-// Sizes that every entry point takes, checked alike.  Strides are in elements;
-// rows, heads and pages lie at 16-byte multiples, and a page's last row within
-// 2^32 16-byte units.
-bool bad_cache(int sequences, int kv_heads, int head_dim, int page_size, int max_pages, int64_t pages, int64_t page_stride,
-               int64_t head_stride, int64_t slot_stride, int dtype) {
-  if (sequences < 1 || sequences > 65535 || kv_heads < 1 || kv_heads > 65535 || page_size < 1 || max_pages < 1 ||
-      pages < 1 || pages > INT32_MAX)
-    return true;
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return true;
-  const int64_t slots = (int64_t)page_size * max_pages;
-  if (slots > (1 << 30) || slots * sequences > INT32_MAX) return true;
-  const int64_t es = element_bytes(dtype);
-  if (page_stride < 0 || head_stride < 0 || slot_stride < head_dim) return true;
-  if ((page_stride * es | head_stride * es | slot_stride * es) & 15) return true;
-  const int64_t limit = 1ll << 36;  // bytes
-  if (page_stride > limit || head_stride > limit || slot_stride > limit) return true;
-  if (page_stride * es > limit / pages || slot_stride * es > limit / page_size) return true;
-  if ((pages - 1) * page_stride * es + (page_size - 1) * slot_stride * es >= limit) return true;
-  return false;
+// The cache and where its results go, checked alike by every entry point: rows,
+// heads and pages lie at 16-byte multiples, and a page's last row within 2^32
+// 16-byte units.  0, or the code to return.
+int check_cache(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, bool scored) {
+  if (!cache || !into) return kBadSize;
+  const prismkv_paged_cache& c = *cache;
+  const prismkv_paged_cache& to = *into;
+  if (c.dtype < kBf16 || c.dtype > kFp32) return kBadMode;
+  if (c.sequences < 1 || c.sequences > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.page_size < 1 ||
+      c.max_pages < 1 || c.pages < 1 || c.pages > INT32_MAX)
+    return kBadSize;
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return kBadSize;
+  const int64_t slots = (int64_t)c.page_size * c.max_pages;
+  if (slots > (1 << 30) || slots * c.sequences > INT32_MAX) return kBadSize;
+  const int64_t es = element_bytes(c.dtype), limit = 1ll << 36;  // bytes
+  if (c.page_stride < 0 || c.head_stride < 0 || c.slot_stride < c.head_dim) return kBadSize;
+  if (c.page_stride > limit || c.head_stride > limit || c.slot_stride > limit) return kBadSize;
+  if ((c.page_stride * es | c.head_stride * es | c.slot_stride * es) & 15) return kBadSize;
+  if (c.page_stride * es > limit / c.pages || c.slot_stride * es > limit / c.page_size) return kBadSize;
+  if ((c.pages - 1) * c.page_stride * es + (c.page_size - 1) * c.slot_stride * es >= limit) return kBadSize;
+  if (to.k != c.k || to.v != c.v || to.table != c.table || to.pages != c.pages || to.page_stride != c.page_stride ||
+      to.head_stride != c.head_stride || to.slot_stride != c.slot_stride || to.sequences != c.sequences ||
+      to.kv_heads != c.kv_heads || to.head_dim != c.head_dim || to.page_size != c.page_size ||
+      to.max_pages != c.max_pages || to.dtype != c.dtype)
+    return kBadSize;
+  if (!c.k || !c.v || !c.table || !c.lengths || !to.lengths || !c.err) return kBadSize;
+  if ((c.k | c.v) & 15 || c.err & 7 ||
+      (c.table | c.lengths | c.seen | c.scores | c.positions | to.lengths | to.seen | to.scores | to.positions) & 3)
+    return kBadSize;
+  const bool some = c.seen || c.scores || c.positions || to.seen || to.scores || to.positions;
+  const bool all = c.seen && c.scores && c.positions && to.seen && to.scores && to.positions;
+  return some != all || (scored && !all) ? kBadSize : 0;
 }
 
 struct WorkLayout {
@@ -1409,127 +1424,118 @@ size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, i
   return attend_layout(sequences, kv_heads, group, head_dim, slots, weigh != 0, dtype).bytes;
 }
 
-int prismkv_paged_attend(uint64_t q, uint64_t k, uint64_t v, uint64_t table, uint64_t lengths, uint64_t scores,
-                         uint64_t scores_out, uint64_t lse, uint64_t paged_work, uint64_t err, uint64_t out, int sequences,
-                         int kv_heads, int group, int head_dim, int page_size, int max_pages, int64_t pages,
-                         int64_t page_stride, int64_t head_stride, int64_t slot_stride, double scale, int dtype,
-                         size_t work_bytes, uint64_t stream) {
-  if (dtype < kBf16 || dtype > kFp32) return kBadMode;
-  if (bad_cache(sequences, kv_heads, head_dim, page_size, max_pages, pages, page_stride, head_stride, slot_stride, dtype))
-    return kBadSize;
-  if (group < 1 || group > 1024 || !(scale == scale)) return kBadSize;
-  if (!q || !k || !v || !table || !lengths || !paged_work || !err || !out || !scores != !scores_out) return kBadSize;
-  if ((q | k | v | paged_work) & 15 || (table | lengths | scores | scores_out | lse) & 3 || err & 7) return kBadSize;
-  const int64_t slots = (int64_t)page_size * max_pages;
-  const WorkLayout w = attend_layout(sequences, kv_heads, group, head_dim, slots, scores != 0, dtype);
+int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t q, uint64_t lse,
+                         uint64_t paged_work, uint64_t out, int group, int flags, double scale, size_t work_bytes,
+                         uint64_t stream) {
+  const bool weigh = flags & 1;
+  if (const int rc = check_cache(cache, into, weigh)) return rc;
+  if (flags & ~3) return kBadMode;
+  const prismkv_paged_cache& c = *cache;
+  if (group < 1 || group > 1024 || !(scale - scale == 0)) return kBadSize;
+  if (!q || !paged_work || !out || (q | paged_work) & 15 || lse & 3 || out & 3) return kBadSize;
+  const int64_t slots = (int64_t)c.page_size * c.max_pages;
+  const WorkLayout w = attend_layout(c.sequences, c.kv_heads, group, c.head_dim, slots, weigh, c.dtype);
   if (work_bytes < w.bytes || w.quanta > INT32_MAX) return kBadSize;  // (quanta are counted in 32 bits)
-  const int es = element_bytes(dtype);
+  const int es = element_bytes(c.dtype);
   PagedAttend a{};
   a.q = reinterpret_cast<const void*>(q);
-  a.k = reinterpret_cast<const void*>(k);
-  a.v = reinterpret_cast<const void*>(v);
-  a.table = reinterpret_cast<const int32_t*>(table);
-  a.lengths = reinterpret_cast<const int32_t*>(lengths);
-  a.scores = reinterpret_cast<const float*>(scores);
-  a.scores_out = reinterpret_cast<float*>(scores_out);
+  a.k = reinterpret_cast<const void*>(c.k);
+  a.v = reinterpret_cast<const void*>(c.v);
+  a.table = reinterpret_cast<const int32_t*>(c.table);
+  a.lengths = reinterpret_cast<const int32_t*>(flags & 2 ? into->lengths : c.lengths);
   a.lse_out = reinterpret_cast<float*>(lse);
   a.out = reinterpret_cast<void*>(out);
   char* work = reinterpret_cast<char*>(paged_work);
   a.counters = reinterpret_cast<unsigned*>(work);
   a.state = reinterpret_cast<float*>(work + w.state);
-  if (scores) {
+  if (weigh) {
+    a.scores = reinterpret_cast<const float*>(c.scores);
+    a.scores_out = reinterpret_cast<float*>(into->scores);
     a.lse_work = reinterpret_cast<float*>(work + w.lse);
     a.logits = reinterpret_cast<float*>(work + w.logits);
   }
-  a.err = reinterpret_cast<unsigned*>(err);
-  a.head_bytes = head_stride * es;
+  a.err = reinterpret_cast<unsigned*>(c.err);
+  a.head_bytes = c.head_stride * es;
   a.logit_stride = w.logit_stride;
   a.slots = slots;
-  a.page_units = (unsigned)(page_stride * es >> 4);
-  a.slot_units = (unsigned)(slot_stride * es >> 4);
+  a.page_units = (unsigned)(c.page_stride * es >> 4);
+  a.slot_units = (unsigned)(c.slot_stride * es >> 4);
   a.state_stride = w.state_stride;
-  a.div = page_div(page_size);
-  a.sequences = sequences;
-  a.kv_heads = kv_heads;
+  a.div = page_div(c.page_size);
+  a.sequences = c.sequences;
+  a.kv_heads = c.kv_heads;
   a.group = group;
   a.tiles = (group + 15) / 16;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.pages = (int)pages;
+  a.page_size = c.page_size;
+  a.max_pages = c.max_pages;
+  a.pages = (int)c.pages;
   a.scale = (float)(scale * 1.4426950408889634);
   const hipStream_t s = (hipStream_t)stream;
   int rc;
-  if (dtype == kBf16) rc = launch_attend_dim<kBf16>(a, head_dim, w.units, s);
-  else if (dtype == kFp16) rc = launch_attend_dim<kFp16>(a, head_dim, w.units, s);
-  else rc = launch_attend_dim<kFp32>(a, head_dim, w.units, s);
-  if (rc || !scores) return rc;
+  if (c.dtype == kBf16) rc = launch_attend_dim<kBf16>(a, c.head_dim, w.units, s);
+  else if (c.dtype == kFp16) rc = launch_attend_dim<kFp16>(a, c.head_dim, w.units, s);
+  else rc = launch_attend_dim<kFp32>(a, c.head_dim, w.units, s);
+  if (rc || !weigh) return rc;
   const int64_t blocks = (slots + kPT - 1) / kPT;
-  hipLaunchKernelGGL(paged_weigh_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024), kv_heads, sequences), dim3(kPT), 0,
-                     s, a);
+  hipLaunchKernelGGL(paged_weigh_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024), c.kv_heads, c.sequences),
+                     dim3(kPT), 0, s, a);
   return (int)hipGetLastError();
 }
 
-int prismkv_paged_append(uint64_t k, uint64_t v, uint64_t k_pages, uint64_t v_pages, uint64_t table, uint64_t offsets,
-                         uint64_t lengths, uint64_t lengths_out, uint64_t seen, uint64_t seen_out, uint64_t scores,
-                         uint64_t scores_out, uint64_t positions, uint64_t positions_out, uint64_t err, int64_t rows,
-                         int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
-                         int sequences, int kv_heads, int head_dim, int page_size, int max_pages, int64_t pages,
-                         int64_t page_stride, int64_t head_stride, int64_t slot_stride, int dtype, uint64_t stream) {
-  if (dtype < kBf16 || dtype > kFp32) return kBadMode;
-  if (bad_cache(sequences, kv_heads, head_dim, page_size, max_pages, pages, page_stride, head_stride, slot_stride, dtype))
-    return kBadSize;
-  if (rows < 0 || rows > INT32_MAX || (!offsets && rows != sequences)) return kBadSize;
-  if (!k_pages || !v_pages || !table || !lengths || !lengths_out || !err || (rows && (!k || !v))) return kBadSize;
-  const bool scored = positions != 0;
-  if (scored && (!positions_out || !scores || !scores_out || !seen || !seen_out)) return kBadSize;
-  const int es = element_bytes(dtype);
-  if ((k | v | k_pages | v_pages) & 15 || err & 7 ||
-      (table | offsets | lengths | lengths_out | seen | seen_out | scores | scores_out | positions | positions_out) & 3)
-    return kBadSize;
-  if ((k_row_stride * es | k_head_stride * es | v_row_stride * es | v_head_stride * es) & 15) return kBadSize;
+int prismkv_paged_append(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t k, uint64_t v,
+                         uint64_t offsets, int64_t rows, int64_t k_row_stride, int64_t k_head_stride,
+                         int64_t v_row_stride, int64_t v_head_stride, uint64_t stream) {
+  if (const int rc = check_cache(cache, into, false)) return rc;
+  const prismkv_paged_cache& c = *cache;
+  if (rows < 0 || rows > INT32_MAX || (!offsets && rows != c.sequences)) return kBadSize;
+  if (rows && (!k || !v)) return kBadSize;
+  const int64_t es = element_bytes(c.dtype), limit = 1ll << 40;
+  for (const int64_t stride : {k_row_stride, k_head_stride, v_row_stride, v_head_stride})
+    if (stride < -limit || stride > limit || stride * es & 15) return kBadSize;
+  if ((k | v) & 15 || offsets & 3) return kBadSize;
   PagedAppend a{};
   a.k = reinterpret_cast<const char*>(k);
   a.v = reinterpret_cast<const char*>(v);
-  a.kp = reinterpret_cast<char*>(k_pages);
-  a.vp = reinterpret_cast<char*>(v_pages);
-  a.table = reinterpret_cast<const int32_t*>(table);
+  a.kp = reinterpret_cast<char*>(c.k);
+  a.vp = reinterpret_cast<char*>(c.v);
+  a.table = reinterpret_cast<const int32_t*>(c.table);
   a.offsets = reinterpret_cast<const int32_t*>(offsets);
-  a.lengths = reinterpret_cast<const int32_t*>(lengths);
-  a.lengths_out = reinterpret_cast<int32_t*>(lengths_out);
-  a.seen = reinterpret_cast<const int32_t*>(seen);
-  a.seen_out = reinterpret_cast<int32_t*>(seen_out);
-  a.positions = reinterpret_cast<int32_t*>(positions);
-  a.positions_out = reinterpret_cast<int32_t*>(positions_out);
-  a.scores = reinterpret_cast<float*>(scores);
-  a.scores_out = reinterpret_cast<float*>(scores_out);
-  a.err = reinterpret_cast<unsigned*>(err);
+  a.lengths = reinterpret_cast<const int32_t*>(c.lengths);
+  a.lengths_out = reinterpret_cast<int32_t*>(into->lengths);
+  a.seen = reinterpret_cast<const int32_t*>(c.seen);
+  a.seen_out = reinterpret_cast<int32_t*>(into->seen);
+  a.positions = reinterpret_cast<int32_t*>(c.positions);
+  a.positions_out = reinterpret_cast<int32_t*>(into->positions);
+  a.scores = reinterpret_cast<float*>(c.scores);
+  a.scores_out = reinterpret_cast<float*>(into->scores);
+  a.err = reinterpret_cast<unsigned*>(c.err);
   a.rows = rows;
   a.k_row = k_row_stride * es;
   a.k_head = k_head_stride * es;
   a.v_row = v_row_stride * es;
   a.v_head = v_head_stride * es;
-  a.page_bytes = page_stride * es;
-  a.head_bytes = head_stride * es;
-  a.slot_bytes = slot_stride * es;
-  a.div = page_div(page_size);
-  a.sequences = sequences;
-  a.kv_heads = kv_heads;
-  while (16 << a.log_pieces < head_dim * es) ++a.log_pieces;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.pages = (int)pages;
-  a.slots = page_size * max_pages;
+  a.page_bytes = c.page_stride * es;
+  a.head_bytes = c.head_stride * es;
+  a.slot_bytes = c.slot_stride * es;
+  a.div = page_div(c.page_size);
+  a.sequences = c.sequences;
+  a.kv_heads = c.kv_heads;
+  while (16 << a.log_pieces < c.head_dim * es) ++a.log_pieces;
+  a.page_size = c.page_size;
+  a.max_pages = c.max_pages;
+  a.pages = (int)c.pages;
+  a.slots = c.page_size * c.max_pages;
   const hipStream_t s = (hipStream_t)stream;
   if (!offsets) {
-    hipLaunchKernelGGL(paged_append_kernel, dim3(sequences), dim3(kPT), 0, s, a);
+    hipLaunchKernelGGL(paged_append_kernel, dim3(c.sequences), dim3(kPT), 0, s, a);
     return (int)hipGetLastError();
   }
   if (rows) {
     hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((rows + kAppendRows - 1) / kAppendRows)), dim3(kPT), 0, s, a);
     const int rc = (int)hipGetLastError();
-    if (rc || lengths_out != lengths) return rc;
+    if (rc || a.lengths_out != a.lengths) return rc;
   }
-  hipLaunchKernelGGL(paged_advance_kernel, dim3((sequences + kPT - 1) / kPT), dim3(kPT), 0, s, a);
+  hipLaunchKernelGGL(paged_advance_kernel, dim3((c.sequences + kPT - 1) / kPT), dim3(kPT), 0, s, a);
   return (int)hipGetLastError();
 }
 
@@ -1538,39 +1544,28 @@ size_t prismkv_paged_evict_work_bytes(int sequences, int kv_heads, int64_t slots
   return evict_layout(sequences, kv_heads, slots).bytes;
 }
 
-int prismkv_paged_evict(uint64_t k_pages, uint64_t v_pages, uint64_t table, uint64_t lengths, uint64_t lengths_out,
-                        uint64_t seen, uint64_t seen_out, uint64_t scores, uint64_t scores_out, uint64_t positions,
-                        uint64_t positions_out, uint64_t keeps, uint64_t paged_work, uint64_t err, int keep, int recent,
-                        int sinks, int sequences, int kv_heads, int head_dim, int page_size, int max_pages, int64_t pages,
-                        int64_t page_stride, int64_t head_stride, int64_t slot_stride, int dtype, size_t work_bytes,
-                        uint64_t stream) {
-  if (dtype < kBf16 || dtype > kFp32) return kBadMode;
-  if (bad_cache(sequences, kv_heads, head_dim, page_size, max_pages, pages, page_stride, head_stride, slot_stride, dtype))
-    return kBadSize;
+int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t keeps,
+                        uint64_t paged_work, int keep, int recent, int sinks, size_t work_bytes, uint64_t stream) {
+  if (const int rc = check_cache(cache, into, true)) return rc;
+  const prismkv_paged_cache& c = *cache;
   if (keep < 0 || recent < 0 || sinks < 0 || (keeps && keep)) return kBadSize;
-  if (!k_pages || !v_pages || !table || !lengths || !lengths_out || !seen || !seen_out || !scores || !scores_out ||
-      !positions || !positions_out || !paged_work || !err)
-    return kBadSize;
-  if ((k_pages | v_pages) & 15 || err & 7 ||
-      (table | lengths | lengths_out | seen | seen_out | scores | scores_out | positions | positions_out | keeps) & 3 ||
-      paged_work & 15)
-    return kBadSize;
-  const int64_t slots = (int64_t)page_size * max_pages;
-  const EvictLayout l = evict_layout(sequences, kv_heads, slots);
+  if (!paged_work || paged_work & 15 || keeps & 3) return kBadSize;
+  const int64_t slots = (int64_t)c.page_size * c.max_pages;
+  const EvictLayout l = evict_layout(c.sequences, c.kv_heads, slots);
   if (work_bytes < l.bytes) return kBadSize;
-  const int es = element_bytes(dtype);
+  const int es = element_bytes(c.dtype);
   PagedEvict a{};
-  a.kp = reinterpret_cast<char*>(k_pages);
-  a.vp = reinterpret_cast<char*>(v_pages);
-  a.table = reinterpret_cast<const int32_t*>(table);
-  a.lengths = reinterpret_cast<const int32_t*>(lengths);
-  a.lengths_out = reinterpret_cast<int32_t*>(lengths_out);
-  a.seen = reinterpret_cast<const int32_t*>(seen);
-  a.seen_out = reinterpret_cast<int32_t*>(seen_out);
-  a.scores = reinterpret_cast<const float*>(scores);
-  a.scores_out = reinterpret_cast<float*>(scores_out);
-  a.positions = reinterpret_cast<const int32_t*>(positions);
-  a.positions_out = reinterpret_cast<int32_t*>(positions_out);
+  a.kp = reinterpret_cast<char*>(c.k);
+  a.vp = reinterpret_cast<char*>(c.v);
+  a.table = reinterpret_cast<const int32_t*>(c.table);
+  a.lengths = reinterpret_cast<const int32_t*>(c.lengths);
+  a.lengths_out = reinterpret_cast<int32_t*>(into->lengths);
+  a.seen = reinterpret_cast<const int32_t*>(c.seen);
+  a.seen_out = reinterpret_cast<int32_t*>(into->seen);
+  a.scores = reinterpret_cast<const float*>(c.scores);
+  a.scores_out = reinterpret_cast<float*>(into->scores);
+  a.positions = reinterpret_cast<const int32_t*>(c.positions);
+  a.positions_out = reinterpret_cast<int32_t*>(into->positions);
   a.keeps = reinterpret_cast<const int32_t*>(keeps);
   char* work = reinterpret_cast<char*>(paged_work);
   a.moves = l.moves;
@@ -1582,17 +1577,17 @@ int prismkv_paged_evict(uint64_t k_pages, uint64_t v_pages, uint64_t table, uint
   a.table_words = l.table_words;
   a.part = (int)l.part;
   a.most_parts = (int)l.parts;
-  a.err = reinterpret_cast<unsigned*>(err);
-  a.page_bytes = page_stride * es;
-  a.head_bytes = head_stride * es;
-  a.slot_bytes = slot_stride * es;
-  a.div = page_div(page_size);
-  a.sequences = sequences;
-  a.kv_heads = kv_heads;
-  while (16 << a.log_pieces < head_dim * es) ++a.log_pieces;
-  a.page_size = page_size;
-  a.max_pages = max_pages;
-  a.pages = (int)pages;
+  a.err = reinterpret_cast<unsigned*>(c.err);
+  a.page_bytes = c.page_stride * es;
+  a.head_bytes = c.head_stride * es;
+  a.slot_bytes = c.slot_stride * es;
+  a.div = page_div(c.page_size);
+  a.sequences = c.sequences;
+  a.kv_heads = c.kv_heads;
+  while (16 << a.log_pieces < c.head_dim * es) ++a.log_pieces;
+  a.page_size = c.page_size;
+  a.max_pages = c.max_pages;
+  a.pages = (int)c.pages;
   a.slots = (int)slots;
   a.keep = keep;
   a.recent = recent;
@@ -1609,11 +1604,11 @@ int prismkv_paged_evict(uint64_t k_pages, uint64_t v_pages, uint64_t table, uint
                                                hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kLongRow * (int)sizeof(unsigned));
       if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(paged_select_kernel, dim3(kv_heads, sequences), dim3(kET), lds, s, a);
+    hipLaunchKernelGGL(paged_select_kernel, dim3(c.kv_heads, c.sequences), dim3(kET), lds, s, a);
     rc = (int)hipGetLastError();
     if (rc || most <= kFew) return rc;
   } else {
-    const dim3 grid((unsigned)l.parts, kv_heads, sequences);
+    const dim3 grid((unsigned)l.parts, c.kv_heads, c.sequences);
     hipLaunchKernelGGL(paged_rank_kernel<0>, grid, dim3(kET), 0, s, a);
     hipLaunchKernelGGL(paged_rank_kernel<1>, grid, dim3(kET), 0, s, a);
     hipLaunchKernelGGL(paged_rank_kernel<2>, grid, dim3(kET), 0, s, a);
@@ -1622,9 +1617,9 @@ int prismkv_paged_evict(uint64_t k_pages, uint64_t v_pages, uint64_t table, uint
     if (rc) return rc;
   }
   const int64_t blocks = (most + (kPT >> a.log_pieces) * kMoveRows - 1) / ((kPT >> a.log_pieces) * kMoveRows);
-  const int64_t room = 4096 / ((int64_t)sequences * kv_heads) + 1;  // workgroups of a row where there are many rows
+  const int64_t room = 4096 / ((int64_t)c.sequences * c.kv_heads) + 1;  // workgroups of a row where there are many rows
   const int64_t grid = blocks < 1 ? 1 : blocks < room ? blocks : room;
-  hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)grid, kv_heads, sequences), dim3(kPT), 0, s, a);
+  hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)grid, c.kv_heads, c.sequences), dim3(kPT), 0, s, a);
   return (int)hipGetLastError();
 }
 

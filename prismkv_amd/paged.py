@@ -127,12 +127,9 @@ class PagedCache:
         self.lib = _lib.load(library)
         if self.lib.missing:
             raise RuntimeError(f"{self.lib.path.name} lacks entry points {self.lib.missing}; rebuild it")
-        self.k, self.v, self.table, self.lengths = k, v, table, lengths
-        self.seen, self.scores, self.positions = seen, scores, positions
+        self._tensors = (k, v, table, lengths, seen, scores, positions)
         self.device = k.device
         self._shape = (sequences, kv_heads, head_dim, page_size, max_pages)
-        self._cache_args = (kv_heads, head_dim, page_size, max_pages, pages, *k.stride()[:3])
-        self._dtype = DTYPES[k.dtype]
         self._free = self._pages = None
         self._attend_work, self._evict_work = {}, None
         if err is None:
@@ -146,8 +143,15 @@ class PagedCache:
                 err[1] = address
             err = (err, host, ctypes.c_int32.from_address(host.data_ptr()))
         self._err = err
+        # what the C entries read of the cache; its tensors are fixed from here on
+        pointers = [0 if x is None else x.data_ptr() for x in self._tensors]
+        self._desc = _lib.PagedCacheDesc(*pointers, err[0].data_ptr(), pages, *k.stride()[:3], *self._shape,
+                                         DTYPES[k.dtype])
+        self._pointer = ctypes.c_void_p(ctypes.addressof(self._desc))
 
     # ------------------------------------------------------------ pages
+
+    k, v, table, lengths, seen, scores, positions = (property(lambda self, i=i: self._tensors[i]) for i in range(7))
 
     @property
     def scored(self):
@@ -261,10 +265,12 @@ class PagedCache:
     def _into(self, into):
         if into is None or into is self:
             return self
-        if not (isinstance(into, PagedCache) and into.k.data_ptr() == self.k.data_ptr()
-                and into.v.data_ptr() == self.v.data_ptr() and into.table.data_ptr() == self.table.data_ptr()
-                and into._cache_args == self._cache_args and into._shape == self._shape
-                and (into.scores is None) == (self.scores is None)):
+        if not isinstance(into, PagedCache) or into.device != self.device:
+            raise ValueError("into must be a fork of this cache")
+        a, b = self._desc, into._desc
+        if (a.k != b.k or a.v != b.v or a.table != b.table or a.pages != b.pages or a.page_stride != b.page_stride
+                or a.head_stride != b.head_stride or a.slot_stride != b.slot_stride or into._shape != self._shape
+                or a.dtype != b.dtype or (a.scores == 0) != (b.scores == 0)):
             raise ValueError("into must be a fork of this cache")
         return into
 
@@ -304,16 +310,8 @@ class PagedCache:
         elif rows != sequences:
             raise ValueError("one row per sequence, or offsets, required")
         self.check_errors()
-        self._call("prismkv_paged_append", kp, vp, self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
-                   0 if offsets is None else offsets.data_ptr(), self.lengths.data_ptr(), to.lengths.data_ptr(),
-                   *self._scored_pointers(to), self._err[0].data_ptr(), rows, ks[0], ks[1], vs[0], vs[1], sequences,
-                   *self._cache_args, self._dtype)
-
-    def _scored_pointers(self, to):
-        if not self.scored:
-            return (0,) * 6
-        return (self.seen.data_ptr(), to.seen.data_ptr(), self.scores.data_ptr(), to.scores.data_ptr(),
-                self.positions.data_ptr(), to.positions.data_ptr())
+        self._call("prismkv_paged_append", self._pointer, to._pointer, kp, vp,
+                   0 if offsets is None else offsets.data_ptr(), rows, ks[0], ks[1], vs[0], vs[1])
 
     def attend(self, q, *, scale=None, accumulate=False, lse=None, into=None):
         """Softmax attention of q [sequences, heads, head_dim] (heads a
@@ -323,7 +321,9 @@ class PagedCache:
         sequence.  `accumulate` adds to every slot's score its weight, summed
         over the heads that share it.  `lse`, an f32 [sequences, heads] tensor,
         receives the logarithm of each softmax's sum (-inf for an empty one)."""
-        return self._attend(q, self.lengths, scale, accumulate, lse, self if into is None else self._into(into))
+        to = self if into is None else self._into(into)
+        group, scale = self._check_q(q, scale, accumulate, lse)
+        return self._attend(q, group, scale, accumulate, lse, to, 0)
 
     def _check_q(self, q, scale, accumulate, lse):
         """The query heads per KV head, and the scale."""
@@ -349,24 +349,20 @@ class PagedCache:
             raise ValueError("lse must be a contiguous float32 [sequences, heads] on the cache's device")
         return group, scale
 
-    def _attend(self, q, lengths, scale, accumulate, lse, to):
-        group, scale = self._check_q(q, scale, accumulate, lse)
+    def _attend(self, q, group, scale, accumulate, lse, to, flags):
         self.check_errors()
-        sequences, kv_heads, head_dim, _, _ = self._shape
         accumulate = bool(accumulate)
         work = self._attend_work.get((group, accumulate))
         if work is None:
             # (the leading counters are zeroed; the kernels leave them so)
+            sequences, kv_heads, head_dim, _, _ = self._shape
             nbytes = self.lib.query("prismkv_paged_attend_work_bytes", sequences, kv_heads, group, head_dim, self.slots,
-                                    int(accumulate), self._dtype)
+                                    int(accumulate), self._desc.dtype)
             work = self._attend_work[(group, accumulate)] = self._workspace(
                 nbytes, 4 * sequences * kv_heads * ((group + 15) // 16))
         out = torch.empty_like(q)
-        scores = (self.scores.data_ptr(), to.scores.data_ptr()) if accumulate else (0, 0)
-        self._call("prismkv_paged_attend", q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
-                   lengths.data_ptr(), *scores, 0 if lse is None else lse.data_ptr(), work.data_ptr(),
-                   self._err[0].data_ptr(), out.data_ptr(), sequences, kv_heads, group, head_dim, *self._cache_args[2:],
-                   scale, self._dtype, work.numel())
+        self._call("prismkv_paged_attend", self._pointer, to._pointer, q.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                   work.data_ptr(), out.data_ptr(), group, flags + accumulate, scale, work.numel())
         return out
 
     def __call__(self, q, k, v, *, scale=None, accumulate=False, lse=None, into=None):
@@ -375,9 +371,9 @@ class PagedCache:
         go there, the new rows into the shared pages behind this cache's
         lengths."""
         to = self if into is None else self._into(into)
-        self._check_q(q, scale, accumulate, lse)  # nothing is appended for a query that is refused
+        group, scale = self._check_q(q, scale, accumulate, lse)  # nothing is appended for a query that is refused
         self.append(k, v, into=into)
-        return self._attend(q, to.lengths, scale, accumulate, lse, to)
+        return self._attend(q, group, scale, accumulate, lse, to, 2)
 
     def evict(self, keep, *, recent=0, sinks=0, into=None):
         """Cuts every sequence longer than `keep` slots (an int, or i32
@@ -401,14 +397,15 @@ class PagedCache:
         if self._evict_work is None:
             self._evict_work = self._workspace(
                 self.lib.query("prismkv_paged_evict_work_bytes", sequences, kv_heads, self.slots), 4 * sequences)
-        self._call("prismkv_paged_evict", self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(),
-                   self.lengths.data_ptr(), to.lengths.data_ptr(), *self._scored_pointers(to), keeps,
-                   self._evict_work.data_ptr(), self._err[0].data_ptr(), keep, recent, sinks, sequences,
-                   *self._cache_args, self._dtype, self._evict_work.numel())
+        self._call("prismkv_paged_evict", self._pointer, to._pointer, keeps, self._evict_work.data_ptr(), keep, recent,
+                   sinks, self._evict_work.numel())
 
     def buffer_bytes(self):
         """Live tensors held here, by name (a fork's pages are its origin's)."""
-        held = {name: x for name, x in vars(self).items() if isinstance(x, torch.Tensor)}
+        names = ("k", "v", "table", "lengths", "seen", "scores", "positions")
+        held = {name: x for name, x in zip(names, self._tensors) if x is not None}
+        if self._evict_work is not None:
+            held["evict_work"] = self._evict_work
         held.update((f"attend_work{key}", x) for key, x in self._attend_work.items())
         return {name: x.numel() * x.element_size() for name, x in held.items()}
 

@@ -1,5 +1,6 @@
 """CPU checks of the paged cache's C entries (refusals before anything is
 enqueued) and of its 64-bit definition (oracle/paged.py)."""
+import ctypes
 import random
 
 import pytest
@@ -8,88 +9,94 @@ import torch
 from oracle import paged
 from tests.test_abi import BIG, call_raw, lib  # noqa: F401
 
-# sequences, kv_heads, head_dim, page_size, max_pages | pages, page_stride, head_stride, slot_stride, dtype
-SHAPE, STRIDES = (3, 8, 128, 16, 10), (40, 8 * 16 * 128, 16 * 128, 128)
+GOOD = dict(k=16, v=16, table=16, lengths=16, seen=16, scores=16, positions=16, err=16, pages=40,
+            page_stride=8 * 16 * 128, head_stride=16 * 128, slot_stride=128, sequences=3, kv_heads=8, head_dim=128,
+            page_size=16, max_pages=10, dtype=0)
 
 
-def attend(lib, pointers=(16,) * 11, shape=SHAPE, group=4, strides=STRIDES, scale=0.1, dtype=0, work=BIG):
-    b, h, d, ps, mp = shape
-    return call_raw(lib, "prismkv_paged_attend", *pointers, b, h, group, d, ps, mp, *strides, scale, dtype, work)
+def desc(**changed):
+    from prismkv_amd._lib import PagedCacheDesc
+    return ctypes.byref(PagedCacheDesc(**{**GOOD, **changed}))
 
 
-def append(lib, pointers=(16,) * 15, rows=5, row_strides=(1024, 128, 1024, 128), shape=SHAPE, strides=STRIDES, dtype=0):
-    return call_raw(lib, "prismkv_paged_append", *pointers, rows, *row_strides, *shape, *strides, dtype)
+def attend(lib, cache=None, into=None, q=16, lse=0, work=16, out=16, group=4, flags=1, scale=0.1, nbytes=BIG):
+    return call_raw(lib, "prismkv_paged_attend", cache or desc(), into or cache or desc(), q, lse, work, out, group, flags,
+                    scale, nbytes)
 
 
-def evict(lib, pointers=(16,) * 11 + (0, 16, 16), keep=5, recent=0, sinks=0, shape=SHAPE, strides=STRIDES, dtype=0,
-          work=BIG):
-    return call_raw(lib, "prismkv_paged_evict", *pointers, keep, recent, sinks, *shape, *strides, dtype, work)
+def append(lib, cache=None, into=None, k=16, v=16, offsets=16, rows=5, strides=(1024, 128, 1024, 128)):
+    return call_raw(lib, "prismkv_paged_append", cache or desc(), into or cache or desc(), k, v, offsets, rows, *strides)
 
 
+def evict(lib, cache=None, into=None, keeps=0, work=16, keep=5, recent=0, sinks=0, nbytes=BIG):
+    return call_raw(lib, "prismkv_paged_evict", cache or desc(), into or cache or desc(), keeps, work, keep, recent, sinks,
+                    nbytes)
+
+
+SHAPE = ("sequences", "kv_heads", "head_dim", "page_size", "max_pages")
+STRIDES = ("pages", "page_stride", "head_stride", "slot_stride")
 BAD_SHAPES = [(0, 8, 128, 16, 10), (65536, 8, 128, 16, 10), (3, 0, 128, 16, 10), (3, 8, 96, 16, 10), (3, 8, 128, 0, 10),
               (3, 8, 128, 16, 0), (3, 8, 128, 1 << 20, 1 << 11), (3, 8, 128, 1 << 30, 1), (2, 8, 128, 1 << 30, 2)]
-BAD_STRIDES = [(0, *STRIDES[1:]), (40, 8 * 16 * 128 + 1, 2048, 128), (40, 16384, 2048 + 4, 128), (40, 16384, 2048, 120),
-               (40, -16384, 2048, 128), (1 << 31, 16384, 2048, 128), (40, 1 << 35, 2048, 128), (40, 1 << 62, 2048, 128),
-               (40, 16384, 2048, 1 << 60)]
+BAD_STRIDES = [(0, 16384, 2048, 128), (40, 8 * 16 * 128 + 1, 2048, 128), (40, 16384, 2048 + 4, 128),
+               (40, 16384, 2048, 120), (40, -16384, 2048, 128), (1 << 31, 16384, 2048, 128), (40, 1 << 35, 2048, 128),
+               (40, 1 << 62, 2048, 128), (40, 16384, 2048, 1 << 60)]
 
 
 @pytest.mark.parametrize("call", [attend, append, evict])
-def test_refused_sizes(lib, call):  # noqa: F811
+def test_refused_caches(lib, call):  # noqa: F811
     for shape in BAD_SHAPES:
-        assert call(lib, shape=shape) == -1, shape
+        assert call(lib, desc(**dict(zip(SHAPE, shape)))) == -1, shape
     for strides in BAD_STRIDES:
-        assert call(lib, strides=strides) == -1, strides
+        assert call(lib, desc(**dict(zip(STRIDES, strides)))) == -1, strides
     for dtype in (-1, 3):
-        assert call(lib, dtype=dtype) == -2
-
-
-def _without(pointers, i, value=0):
-    return tuple(value if j == i else x for j, x in enumerate(pointers))
-
-
-def test_refused_pointers(lib):  # noqa: F811
-    good = (16,) * 11
-    for i in (0, 1, 2, 3, 4, 5, 6, 8, 9, 10):  # scores and their destination come together
-        assert attend(lib, _without(good, i)) == -1, i
-    for i, off in ((0, 24), (1, 24), (2, 24), (3, 18), (4, 18), (7, 18), (8, 24), (9, 20)):
-        assert attend(lib, _without(good, i, off)) == -1, i
-    good = (16,) * 15
-    for i in (0, 1, 2, 3, 4, 6, 7, 8, 9, 10, 11, 13, 14):  # (0: no offsets; 12: not scored)
-        assert append(lib, _without(good, i)) == -1, i
-    for i, off in ((0, 24), (2, 24), (5, 18), (12, 18), (14, 20)):
-        assert append(lib, _without(good, i, off)) == -1, i
-    good = (16,) * 11 + (0, 16, 16)
-    for i in range(14):
-        if i != 11:
-            assert evict(lib, _without(good, i)) == -1, i
-    assert evict(lib, _without(good, 12, 24)) == -1 and evict(lib, _without(good, 13, 20)) == -1
+        assert call(lib, desc(dtype=dtype)) == -2
+    for name in ("k", "v", "table", "lengths", "err"):
+        assert call(lib, desc(**{name: 0})) == -1, name
+    for name in ("seen", "scores", "positions"):  # all of a scored cache, or none
+        assert call(lib, desc(**{name: 0})) == -1, name
+    for name in ("k", "v"):
+        assert call(lib, desc(**{name: 24})) == -1, name
+    for name in ("table", "lengths", "seen", "scores", "positions", "err"):
+        assert call(lib, desc(**{name: 18})) == -1, name
+    # results go to a cache over the same pages and table
+    for name in ("k", "v", "table", *STRIDES, *SHAPE, "dtype"):
+        other = {"dtype": 1, "head_dim": 64, "slot_stride": 256, "head_stride": 4096}.get(name, 2 * GOOD[name])
+        assert call(lib, desc(), desc(**{name: other})) == -1, name
+    assert call(lib, desc(), desc(seen=0, scores=0, positions=0)) == -1
+    name = "prismkv_paged_" + call.__name__
+    assert call_raw(lib, name, *[0] * (len(getattr(lib.cdll, name).argtypes) - 1)) == -1  # no cache
 
 
 def test_refused_arguments(lib):  # noqa: F811
-    assert attend(lib, group=0) == -1 and attend(lib, group=1025) == -1
-    assert attend(lib, scale=float("nan")) == -1
-    assert append(lib, rows=-1) == -1 and append(lib, rows=1 << 31) == -1
-    no_offsets = _without((16,) * 15, 5)
-    assert append(lib, no_offsets, rows=4) == -1  # one row per sequence without offsets
+    plain = desc(seen=0, scores=0, positions=0)
+    assert attend(lib, plain, flags=1) == -1 and evict(lib, plain) == -1  # not scored
+    for bad in (dict(q=0), dict(q=24), dict(work=0), dict(work=24), dict(out=0), dict(out=18), dict(lse=18),
+                dict(group=0), dict(group=1025), dict(scale=float("nan")), dict(scale=float("inf"))):
+        assert attend(lib, **bad) == -1, bad
+    assert attend(lib, flags=4) == -2
+    for bad in (dict(k=0), dict(v=0), dict(k=24), dict(offsets=18), dict(rows=-1), dict(rows=1 << 31),
+                dict(offsets=0, rows=4)):  # (one row per sequence without offsets)
+        assert append(lib, **bad) == -1, bad
     for i in range(4):
-        assert append(lib, row_strides=_without((1024, 128, 1024, 128), i, 1028)) == -1
-    for bad in (dict(keep=-1), dict(recent=-1), dict(sinks=-1)):
-        assert evict(lib, **bad) == -1
-    assert evict(lib, (16,) * 14, keep=5) == -1  # a budget for all and one for each
+        for bad in (1028, 1 << 41, -(1 << 41), 1 << 62):
+            assert append(lib, strides=[bad if j == i else 1024 for j in range(4)]) == -1
+    for bad in (dict(keep=-1), dict(recent=-1), dict(sinks=-1), dict(work=0), dict(work=24), dict(keeps=18, keep=0),
+                dict(keeps=16, keep=5)):  # (a budget for all and one for each)
+        assert evict(lib, **bad) == -1, bad
 
 
 def test_workspace_sizes(lib):  # noqa: F811
     need = lib.query("prismkv_paged_attend_work_bytes", 3, 8, 4, 128, 160, 1, 0)
     # the weighed logits of every query head and slot, at least
     assert need >= 3 * 32 * 160 * 4 + lib.query("prismkv_paged_attend_work_bytes", 3, 8, 4, 128, 160, 0, 0)
-    assert attend(lib, work=need - 1) == -1
-    assert attend(lib, work=need) not in (0, -1, -2)  # past every host check, refused by the runtime (no device)
+    assert attend(lib, nbytes=need - 1) == -1
+    assert attend(lib, nbytes=need) not in (0, -1, -2)  # past every host check, refused by the runtime (no device)
     for bad in ((0, 8, 4, 128, 160, 0, 0), (3, 0, 4, 128, 160, 0, 0), (3, 8, 0, 128, 160, 0, 0), (3, 8, 4, 128, 0, 0, 0),
                 (3, 8, 4, 128, 160, 0, 3)):
         assert lib.query("prismkv_paged_attend_work_bytes", *bad) == 0
     need = lib.query("prismkv_paged_evict_work_bytes", 3, 8, 160)
     assert need >= 24 * 160 * 4
-    assert evict(lib, work=need - 1) == -1 and evict(lib, work=need) not in (0, -1, -2)
+    assert evict(lib, nbytes=need - 1) == -1 and evict(lib, nbytes=need) not in (0, -1, -2)
     assert lib.query("prismkv_paged_evict_work_bytes", 0, 8, 160) == 0
     assert append(lib) not in (0, -1, -2)
 
