@@ -426,8 +426,9 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *            where nothing is scored);
  *   err      16 bytes, 8-byte aligned: the error word, set to 4 when a slot
  *            below a length has no page (a row to append to it is dropped;
- *            attention reads page 0 in its place; a move is left out), and at
- *            byte offset 8 the optional host word's address, as in a workspace.
+ *            attention reads page 0 in its place; a move is left out) and to 8
+ *            when an append's offsets do not cover its rows, and at byte offset 8
+ *            the optional host word's address, as in a workspace.
  * Results go to a second cache `into` over the same pages and table: the first
  * itself, or one whose lengths, seen, scores and positions do not overlap the
  * first's.  A page that belongs to several tables may be read, not written.

@@ -7,7 +7,9 @@ namespace prismkv {
 namespace {
 
 constexpr int kPT = 256;  // threads of the paged kernels but the selection
-constexpr unsigned kErrPages = 4u;  // error word: a slot within a sequence's length has no page of the cache
+// Error word: a slot within a sequence's length has no page of the cache; an append's
+// offsets do not cover its rows.
+constexpr unsigned kErrPages = 4u, kErrRows = 8u;
 
 // Element types of the C ABI (`dtype`).
 constexpr int kBf16 = 0, kFp16 = 1, kFp32 = 2;
@@ -113,53 +115,48 @@ struct PagedSpan {
   int at, end, b, hh, n, first;
 };
 
-// Calls f(i, n, c) for the lengths n and quanta c of 64 sequences from i on at a
-// time (a lane each, 0 past the last), until it returns true.
-template <int kL, typename F>
-__device__ __forceinline__ void each_64(const PagedAttend& a, F f) {
-  const int lane = threadIdx.x & 63;
-  for (int i = 0; i < a.sequences; i += 64) {
-    const bool in = i + lane < a.sequences;
-    const int n = in ? clamp_length(a, a.lengths[i + lane]) : 0;
-    if (f(i, n, in ? quanta_of<kL>(n) : 0)) return;
-  }
+// Quanta of the first `count` sequences, for one KV head and head tile.
+template <int kL>
+__device__ __forceinline__ int quanta_before(const PagedAttend& a, int count) {
+  int sum = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < count; i += 64) sum += quanta_of<kL>(clamp_length(a, a.lengths[i]));
+  return wave_sum_i(sum);
 }
 
-// Every wave finds its workgroup's share by itself (uniform; one load of the
-// lengths and a lane scan for up to 64 sequences), so that a long sequence among
+// Every wave finds its workgroup's share by itself (uniform; two loads of the
+// lengths and a lane scan for every 64 sequences), so that a long sequence among
 // short ones is spread over as many workgroups as its share of the rows.
 template <int kL>
 __device__ __forceinline__ PagedSpan<kL> find_span(const PagedAttend& a, int unit) {
-  const int heads = a.kv_heads * a.tiles;
+  const int lane = threadIdx.x & 63, heads = a.kv_heads * a.tiles;
+  auto length = [&](int i) { return i < a.sequences ? clamp_length(a, a.lengths[i]) : 0; };
+  int n = length(lane);
   PagedSpan<kL> u;
-  u.deal.total = 0;
-  each_64<kL>(a, [&](int, int, int c) {
-    u.deal.total += wave_sum_i(c);
-    return false;
-  });
-  u.deal.total *= heads;
+  u.deal.total = quanta_before<kL>(a, a.sequences) * heads;
   u.at = u.deal.begin(unit);
   u.end = u.deal.begin(unit + 1);
   if (u.at >= u.end) return u;
   const int to = u.at / heads;  // (a sequence's quanta begin at a multiple of heads)
   int base = 0;
-  each_64<kL>(a, [&](int i, int n, int c) {
+  for (int i = 0;; i += 64) {  // (`to` lies in some sequence)
+    const int next = length(i + 64 + lane);
+    const int c = i + lane < a.sequences ? quanta_of<kL>(n) : 0;
     const int incl = (int)wave_incl_scan((unsigned)c);
     const int sum = __builtin_amdgcn_readlane(incl, 63);
-    if (to - base >= sum) {
-      base += sum;
-      return false;
+    if (to - base < sum || i + 64 >= a.sequences) {
+      const int l = max(__ffsll((unsigned long long)__ballot(incl > to - base)) - 1, 0);
+      const int own = __builtin_amdgcn_readlane(c, l);
+      const int in = u.at - (base + __builtin_amdgcn_readlane(incl, l) - own) * heads;  // within the sequence
+      u.b = i + l;
+      u.n = __builtin_amdgcn_readlane(n, l);
+      u.hh = in / own;
+      u.first = in - u.hh * own;
+      return u;
     }
-    const int l = __ffsll((unsigned long long)__ballot(incl > to - base)) - 1;
-    const int own = __builtin_amdgcn_readlane(c, l);
-    const int in = u.at - (base + __builtin_amdgcn_readlane(incl, l) - own) * heads;  // within the sequence
-    u.b = i + l;
-    u.n = __builtin_amdgcn_readlane(n, l);
-    u.hh = in / own;
-    u.first = in - u.hh * own;
-    return true;
-  });
-  return u;
+    base += sum;
+    n = next;
+  }
 }
 
 // log2 of a softmax's sum from its maximum and the sum held times 2^kBias.

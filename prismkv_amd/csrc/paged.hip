@@ -436,8 +436,6 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
         s[i][r] = DT == kFp32 ? d[r] + d2[r] : d[r];
         bm = fmaxf(bm, t0 + 16 * i + 4 * q + r < end ? s[i][r] * a.scale : -INFINITY);
       }
-      if (logits && j < rows)
-        *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
     }
     rows_of.move();
     rows_of.load_k(t);
@@ -494,6 +492,13 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
       pv_columns<0, DT, D>(acc, t, ph, pl);
     }
     rows_of.load_v(t);
+    // behind the loads: memory answers stores in the same order, and what the next
+    // step waits for must not be behind them (16 sequences of 4099: 47.5 us before)
+    if (logits && j < rows) {
+#pragma unroll
+      for (int i = 0; i < T::kBlocks; ++i)
+        *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+    }
   }
   if (__ballot(rows_of.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
 
@@ -584,20 +589,13 @@ constexpr int kJoinColumns = 16;
 template <int DT, int D>
 __global__ __launch_bounds__(kPT) void paged_join_kernel(PagedAttend a) {
   extern __shared__ float lds[];
-  const int b = blockIdx.z, lane = threadIdx.x & 63;
+  const int b = blockIdx.z;
   const int h = blockIdx.y / a.tiles, tile = blockIdx.y - h * a.tiles;
   const int rows = min(a.group - 16 * tile, 16), col0 = blockIdx.x * kJoinColumns;
   if (col0 >= rows * D / 4) return;
   constexpr int kL = kLeast<DT, D>;
-  PagedDeal<kL> deal{0};
-  int from = 0, n = 0;  // quanta before sequence b, its length
-  each_64<kL>(a, [&](int i, int len, int c) {
-    deal.total += wave_sum_i(c);
-    from += wave_sum_i(i + lane < b ? c : 0);
-    if (i <= b && b < i + 64) n = __builtin_amdgcn_readlane(len, b - i);
-    return false;
-  });
-  deal.total *= a.kv_heads * a.tiles;
+  const PagedDeal<kL> deal{quanta_before<kL>(a, a.sequences) * a.kv_heads * a.tiles};
+  const int from = quanta_before<kL>(a, b), n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[b]));
   const int quanta = quanta_of<kL>(n);
   const PagedParts parts(deal, from * a.kv_heads * a.tiles + (int)blockIdx.y * quanta, quanta);
   if (parts.chunks == 1) return;  // its workgroup has finished it
@@ -614,9 +612,21 @@ __global__ __launch_bounds__(kPT) void paged_weigh_kernel(PagedAttend a) {
   const float* logits = a.logits + ((size_t)b * a.kv_heads + h) * a.group * a.logit_stride;
   const size_t at = ((size_t)b * a.kv_heads + h) * a.slots;
   for (int t = blockIdx.x * kPT + threadIdx.x; t < n; t += gridDim.x * kPT) {
+    const float before = a.scores[at + t];
     float sum = 0.f;
-    for (int g = 0; g < a.group; ++g) sum += weight(logits[(size_t)g * a.logit_stride + t], a.scale, no_less(lse[g]));
-    a.scores_out[at + t] = a.scores[at + t] + sum;
+    for (int g0 = 0; g0 < a.group; g0 += 4) {  // (four heads' loads together)
+      float s[4], l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int g = min(g0 + e, a.group - 1);
+        s[e] = logits[(size_t)g * a.logit_stride + t];
+        l[e] = lse[g];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (g0 + e < a.group) sum += weight(s[e], a.scale, no_less(l[e]));
+    }
+    a.scores_out[at + t] = before + sum;
   }
 }
 
@@ -664,8 +674,12 @@ __device__ __forceinline__ AppendPlace append_place(const PagedAppend& a, int64_
   return p;
 }
 
-// lengths and tokens seen of sequence b with `more` rows
-__device__ __forceinline__ void advance(const PagedAppend& a, int b, int more) {
+// lengths and tokens seen of sequence b with its packed rows; offsets that do not
+// cover the rows, ascending from 0, are reported
+__device__ __forceinline__ void advance(const PagedAppend& a, int b) {
+  const int from = a.offsets[b], to = a.offsets[b + 1], more = max(to - from, 0);
+  if (from > to || (b == 0 && from) || (b == a.sequences - 1 && to != a.rows))
+    report_error(a.err, error_host_slot(a.err), kErrRows);
   a.lengths_out[b] = (int)min((int64_t)max(a.lengths[b], 0) + more, (int64_t)a.slots);
   if (a.positions) a.seen_out[b] = a.seen[b] + more;
 }
@@ -729,14 +743,14 @@ __global__ __launch_bounds__(kPT) void paged_append_kernel(PagedAppend a) {
     }
   } else if (a.lengths_out != a.lengths) {
     for (int64_t b = (int64_t)blockIdx.x * kPT + tid; b < a.sequences; b += (int64_t)gridDim.x * kPT)
-      advance(a, (int)b, max(a.offsets[b + 1] - a.offsets[b], 0));
+      advance(a, (int)b);
   }
 }
 
 // Packed rows onto lengths that are advanced in place: after every workgroup has read them.
 __global__ __launch_bounds__(kPT) void paged_advance_kernel(PagedAppend a) {
   const int b = blockIdx.x * kPT + threadIdx.x;
-  if (b < a.sequences) advance(a, b, max(a.offsets[b + 1] - a.offsets[b], 0));
+  if (b < a.sequences) advance(a, b);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -1012,6 +1026,7 @@ __global__ __launch_bounds__(kET) void paged_select_kernel(PagedEvict a) {
   extern __shared__ unsigned keys[];  // of whole 64-slot steps
   for (int i = tid; i < 3 * 2048; i += kET) (&hist[0][0])[i] = 0u;
   const EvictRow r(a, b, h);
+  asm volatile("" ::"s"(r.n), "s"(r.m));  // (read, not only asked for, before others may write the length)
   __syncthreads();
   const bool cut = r.n > r.m && r.m > 0;
   const int steps = (r.n + 64 * kEWaves - 1) / (64 * kEWaves);  // of 64 slots per wave

@@ -24,7 +24,9 @@ from . import _lib
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 HEAD_DIMS = (64, 128, 256)
-ERR_PAGES = 4
+ERR_PAGES, ERR_ROWS = 4, 8  # codes of the error word, as the kernels write them
+ERROR_MESSAGES = {ERR_PAGES: "a slot below a sequence's length has no page",
+                  ERR_ROWS: "the offsets of an append did not ascend from 0 to its number of rows"}
 _SCORED = ("seen", "scores", "positions")
 
 
@@ -241,18 +243,20 @@ class PagedCache:
 
     def check_errors(self):
         """RuntimeError if an earlier launch found a slot below a sequence's
-        length without a page: the results since the last check are invalid.
-        Reads a host-mapped word (no synchronisation, launches that have not
-        run yet are not seen) and clears it."""
+        length without a page, or offsets that do not cover an append's rows:
+        the results since the last check are invalid.  Reads a host-mapped word
+        (no synchronisation, launches that have not run yet are not seen) and
+        clears it."""
         err, host, word = self._err  # (word: host's first element, read without a tensor operation)
-        if word.value:
+        code = word.value
+        if code:
             with torch.cuda.device(self.device):
                 torch.cuda.synchronize()
                 err[:1].zero_()
                 host.zero_()
                 torch.cuda.synchronize()
-            raise RuntimeError("paged cache: a slot below a sequence's length has no page; the results of the launches "
-                               "since the last check are invalid")
+            raise RuntimeError(f"paged cache: {ERROR_MESSAGES.get(code, code)}; the results of the launches since the "
+                               "last check are invalid")
 
     def _call(self, name, *args):
         index = self.device.index

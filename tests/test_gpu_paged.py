@@ -525,6 +525,63 @@ def test_slots_without_pages_are_reported():
     full.check_errors()
 
 
+@pytest.mark.parametrize("bad", [[0, 2, 4], [0, 4, 3], [1, 2, 3], [0, 3, 2], [-1, 2, 3]])
+def test_offsets_that_do_not_fit_are_reported(bad):
+    for apart in (False, True):
+        cache, _ = make([20, 3], 2, 64, 16, BF16, room=8, scored=True)
+        rows = torch.zeros(3, 2, 64, dtype=BF16, device="cuda")
+        cache.append(rows, rows, torch.tensor(bad, dtype=torch.int32, device="cuda"), into=cache.fork() if apart else None)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="offsets"):
+            cache.check_errors()
+
+
+def test_many_sequences():
+    """More sequences than one load of the lengths finds, short and empty ones
+    between a long one's."""
+    lengths = [(7 * b) % 40 for b in range(700)]
+    lengths[3], lengths[411], lengths[699] = 3000, 900, 0
+    cache, host = make(lengths, 1, 64, 32, BF16, scored=True)
+    q = queries(cache, 2)
+    out = cache.attend(q.cuda(), accumulate=True, into=cache.fork())
+    pick = list(range(0, 20)) + list(range(400, 420)) + list(range(690, 700))
+    few = dict(host, table=host["table"][pick])
+    check_attend(q[pick], few, [lengths[b] for b in pick], out[pick])
+
+
+@pytest.mark.parametrize("dim,group,dtype", [(128, 16, BF16), (256, 16, FP16), (128, 16, FP32), (64, 40, BF16)])
+def test_wide_calls_in_a_graph(dim, group, dtype):
+    """The calls that take most LDS and a second launch, captured."""
+    lengths = [9000, 300]
+    cache, host = make(lengths, 1, dim, 64, dtype, scored=True, fill=0.0)
+    q = queries(cache, group).cuda()
+    fork = cache.fork()
+    want = cache.attend(q, accumulate=True, into=fork)
+    scores = fork.scores.clone()
+    check_attend(q.cpu(), host, lengths, want)
+    after = cache.fork()
+    cache.evict(7000, recent=5, into=after)
+    positions = after.positions[:, :, :300].clone()
+    cache.k.copy_(host["k"])
+    cache.v.copy_(host["v"])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, accumulate=True, into=fork)
+        cache.evict(7000, recent=5, into=after)
+    for _ in range(3):
+        for x in (fork.scores, after.positions, after.lengths):
+            x.zero_()
+        cache.k.copy_(host["k"])
+        cache.v.copy_(host["v"])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(bits(out), bits(want)) and after.lengths.tolist() == [7000, 300]
+        for b, n in enumerate(lengths):
+            assert torch.equal(fork.scores[b, :, :n], scores[b, :, :n])
+        assert torch.equal(after.positions[:, :, :300], positions)
+
+
 def test_reserve_and_release():
     cache = PagedCache(2, 6, 4, page_size=16, kv_heads=1, head_dim=64)
     cache.reserve([17, 1])
