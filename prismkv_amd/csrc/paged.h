@@ -57,6 +57,7 @@ struct PagedAttend {
   PageDiv div;
   int sequences, kv_heads, group, tiles, page_size, max_pages, pages;
   float scale;  // log2(e) times the caller's
+  bool many;    // kSoloPairs pairs or more
 };
 
 // 16 bytes that another workgroup wrote through (agent scope, as ld_dev).
@@ -113,30 +114,49 @@ template <int kL>
 struct PagedSpan {
   PagedDeal<kL> deal;
   int at, end, b, hh, n, first;
+  bool alone;  // a wave for each pair instead
 };
 
-// Quanta of the first `count` sequences, for one KV head and head tile.
+// Quanta of the first `count` sequences, for one KV head and head tile; `longest`
+// is raised to their longest.
 template <int kL>
-__device__ __forceinline__ int quanta_before(const PagedAttend& a, int count) {
-  int sum = 0;
+__device__ __forceinline__ int quanta_before(const PagedAttend& a, int count, int& longest) {
+  int sum = 0, most = 0;
 #pragma unroll 4
-  for (int i = threadIdx.x & 63; i < count; i += 64) sum += quanta_of<kL>(clamp_length(a, a.lengths[i]));
+  for (int i = threadIdx.x & 63; i < count; i += 64) {
+    const int n = clamp_length(a, a.lengths[i]);
+    sum += quanta_of<kL>(n);
+    most = max(most, n);
+  }
+  most = (int)wave_max((float)min(most, 1 << 20));  // (exact as far as it matters)
+  longest = max(longest, most);
   return wave_sum_i(sum);
+}
+
+// Many short pairs: a wave for each by itself, where a workgroup for each would
+// take them one after another and leave most of its waves without a tile (256
+// sequences of 100 tokens, 8 heads: 23.8 us, 42.8 by workgroups; 128 of 500 44.5
+// and 51.4; with fewer pairs, or longer ones, the workgroups are as fast or faster:
+// 256 pairs of 250 11.2 us against 14.6, 512 of 1000 46 against 116).
+constexpr int kSoloTokens = 512, kSoloPairs = 512;
+__device__ __forceinline__ bool pairs_alone(const PagedAttend& a, int longest) {
+  return a.many && longest <= kSoloTokens;
 }
 
 // Every wave finds its workgroup's share by itself (uniform; two loads of the
 // lengths and a lane scan for every 64 sequences), so that a long sequence among
 // short ones is spread over as many workgroups as its share of the rows.
-template <int kL>
+template <int kL, bool kMany>
 __device__ __forceinline__ PagedSpan<kL> find_span(const PagedAttend& a, int unit) {
   const int lane = threadIdx.x & 63, heads = a.kv_heads * a.tiles;
   auto length = [&](int i) { return i < a.sequences ? clamp_length(a, a.lengths[i]) : 0; };
-  int n = length(lane);
+  int n = length(lane), longest = 0;
   PagedSpan<kL> u;
-  u.deal.total = quanta_before<kL>(a, a.sequences) * heads;
+  u.deal.total = quanta_before<kL>(a, a.sequences, longest) * heads;
+  u.alone = kMany && pairs_alone(a, longest);
   u.at = u.deal.begin(unit);
   u.end = u.deal.begin(unit + 1);
-  if (u.at >= u.end) return u;
+  if (u.alone || u.at >= u.end) return u;
   const int to = u.at / heads;  // (a sequence's quanta begin at a multiple of heads)
   int base = 0;
   for (int i = 0;; i += 64) {  // (`to` lies in some sequence)

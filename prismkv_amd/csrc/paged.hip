@@ -365,7 +365,7 @@ struct Rows<DT, D, false> {
 
 // `count` quanta of one pair from its quantum u.first on: this workgroup's state
 // of them, and the pair's output if it is the only or the last to come.
-template <int DT, int D, bool kAligned>
+template <int DT, int D, bool kAligned, bool kMany>
 __device__ __forceinline__ void attend_segment(const PagedAttend& a, const PagedSpan<kLeast<DT, D>>& u, int quanta, int count, float* lds) {
   typedef Tile<DT, D> T;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
@@ -373,6 +373,9 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   const int h = u.hh / a.tiles, g0 = 16 * (u.hh - h * a.tiles);
   const int rows = min(a.group - g0, 16);  // query heads of this tile
   const int start = min(u.first * kQuantum, u.n), end = min(start + count * kQuantum, u.n);
+  // (a pair alone: all tiles are this wave's)
+  const bool alone = kMany && u.alone;
+  const int step = alone ? T::kTokens : kAWaves<D> * T::kTokens;
 
   // Q^T: column j is head j (zero past the tile's heads)
   u32x4 qop[T::kKLoads];
@@ -397,19 +400,18 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   // requested as soon as this one's are used up by the scores, its values after
   // the products with this one's, and the pages of the tile after that in
   // between (memory answers in order: whatever is waited for was asked first).
-  constexpr int kStep = kAWaves<D> * T::kTokens;
-  int t0 = start + T::kTokens * w;
+  int t0 = start + (alone ? 0 : T::kTokens * w);
   T t;
   if (t0 < end) {
     rows_of.ask(t0);
     rows_of.move();
     rows_of.load_k(t);
-    rows_of.ask(t0 + kStep);
+    rows_of.ask(t0 + step);
     rows_of.load_v(t);
   }
   // (the loads of the tile behind the last are issued too: on every path as many
   // are in flight, so that the compiler's wait counts are exact)
-  for (; t0 < end; t0 += kStep) {
+  for (; t0 < end; t0 += step) {
     // scores: lane (j, q) gets tokens 16i + 4q + r of head j
     float s[T::kBlocks][4];
     float bm = -INFINITY;
@@ -439,7 +441,7 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
     }
     rows_of.move();
     rows_of.load_k(t);
-    rows_of.ask(t0 + 2 * kStep);
+    rows_of.ask(t0 + 2 * step);
     bm = fmaxf(bm, xor16(bm));
     bm = fmaxf(bm, xor32(bm));
     if (__ballot(bm > m)) {
@@ -502,12 +504,24 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   }
   if (__ballot(rows_of.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
 
+  z += xor16(z);
+  z += xor32(z);
+  const size_t head0 = ((size_t)u.b * a.kv_heads + h) * a.group + g0;  // this tile's first query head
+  if (alone) {  // lane (j, q) has dims dim(n, j) of heads 4q + r
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float M = __shfl(m, 4 * q + r), den = __shfl(z, 4 * q + r);
+      if (4 * q + r < rows) {
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) finish<DT, D>(a, head0, (4 * q + r) * D + T::dim(n, j), M, den, acc[n][r]);
+      }
+    }
+    return;
+  }
   // the waves' states meet in LDS
   float* sm = lds;  // [waves][16] maxima
   float* sz = sm + 16 * kAWaves<D>;   // [waves][16] sums
   float* sacc = sz + 16 * kAWaves<D>; // [waves][rows][D]
-  z += xor16(z);
-  z += xor32(z);
   if (lane < 16) {
     sm[16 * w + j] = m;
     sz[16 * w + j] = z;
@@ -521,7 +535,6 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
         *reinterpret_cast<float4*>(dst + T::dim(n, j)) = make_float4(acc[n][r], acc[n + 1][r], acc[n + 2][r], acc[n + 3][r]);
     }
   __syncthreads();
-  const size_t head0 = ((size_t)u.b * a.kv_heads + h) * a.group + g0;  // this tile's first query head
   const int pair0 = u.at - u.first, unit = (int)blockIdx.x;
   const bool whole = count == quanta;
   float* state = a.state + (size_t)(2 * unit + (u.at != u.deal.begin(unit))) * a.state_stride;  // {max, sum}[rows], [rows][D]
@@ -564,14 +577,30 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   join_states<DT, D, 64 * kAWaves<D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
 }
 
-template <int DT, int D, bool kAligned>
+template <int DT, int D, bool kAligned, bool kMany>
 __global__ __launch_bounds__(64 * kAWaves<D>, kAWaves<D> / 4) void paged_attend_kernel(PagedAttend a) {
   extern __shared__ float lds[];
-  PagedSpan<kLeast<DT, D>> u = find_span<kLeast<DT, D>>(a, blockIdx.x);
+  constexpr int kL = kLeast<DT, D>;
+  PagedSpan<kL> u = find_span<kL, kMany>(a, blockIdx.x);
+  if constexpr (kMany) {
+    if (u.alone) {
+      const int heads = a.kv_heads * a.tiles;
+      u.first = 0;
+      for (int pair = blockIdx.x + gridDim.x * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); pair < a.sequences * heads;
+           pair += gridDim.x * kAWaves<D>) {
+        u.b = pair / heads;
+        u.hh = pair - u.b * heads;
+        u.n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[u.b]));
+        const int quanta = quanta_of<kL>(u.n);
+        attend_segment<DT, D, kAligned, kMany>(a, u, quanta, quanta, lds);
+      }
+      return;
+    }
+  }
   while (u.at < u.end) {  // the pairs that this workgroup's share lies in
-    const int quanta = quanta_of<kLeast<DT, D>>(u.n);
+    const int quanta = quanta_of<kL>(u.n);
     const int count = min(quanta - u.first, u.end - u.at);
-    attend_segment<DT, D, kAligned>(a, u, quanta, count, lds);
+    attend_segment<DT, D, kAligned, kMany>(a, u, quanta, count, lds);
     u.at += count;
     u.first = 0;
     if (++u.hh == a.kv_heads * a.tiles) {
@@ -594,8 +623,10 @@ __global__ __launch_bounds__(kPT) void paged_join_kernel(PagedAttend a) {
   const int rows = min(a.group - 16 * tile, 16), col0 = blockIdx.x * kJoinColumns;
   if (col0 >= rows * D / 4) return;
   constexpr int kL = kLeast<DT, D>;
-  const PagedDeal<kL> deal{quanta_before<kL>(a, a.sequences) * a.kv_heads * a.tiles};
-  const int from = quanta_before<kL>(a, b), n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[b]));
+  int longest = 0;
+  const PagedDeal<kL> deal{quanta_before<kL>(a, a.sequences, longest) * a.kv_heads * a.tiles};
+  if (pairs_alone(a, longest)) return;
+  const int from = quanta_before<kL>(a, b, longest), n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[b]));
   const int quanta = quanta_of<kL>(n);
   const PagedParts parts(deal, from * a.kv_heads * a.tiles + (int)blockIdx.y * quanta, quanta);
   if (parts.chunks == 1) return;  // its workgroup has finished it
@@ -1387,14 +1418,15 @@ EvictLayout evict_layout(int sequences, int kv_heads, int64_t slots) {
   return w;
 }
 
-template <int DT, int D, bool kAligned>
+template <int DT, int D, bool kAligned, bool kMany>
 int launch_attend_rows(const PagedAttend& a, int64_t units, int lds, hipStream_t stream) {
+  const auto kernel = paged_attend_kernel<DT, D, kAligned, kMany>;
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_attend_kernel<DT, D, kAligned>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL((paged_attend_kernel<DT, D, kAligned>), dim3((unsigned)units), dim3(64 * kAWaves<D>), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(64 * kAWaves<D>), lds, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -1414,8 +1446,10 @@ int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
   if (apart) a.counters = nullptr;
   // a lane's offset within a block is 32 bits
   const bool aligned = a.page_size % 16 == 0 && a.slot_units < (1u << 23);
-  const int rc = aligned ? launch_attend_rows<DT, D, true>(a, units, lds, stream)
-                         : launch_attend_rows<DT, D, false>(a, units, lds, stream);
+  a.many = (int64_t)a.sequences * a.kv_heads * a.tiles >= kSoloPairs;
+  const auto launch = aligned ? a.many ? launch_attend_rows<DT, D, true, true> : launch_attend_rows<DT, D, true, false>
+                              : a.many ? launch_attend_rows<DT, D, false, true> : launch_attend_rows<DT, D, false, false>;
+  const int rc = launch(a, units, lds, stream);
   if (rc || !apart) return rc;
   hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3((rows * D / 4 + kJoinColumns - 1) / kJoinColumns,
                      a.kv_heads * a.tiles, a.sequences), dim3(kPT), (4 * kPT + sums) * (int)sizeof(float), stream, a);

@@ -549,6 +549,36 @@ def test_many_sequences():
     check_attend(q[pick], few, [lengths[b] for b in pick], out[pick])
 
 
+@pytest.mark.parametrize("kv_heads,group,dim,page,dtype", [(1, 17, 64, 16, BF16), (2, 4, 128, 16, FP16), (1, 3, 256, 24, BF16),
+                                                           (2, 16, 128, 7, FP32), (3, 1, 256, 32, FP32)])
+def test_many_short_sequences(kv_heads, group, dim, page, dtype):
+    """A wave for each pair: up to 512 tokens, 512 pairs or more; as soon as one
+    sequence is longer, workgroups again, with the same bounds."""
+    lengths = [(37 * b) % 513 for b in range(520 // kv_heads)]
+    lengths[-1], lengths[100] = 512, 0
+    cache, host = make(lengths, kv_heads, dim, page, dtype, room=1, scored=True)
+    q = queries(cache, group)
+    pick = [0, 1, 2, 99, 100, 101, 120, len(lengths) - 1]
+    few = dict(host, table=host["table"][pick])
+    for longest in (512, 513):
+        fork = cache.fork()
+        fork.scores.fill_(-7.0)
+        cache.scores.zero_()
+        lse = torch.zeros(q.shape[:2], device="cuda")
+        if longest == 513:  # (one more token: a row of zeros)
+            at = host["table"][-1, 512 // page]
+            for x in (cache.k, cache.v, few["k"], few["v"]):
+                x[at, :, 512 % page] = 0
+            cache.lengths[-1] = 513
+            lengths[-1] = 513
+        out = cache.attend(q.cuda(), accumulate=True, lse=lse, into=fork)
+        check_attend(q[pick], few, [lengths[b] for b in pick], out[pick], fork.scores[pick].cpu(), lse[pick].cpu())
+        for b in pick:
+            assert (fork.scores[b, :, lengths[b]:] == -7).all()
+        assert torch.equal(bits(cache.attend(q.cuda())), bits(out))
+    cache.check_errors()
+
+
 @pytest.mark.parametrize("dim,group,dtype", [(128, 16, BF16), (256, 16, FP16), (128, 16, FP32), (64, 40, BF16)])
 def test_wide_calls_in_a_graph(dim, group, dtype):
     """The calls that take most LDS and a second launch, captured."""
