@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections import deque
 
 import torch
 
@@ -45,6 +46,36 @@ def _i32(x, shape, device, what):
     _check(isinstance(x, torch.Tensor) and x.dtype == torch.int32 and tuple(x.shape) == shape and x.is_contiguous()
            and x.device == device, f"{what} must be a contiguous int32 {list(shape)} on the cache's device")
     return x
+
+
+class _ErrorWord:
+    """A cache's (and its forks') error word, in pinned host memory that the
+    kernels write and a call reads without a tensor operation: 16 bytes of a
+    page of them, since pinning memory for each takes longer than the rest of a
+    cache's set-up.  Given back when the last of the caches is gone, behind all
+    that are free."""
+
+    free: dict = {}  # device index -> words
+    pages: list = []
+
+    def __init__(self, lib, device):
+        self.home = self.free.setdefault(device.index, deque())
+        if not self.home:
+            with torch.cuda.device(device):
+                page = torch.zeros(256, 4, dtype=torch.int32, pin_memory=True)
+                address = lib.query("prismkv_mapped_pointer", page.data_ptr())
+            if not address:
+                raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")
+            self.pages.append(page)
+            self.home.extend((address + 16 * i, page.data_ptr() + 16 * i) for i in range(256))
+        self.slot = self.home.popleft()
+        self.address = self.slot[0]
+        self.word = ctypes.c_int32.from_address(self.slot[1])
+        self.word.value = 0
+
+    def __del__(self):
+        if hasattr(self, "slot"):
+            self.home.append(self.slot)
 
 
 class PagedCache:
@@ -134,20 +165,10 @@ class PagedCache:
         self._shape = (sequences, kv_heads, head_dim, page_size, max_pages)
         self._free = self._pages = None
         self._attend_work, self._evict_work = {}, None
-        if err is None:
-            with torch.cuda.device(self.device):
-                # the error word, with the address of a host-mapped one that the next call reads
-                host = torch.zeros(4, dtype=torch.int32, pin_memory=True)
-                address = self.lib.query("prismkv_mapped_pointer", host.data_ptr())
-                if not address:
-                    raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")
-                err = torch.zeros(2, dtype=torch.int64, device=self.device)
-                err[1] = address
-            err = (err, host, ctypes.c_int32.from_address(host.data_ptr()))
-        self._err = err
+        self._err = _ErrorWord(self.lib, self.device) if err is None else err
         # what the C entries read of the cache; its tensors are fixed from here on
         pointers = [0 if x is None else x.data_ptr() for x in self._tensors]
-        self._desc = _lib.PagedCacheDesc(*pointers, err[0].data_ptr(), pages, *k.stride()[:3], *self._shape,
+        self._desc = _lib.PagedCacheDesc(*pointers, self._err.address, pages, *k.stride()[:3], *self._shape,
                                          DTYPES[k.dtype])
         self._pointer = ctypes.c_void_p(ctypes.addressof(self._desc))
 
@@ -247,14 +268,10 @@ class PagedCache:
         the results since the last check are invalid.  Reads a host-mapped word
         (no synchronisation, launches that have not run yet are not seen) and
         clears it."""
-        err, host, word = self._err  # (word: host's first element, read without a tensor operation)
-        code = word.value
+        code = self._err.word.value
         if code:
-            with torch.cuda.device(self.device):
-                torch.cuda.synchronize()
-                err[:1].zero_()
-                host.zero_()
-                torch.cuda.synchronize()
+            torch.cuda.synchronize(self.device)
+            self._err.word.value = 0
             raise RuntimeError(f"paged cache: {ERROR_MESSAGES.get(code, code)}; the results of the launches since the "
                                "last check are invalid")
 
