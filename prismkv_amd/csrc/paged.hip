@@ -31,9 +31,9 @@ namespace {
 // order of arrival.
 //
 // Measured (MI355X, launches after one another in a graph): 65792 tokens, 8 x 4
-// heads, bf16, 47.8 us = 5.6 TB/s; 32 sequences of 6.4K tokens 136 us = 6.2 TB/s
+// heads, bf16, 47.5 us = 5.7 TB/s; 32 sequences of 6.4K tokens 136 us = 6.2 TB/s
 // (a plain read of as much memory reaches 6.9); 16 x 8192 of head_dim 256 in fp32
-// 93 us = 5.8; of head_dim 64 50 us = 5.3; 75 tokens 6.7 us.  About 6 us of a call
+// 93 us = 5.8; of head_dim 64 50 us = 5.3; 75 tokens 6.6 us.  About 6 us of a call
 // are the launch and the chain lengths -> page -> rows, 4 more the join.
 
 // 16-bit types: P is a head and a remainder of the type (two products into one
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(kPT) void paged_weigh_kernel(PagedAttend a) {
 // of its rows (one of a sequence each, or kAppendRows packed ones) with a thread
 // per row, then copies them with 16 bytes per thread, kU loads each of K and V in
 // flight.  20011 rows of 8 heads and 128 dims in bf16 (164 MB read and written):
-// 31.7 us = 5.2 TB/s (a copy as large: 32.2); 128 single rows 3.4 us.
+// 31.7 us = 5.2 TB/s (a copy as large: 32.2); 128 single rows 3.5 us.
 
 constexpr int kAppendRows = 8;
 
@@ -1314,7 +1314,7 @@ __global__ __launch_bounds__(kET) void paged_pick_kernel(PagedEvict a) {
 
 // Moves the kept rows into the holes where the selection has not: a copy, bound by
 // the rows it reads and writes.  No source is another move's destination.  100 MB
-// of 256-byte rows read and written: 23 us = 4.4 TB/s (4 or 8 rows in flight per
+// of 256-byte rows read and written: 23.5 us = 4.4 TB/s (4 or 8 rows in flight per
 // thread: fewer workgroups, and 1 to 4 us more).
 constexpr int kMoveRows = 2;
 
