@@ -50,7 +50,8 @@ struct PagedAttend {
   const float* scores;  // weigh: the scores read and written, or null
   float *scores_out, *lse_out;
   void* out;
-  float *logits, *lse_work, *state;  // workspace: unscaled scores and log-sums (to be weighed), partial states
+  float *logits, *state;  // workspace: unscaled scores (to be weighed), partial states
+  float2* sums_work;      // workspace: each softmax's maximum and its sum's reciprocal (to be weighed)
   unsigned *counters, *err;          // counters: null where a second launch joins the states
   int64_t head_bytes, logit_stride, slots;
   unsigned page_units, slot_units, state_stride;  // 16-byte units; floats per partial state
@@ -182,7 +183,7 @@ __device__ __forceinline__ PagedSpan<kL> find_span(const PagedAttend& a, int uni
 // log2 of a softmax's sum from its maximum and the sum held times 2^kBias.
 template <int DT>
 __device__ __forceinline__ float log_sum(float M, float den) {
-  return den == 0.f ? -INFINITY : M + log2f(den) - kBias<DT>;
+  return den == 0.f ? -INFINITY : M + (log2f(den) - kBias<DT>);
 }
 
 // Writes output element i (query head i / D of the tile, dim i % D) from the
@@ -195,9 +196,10 @@ __device__ __forceinline__ void finish(const PagedAttend& a, size_t head0, int i
   else if constexpr (DT == kFp16) reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)y;
   else reinterpret_cast<float*>(a.out)[at] = y;
   if (i % D == 0) {
-    const float l2 = log_sum<DT>(M, den);
-    if (a.lse_out) a.lse_out[head0 + i / D] = l2 * 0.693147180559945309f;
-    if (a.lse_work) a.lse_work[head0 + i / D] = l2;
+    if (a.lse_out) a.lse_out[head0 + i / D] = log_sum<DT>(M, den) * 0.693147180559945309f;
+    if (a.sums_work)
+      a.sums_work[head0 + i / D] =
+          den == 0.f ? make_float2(0.f, 0.f) : make_float2(M, (float)(1 << kBias<DT>) / den);
   }
 }
 

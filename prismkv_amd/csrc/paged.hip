@@ -139,10 +139,16 @@ __device__ __forceinline__ void pv_columns(f32x4 (&acc)[D / 16], const Tile<DT, 
   }
 }
 
-// 2^(scale s - m): one rounding of the difference, however large the two are.  m
-// is finite or +infinity (no_less): where no score is above -infinity, 0 serves.
+// 2^(scale s - m): one rounding of the difference.  m is a rounded product itself;
+// from 2^22 on, where its rounding is 1/8 and more (and at 2^32 takes all of the
+// exponent's range), the other products are rounded as it was, so that the largest
+// score's weight is 1.  m is finite or +infinity (no_less): where no score is above
+// -infinity, 0 serves.
 __device__ __forceinline__ float weight(float s, float scale, float m) {
-  return __builtin_amdgcn_exp2f(fmaf(s, scale, -m));
+#pragma clang fp contract(off)
+  const float product = s * scale;
+  const float rounded = product - m;
+  return __builtin_amdgcn_exp2f(fabsf(m) < 0x1p22f ? fmaf(s, scale, -m) : rounded);
 }
 __device__ __forceinline__ float no_less(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -633,29 +639,31 @@ __global__ __launch_bounds__(kPT) void paged_join_kernel(PagedAttend a) {
   join_states<DT, D, kPT>(a, ((size_t)b * a.kv_heads + h) * a.group + 16 * tile, rows, parts, col0, kJoinColumns, lds);
 }
 
-// scores_out[t] = scores[t] + sum over the group's heads of e^(s_t - lse): a
-// thread per slot; bound by the scores that it reads (4 bytes per query head and
+// scores_out[t] = scores[t] + sum over the group's heads of its weight, from their
+// maxima and sums as the attention had them (a log-sum's rounding, 2^-24 of it, would
+// be the weights' error: 4e-4 at scores of 2e4): a thread per slot; bound by the scores that it reads (4 bytes per query head and
 // slot) and the two score arrays.
 __global__ __launch_bounds__(kPT) void paged_weigh_kernel(PagedAttend a) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int n = clamp_length(a, a.lengths[b]);
-  const float* lse = a.lse_work + ((size_t)b * a.kv_heads + h) * a.group;
+  const float2* sums = a.sums_work + ((size_t)b * a.kv_heads + h) * a.group;
   const float* logits = a.logits + ((size_t)b * a.kv_heads + h) * a.group * a.logit_stride;
   const size_t at = ((size_t)b * a.kv_heads + h) * a.slots;
   for (int t = blockIdx.x * kPT + threadIdx.x; t < n; t += gridDim.x * kPT) {
     const float before = a.scores[at + t];
     float sum = 0.f;
     for (int g0 = 0; g0 < a.group; g0 += 4) {  // (four heads' loads together)
-      float s[4], l[4];
+      float s[4];
+      float2 z[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int g = min(g0 + e, a.group - 1);
         s[e] = logits[(size_t)g * a.logit_stride + t];
-        l[e] = lse[g];
+        z[e] = sums[g];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (g0 + e < a.group) sum += weight(s[e], a.scale, no_less(l[e]));
+        if (g0 + e < a.group) sum = fmaf(weight(s[e], a.scale, z[e].x), z[e].y, sum);
     }
     a.scores_out[at + t] = before + sum;
   }
@@ -1375,7 +1383,7 @@ int check_cache(const prismkv_paged_cache* cache, const prismkv_paged_cache* int
 }
 
 struct WorkLayout {
-  size_t lse, state, logits, bytes;  // counters first
+  size_t sums, state, logits, bytes;  // counters first
   unsigned state_stride;
   int64_t logit_stride, quanta, units;
 };
@@ -1390,8 +1398,8 @@ WorkLayout attend_layout(int sequences, int kv_heads, int group, int head_dim, i
   w.state_stride = (unsigned)((group < 16 ? group : 16) * (head_dim + 2));
   w.logit_stride = (slots + 31) & ~31ll;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  w.lse = up((size_t)sequences * heads * sizeof(unsigned));
-  w.state = w.lse + up((size_t)sequences * kv_heads * group * sizeof(float));
+  w.sums = up((size_t)sequences * heads * sizeof(unsigned));
+  w.state = w.sums + up((size_t)sequences * kv_heads * group * sizeof(float2));
   w.logits = w.state + up((size_t)2 * w.units * w.state_stride * sizeof(float));
   w.bytes = w.logits + (weigh ? (size_t)sequences * kv_heads * group * w.logit_stride * sizeof(float) : 0);
   return w;
@@ -1500,7 +1508,7 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   if (weigh) {
     a.scores = reinterpret_cast<const float*>(c.scores);
     a.scores_out = reinterpret_cast<float*>(into->scores);
-    a.lse_work = reinterpret_cast<float*>(work + w.lse);
+    a.sums_work = reinterpret_cast<float2*>(work + w.sums);
     a.logits = reinterpret_cast<float*>(work + w.logits);
   }
   a.err = reinterpret_cast<unsigned*>(c.err);

@@ -144,6 +144,46 @@ def test_attend_peaked_and_wide_scores(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attend_scores_of_large_size(dtype, page):
+    """Scores far above 2^24, where the rounding of score times scale is itself
+    many units: the largest one's slot still has all the weight, once."""
+    lengths, dim, group = [250, 65], 64, 3
+    cache, host = make(lengths, 1, dim, page, dtype, scored=True)
+    gen = torch.Generator().manual_seed(3)
+    sign = torch.where(torch.rand(dim, generator=gen) < 0.5, -1.0, 1.0)
+    first, last = [], []  # the slots of the smallest and largest score
+    for b, n in enumerate(lengths):
+        size = 1 + torch.randperm(n, generator=gen)  # (integers below 256: exact in every type)
+        for t in range(n):
+            host["k"][host["table"][b, t // page], 0, t % page] = (sign * size[t]).to(dtype)
+        first.append(int(size.argmin()))
+        last.append(int(size.argmax()))
+    cache.k.copy_(host["k"])
+    q = sign.expand(2, group, dim).contiguous().to(dtype)  # scores 64 * size, exact in fp32
+    eps = {BF16: 2.0 ** -8, FP16: 2.0 ** -11, FP32: 2.0 ** -24}[dtype]
+    lse = torch.zeros(2, group, device="cuda")
+    for power in (3, 9, 12, 15, 17, 20, 22, 27, 31, 60, 100):
+        for factor in (0.1234, 0.777, 1.3, -0.9173):
+            # (neighbouring scores lie 64 * 8 * 0.12 apart at least: e^-63 to 1)
+            scale = factor * 2.0 ** power
+            cache.scores.zero_()
+            out = cache.attend(q.cuda(), scale=scale, accumulate=True, lse=lse).cpu().double()
+            for b, n in enumerate(lengths):
+                at = last[b] if scale > 0 else first[b]
+                want = host["v"][host["table"][b, at // page], 0, at % page].double()
+                # the rounding to the type, and four in 32 bits (two products, their sum, the quotient)
+                assert ((out[b] - want).abs() <= want.abs() * (eps + 2.0 ** -21)).all(), (scale, b)
+                weights = cache.scores[b, 0, :n].cpu().double()
+                assert abs(float(weights[at]) - group) <= group * 2.0 ** -21, (scale, b)
+                weights[at] = 0
+                assert (weights <= group * 2.0 ** -60).all(), (scale, b)
+                top = 64 * (n if scale > 0 else 1) * scale
+                # five roundings: the scale's, the product's, the sum's, and with ln 2 two
+                assert ((lse[b].cpu().double() - top).abs() <= abs(top) * 2.0 ** -21).all(), (scale, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 def test_attend_infinities(dtype):
     """An infinite value is the output's where its slot has weight; -infinite
     scores have none; NaN reaches the outputs of its own sequence only."""
