@@ -3,8 +3,9 @@ the routed one: `PagedCache.append` writes new rows, `attend` runs one new
 query token of every sequence over its pages, and `evict` bounds a cache by
 accumulated attention weight.  No counterpart in the reference.
 
-Any head layout with head_dim 64, 128 or 256 (NotImplementedError otherwise),
-bf16, fp16 or fp32.  As for `Native8B`: validation happens on the host before
+Any head layout with head_dim 64, 128 or 256 in bf16, fp16 or fp32, and up to 64
+GiB each of k and v pages (NotImplementedError otherwise); for inference, without
+gradients.  As for `Native8B`: validation happens on the host before
 anything is enqueued (ValueError), calls go to the current stream of the
 cache's device, never synchronise and can be captured into a HIP graph after
 one eager call has made their workspaces; lengths and page table are read on
@@ -106,6 +107,8 @@ class PagedCache:
         shape = (int(pages), int(kv_heads), int(page_size), int(head_dim))
         slots = int(max_pages) * int(page_size)
         _check_slots(int(sequences), slots)
+        if math.prod(shape) * dtype.itemsize > 1 << 36:
+            raise NotImplementedError("pages that span at most 64 GiB (of k, and of v)")
         k = torch.zeros(shape, dtype=dtype, device=device)
         v = torch.zeros(shape, dtype=dtype, device=device)
         table = torch.full((int(sequences), int(max_pages)), -1, dtype=torch.int32, device=device)
@@ -142,6 +145,8 @@ class PagedCache:
                "K/V rows must be 16-byte aligned")
         _check(k.stride(2) >= head_dim and (pages == 1 or k.stride(0) >= head_dim) and
                (kv_heads == 1 or k.stride(1) >= head_dim), "K/V rows must not overlap")
+        if max(pages * k.stride(0), (pages - 1) * k.stride(0) + page_size * k.stride(2)) * es > 1 << 36:
+            raise NotImplementedError("pages that span at most 64 GiB (of k, and of v)")
         _check(table.dim() == 2 and min(table.shape) >= 1, "an int32 page table [sequences, max_pages] required")
         sequences, max_pages = table.shape
         slots = max_pages * page_size

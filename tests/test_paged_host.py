@@ -112,6 +112,15 @@ def test_host_only_tensors_are_refused():
         PagedCache(0, 4, 4)
 
 
+def test_too_large_caches_are_refused():
+    """By the constructor, before anything is allocated: 2^25 pages of 16 x 128 bf16 rows."""
+    from prismkv_amd import PagedCache
+    with pytest.raises(NotImplementedError, match="64 GiB"):
+        PagedCache(1, 1 << 25, 1 << 10, page_size=16, kv_heads=1, device="cuda:0")
+    with pytest.raises(NotImplementedError, match="slots"):
+        PagedCache(1, 4, 1 << 27, page_size=16, kv_heads=1, device="cuda:0")
+
+
 def test_definition_of_attend():
     """The oracle's rows, weights and log-sum against softmax on gathered rows."""
     torch.manual_seed(0)
