@@ -36,10 +36,12 @@ namespace {
 // 93 us = 5.8; of head_dim 64 50 us = 5.3; 75 tokens 6.6 us.  About 6 us of a call
 // are the launch and the chain lengths -> page -> rows, 4 more the join.
 
-// 16-bit types: P is a head and a remainder of the type (two products into one
-// accumulator: about twice the type's significant bits).  The head is taken from
-// slightly below p, so that both are positive wherever p is and an infinite V
-// is not multiplied by a remainder of 0.
+// 16-bit types: P is a sum of terms of the type, each with a product of its own into
+// one accumulator: bf16 takes three, which hold all 24 bits of an fp32 p (with two,
+// outputs that cancel are off by 2^-17 of their terms; 65792 tokens, 8 x 4 heads take
+// as long with either), fp16 a head and a remainder (about twice its significant
+// bits).  Every term is positive wherever p is, so that an infinite V is not
+// multiplied by a term of 0.
 // The tile of one step as loaded.  16-bit (32 tokens, two 16-token blocks):
 // lane (j, q) holds row j of each block at dims 32c + 8q .. +8 (K, the A operand
 // of the 16x16x32 product) and of rows 4q + t (V) 16 bytes out of every 256 (8 of
@@ -113,29 +115,42 @@ __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// p as a head and a remainder of the 16-bit type.
+// p >= 0 as terms of the 16-bit type, each in the upper half of a word.
 template <int DT>
-__device__ __forceinline__ void split16(float p, unsigned& hi, unsigned& lo) {
+constexpr int kTerms = DT == kBf16 ? 3 : 2;
+template <int DT>
+__device__ __forceinline__ void split16(float p, unsigned (&term)[kTerms<DT>]) {
   if constexpr (DT == kBf16) {
-    const unsigned u = __float_as_uint(p * (1.f - 0x1p-9f)) & 0xffff0000u;
-    hi = u >> 16;
-    lo = f32_to_bf16(p - __uint_as_float(u));
+    // 8 bits each from the top, which is exact; at least the least bf16 number
+    // (as signed integers: a remainder below 0 behind a term that was raised to it).
+    // A NaN may be lost here: the sum of the weights has it.
+    const int least = p > 0.f ? 0x10000 : 0;
+    const int hi = max(__float_as_int(p) & (int)0xffff0000, least);
+    const float rest = p - __int_as_float(hi);
+    const int mid = max(__float_as_int(rest) & (int)0xffff0000, least);
+    term[0] = (unsigned)hi;
+    term[1] = (unsigned)mid;
+    term[2] = (unsigned)max(__float_as_int(rest - __int_as_float(mid)), least);
   } else {
     const _Float16 h = (_Float16)(p * (1.f - 0x1p-10f));
     const _Float16 l = (_Float16)(p - (float)h);
-    hi = __builtin_bit_cast(unsigned short, h);
-    lo = __builtin_bit_cast(unsigned short, l);
+    term[0] = (unsigned)__builtin_bit_cast(unsigned short, h) << 16;
+    term[1] = (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
   }
 }
 
+// The upper halves of two words (low half from a).
+__device__ __forceinline__ unsigned upper16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
 template <int N, int DT, int D>
-__device__ __forceinline__ void pv_columns(f32x4 (&acc)[D / 16], const Tile<DT, D>& t, u32x4 ph, u32x4 pl) {
+__device__ __forceinline__ void pv_columns(f32x4 (&acc)[D / 16], const Tile<DT, D>& t,
+                                           const u32x4 (&p)[kTerms<DT>]) {
   if constexpr (N < D / 16) {
     const u32x4 vb = {pair16<N>(t.v[0][0], t.v[0][1]), pair16<N>(t.v[0][2], t.v[0][3]),
                       pair16<N>(t.v[1][0], t.v[1][1]), pair16<N>(t.v[1][2], t.v[1][3])};
-    acc[N] = mfma32<DT>(ph, vb, acc[N]);
-    acc[N] = mfma32<DT>(pl, vb, acc[N]);
-    pv_columns<N + 1, DT, D>(acc, t, ph, pl);
+#pragma unroll
+    for (int i = 0; i < kTerms<DT>; ++i) acc[N] = mfma32<DT>(p[i], vb, acc[N]);
+    pv_columns<N + 1, DT, D>(acc, t, p);
   }
 }
 
@@ -490,14 +505,17 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
         for (int n = 0; n < D / 16; ++n)
           acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][r], __uint_as_float(t.v[0][r][n]), acc[n], 0, 0, 0);
     } else {
-      unsigned hi[8], lo[8];
+      unsigned term[8][kTerms<DT>];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) split16<DT>(p[i][r], hi[4 * i + r], lo[4 * i + r]);
-      const u32x4 ph = {hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, hi[4] | hi[5] << 16, hi[6] | hi[7] << 16};
-      const u32x4 pl = {lo[0] | lo[1] << 16, lo[2] | lo[3] << 16, lo[4] | lo[5] << 16, lo[6] | lo[7] << 16};
-      pv_columns<0, DT, D>(acc, t, ph, pl);
+        for (int r = 0; r < 4; ++r) split16<DT>(p[i][r], term[4 * i + r]);
+      u32x4 pw[kTerms<DT>];
+#pragma unroll
+      for (int k = 0; k < kTerms<DT>; ++k)
+        pw[k] = u32x4{upper16(term[0][k], term[1][k]), upper16(term[2][k], term[3][k]), upper16(term[4][k], term[5][k]),
+                      upper16(term[6][k], term[7][k])};
+      pv_columns<0, DT, D>(acc, t, pw);
     }
     rows_of.load_v(t);
     // behind the loads: memory answers stores in the same order, and what the next

@@ -1,0 +1,65 @@
+"""The paged cache where its operators are easily wrong: outputs that cancel,
+infinite values of little weight, wide page tables, shared buffers, the
+largest calls.  Bounds are derived beside each test."""
+import math
+
+import pytest
+import torch
+
+from prismkv_amd import PagedCache
+from tests.gpu_util import log
+from tests.test_gpu_paged import BF16, FP16, FP32, bits
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_outputs_that_cancel(dtype):
+    """Sums of p v that are near 0 beside their terms, where the output's own
+    rounding hides nothing: p is used with 32 bits in every type.
+
+    Four tokens a sequence, one query head to a KV head.  A score is one product
+    (the other dims of q are 0), exact in fp32, and the largest is 0.  A weight's
+    exponent has two roundings, the scale's and its own: with the exponential's,
+    2^-23, p is off by less than 2 * 2^-23 + 2^-23 < 2^-21 of itself where |s| <= 2, and
+    by 2^-19 for the token of 6.24, whose term is 2^-8 of the others at most.  As
+    the terms' sum is near 0 the denominator's error does not count.  p as terms of
+    the type is exact (three of bf16; fp32 itself) or off by 2^-23 (two of fp16).
+    The products are exact in fp32 and the first terms' sum takes four roundings,
+    of 2^-23 each where the matrix cores should truncate; the other terms add to
+    what that left, 2^-7 of it.  All together: (0.5 + 0.01 + 0.13 + 0.52) 2^-20 of
+    sum p |v|, held to 2^-19, and the output's own rounding."""
+    gen = torch.Generator().manual_seed(11)
+    sequences, heads, dim = 64, 4, 64
+    step = {BF16: 2.0 ** -8, FP16: 2.0 ** -11, FP32: 2.0 ** -24}[dtype]
+    # scores 0, two in [-2, 0], -6.24: one product each
+    s = torch.zeros(sequences, heads, 4, dtype=torch.float64)
+    s[:, :, 1:3] = -2 * torch.rand(sequences, heads, 2, generator=gen, dtype=torch.float64)
+    s[:, :, 3] = -6.24
+    k = torch.zeros(sequences, heads, 16, dim)
+    k[:, :, :4, 0] = s.float()
+    k = k.to(dtype)
+    q = torch.zeros(sequences, heads, dim, dtype=dtype)
+    q[:, :, 0] = 1
+    p = torch.exp(k[:, :, :4, 0].double())
+    p /= p.sum(-1, keepdim=True)
+    # values: two at random, then what cancels, rounded, and once more for the rest
+    v = torch.zeros(sequences, heads, 16, dim, dtype=dtype)
+    v[:, :, :2] = torch.randn(sequences, heads, 2, dim, generator=gen).to(dtype)
+    for t in (2, 3):
+        rest = (p[..., None] * v[:, :, :4].double()).sum(2)
+        v[:, :, t] = (-rest / p[:, :, t, None]).to(dtype)
+    want = (p[..., None] * v[:, :, :4].double()).sum(2)
+    spread = (p[..., None] * v[:, :, :4].double().abs()).sum(2)
+    assert (want.abs() * step < 2.0 ** -22 * spread).all()  # (they do cancel)
+    cache = PagedCache.from_tensors(k.cuda(), v.cuda(), torch.arange(sequences, dtype=torch.int32, device="cuda")[:, None],
+                                    i32(*[4] * sequences))
+    out = cache.attend(q.cuda(), scale=1.0).cpu().double()
+    smallest = {BF16: 2.0 ** -134, FP16: 2.0 ** -25, FP32: 2.0 ** -150}[dtype]  # half the least subnormal
+    error = (out - want).abs() / (spread * 2.0 ** -19 + want.abs() * step + smallest)
+    log("largest error over its bound", dtype, float(error.max()))
+    assert (error <= 1).all()
