@@ -21,8 +21,9 @@ def attend(q, k_pages, v_pages, table, lengths, scale=None):
     sum |q_i k_i| (the order is free; the 8 cover the scaling); with delta the
     largest such error of a head's scores, a weight is off by a factor within
     2 delta (its own and the denominator's) and the exponentials' and the
-    sums' own steps, 2^-20 + n 2^-24.  fp16 multiplies V with P as a head and a
-    remainder: 2^-15 at most (bf16 with three terms, which is exact)."""
+    sums' own steps, 2^-20 + n 2^-24.  bf16 multiplies V with P as three terms,
+    which is exact, fp16 as two, 2^-22 and, as each is 2^-39 of the largest weight
+    at least, 2^-38 |v| a slot."""
     B, heads, D = q.shape
     H = k_pages.shape[1]
     scale = 1 / math.sqrt(D) if scale is None else scale
@@ -46,10 +47,11 @@ def attend(q, k_pages, v_pages, table, lengths, scale=None):
         out = (p[:, :, None] * v).sum(1)
         rel = 2 * delta + 2.0 ** -20 + n * 2.0 ** -24
         spread = (p[:, :, None] * v.abs()).sum(1)
-        split = 2.0 ** -15 if q.dtype == torch.float16 else 0
+        split, least = (2.0 ** -22, 2.0 ** -38) if q.dtype == torch.float16 else (0, 0)
         # (a subnormal output is off by half of the type's smallest step)
         floor = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}[q.dtype]
-        out_bound = out.abs() * eps + spread * (rel[:, None] + split) * (1 + eps) + floor
+        lost = spread * (rel[:, None] + split) + least * (p.amax(-1)[:, None, None] * v.abs()).sum(1)
+        out_bound = out.abs() * eps + lost * (1 + eps) + floor
         group = heads // H
         weights = p.view(H, group, n).sum(1)
         weights_bound = (p * rel[:, None]).view(H, group, n).sum(1) + weights * (group + 2) * 2.0 ** -24

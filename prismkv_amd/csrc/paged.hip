@@ -39,9 +39,9 @@ namespace {
 // 16-bit types: P is a sum of terms of the type, each with a product of its own into
 // one accumulator: bf16 takes three, which hold all 24 bits of an fp32 p (with two,
 // outputs that cancel are off by 2^-17 of their terms; 65792 tokens, 8 x 4 heads take
-// as long with either), fp16 a head and a remainder (about twice its significant
-// bits).  Every term is positive wherever p is, so that an infinite V is not
-// multiplied by a term of 0.
+// as long with either), fp16 two, 22 bits.  Every term is positive wherever p is, so
+// that an infinite V is not multiplied by a term of 0: at least the type's least
+// number, which for fp16, with its bias, is 2^-39 of the maximum's weight.
 // The tile of one step as loaded.  16-bit (32 tokens, two 16-token blocks):
 // lane (j, q) holds row j of each block at dims 32c + 8q .. +8 (K, the A operand
 // of the 16x16x32 product) and of rows 4q + t (V) 16 bytes out of every 256 (8 of
@@ -115,15 +115,15 @@ __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// p >= 0 as terms of the 16-bit type, each in the upper half of a word.
+// p >= 0 as terms of the 16-bit type, each in the upper half of a word.  A NaN may be
+// lost here: the sum of the weights has it.
 template <int DT>
 constexpr int kTerms = DT == kBf16 ? 3 : 2;
 template <int DT>
 __device__ __forceinline__ void split16(float p, unsigned (&term)[kTerms<DT>]) {
   if constexpr (DT == kBf16) {
-    // 8 bits each from the top, which is exact; at least the least bf16 number
-    // (as signed integers: a remainder below 0 behind a term that was raised to it).
-    // A NaN may be lost here: the sum of the weights has it.
+    // 8 bits each from the top, which is exact (as signed integers: a remainder
+    // below 0 is left behind a term that was raised)
     const int least = p > 0.f ? 0x10000 : 0;
     const int hi = max(__float_as_int(p) & (int)0xffff0000, least);
     const float rest = p - __int_as_float(hi);
@@ -132,9 +132,11 @@ __device__ __forceinline__ void split16(float p, unsigned (&term)[kTerms<DT>]) {
     term[1] = (unsigned)mid;
     term[2] = (unsigned)max(__float_as_int(rest - __int_as_float(mid)), least);
   } else {
-    const _Float16 h = (_Float16)(p * (1.f - 0x1p-10f));
-    const _Float16 l = (_Float16)(p - (float)h);
-    term[0] = (unsigned)__builtin_bit_cast(unsigned short, h) << 16;
+    // the head rounded down, so that the remainder is positive
+    const float least = p > 0.f ? 0x1p-24f : 0.f, head = fmaxf(p, least);
+    const auto h = __builtin_amdgcn_cvt_pkrtz(0.f, head);  // {0, head}
+    const _Float16 l = (_Float16)fmaxf(head - (float)h[1], least);
+    term[0] = __builtin_bit_cast(unsigned, h);
     term[1] = (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
   }
 }

@@ -28,10 +28,10 @@ def test_outputs_that_cancel(dtype):
     2^-23, p is off by less than 2 * 2^-23 + 2^-23 < 2^-21 of itself where |s| <= 2, and
     by 2^-19 for the token of 6.24, whose term is 2^-8 of the others at most.  As
     the terms' sum is near 0 the denominator's error does not count.  p as terms of
-    the type is exact (three of bf16; fp32 itself) or off by 2^-23 (two of fp16).
+    the type is exact (three of bf16; fp32 itself) or off by 2^-22 (two of fp16).
     The products are exact in fp32 and the first terms' sum takes four roundings,
     of 2^-23 each where the matrix cores should truncate; the other terms add to
-    what that left, 2^-7 of it.  All together: (0.5 + 0.01 + 0.13 + 0.52) 2^-20 of
+    what that left, 2^-7 of it.  All together: (0.5 + 0.01 + 0.25 + 0.52) 2^-20 of
     sum p |v|, held to 2^-19, and the output's own rounding."""
     gen = torch.Generator().manual_seed(11)
     sequences, heads, dim = 64, 4, 64
@@ -63,3 +63,38 @@ def test_outputs_that_cancel(dtype):
     error = (out - want).abs() / (spread * 2.0 ** -19 + want.abs() * step + smallest)
     log("largest error over its bound", dtype, float(error.max()))
     assert (error <= 1).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("page", [16, 24])
+def test_infinite_values_of_little_weight(dtype, page):
+    """An infinite value is the output's wherever its slot has weight in 32 bits
+    (2^-126 of the largest and more), and changes no other dim.
+
+    The other dims: weight 1 and one of 2^-10 at most, the bounds of
+    test_outputs_that_cancel; fp16 terms no less than 2^-24 of 2^15 add
+    2 * 2^-39 |v|."""
+    powers = [10, 20, 29, 31, 36, 40, 45, 60, 100, 120]
+    dim = 64
+    gen = torch.Generator().manual_seed(4)
+    k, v = (torch.zeros(len(powers), 1, page, dim, dtype=dtype) for _ in range(2))
+    k[:, 0, 1, 0] = -math.log(2) * torch.tensor(powers).to(dtype)
+    v[:, 0, :2] = torch.randn(len(powers), 2, dim, generator=gen).to(dtype)
+    p = torch.exp(k[:, 0, :2, 0].double())
+    p /= p.sum(-1, keepdim=True)
+    want = (p[..., None] * v[:, 0, :2].double()).sum(1)
+    spread = (p[..., None] * v[:, 0, :2].double().abs()).sum(1)
+    v[:, 0, 1, 5], v[:, 0, 1, 40] = math.inf, -math.inf
+    q = torch.zeros(len(powers), 1, dim, dtype=dtype)
+    q[..., 0] = 1
+    cache = PagedCache.from_tensors(k.cuda(), v.cuda(), torch.arange(len(powers), dtype=torch.int32, device="cuda")[:, None],
+                                    i32(*[2] * len(powers)))
+    out = cache.attend(q.cuda(), scale=1.0).cpu()[:, 0].double()
+    assert (out[:, 5] == math.inf).all(), out[:, 5]
+    assert (out[:, 40] == -math.inf).all(), out[:, 40]
+    step = {BF16: 2.0 ** -8, FP16: 2.0 ** -11, FP32: 2.0 ** -24}[dtype]
+    smallest = {BF16: 2.0 ** -134, FP16: 2.0 ** -25, FP32: 2.0 ** -150}[dtype]
+    other = [d for d in range(dim) if d not in (5, 40)]
+    v_max = v[:, 0, :2, other].double().abs().amax()
+    bound = want.abs() * step + spread * 2.0 ** -19 + v_max * 2.0 ** -38 + smallest
+    assert ((out - want).abs() <= bound)[:, other].all()
