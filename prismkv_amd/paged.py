@@ -50,7 +50,7 @@ def _i32(x, shape, device, what):
 
 
 class _ErrorWord:
-    """A cache's (and its forks') error word, in pinned host memory that the
+    """A cache's (and its forks', and what it was resized to) error word, in pinned host memory that the
     kernels write and a call reads without a tensor operation: 16 bytes of a
     page of them, since pinning memory for each takes longer than the rest of a
     cache's set-up.  Given back when the last of the caches is gone, behind all
@@ -95,7 +95,7 @@ class PagedCache:
     scores and positions, so that a step can be taken back."""
 
     def __init__(self, sequences, pages, max_pages, *, page_size=64, kv_heads=8, head_dim=128, dtype=torch.bfloat16,
-                 scored=False, device="cuda", library=None):
+                 scored=False, device="cuda", library=None, _err=None):
         for value, what in ((sequences, "sequences"), (pages, "pages"), (max_pages, "max_pages"),
                             (page_size, "page_size"), (kv_heads, "kv_heads")):
             _check(int(value) >= 1, f"{what} must be positive")
@@ -118,7 +118,7 @@ class PagedCache:
             meta = dict(seen=torch.zeros_like(lengths),
                         scores=torch.zeros(int(sequences), int(kv_heads), slots, device=device),
                         positions=torch.zeros(int(sequences), int(kv_heads), slots, dtype=torch.int32, device=device))
-        self._setup(k, v, table, lengths, library=library, **meta)
+        self._setup(k, v, table, lengths, library=library, err=_err, **meta)
         self._free = list(range(int(pages)))[::-1]
         self._pages = [[] for _ in range(int(sequences))]
 
@@ -234,13 +234,14 @@ class PagedCache:
         this one's contents: per sequence its first max_pages pages, which the
         caller knows to hold its length, their scores and positions.  (A cut
         cache in the table of its longest prompt would keep that prompt's memory,
-        and its cuts the cost of that many slots.)"""
+        and its cuts the cost of that many slots.)  Reports of this cache's launches
+        go to it as well."""
         self._owns_pages()
         sequences, kv_heads, head_dim, page_size, _ = self._shape
         counts = [min(len(held), int(max_pages)) for held in self._pages]
         _check(sum(counts) <= int(pages), "the sequences' pages do not fit")
         new = PagedCache(sequences, pages, max_pages, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim,
-                         dtype=self.k.dtype, scored=self.scored, device=self.device, library=self.lib.path)
+                         dtype=self.k.dtype, scored=self.scored, device=self.device, library=self.lib.path, _err=self._err)
         new.reserve([count * page_size for count in counts])
         for held, own, count in zip(self._pages, new._pages, counts):
             new.k[own] = self.k[held[:count]]

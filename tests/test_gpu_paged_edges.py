@@ -98,3 +98,56 @@ def test_infinite_values_of_little_weight(dtype, page):
     v_max = v[:, 0, :2, other].double().abs().amax()
     bound = want.abs() * step + spread * 2.0 ** -19 + v_max * 2.0 ** -38 + smallest
     assert ((out - want).abs() <= bound)[:, other].all()
+
+
+def test_a_report_outlives_resizing():
+    """Rows dropped for want of a page are reported to the cache that takes
+    this one's place."""
+    for fork in (False, True):
+        cache = PagedCache(2, 8, 4, page_size=16, kv_heads=2, head_dim=64, scored=True)
+        cache.reserve([16, 0])
+        rows = torch.ones(20, 2, 64, dtype=BF16, device="cuda")
+        cache.append(rows, rows, i32(0, 16, 20), into=cache.fork() if fork else None)  # (the second sequence has no page)
+        cache = cache.resized(6, 3)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="has no page"):
+            cache.check_errors()
+        cache.check_errors()
+
+
+def test_resized():
+    """The contents of sequences of different page counts, and what runs on them."""
+    gen = torch.Generator().manual_seed(2)
+    lengths = [37, 0, 64, 5]
+    cache = PagedCache(4, 20, 8, page_size=16, kv_heads=2, head_dim=64, scored=True)
+    cache.reserve([50, 20, 64, 5])  # (more than the lengths)
+    rows = torch.randn(sum(lengths), 2, 64, generator=gen).bfloat16().cuda()
+    ends = i32(0, 37, 37, 101, 106)
+    cache.append(rows, -rows, ends)
+    q = torch.randn(4, 4, 64, generator=gen).bfloat16().cuda()
+    cache.attend(q, accumulate=True)
+    cache.release(1)
+    for pages, max_pages in ((9, 4), (30, 12)):
+        new = cache.resized(pages, max_pages)
+        assert new.k.shape[0] == pages and new.table.shape[1] == max_pages
+        assert (new.table >= 0).sum(1).tolist() == [4, 0, 4, 1]
+        used = new.table[new.table >= 0].tolist()
+        assert len(set(used)) == 9
+        for b, n in enumerate(lengths):
+            at = torch.arange(n, device="cuda")
+            place = [(c.table[b, at // 16].long(), at % 16) for c in (cache, new)]
+            for x, y in ((cache.k, new.k), (cache.v, new.v)):
+                assert torch.equal(bits(x[place[0][0], :, place[0][1]]), bits(y[place[1][0], :, place[1][1]]))
+            assert torch.equal(new.scores[b, :, :n], cache.scores[b, :, :n])
+            assert torch.equal(new.positions[b, :, :n], cache.positions[b, :, :n])
+        assert torch.equal(new.lengths, cache.lengths) and torch.equal(new.seen, cache.seen)
+        assert torch.equal(bits(new.attend(q)), bits(cache.attend(q)))
+        new.evict(20, recent=3)
+        old = cache.resized(20, 8)
+        old.evict(20, recent=3)
+        for b in range(4):
+            m = min(lengths[b], 20)
+            assert torch.equal(new.positions[b, :, :m], old.positions[b, :, :m])
+        new.check_errors()
+    with pytest.raises(ValueError, match="do not fit"):
+        cache.resized(8, 4)
