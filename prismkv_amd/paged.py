@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from collections import deque
 
 import torch
@@ -50,29 +51,45 @@ def _i32(x, shape, device, what):
 
 
 class _ErrorWord:
-    """A cache's (and its forks', and what it was resized to) error word, in pinned host memory that the
-    kernels write and a call reads without a tensor operation: 16 bytes of a
-    page of them, since pinning memory for each takes longer than the rest of a
-    cache's set-up.  Given back when the last of the caches is gone, behind all
-    that are free."""
+    """The error word of a cache, its forks and what it was resized to, in pinned
+    host memory that the kernels write and a call reads without a tensor operation:
+    16 bytes of a page of them, since pinning memory for each takes longer than the
+    rest of a cache's set-up.  Given back when the last of the caches is gone; as
+    launches that may write it can still be queued then, another cache gets it only
+    after the device has been waited for, once for every PER_PAGE words."""
 
-    free: dict = {}  # device index -> words
+    PER_PAGE = 256
+    homes: dict = {}  # device index -> (words that nothing enqueued writes, words given back)
     pages: list = []
+    lock = threading.Lock()  # for refilling (not for giving back, which the collector may do at any time)
 
     def __init__(self, lib, device):
-        self.home = self.free.setdefault(device.index, deque())
-        if not self.home:
-            with torch.cuda.device(device):
-                page = torch.zeros(256, 4, dtype=torch.int32, pin_memory=True)
-                address = lib.query("prismkv_mapped_pointer", page.data_ptr())
-            if not address:
-                raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")
-            self.pages.append(page)
-            self.home.extend((address + 16 * i, page.data_ptr() + 16 * i) for i in range(256))
-        self.slot = self.home.popleft()
+        fresh, self.home = self.homes.setdefault(device.index, (deque(), deque()))
+        while not hasattr(self, "slot"):
+            try:
+                self.slot = fresh.popleft()
+            except IndexError:
+                with self.lock:
+                    if not fresh:
+                        self._refill(lib, device, fresh, self.home)
         self.address = self.slot[0]
         self.word = ctypes.c_int32.from_address(self.slot[1])
         self.word.value = 0
+
+    @classmethod
+    def _refill(cls, lib, device, fresh, given_back):
+        count = len(given_back)
+        with torch.cuda.device(device):
+            if count >= cls.PER_PAGE and not torch.cuda.is_current_stream_capturing():
+                torch.cuda.synchronize(device)
+                fresh.extend(given_back.popleft() for _ in range(count))
+                return
+            page = torch.zeros(cls.PER_PAGE, 4, dtype=torch.int32, pin_memory=True)
+            address = lib.query("prismkv_mapped_pointer", page.data_ptr())
+        if not address:
+            raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")
+        cls.pages.append(page)
+        fresh.extend((address + 16 * i, page.data_ptr() + 16 * i) for i in range(cls.PER_PAGE))
 
     def __del__(self):
         if hasattr(self, "slot"):

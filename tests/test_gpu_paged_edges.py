@@ -151,3 +151,21 @@ def test_resized():
         new.check_errors()
     with pytest.raises(ValueError, match="do not fit"):
         cache.resized(8, 4)
+
+
+def test_more_caches_than_a_page_of_error_words():
+    """Made and let go one after another with work queued: a report reaches its own cache only."""
+    q = torch.zeros(1, 1, 64, dtype=BF16, device="cuda")
+    for i in range(700):
+        cache = PagedCache(1, 1, 1, page_size=16, kv_heads=1, head_dim=64)
+        if i % 3:
+            cache.reserve(1)
+        cache.lengths.fill_(1)
+        cache.attend(q)
+        if i % 50 < 3:
+            torch.cuda.synchronize()
+            if i % 3:
+                cache.check_errors()
+            else:
+                with pytest.raises(RuntimeError, match="has no page"):
+                    cache.check_errors()

@@ -188,3 +188,66 @@ def test_evict_session_on_host():
     assert torch.allclose(session._observed[0], whole, atol=1e-5)
     session.close()
     assert model.config._attn_implementation == "sdpa" and not session._observed
+
+
+@pytest.fixture
+def words(monkeypatch):
+    """_ErrorWord without a device: (made words' class, device, the synchronisations so far)."""
+    import contextlib
+    from prismkv_amd import paged as module
+    zeros, synced = torch.zeros, []
+    monkeypatch.setattr(torch, "zeros", lambda *a, pin_memory=False, **k: zeros(*a, **k))
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda d=None: synced.append(d))
+
+    class Lib:
+        def query(self, name, address):
+            return address
+
+    device = torch.device("cuda", 97)  # (no other test's)
+    return lambda: module._ErrorWord(Lib(), device), synced
+
+
+def test_error_words_are_used_again_only_behind_a_synchronisation(words):
+    """A launch still queued when its cache goes may write the word: it is another
+    cache's only after everything enqueued before has run."""
+    make, synced = words
+    retired = {}  # address -> synchronisations when it was given back
+    held = []
+    for i in range(3000):
+        word = make()
+        assert word.word.value == 0 and word.address not in [w.address for w in held]
+        if word.address in retired:
+            assert len(synced) > retired[word.address], i
+        word.word.value = 4  # (a late report)
+        held.append(word)
+        if len(held) > 5:
+            gone = held.pop(0)
+            retired[gone.address] = len(synced)
+            del gone
+    assert len(set(retired)) < 1000  # (they are used again)
+    assert len(synced) < 30
+
+
+def test_error_words_of_several_threads(words):
+    import threading
+    make, _ = words
+    problems = []
+
+    def run():
+        try:
+            for _ in range(2000):
+                word = make()
+                word.word.value = token = threading.get_ident() % 2 ** 30 + 1
+                if make().address == word.address or word.word.value != token:
+                    problems.append("a word of two caches")
+        except Exception as e:  # noqa: BLE001
+            problems.append(repr(e))
+
+    threads = [threading.Thread(target=run) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not problems
