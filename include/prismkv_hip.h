@@ -431,7 +431,7 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *            the optional host word's address, as in a workspace.
  * Results go to a second cache `into` over the same pages and table: the first
  * itself, or one whose lengths, seen, scores and positions do not overlap the
- * first's.  A page that belongs to several tables may be read, not written.
+ * first's (refused).  A page that belongs to several tables may be read, not written.
  * `paged_work` is scratch, 16-byte aligned, of the matching *_work_bytes for the
  * call's own sizes; its leading counters (prismkv_paged_attend: sequences *
  * kv_heads * ceil(group / 16) words, prismkv_paged_evict: sequences) must be zero

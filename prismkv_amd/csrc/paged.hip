@@ -1368,6 +1368,19 @@ PageDiv page_div(int page_size) {
 
 int element_bytes(int dtype) { return dtype == kFp32 ? 4 : 2; }
 
+// The second cache's lengths, tokens seen, scores and positions are all the first's or
+// lie apart from all of them: a launch reads the first's while it writes the second's.
+bool results_fit(const prismkv_paged_cache& c, const prismkv_paged_cache& to) {
+  if (to.lengths == c.lengths && to.seen == c.seen && to.scores == c.scores && to.positions == c.positions) return true;
+  const uint64_t few = 4ull * c.sequences, many = few * c.kv_heads * c.page_size * c.max_pages;
+  const uint64_t from[4] = {c.lengths, c.seen, c.scores, c.positions}, into[4] = {to.lengths, to.seen, to.scores, to.positions};
+  const uint64_t size[4] = {few, few, many, many};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j)
+      if (from[i] && into[j] && from[i] < into[j] + size[j] && into[j] < from[i] + size[i]) return false;
+  return true;
+}
+
 // The cache and where its results go, checked alike by every entry point: rows,
 // heads and pages lie at 16-byte multiples, and a page's last row within 2^32
 // 16-byte units.  0, or the code to return.
@@ -1399,7 +1412,7 @@ int check_cache(const prismkv_paged_cache* cache, const prismkv_paged_cache* int
     return kBadSize;
   const bool some = c.seen || c.scores || c.positions || to.seen || to.scores || to.positions;
   const bool all = c.seen && c.scores && c.positions && to.seen && to.scores && to.positions;
-  return some != all || (scored && !all) ? kBadSize : 0;
+  return some != all || (scored && !all) || !results_fit(c, to) ? kBadSize : 0;
 }
 
 struct WorkLayout {

@@ -17,6 +17,7 @@ sequence's length that has no page is reported at the next call
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 import threading
 from collections import deque
@@ -185,6 +186,10 @@ class PagedCache:
         self._tensors = (k, v, table, lengths, seen, scores, positions)
         self.device = k.device
         self._shape = (sequences, kv_heads, head_dim, page_size, max_pages)
+        # the buffers that calls read and write besides the pages, as [from, to)
+        self._spans = tuple((x.data_ptr(), x.data_ptr() + 4 * x.numel()) for x in self._tensors[3:] if x is not None)
+        _check(not any(_overlap(x, y) for x, y in itertools.combinations(self._spans, 2)),
+               "lengths, seen, scores and positions must not overlap")
         self._free = self._pages = None
         self._attend_work, self._evict_work = {}, None
         self._err = _ErrorWord(self.lib, self.device) if err is None else err
@@ -316,6 +321,10 @@ class PagedCache:
                 or a.head_stride != b.head_stride or a.slot_stride != b.slot_stride or into._shape != self._shape
                 or a.dtype != b.dtype or (a.scores == 0) != (b.scores == 0)):
             raise ValueError("into must be a fork of this cache")
+        # (what `fork` made has buffers of its own)
+        if into._err is not self._err and into._spans != self._spans and any(
+                _overlap(x, y) for x in self._spans for y in into._spans):
+            raise ValueError("into's lengths, seen, scores and positions must be all of this cache's or overlap none")
         return into
 
     def _workspace(self, nbytes, zero):
@@ -452,6 +461,10 @@ class PagedCache:
             held["evict_work"] = self._evict_work
         held.update((f"attend_work{key}", x) for key, x in self._attend_work.items())
         return {name: x.numel() * x.element_size() for name, x in held.items()}
+
+
+def _overlap(x, y):
+    return x[0] < y[1] and y[0] < x[1]
 
 
 def _native_types(head_dim, dtype):

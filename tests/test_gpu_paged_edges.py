@@ -169,3 +169,43 @@ def test_more_caches_than_a_page_of_error_words():
             else:
                 with pytest.raises(RuntimeError, match="has no page"):
                     cache.check_errors()
+
+
+def test_buffers_that_overlap_are_refused():
+    """Lengths, tokens seen, scores and positions are buffers of their own, and a
+    cache that results go to has either all of this one's or none."""
+    k = torch.zeros(4, 2, 16, 64, dtype=BF16, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    q = torch.zeros(2, 4, 64, dtype=BF16, device="cuda")
+
+    def state():
+        return dict(lengths=i32(3, 4), seen=i32(3, 4), scores=torch.zeros(2, 2, 32, device="cuda"),
+                    positions=torch.zeros(2, 2, 32, dtype=torch.int32, device="cuda"))
+
+    def made(x):
+        return PagedCache.from_tensors(k, v, table, x["lengths"], seen=x["seen"], scores=x["scores"], positions=x["positions"])
+
+    own = state()
+    with pytest.raises(ValueError, match="overlap"):
+        made(dict(own, seen=own["lengths"]))
+    with pytest.raises(ValueError, match="overlap"):
+        made(dict(own, positions=own["scores"].view(torch.int32)))
+    words = torch.zeros(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        made(dict(own, lengths=words[:2], seen=words[1:]))
+    cache = made(own)
+    for name in own:
+        with pytest.raises(ValueError, match="overlap"):
+            cache.attend(q, into=made(dict(state(), **{name: own[name]})))
+    longer = torch.zeros(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        made(dict(own, lengths=longer[:2])).attend(q, into=made(dict(state(), seen=longer[1:])))
+    cache.attend(q, into=made(own))      # all of them: the cache itself
+    cache.attend(q, into=made(state()))  # none
+    cache.attend(q, into=cache.fork())
+    fork = cache.fork()
+    fork.attend(q, into=fork.fork())
+    unscored = [PagedCache.from_tensors(k, v, table, x) for x in (own["lengths"], own["lengths"], own["seen"])]
+    unscored[0].attend(q, into=unscored[1])
+    unscored[0].attend(q, into=unscored[2])

@@ -251,3 +251,25 @@ def test_error_words_of_several_threads(words):
     for t in threads:
         t.join()
     assert not problems
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="the addresses are made up: host checks only")
+def test_overlapping_results_are_refused(lib):  # noqa: F811
+    """Buffers of the second cache that are not all the first's lie apart from all of the first's."""
+    size = dict(lengths=4 * 3, seen=4 * 3, scores=4 * 3 * 8 * 160, positions=4 * 3 * 8 * 160)
+    own = dict(lengths=1 << 20, seen=2 << 20, scores=3 << 20, positions=4 << 20)
+    apart = {name: at + (8 << 20) for name, at in own.items()}
+    for call in (attend, append, evict):
+        assert call(lib, desc(**own), desc(**own)) not in (0, -1, -2)  # past every host check (no device)
+        assert call(lib, desc(**own), desc(**apart)) not in (0, -1, -2)
+        for name in own:
+            assert call(lib, desc(**own), desc(**{**apart, name: own[name]})) == -1, name
+            for other in own:
+                for at in (own[other] + size[other] - 4, own[other] - size[name] + 4):
+                    assert call(lib, desc(**own), desc(**{**apart, name: at})) == -1, (name, other)
+                for at in (own[other] + size[other], own[other] - size[name]):  # next to each other
+                    assert call(lib, desc(**own), desc(**{**apart, name: at})) not in (0, -1, -2), (name, other)
+    plain = dict(seen=0, scores=0, positions=0)
+    for at, ok in ((1 << 20, True), ((1 << 20) + 4, False), ((1 << 20) + 12, True)):
+        code = attend(lib, desc(lengths=1 << 20, **plain), desc(lengths=at, **plain), flags=0)
+        assert (code not in (0, -1, -2)) if ok else code == -1
