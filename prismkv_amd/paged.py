@@ -134,7 +134,7 @@ class PagedCache:
         meta = {}
         if scored:
             meta = dict(seen=torch.zeros_like(lengths),
-                        scores=torch.zeros(int(sequences), int(kv_heads), slots, device=device),
+                        scores=torch.zeros(int(sequences), int(kv_heads), slots, dtype=torch.float32, device=device),
                         positions=torch.zeros(int(sequences), int(kv_heads), slots, dtype=torch.int32, device=device))
         self._setup(k, v, table, lengths, library=library, err=_err, **meta)
         self._free = list(range(int(pages)))[::-1]

@@ -209,3 +209,16 @@ def test_buffers_that_overlap_are_refused():
     unscored = [PagedCache.from_tensors(k, v, table, x) for x in (own["lengths"], own["lengths"], own["seen"])]
     unscored[0].attend(q, into=unscored[1])
     unscored[0].attend(q, into=unscored[2])
+
+
+@pytest.mark.parametrize("default", [BF16, FP16, torch.float64])
+def test_default_types_do_not_matter(default):
+    """Scores are float32 whatever torch's default type is."""
+    torch.set_default_dtype(default)
+    try:
+        cache = PagedCache(1, 4, 4, page_size=16, kv_heads=1, head_dim=64, scored=True)
+        cache.reserve(20)
+        new = cache.resized(2, 2)
+    finally:
+        torch.set_default_dtype(FP32)
+    assert cache.scores.dtype == new.scores.dtype == FP32
