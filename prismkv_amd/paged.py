@@ -85,7 +85,7 @@ class _ErrorWord:
                 torch.cuda.synchronize(device)
                 fresh.extend(given_back.popleft() for _ in range(count))
                 return
-            page = torch.zeros(cls.PER_PAGE, 4, dtype=torch.int32, pin_memory=True)
+            page = torch.zeros(cls.PER_PAGE, 4, dtype=torch.int32, device="cpu", pin_memory=True)
             address = lib.query("prismkv_mapped_pointer", page.data_ptr())
         if not address:
             raise RuntimeError("prismkv_mapped_pointer: the pinned error word is not device-accessible")

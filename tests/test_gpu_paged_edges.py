@@ -222,3 +222,16 @@ def test_default_types_do_not_matter(default):
     finally:
         torch.set_default_dtype(FP32)
     assert cache.scores.dtype == new.scores.dtype == FP32
+
+
+def test_default_devices_do_not_matter(monkeypatch):
+    """The error word lies in host memory whatever torch's default device is."""
+    from prismkv_amd import paged as module
+    monkeypatch.setattr(module._ErrorWord, "homes", {})  # (the first cache makes its page of words)
+    with torch.device("cuda"):
+        cache = PagedCache(2, 4, 4, page_size=16, kv_heads=1, head_dim=64, scored=True)
+        cache.reserve([20, 3])
+        new = cache.resized(3, 2)
+        q = torch.zeros(2, 1, 64, dtype=BF16)
+        assert not new.attend(q).any() and not new.fork().attend(q).any()
+    new.check_errors()
