@@ -144,3 +144,101 @@ def test_other_heads_and_a_new_request():
     again = decode(model, session, ids, 80)
     assert torch.equal(first, again)
     session.close()
+
+
+def record_calls(session, model, prompt, steps, seed):
+    """A decode of layer 0, with what every step was given and left."""
+    calls, forward = [], session.forward
+
+    def keep(module, q, k, v, mask, **kw):
+        observed = session._observed.get(0)
+        out = forward(module, q, k, v, mask, **kw)
+        if 0 in session.ops:  # (a decode step: a prompt, also one of a token, has no cache yet)
+            op = session.ops[0]
+            calls.append(dict(q=q[0, :, 0].cpu(), k=k[0].cpu(), v=v[0].cpu(), out=out[0][0, 0].cpu(),
+                              observed=None if observed is None else observed.cpu(), held=op.held,
+                              positions=op.cache.positions[0, :, :op.held].cpu(),
+                              scores=op.cache.scores[0, :, :op.held].cpu()))
+        return out
+
+    session.forward = keep
+    ids = torch.randint(0, 256, (1, prompt + steps), generator=torch.Generator().manual_seed(seed)).cuda()
+    decode(model, session, ids, prompt)
+    return calls
+
+
+def follow(calls, prompt, budget, recent, sinks, every):
+    """The definition, head by head, from the queries, keys and values that the
+    session was given: the prompt's observed queries, then every step.  Scores are
+    compared at every step within the sum of the weights' bounds (oracle/paged.py)
+    and a rounding for each addition; a slot may stay or leave against the
+    definition only where its score and the edge's are within their bounds.  After
+    each step the slots are the session's.  Returns the comparisons made."""
+    heads = calls[0]["k"].shape[0]
+    group = calls[0]["q"].shape[0] // heads
+
+    def weigh(call, queries, tokens, h):
+        keys, values = (x[h:h + 1, tokens].permute(1, 0, 2)[:, :, None] for x in (call["k"], call["v"]))
+        (out, weights, _), (tol, w_tol, _) = paged.attend(queries[None, group * h:group * (h + 1)], keys, values,
+                                                          torch.arange(len(tokens))[None], [len(tokens)])[0]
+        return out, weights[0], tol, w_tol[0]
+
+    compared = 0
+    for h in range(heads):
+        held = torch.arange(prompt)
+        score, bound = (torch.zeros(prompt, dtype=torch.float64) for _ in range(2))
+
+        def add(call, queries, n):
+            out, w, tol, w_tol = weigh(call, queries, held[:n], h)
+            score[:n] += w
+            bound[:n] += w_tol + score[:n] * 2.0 ** -24
+            return out, tol
+
+        def cut(seen):
+            """(held, score, bound) of the slots that stay, and how many others may have."""
+            guarded = (held >= seen - recent) | (held < sinks)
+            rank = torch.where(guarded, torch.inf, score)
+            order = torch.sort(rank, descending=True, stable=True).indices[:budget]
+            edge, slack = rank[order[-1]], bound[order[-1]]
+            close = int((((rank - edge).abs() <= bound + slack) & ~guarded).sum()) - 1
+            return held[order], score[order], bound[order], close
+
+        observed = calls[0]["observed"]
+        for i in range(0 if observed is None else observed.shape[1]):
+            add(calls[0], observed[:, i], prompt - observed.shape[1] + 1 + i)
+        close = 0
+        if prompt > budget:
+            held, score, bound, close = cut(prompt)
+        for step, call in enumerate(calls):
+            if len(held) >= budget + every:
+                held, score, bound, close = cut(prompt + step)
+            held = torch.cat((held, torch.tensor([prompt + step])))
+            got = call["positions"][h].long()
+            assert len(set(got.tolist())) == len(got) == call["held"] == len(held), (step, h)
+            assert len(set(got.tolist()) ^ set(held.tolist())) <= 2 * close, (step, h, close)
+            index = {int(t): i for i, t in enumerate(held)}
+            same = torch.tensor([index.get(int(t), -1) for t in got])
+            known, score, bound = same >= 0, *(torch.cat((x, torch.zeros(1, dtype=x.dtype)))[same.clamp(min=0)]
+                                               for x in (score, bound))
+            held, close = got, 0
+            out, tol = add(call, call["q"], len(held))
+            assert ((call["out"][group * h:group * (h + 1)].double() - out).abs() <= tol).all(), (step, h)
+            have = call["scores"][h].double()
+            assert ((have - score).abs() <= bound)[known].all(), (step, h, float((have - score).abs()[known].max()))
+            compared += int(known.sum())
+            score = torch.where(known, score, have)  # (a slot that the definition would have let go)
+    return compared
+
+
+@pytest.mark.parametrize("prompt,observe", [(300, 24), (300, 0), (97, 24)])
+def test_every_score_of_a_small_budget(prompt, observe):
+    from prismkv_amd.hf import HFNative
+    budget, recent, sinks, every, steps = 96, 16, 4, 8, 40
+    model = tiny_qwen3(1)
+    session = HFNative(model, {}, mode="evict", cache_budget=budget, cache_recent=recent, cache_sinks=sinks,
+                       evict_every=every, observe=observe)
+    calls = record_calls(session, model, prompt, steps, 2)
+    compared = follow(calls, prompt, budget, recent, sinks, every)
+    session.close()
+    log("scores compared", compared, "of", sum(8 * call["held"] for call in calls))
+    assert compared >= 0.99 * sum(8 * call["held"] for call in calls)
