@@ -22,11 +22,11 @@ own attention over the whole cache.
 Mode "evict" (no reference counterpart) is the other control of the routed
 decode's cost: per layer a `PagedCache` of at most `cache_budget` slots and the
 `evict_every` latest tokens.  The prompt's keys and values are weighed by its
-last `observe` queries and cut to the budget; every decode step then appends
-its token, attends to what is held and adds the step's weights to the scores,
-and a cache that has grown by `evict_every` tokens is cut again: the
-`cache_recent` newest and `cache_sinks` first tokens stay, then the highest
-scores.  Any number of KV and query heads with head_dim 64, 128 or 256;
+last `observe` queries and, if it is longer, cut to the budget; every decode
+step then appends its token, attends to what is held and adds the step's
+weights to the scores, and a cache that has grown by `evict_every` tokens is
+cut again: the `cache_recent` newest and `cache_sinks` first tokens stay, then
+the highest scores.  Any number of KV and query heads with head_dim 64, 128 or 256;
 encoders are not used.  (The model's own cache object still grows; it is not
 read.)
 
@@ -238,8 +238,9 @@ class _BoundedLayer:
         cache.reserve(prefix)
         ends = torch.tensor([0, prefix], dtype=torch.int32, device=K.device)
         cache.append(K[:, :prefix].transpose(0, 1), V[:, :prefix].transpose(0, 1), ends)
-        if observed is not None and prefix > session.cache_budget:
-            # the prompt's last queries, each over the tokens up to its own
+        if observed is not None:
+            # the prompt's last queries, each over the tokens up to its own (also where
+            # the first cut comes later: it ranks the prompt's slots by these)
             queries = observed.transpose(0, 1).contiguous()
             for i in range(len(queries)):
                 cache.lengths.fill_(prefix - len(queries) + 1 + i)

@@ -242,3 +242,19 @@ def test_every_score_of_a_small_budget(prompt, observe):
     session.close()
     log("scores compared", compared, "of", sum(8 * call["held"] for call in calls))
     assert compared >= 0.99 * sum(8 * call["held"] for call in calls)
+
+
+@pytest.mark.parametrize("prompt,observe", [(96, 24), (60, 24), (10, 24), (1, 24)])
+def test_prompts_within_the_budget_are_weighed_too(prompt, observe):
+    """Their slots are ranked by the same queries as a longer prompt's when the
+    decode steps make the first cut."""
+    from prismkv_amd.hf import HFNative
+    budget, recent, sinks, every = 96, 16, 4, 8
+    model = tiny_qwen3(1)
+    session = HFNative(model, {}, mode="evict", cache_budget=budget, cache_recent=recent, cache_sinks=sinks,
+                       evict_every=every, observe=observe)
+    calls = record_calls(session, model, prompt, max(30, 120 - prompt), 5)
+    assert calls[0]["observed"].shape[1] == min(prompt, observe)
+    compared = follow(calls, prompt, budget, recent, sinks, every)
+    session.close()
+    assert compared >= 0.99 * sum(8 * call["held"] for call in calls)
