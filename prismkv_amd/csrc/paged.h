@@ -210,7 +210,8 @@ struct PagedAppend {
   int32_t *lengths_out, *seen_out, *positions, *positions_out;
   float *scores, *scores_out;
   unsigned* err;
-  int64_t rows, k_row, k_head, v_row, v_head;  // bytes
+  int64_t first_row, rows;                     // this launch's first, all
+  int64_t k_row, k_head, v_row, v_head;        // bytes
   int64_t page_bytes, head_bytes, slot_bytes;
   PageDiv div;
   int sequences, kv_heads, log_pieces, page_size, max_pages, pages, slots;  // log_pieces: 16-byte pieces of a row

@@ -698,6 +698,7 @@ __global__ __launch_bounds__(kPT) void paged_weigh_kernel(PagedAttend a) {
 // 31.7 us = 5.2 TB/s (a copy as large: 32.2); 128 single rows 3.5 us.
 
 constexpr int kAppendRows = 8;
+constexpr int64_t kLaunchRows = 1 << 26;  // (a launch has fewer than 2^32 threads: 2^27 rows)
 
 struct AppendPlace {
   size_t at;  // bytes from the pages' base
@@ -746,7 +747,7 @@ __device__ __forceinline__ void advance(const PagedAppend& a, int b) {
 __global__ __launch_bounds__(kPT) void paged_append_kernel(PagedAppend a) {
   __shared__ AppendPlace places[kAppendRows];
   const int tid = threadIdx.x, each = a.offsets ? kAppendRows : 1;
-  const int64_t row0 = (int64_t)blockIdx.x * each;
+  const int64_t row0 = a.first_row + (int64_t)blockIdx.x * each;
   const int rows = (int)min((int64_t)each, a.rows - row0);
   const int log = a.log_pieces, per_row = a.kv_heads << log, items = rows * per_row;  // pieces of 16 bytes
   constexpr int kU = 4;
@@ -1620,11 +1621,12 @@ int prismkv_paged_append(const prismkv_paged_cache* cache, const prismkv_paged_c
     hipLaunchKernelGGL(paged_append_kernel, dim3(c.sequences), dim3(kPT), 0, s, a);
     return (int)hipGetLastError();
   }
-  if (rows) {
-    hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((rows + kAppendRows - 1) / kAppendRows)), dim3(kPT), 0, s, a);
-    const int rc = (int)hipGetLastError();
-    if (rc || a.lengths_out != a.lengths) return rc;
+  for (; a.first_row < rows; a.first_row += kLaunchRows) {
+    const int64_t more = rows - a.first_row < kLaunchRows ? rows - a.first_row : kLaunchRows;
+    hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((more + kAppendRows - 1) / kAppendRows)), dim3(kPT), 0, s, a);
+    if (const int rc = (int)hipGetLastError()) return rc;
   }
+  if (rows && a.lengths_out != a.lengths) return 0;  // (advanced by the rows' launches)
   hipLaunchKernelGGL(paged_advance_kernel, dim3((c.sequences + kPT - 1) / kPT), dim3(kPT), 0, s, a);
   return (int)hipGetLastError();
 }

@@ -235,3 +235,43 @@ def test_default_devices_do_not_matter(monkeypatch):
         q = torch.zeros(2, 1, 64, dtype=BF16)
         assert not new.attend(q).any() and not new.fork().attend(q).any()
     new.check_errors()
+
+
+def test_rows_beyond_one_launch():
+    """More packed rows than one launch has threads for (2^27 rows of 8 a
+    workgroup of 256 would take 2^32), on two sequences, in place and into a fork."""
+    rows, page = (1 << 27) + 1000, 1 << 16
+    gen = torch.Generator().manual_seed(0)
+    few = 1 << 12
+    pages = [rows // page, 2]
+    shape = (sum(pages), 1, page, 64)
+    k = torch.zeros(shape, dtype=BF16, device="cuda")
+    v = torch.zeros(shape, dtype=BF16, device="cuda")
+    table = torch.full((2, pages[0]), -1, dtype=torch.int32)
+    table[0] = torch.arange(pages[0]).flip(0)
+    table[1, :2] = torch.arange(pages[0], sum(pages))
+    cache = PagedCache.from_tensors(k, v, table.cuda(), i32(0, 5))
+    one = torch.randn(few, 64, generator=gen).bfloat16().cuda()
+    new = torch.empty(rows, 1, 64, dtype=BF16, device="cuda")
+    for at in range(0, rows, few):  # (block i of the rows: `one` turned by i)
+        n = min(few, rows - at)
+        new[at:at + n, 0] = one.roll(at // few, 0)[:n]
+    first = pages[0] * page  # rows of the first sequence; the rest is the second's
+    ends = i32(0, first, rows)
+    fork = cache.fork()
+    for to in (fork, cache):
+        k.zero_()
+        v.zero_()
+        cache.append(new, new, ends, into=to)
+        torch.cuda.synchronize()
+        cache.check_errors()
+        assert to.lengths.tolist() == [first, 5 + rows - first]
+        for x in (k, v):
+            for b in range(pages[0]):
+                assert torch.equal(x[int(table[0, b]), 0], new[b * page:(b + 1) * page, 0])
+            flat = x[pages[0]:].view(-1, 64)
+            assert torch.equal(flat[5:5 + rows - first], new[first:, 0])
+            assert not flat[:5].any() and not flat[5 + rows - first:].any()
+    assert fork.lengths.tolist() == cache.lengths.tolist()
+    del x, k, v, new, flat, cache, fork, to
+    torch.cuda.empty_cache()
