@@ -721,7 +721,7 @@ __device__ __forceinline__ AppendPlace append_place(const PagedAppend& a, int64_
     step = row - a.offsets[lo];
     if (step < 0 || row >= a.offsets[lo + 1]) return p;  // a row of no sequence
   }
-  p.length = max(a.lengths[p.b], 0);
+  p.length = min(max(a.lengths[p.b], 0), a.slots);
   if (a.positions) p.position = a.seen[p.b] + (int)step;
   const int64_t slot = p.length + step;
   const int page = slot < a.slots ? a.table[(size_t)p.b * a.max_pages + a.div.of((int)slot)] : -1;

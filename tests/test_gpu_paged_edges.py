@@ -275,3 +275,19 @@ def test_rows_beyond_one_launch():
     assert fork.lengths.tolist() == cache.lengths.tolist()
     del x, k, v, new, flat, cache, fork, to
     torch.cuda.empty_cache()
+
+
+def test_lengths_past_the_table():
+    """Read as the table's slots: a row is dropped and reported, the length stays there."""
+    for far in (33, 2 ** 31 - 1):
+        for offsets in (None, i32(0, 1, 2)):
+            cache = PagedCache(2, 4, 2, page_size=16, kv_heads=1, head_dim=64)
+            cache.reserve(32)
+            cache.lengths.copy_(i32(far, 3))
+            rows = torch.ones(2, 1, 64, dtype=BF16, device="cuda")
+            cache.append(rows, rows, offsets)
+            assert cache.lengths.tolist() == [32, 4]
+            assert int(cache.k.count_nonzero()) == 64
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError, match="has no page"):
+                cache.check_errors()
