@@ -455,7 +455,8 @@ int prismkv_paged_append(const prismkv_paged_cache* cache, const prismkv_paged_c
 /* q [sequences][kv_heads * group][head_dim] -> out of the same shape and type:
  * softmax(scale q.k) v over each sequence's slots [0, lengths[b]), 0 where there
  * is none; lse f32 [sequences][kv_heads * group] (or 0) <- the natural logarithm
- * of the softmax's sum, -infinity for an empty one.  Scores, sums and products
+ * of the softmax's sum, -infinity for an empty one.  scale log2(e) is finite in fp32
+ * (-1 otherwise).  Scores, sums and products
  * are accumulated in fp32.  flags & 1: into's scores[t] = scores[t] + slot t's
  * weights summed over the group's heads, for t < lengths[b].  flags & 2: the
  * lengths are into's (an append that went there is attended to). */

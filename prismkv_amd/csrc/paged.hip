@@ -9,6 +9,8 @@
 // through.
 #include "paged.h"
 
+#include <cfloat>
+
 #include "prismkv_hip.h"
 
 namespace prismkv {
@@ -1522,7 +1524,8 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   if (const int rc = check_cache(cache, into, weigh)) return rc;
   if (flags & ~3) return kBadMode;
   const prismkv_paged_cache& c = *cache;
-  if (group < 1 || group > 1024 || !(scale - scale == 0)) return kBadSize;
+  const double scale2 = scale * 1.4426950408889634;  // the exponents are powers of 2, in fp32
+  if (group < 1 || group > 1024 || !(scale2 >= -FLT_MAX && scale2 <= FLT_MAX)) return kBadSize;
   if (!q || !paged_work || !out || (q | paged_work) & 15 || lse & 3 || out & 3) return kBadSize;
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
   const WorkLayout w = attend_layout(c.sequences, c.kv_heads, group, c.head_dim, slots, weigh, c.dtype);
@@ -1560,7 +1563,7 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   a.page_size = c.page_size;
   a.max_pages = c.max_pages;
   a.pages = (int)c.pages;
-  a.scale = (float)(scale * 1.4426950408889634);
+  a.scale = (float)scale2;
   const hipStream_t s = (hipStream_t)stream;
   int rc;
   if (c.dtype == kBf16) rc = launch_attend_dim<kBf16>(a, c.head_dim, w.units, s);

@@ -28,6 +28,7 @@ from . import _lib
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 HEAD_DIMS = (64, 128, 256)
+MAX_SCALE = torch.finfo(torch.float32).max / 1.4426950408889634
 ERR_PAGES, ERR_ROWS = 4, 8  # codes of the error word, as the kernels write them
 ERROR_MESSAGES = {ERR_PAGES: "a slot below a sequence's length has no page",
                   ERR_ROWS: "the offsets of an append did not ascend from 0 to its number of rows"}
@@ -395,8 +396,8 @@ class PagedCache:
         if accumulate and self.scores is None:
             raise ValueError("accumulate needs a scored cache")
         scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-        if not math.isfinite(scale):
-            raise ValueError("a finite scale required")
+        if not abs(scale) <= MAX_SCALE:
+            raise ValueError("a scale that is finite in float32, as times log2(e), required")
         if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()
                                 or lse.device != self.device):
             raise ValueError("lse must be a contiguous float32 [sequences, heads] on the cache's device")

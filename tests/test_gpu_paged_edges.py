@@ -291,3 +291,15 @@ def test_lengths_past_the_table():
             torch.cuda.synchronize()
             with pytest.raises(RuntimeError, match="has no page"):
                 cache.check_errors()
+
+
+def test_scales_that_32_bits_do_not_hold_are_refused():
+    cache = PagedCache(1, 1, 1, page_size=16, kv_heads=1, head_dim=64)
+    cache.reserve(1)
+    cache.lengths.fill_(1)
+    q = torch.zeros(1, 1, 64, dtype=BF16, device="cuda")
+    for scale in (3e38, -3e38, 1e300):  # (times log2(e), as the kernels have it)
+        with pytest.raises(ValueError, match="finite"):
+            cache.attend(q, scale=scale)
+    for scale in (2e38, 0.0, 1e-300):
+        assert not cache.attend(q, scale=scale).any()

@@ -273,3 +273,8 @@ def test_overlapping_results_are_refused(lib):  # noqa: F811
     for at, ok in ((1 << 20, True), ((1 << 20) + 4, False), ((1 << 20) + 12, True)):
         code = attend(lib, desc(lengths=1 << 20, **plain), desc(lengths=at, **plain), flags=0)
         assert (code not in (0, -1, -2)) if ok else code == -1
+
+
+def test_scales_that_32_bits_do_not_hold_are_refused(lib):  # noqa: F811
+    for scale in (3e38, -3e38, 1e300):  # (times log2(e))
+        assert attend(lib, scale=scale) == -1
