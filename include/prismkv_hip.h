@@ -459,7 +459,10 @@ int prismkv_paged_append(const prismkv_paged_cache* cache, const prismkv_paged_c
  * (-1 otherwise).  Scores, sums and products
  * are accumulated in fp32.  flags & 1: into's scores[t] = scores[t] + slot t's
  * weights summed over the group's heads, for t < lengths[b].  flags & 2: the
- * lengths are into's (an append that went there is attended to). */
+ * lengths are into's (an append that went there is attended to).  Refused (-1, and
+ * 0 work bytes): 2^31 quanta of 32 slots and more, a sequence's table rounded up to
+ * 256 (of head_dim 256 or fp32 128, of both 64), for each sequence, KV head and 16
+ * query heads on it. */
 size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh,
                                        int dtype);
 int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t q, uint64_t lse,

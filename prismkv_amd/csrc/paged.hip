@@ -1514,7 +1514,8 @@ extern "C" {
 size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh,
                                        int dtype) {
   if (dtype < kBf16 || dtype > kFp32 || sequences < 1 || kv_heads < 1 || group < 1 || head_dim < 1 || slots < 1) return 0;
-  return attend_layout(sequences, kv_heads, group, head_dim, slots, weigh != 0, dtype).bytes;
+  const WorkLayout w = attend_layout(sequences, kv_heads, group, head_dim, slots, weigh != 0, dtype);
+  return w.quanta > INT32_MAX ? 0 : w.bytes;  // (refused: quanta are counted in 32 bits)
 }
 
 int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t q, uint64_t lse,
@@ -1529,7 +1530,7 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   if (!q || !paged_work || !out || (q | paged_work) & 15 || lse & 3 || out & 3) return kBadSize;
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
   const WorkLayout w = attend_layout(c.sequences, c.kv_heads, group, c.head_dim, slots, weigh, c.dtype);
-  if (work_bytes < w.bytes || w.quanta > INT32_MAX) return kBadSize;  // (quanta are counted in 32 bits)
+  if (work_bytes < w.bytes || w.quanta > INT32_MAX) return kBadSize;
   const int es = element_bytes(c.dtype);
   PagedAttend a{};
   a.q = reinterpret_cast<const void*>(q);

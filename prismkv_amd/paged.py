@@ -377,7 +377,8 @@ class PagedCache:
         receives the logarithm of each softmax's sum (-inf for an empty one)."""
         to = self if into is None else self._into(into)
         group, scale = self._check_q(q, scale, accumulate, lse)
-        return self._attend(q, group, scale, accumulate, lse, to, 0)
+        accumulate = bool(accumulate)
+        return self._attend(q, group, scale, accumulate, lse, to, 0, self._attend_workspace(group, accumulate))
 
     def _check_q(self, q, scale, accumulate, lse):
         """The query heads per KV head, and the scale."""
@@ -403,17 +404,22 @@ class PagedCache:
             raise ValueError("lse must be a contiguous float32 [sequences, heads] on the cache's device")
         return group, scale
 
-    def _attend(self, q, group, scale, accumulate, lse, to, flags):
-        self.check_errors()
-        accumulate = bool(accumulate)
+    def _attend_workspace(self, group, accumulate):
         work = self._attend_work.get((group, accumulate))
         if work is None:
             # (the leading counters are zeroed; the kernels leave them so)
             sequences, kv_heads, head_dim, _, _ = self._shape
             nbytes = self.lib.query("prismkv_paged_attend_work_bytes", sequences, kv_heads, group, head_dim, self.slots,
                                     int(accumulate), self._desc.dtype)
+            if not nbytes:
+                raise NotImplementedError("less than 2^31 blocks of 32 slots in all (of every sequence's table, KV head "
+                                          "and 16 query heads on it)")
             work = self._attend_work[(group, accumulate)] = self._workspace(
                 nbytes, 4 * sequences * kv_heads * ((group + 15) // 16))
+        return work
+
+    def _attend(self, q, group, scale, accumulate, lse, to, flags, work):
+        self.check_errors()
         out = torch.empty_like(q)
         self._call("prismkv_paged_attend", self._pointer, to._pointer, q.data_ptr(), 0 if lse is None else lse.data_ptr(),
                    work.data_ptr(), out.data_ptr(), group, flags + accumulate, scale, work.numel())
@@ -425,9 +431,12 @@ class PagedCache:
         go there, the new rows into the shared pages behind this cache's
         lengths."""
         to = self if into is None else self._into(into)
-        group, scale = self._check_q(q, scale, accumulate, lse)  # nothing is appended for a query that is refused
+        # nothing is appended for a query that is refused
+        group, scale = self._check_q(q, scale, accumulate, lse)
+        accumulate = bool(accumulate)
+        work = self._attend_workspace(group, accumulate)
         self.append(k, v, into=into)
-        return self._attend(q, group, scale, accumulate, lse, to, 2)
+        return self._attend(q, group, scale, accumulate, lse, to, 2, work)
 
     def evict(self, keep, *, recent=0, sinks=0, into=None):
         """Cuts every sequence longer than `keep` slots (an int, or i32

@@ -303,3 +303,33 @@ def test_scales_that_32_bits_do_not_hold_are_refused():
             cache.attend(q, scale=scale)
     for scale in (2e38, 0.0, 1e-300):
         assert not cache.attend(q, scale=scale).any()
+
+
+def test_a_step_that_is_refused_appends_nothing():
+    """Also where it is the size of the call that cannot be attended to."""
+    k = torch.zeros(1, 1, 1 << 20, 64, dtype=BF16, device="cuda")
+    cache = PagedCache.from_tensors(k, torch.zeros_like(k), torch.zeros(1, 1 << 10, dtype=torch.int32, device="cuda"), i32(3))
+    q = torch.zeros(1, 1024, 64, dtype=BF16, device="cuda")
+    row = torch.ones(1, 1, 64, dtype=BF16, device="cuda")
+    for call in (lambda: cache(q, row, row), lambda: cache.attend(q)):
+        with pytest.raises(NotImplementedError, match="2\\^31"):
+            call()
+    assert cache.lengths.tolist() == [3] and not k.any()
+    cache(q[:, :512].contiguous(), row, row)  # half as many query heads
+    assert cache.lengths.tolist() == [4]
+
+
+def test_a_step_without_its_workspace_is_not_captured():
+    cache = PagedCache(1, 2, 2, page_size=16, kv_heads=1, head_dim=64)
+    cache.reserve(20)
+    q = torch.zeros(1, 2, 64, dtype=BF16, device="cuda")
+    row = torch.ones(1, 1, 64, dtype=BF16, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        filler = q + 1
+        with pytest.raises(RuntimeError, match="before the capture"):
+            cache(q, row, row)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert cache.lengths.tolist() == [0] and not cache.k.any() and filler.bool().all()

@@ -278,3 +278,13 @@ def test_overlapping_results_are_refused(lib):  # noqa: F811
 def test_scales_that_32_bits_do_not_hold_are_refused(lib):  # noqa: F811
     for scale in (3e38, -3e38, 1e300):  # (times log2(e))
         assert attend(lib, scale=scale) == -1
+
+
+def test_too_many_quanta_have_no_workspace(lib):  # noqa: F811
+    """2^30 slots of 1024 query heads on a KV head are 2^31 quanta of 32 slots; of 512 heads half of it."""
+    for group, fits in ((1024, False), (512, True)):
+        need = lib.query("prismkv_paged_attend_work_bytes", 1, 1, group, 64, 1 << 30, 0, 0)
+        assert (need > 0) == fits
+    wide = dict(sequences=1, kv_heads=1, page_size=1 << 20, max_pages=1 << 10, pages=1, page_stride=128 << 20,
+                head_stride=128 << 20)
+    assert attend(lib, desc(**wide), group=1024, flags=0) == -1
