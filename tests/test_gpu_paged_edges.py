@@ -333,3 +333,39 @@ def test_a_step_without_its_workspace_is_not_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert cache.lengths.tolist() == [0] and not cache.k.any() and filler.bool().all()
+
+
+@pytest.mark.parametrize("width", [40, 2048])
+def test_tables_wider_than_the_sequences(width):
+    """Room for far longer sequences than there are: a step that weighs, cuts (by
+    one launch, and by the launches of rows as long as the table) and steps again."""
+    from oracle import paged
+    from tests.test_gpu_paged import check_attend, check_evict, make, queries
+    lengths, heads, page = [300, 0, 41], 2, 16
+    narrow, host = make(lengths, heads, 64, page, BF16, room=20, scored=True)
+    slots = width * page
+    table = torch.full((3, width), -1, dtype=torch.int32)
+    table[:, :host["table"].shape[1]] = host["table"]
+    gen = torch.Generator().manual_seed(1)
+    host.update(table=table, scores=torch.zeros(3, heads, slots), seen=torch.tensor(lengths, dtype=torch.int32),
+                positions=torch.arange(slots, dtype=torch.int32).expand(3, heads, slots).clone())
+    cache = PagedCache.from_tensors(narrow.k, narrow.v, table.cuda(), narrow.lengths, seen=host["seen"].cuda(),
+                                    scores=host["scores"].cuda(), positions=host["positions"].cuda())
+    for keep in (None, 120, 60, 4):
+        q = queries(cache, 4, seed=keep or 0)
+        k, v = (torch.randn(3, heads, 64, generator=gen).bfloat16() for _ in range(2))
+        before = cache.scores.cpu()
+        out = cache(q.cuda(), k.cuda(), v.cuda(), accumulate=True)
+        lengths = [n + 1 for n in lengths]
+        state = {n: getattr(cache, n).cpu() for n in ("k", "v", "table", "scores", "positions", "seen")}
+        check_attend(q, state, lengths, out)
+        for b, ((_, w, _), (_, tol, _)) in enumerate(paged.attend(q, state["k"], state["v"], table, lengths)):
+            old = before[b, :, :lengths[b]].double()
+            old[:, -1] = 0
+            got = cache.scores[b, :, :lengths[b]].cpu().double()
+            assert ((got - old - w).abs() <= tol + (old + w) * 2.0 ** -24).all()
+        if keep:
+            cache.evict(keep, recent=5, sinks=1)
+            check_evict(state, lengths, [keep] * 3, cache, cache, 5, 1)
+            lengths = [min(n, keep) for n in lengths]
+    cache.check_errors()
