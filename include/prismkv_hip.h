@@ -474,7 +474,9 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
  * first in the order protected (position >= seen[b] - recent or position <
  * sinks) before others, then NaN scores, then score descending, then slot
  * ascending.  The i-th staying slot at or behind the new length moves, with its
- * K and V rows, score and position, into the i-th leaving slot before it. */
+ * K and V rows, score and position, into the i-th leaving slot before it.  The rows
+ * move in the pages that cache and into share: where those are two, the first still
+ * lists slots that were overwritten, and may only be cut in the same way again. */
 size_t prismkv_paged_evict_work_bytes(int sequences, int kv_heads, int64_t slots);
 int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t keeps,
                         uint64_t paged_work, int keep, int recent, int sinks, size_t work_bytes, uint64_t stream);

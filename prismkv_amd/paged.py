@@ -111,7 +111,10 @@ class PagedCache:
 
     `reserve` and `release` hand out pages on the host; calls that take `into`
     (a `fork`) write their results there and leave this cache's own lengths,
-    scores and positions, so that a step can be taken back."""
+    scores and positions, so that an `append`, an `attend` or a step can be taken
+    back.  An `evict` cannot: it moves rows in the shared pages.  A fork holds what
+    this cache held when it was made, and a call into it writes what that call
+    changes; it is made anew when this cache has gone on by itself."""
 
     def __init__(self, sequences, pages, max_pages, *, page_size=64, kv_heads=8, head_dim=128, dtype=torch.bfloat16,
                  scored=False, device="cuda", library=None, _err=None):
@@ -216,7 +219,7 @@ class PagedCache:
     def fork(self):
         """A cache over the same pages and page table with copies of this
         one's lengths, scores and positions: the `into` of a step that may be
-        taken back.  (Rows that `evict` moved stay moved.)"""
+        taken back.  (Rows that `evict` moves are moved for both.)"""
         obj = PagedCache.__new__(PagedCache)
         meta = {name: getattr(self, name).clone() for name in _SCORED} if self.scored else {}
         obj._setup(self.k, self.v, self.table, self.lengths.clone(), library=self.lib.path, err=self._err, **meta)
@@ -446,7 +449,10 @@ class PagedCache:
         fewest rows move: a slot that stays and lies behind the budget goes
         into one that became free, in ascending order, with its score and
         position; the order of the slots is not that of the tokens afterwards.
-        The pages stay reserved (`release`)."""
+        The pages stay reserved (`release`).  With `into` the rows move in the
+        shared pages all the same, over rows that this cache still lists: it may
+        then repeat the same cut, into a fork or itself, but not be attended to,
+        appended to or cut otherwise."""
         to = self if into is None else self._into(into)
         _check(self.scored, "evict needs a scored cache")
         sequences, kv_heads, _, _, _ = self._shape

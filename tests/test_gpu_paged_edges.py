@@ -369,3 +369,25 @@ def test_tables_wider_than_the_sequences(width):
             check_evict(state, lengths, [keep] * 3, cache, cache, 5, 1)
             lengths = [min(n, keep) for n in lengths]
     cache.check_errors()
+
+
+def test_a_cut_into_a_fork_may_be_repeated_only():
+    """The rows move in the pages that the original shares: the same cut, into another
+    fork or in place, leaves the same; attending to the original would read moved rows."""
+    from tests.test_gpu_paged import make, queries
+    cache, host = make([300, 90], 2, 64, 16, BF16, scored=True)
+    q = queries(cache, 2).cuda()
+    first, second = cache.fork(), cache.fork()
+    before = bits(cache.attend(q))
+    cache.evict(50, recent=4, into=first)
+    pages, out = bits(cache.k), bits(first.attend(q))
+    assert cache.lengths.tolist() == [300, 90] and not torch.equal(bits(cache.attend(q)), before)
+    cache.evict(50, recent=4, into=second)
+    cache.evict(50, recent=4)
+    assert torch.equal(bits(cache.k), pages)
+    for other in (second, cache):
+        assert torch.equal(bits(other.attend(q)), out)
+        for name in ("lengths", "seen"):
+            assert torch.equal(getattr(other, name), getattr(first, name))
+        for name in ("scores", "positions"):
+            assert torch.equal(getattr(other, name)[:, :, :50], getattr(first, name)[:, :, :50])
