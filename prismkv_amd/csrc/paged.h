@@ -136,9 +136,10 @@ __device__ __forceinline__ int quanta_before(const PagedAttend& a, int count, in
 
 // Many short pairs: a wave for each by itself, where a workgroup for each would
 // take them one after another and leave most of its waves without a tile (256
-// sequences of 100 tokens, 8 heads: 23.8 us, 42.8 by workgroups; 128 of 500 44.5
-// and 51.4; with fewer pairs, or longer ones, the workgroups are as fast or faster:
-// 256 pairs of 250 11.2 us against 14.6, 512 of 1000 46 against 116).
+// sequences of 100 tokens, 8 heads: 23.7 us, 42.9 by workgroups; 128 of 500 44.5
+// and 51.8).  Fewer pairs are faster by workgroups (256 of 250 tokens 11.4 us against
+// 13.9), longer ones as fast or, ragged, faster: 512 of 1000 tokens 47 us against 45,
+// 512 ragged up to 1000 27.6 against 34.5.
 constexpr int kSoloTokens = 512, kSoloPairs = 512;
 __device__ __forceinline__ bool pairs_alone(const PagedAttend& a, int longest) {
   return a.many && longest <= kSoloTokens;

@@ -33,10 +33,11 @@ namespace {
 // order of arrival.
 //
 // Measured (MI355X, launches after one another in a graph): 65792 tokens, 8 x 4
-// heads, bf16, 47.5 us = 5.7 TB/s; 32 sequences of 6.4K tokens 136 us = 6.2 TB/s
-// (a plain read of as much memory reaches 6.9); 16 x 8192 of head_dim 256 in fp32
-// 93 us = 5.8; of head_dim 64 50 us = 5.3; 75 tokens 6.6 us.  About 6 us of a call
-// are the launch and the chain lengths -> page -> rows, 4 more the join.
+// heads, bf16, 47.3 us = 5.7 TB/s; 32 sequences of 6.4K tokens 136 us = 6.2 TB/s
+// (a plain read of as much memory reaches 6.9); 16 x 8192 of head_dim 256 in fp32, 2
+// x 4 heads, 92 us = 5.9; of head_dim 64, 8 x 4 heads, 48 us = 5.6; 75 tokens 6.4 us.
+// About 6 us of a call are the launch and the chain lengths -> page -> rows, 3.7 more
+// the join (65792 tokens 43.7 us without it).
 
 // 16-bit types: P is a sum of terms of the type, each with a product of its own into
 // one accumulator: bf16 takes three, which hold all 24 bits of an fp32 p (with two,
@@ -1071,9 +1072,9 @@ __device__ __forceinline__ void evict_lengths(const PagedEvict& a, const EvictRo
 // LDS, the budget-th largest by three histogram passes (11, 11 and 10 bits), then
 // the slots that move, found by each wave in its own share, and, if they are few,
 // their rows.  Bound by the latency of its steps and, its 16 waves on one CU, the
-// instructions of each 64 slots: 2112 slots to 2048, 8 x 8 rows, 11.1 us in all (the
-// reads 1.0, the passes 2.4, the writing of the moves 1.7, the moves 2.8); up to
-// 9001 slots, 16 x 4 rows, 14.7.
+// instructions of each 64 slots: 2112 slots to 2048, 8 x 8 rows, 11.5 us, of which by
+// clock reads the reads and the first counts 1.4, the passes 2.4, counts and lists of
+// the moves 3.0, the moves 1.8; up to 9001 slots, 16 x 4 rows, 15 traced.
 // Up to this many slots; twice as many where the rows fill the CUs by themselves (31
 // steps of 64 slots a wave: one row of 32000 slots 45 us, 43 in parts; 64 rows 59,
 // 75 in parts).
@@ -1345,7 +1346,7 @@ __global__ __launch_bounds__(kET) void paged_pick_kernel(PagedEvict a) {
 
 // Moves the kept rows into the holes where the selection has not: a copy, bound by
 // the rows it reads and writes.  No source is another move's destination.  100 MB
-// of 256-byte rows read and written: 23.5 us = 4.4 TB/s (4 or 8 rows in flight per
+// of 256-byte rows read and written: 23.2 us = 4.4 TB/s (4 or 8 rows in flight per
 // thread: fewer workgroups, and 1 to 4 us more).
 constexpr int kMoveRows = 2;
 
@@ -1480,9 +1481,9 @@ int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
   const int64_t longest = a.slots / (kLeast<DT, D> * kQuantum) + 2;
   const int64_t most = kUnits / (a.kv_heads * a.tiles) + 2;  // (a sequence's pairs are alike)
   const int chunks = (int)(longest < most ? longest : most);  // of one pair at most
-    // Where a pair's states may be many and wide a second launch joins them: 65536
-  // tokens of one KV head and 16 query heads (264K floats) 20.0 us, 47.5 by the last
-  // workgroup; of 8 KV heads and 4 (17K) 48.2 against 47.8.
+  // Where a pair's states may be many and wide a second launch joins them: 65536
+  // tokens of one KV head and 16 query heads (264K floats) 20.3 us, 44.9 by the last
+  // workgroup; of 8 KV heads and 4 (17K) 48.5 against 47.3.
   const bool apart = (int64_t)chunks * rows * D > 49152;
   const int merge = 32 * kAWaves<D> + kAWaves<D> * rows * D, sums = 32 + chunks * rows;
   const int join = apart ? 0 : 256 * kAWaves<D> + sums;

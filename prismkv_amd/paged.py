@@ -35,8 +35,8 @@ ERROR_MESSAGES = {ERR_PAGES: "a slot below a sequence's length has no page",
 _SCORED = ("seen", "scores", "positions")
 
 
-# The current stream's handle; building a torch.cuda.Stream for it takes 2.7 us of a
-# call's 13.
+# The current stream's handle; building a torch.cuda.Stream for it takes 1 us beside a
+# call's 7.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
