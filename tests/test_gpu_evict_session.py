@@ -258,3 +258,47 @@ def test_prompts_within_the_budget_are_weighed_too(prompt, observe):
     compared = follow(calls, prompt, budget, recent, sinks, every)
     session.close()
     assert compared >= 0.99 * sum(8 * call["held"] for call in calls)
+
+
+def test_prompts_in_chunks_and_a_second_turn():
+    """A prompt in chunks, one of a token, is observed as a whole; tokens appended by
+    a chunk after decode steps make a new prefix, weighed by the chunk's queries."""
+    from transformers import DynamicCache
+    from prismkv_amd.hf import HFNative
+    budget, recent, sinks, every, observe = 96, 16, 4, 8, 24
+    model = tiny_qwen3(1)
+    session = HFNative(model, {}, mode="evict", cache_budget=budget, cache_recent=recent, cache_sinks=sinks,
+                       evict_every=every, observe=observe)
+    ids = torch.randint(0, 256, (1, 400), generator=torch.Generator().manual_seed(9)).cuda()
+    cache = DynamicCache(config=model.config)
+    calls, forward = [], session.forward
+
+    def keep(module, q, k, v, mask, **kw):
+        observed = session._observed.get(0)
+        out = forward(module, q, k, v, mask, **kw)
+        if 0 in session.ops:
+            op = session.ops[0]
+            calls.append(dict(q=q[0, :, 0].cpu(), k=k[0].cpu(), v=v[0].cpu(), out=out[0][0, 0].cpu(),
+                              observed=None if observed is None else observed.cpu(), held=op.held,
+                              positions=op.cache.positions[0, :, :op.held].cpu(),
+                              scores=op.cache.scores[0, :, :op.held].cpu()))
+        return out
+
+    session.forward = keep
+    with torch.no_grad():
+        with session.prefill():
+            for lo, hi in ((0, 90), (90, 105), (105, 106), (106, 120)):
+                model(ids[:, lo:hi], past_key_values=cache, use_cache=True)
+        for s in range(120, 140):
+            model(ids[:, s:s + 1], past_key_values=cache, use_cache=True)
+        first, calls = calls, []
+        model(ids[:, 140:155], past_key_values=cache, use_cache=True)
+        assert 0 not in session.ops and not calls
+        for s in range(155, 180):
+            model(ids[:, s:s + 1], past_key_values=cache, use_cache=True)
+    assert len(first) == 20 and len(calls) == 25
+    assert first[0]["observed"].shape[1] == observe and calls[0]["observed"].shape[1] == 15
+    for turn, prompt in ((first, 120), (calls, 155)):
+        assert follow(turn, prompt, budget, recent, sinks, every) >= 0.99 * sum(8 * call["held"] for call in turn)
+    session.check_errors()
+    session.close()

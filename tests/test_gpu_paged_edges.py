@@ -391,3 +391,61 @@ def test_a_cut_into_a_fork_may_be_repeated_only():
             assert torch.equal(getattr(other, name), getattr(first, name))
         for name in ("scores", "positions"):
             assert torch.equal(getattr(other, name)[:, :, :50], getattr(first, name)[:, :, :50])
+
+
+def plain_attend(q, k, v, n):
+    """Softmax attention in 64 bits of q [..., G, D] over k, v [..., S, D], slots [0, n) of each."""
+    s = (q.double() @ k.double().transpose(-1, -2).contiguous()) / math.sqrt(q.shape[-1])
+    s = s.masked_fill(torch.arange(k.shape[-2]) >= n[..., None, None], -math.inf)
+    p = torch.nan_to_num(torch.softmax(s, -1))  # (no slot: no weight)
+    return p @ v.double(), p, (p @ v.double().abs())
+
+
+@pytest.mark.parametrize("many", ["sequences", "heads"])
+def test_the_most_sequences_and_heads(many):
+    """65535 of each: append, a weighed step and a cut, against all of them in 64
+    bits.  The sums of 64 |q k| stay below 8, scores are off by (64 + 8) 2^-24 of an
+    eighth of that, less than 2^-17.8, weights and outputs by twice that and the
+    exponential's 2^-20: 2^-16, and fp32's rounding."""
+    count, page, dim, group = 65535, 4, 64, 2
+    B, H = (count, 1) if many == "sequences" else (1, count)
+    gen = torch.Generator().manual_seed(7)
+    cache = PagedCache(B, B, 1, page_size=page, kv_heads=H, head_dim=dim, dtype=FP32, scored=True)
+    cache.reserve(page)
+    new = torch.randint(0, 4, (B,), generator=gen) if B > 1 else torch.tensor([3])
+    rows = int(new.sum())
+    k, v = (torch.rand(rows, H, dim, generator=gen) - 0.5 for _ in range(2))
+    ends = torch.cat((torch.zeros(1, dtype=torch.int64), new.cumsum(0))).int().cuda()
+    cache.append(k.cuda(), v.cuda(), ends)
+    assert torch.equal(cache.lengths.cpu(), new.int())
+    q = torch.rand(B, H * group, dim, generator=gen) - 0.5
+    one = torch.rand(2, B, H, dim, generator=gen) - 0.5
+    out = cache(q.cuda(), one[0].cuda(), one[1].cuda(), accumulate=True).cpu()
+    n = new + 1
+    # [B, H, page, dim] of what was written
+    full = torch.zeros(2, B, H, page, dim)
+    b = torch.repeat_interleave(torch.arange(B), new)
+    slot = torch.arange(rows) - torch.repeat_interleave(new.cumsum(0) - new, new)
+    full[0][b, :, slot], full[1][b, :, slot] = k, v
+    full[0][torch.arange(B), :, new], full[1][torch.arange(B), :, new] = one[0], one[1]
+    order = cache.table[:, 0].long()
+    used = torch.arange(page) < n[:, None]
+    for x, y in ((cache.k, full[0]), (cache.v, full[1])):
+        assert torch.equal(x[order].cpu().transpose(1, 2)[used], y.transpose(1, 2)[used])
+    want, p, spread = plain_attend(q.view(B, H, group, dim), full[0], full[1], n[:, None].expand(B, H))
+    assert ((out.view(want.shape).double() - want).abs() <= spread * 2.0 ** -16 + want.abs() * 2.0 ** -24).all()
+    weights = p.sum(2)
+    got = cache.scores.cpu()
+    assert ((got.double() - weights).abs() <= weights * 2.0 ** -16)[used[:, None].expand_as(got)].all()
+    # two slots stay: the newest and the heaviest other
+    before = {name: getattr(cache, name).cpu() for name in ("k", "v", "positions", "scores")}
+    cache.evict(2, recent=1)
+    assert torch.equal(cache.lengths.cpu(), n.clamp(max=2).int())
+    rank = before["scores"].masked_fill(~used[:, None], -1.0)
+    newest = torch.arange(page) == (n - 1)[:, None]
+    rank = rank.masked_fill(newest[:, None], 1e9)
+    kept = torch.sort(rank, dim=-1, descending=True, stable=True).indices[..., :2].sort(-1).values
+    held = cache.positions.cpu()[..., :2].sort(-1).values
+    live = (n >= 2)[:, None, None].expand_as(kept)
+    assert torch.equal(held[live].long(), kept[live])
+    cache.check_errors()
