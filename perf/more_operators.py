@@ -413,7 +413,7 @@ def run(state):
         return {"q": q, "k": state["k"], "v": state["v"], **into}
     if own:
         state["cache"].append(state["new_k"], state["new_v"], packed, into=state["fork"])
-        k, v = state["fork"].read(packed)
+        k, v = state["fork"].read(packed, rows=state["new_k"].shape[0])
     else:
         place = _plain_append(state, state["new_k"], into)
         k, v = (_widen(state[name][place[0], :, place[1]], state[name + "_scales"][place[0], :, place[1]])
