@@ -415,6 +415,17 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *            1 fp16, 2 fp32; -2 for another), head_dim 64, 128 or 256, the same
  *            strides for both, of 16-byte multiples with contiguous rows, all
  *            rows of a head within 2^36 bytes;
+ *            dtype 16 and 17: rows that go in and out are bf16 or fp16, the pages
+ *            hold them in 4 bits, as u8 [pages][kv_heads][page_size][head_dim / 2]
+ *            of codes (the even dim in the lower half of a byte; strides in
+ *            bytes) and
+ *   k_scales, v_scales  u8 [pages][kv_heads][page_size][head_dim / 32], strides in
+ *            bytes (multiples of head_dim / 32, as are the addresses): for every
+ *            32 dims a byte s >= 2, the codes 0 .. 7 standing for 0, 0.5, 1, 1.5,
+ *            2, 3, 4 and 6 times 2^(s - 127), 8 .. 15 for their negatives; all are
+ *            NaN where s is 255.  A row is held with the smallest s >= 2 for which
+ *            no value is above 7 times that (at most 252, and 255 for infinities and
+ *            NaN) and the nearest codes, ties to even;
  *   table    i32 [sequences][max_pages]: the page of slots [i page_size,
  *            (i + 1) page_size) of a sequence; an entry outside [0, pages) is no
  *            page.  slots = max_pages * page_size <= 2^30, sequences * slots <
@@ -426,9 +437,11 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *            where nothing is scored);
  *   err      16 bytes, 8-byte aligned: the error word, set to 4 when a slot
  *            below a length has no page (a row to append to it is dropped;
- *            attention reads page 0 in its place; a move is left out) and to 8
- *            when an append's offsets do not cover its rows, and at byte offset 8
- *            the optional host word's address, as in a workspace.
+ *            attention reads page 0 in its place; a move is left out), to 8 when
+ *            an append's offsets do not cover its rows, to 16 when those of a
+ *            prompt or a read do not and to 32 when these ask for more rows than a
+ *            sequence holds, and at byte offset 8 the optional host word's address,
+ *            as in a workspace.
  * Results go to a second cache `into` over the same pages and table: the first
  * itself, or one whose lengths, seen, scores and positions do not overlap the
  * first's (refused).  A page that belongs to several tables may be read, not written.
@@ -440,6 +453,8 @@ typedef struct prismkv_paged_cache {
   uint64_t k, v, table, lengths, seen, scores, positions, err;
   int64_t pages, page_stride, head_stride, slot_stride;
   int32_t sequences, kv_heads, head_dim, page_size, max_pages, dtype;
+  uint64_t k_scales, v_scales;                                            /* these five of dtype 16 and 17 only */
+  int64_t scale_page_stride, scale_head_stride, scale_slot_stride;
 } prismkv_paged_cache;
 
 /* Row i of sequence b's new rows (rows offsets[b] .. offsets[b + 1] of k and v
@@ -480,6 +495,36 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
 size_t prismkv_paged_evict_work_bytes(int sequences, int kv_heads, int64_t slots);
 int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t keeps,
                         uint64_t paged_work, int keep, int recent, int sinks, size_t work_bytes, uint64_t stream);
+
+/* prismkv_paged_append with the rows of k, and of q [rows][heads][head_dim], turned by
+ * their positions p on the way (lengths[b] + i, of a scored cache seen[b] + i): dims x
+ * and y of a pair become x cos - y sin and y cos + x sin, times `amplitude`, of the angle
+ * p turns[j] / 2^64 of a full turn; pair j is dims j and j + rotary_dim / 2, or with
+ * `interleaved` 2j and 2j + 1, of the first rotary_dim (a multiple of 16, up to
+ * head_dim) dims; turns is u64 [rotary_dim / 2].  The turned q goes to q_out, contiguous;
+ * strides of q as of k and v.  q may be 0 (heads 0).  turns 0: nothing is turned, and q
+ * is 0.  Turned rows are rounded to their type before they are held in 4 bits. */
+int prismkv_paged_append_rows(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t k, uint64_t v,
+                              uint64_t q, uint64_t q_out, uint64_t offsets, uint64_t turns, int64_t rows,
+                              int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                              int64_t q_row_stride, int64_t q_head_stride, int heads, int rotary_dim, int interleaved,
+                              double amplitude, uint64_t stream);
+
+/* The last offsets[b + 1] - offsets[b] slots of every sequence (offsets as for the
+ * append; 0: one each) -> k_out, v_out [rows][kv_heads][head_dim], contiguous, of the
+ * rows' type; rows of slots before a sequence's first are 0. */
+int prismkv_paged_read(const prismkv_paged_cache* cache, uint64_t offsets, uint64_t k_out, uint64_t v_out, int64_t rows,
+                       uint64_t stream);
+
+/* Causal attention of the last m = offsets[b + 1] - offsets[b] slots' queries of every
+ * sequence (q [rows][kv_heads * group][head_dim], packed; offsets as above) over its
+ * slots: row i sees slots t <= lengths[b] - m + i; out as q, 0 where there is none; lse
+ * f32 [rows][kv_heads * group] (or 0) as for prismkv_paged_attend.  The workspace
+ * needs no preparation. */
+size_t prismkv_paged_prompt_work_bytes(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots,
+                                       int dtype);
+int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t offsets, uint64_t lse, uint64_t paged_work,
+                         uint64_t out, int64_t rows, int group, double scale, size_t work_bytes, uint64_t stream);
 
 #ifdef __cplusplus
 }

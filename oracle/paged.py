@@ -74,3 +74,104 @@ def evict(scores, positions, n, keep, seen, recent=0, sinks=0):
     sources = [t for t in range(m, n) if t in kept]
     holes = [t for t in range(m) if t not in kept]
     return list(zip(sources, holes))
+
+
+# ------------------------------------------------------------------ whole prompts
+
+def prompt(q, k, v, new, dtype=None, scale=None):
+    """Causal attention of one sequence's last `new` slots: q [new, heads, D], its rows
+    k, v [kv_heads, n, D] -> (out [new, heads, D], lse [new, heads]) in fp64 and bounds
+    of what the device may change of them.
+
+    As for `attend`, and P is rounded once to q's type (half a step, `half`, of
+    each weight; fp16 weights below 2^-29 of the largest, and at least 2^-39 of
+    it, by 2^-39 more), which fp32 is not."""
+    m, heads, D = q.shape
+    H, n = k.shape[0], k.shape[1]
+    scale = 1 / math.sqrt(D) if scale is None else scale
+    dtype = q.dtype if dtype is None else dtype
+    half = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}[dtype]
+    out, bound = (torch.zeros(m, heads, D, dtype=torch.float64) for _ in range(2))
+    lse, lse_bound = torch.full((m, heads), -math.inf, dtype=torch.float64), torch.zeros(m, heads, dtype=torch.float64)
+    later = torch.arange(n)[None] > (n - m + torch.arange(m))[:, None]
+    for g in range(heads):
+        kd, vd, qd = k[g * H // heads].double(), v[g * H // heads].double(), q[:, g].double()
+        s = (qd @ kd.T * scale).masked_fill(later, -math.inf)
+        delta = ((qd.abs() @ kd.abs().T).masked_fill(later, 0).amax(-1) * abs(scale)) * (D + 8) * 2.0 ** -24
+        lse[:, g] = torch.logsumexp(s, -1)
+        p = torch.exp(s - lse[:, g, None])
+        p[torch.isinf(lse[:, g])] = 0
+        out[:, g] = p @ vd
+        rel = 2 * delta + 2.0 ** -20 + n * 2.0 ** -24
+        rounded, least = (0, 0) if dtype == torch.float32 else (half, 2.0 ** -38 if dtype == torch.float16 else 0)
+        lost = (p @ vd.abs()) * (rel[:, None] + rounded) + least * p.amax(-1)[:, None] * ((~later).double() @ vd.abs())
+        floor = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}[dtype]
+        bound[:, g] = out[:, g].abs() * half + lost * (1 + half) + floor
+        lse_bound[:, g] = delta + 2.0 ** -20 + n * 2.0 ** -24 + lse[:, g].abs() * 2.0 ** -22
+    return (out, lse), (bound, lse_bound)
+
+
+# ------------------------------------------------------------------ 4 bits
+
+SIZES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def hold(x):
+    """Codes [..., D] (0 .. 15) and scale bytes [..., D / 32] of rows [..., D], by the
+    definition: the smallest power of two, at least 2^-125 and at most 2^125, for which no value
+    is above 7 times it; the nearest of the sizes, the even code on ties."""
+    y = x.double().unflatten(-1, (-1, 32))
+    amax = y.abs().amax(-1)
+    special = ~torch.isfinite(amax)
+    e = torch.full(amax.shape, -125, dtype=torch.int32)
+    for power in range(-125, 125):
+        e[amax > 7 * 2.0 ** power] = power + 1
+    unit = torch.pow(torch.tensor(2.0, dtype=torch.float64), e.double())[..., None]
+    size = torch.nan_to_num(y.abs() / unit, nan=0.0, posinf=0.0)
+    distance = (size[..., None] - torch.tensor(SIZES, dtype=torch.float64)).abs()
+    nearest = distance.amin(-1, keepdim=True)
+    even = torch.tensor([i % 2 == 0 for i in range(8)])
+    tie = ((distance == nearest) & even).any(-1) & ((distance == nearest).sum(-1) > 1)
+    code = torch.where(tie, ((distance == nearest) & even).double().argmax(-1), distance.argmin(-1))
+    code = code + 8 * torch.signbit(y).long()
+    byte = torch.where(special, 255, e + 127)
+    return code.flatten(-2).to(torch.uint8), byte.to(torch.uint8)
+
+
+def pack(codes):
+    """Two codes a byte, the even dim's in the lower half."""
+    return codes[..., 0::2] | (codes[..., 1::2] << 4)
+
+
+def value(codes, scales):
+    """What codes [..., D] (0 .. 15) and scale bytes stand for, in fp64."""
+    sizes = torch.tensor(SIZES + tuple(-s for s in SIZES), dtype=torch.float64)[codes.long()]
+    unit = torch.pow(torch.tensor(2.0, dtype=torch.float64), scales.double() - 127)
+    unit[scales == 255] = math.nan
+    return (sizes.unflatten(-1, (-1, 32)) * unit[..., None]).flatten(-2)
+
+
+def unpack(packed):
+    return torch.stack((packed & 15, packed >> 4), -1).flatten(-2)
+
+
+# ------------------------------------------------------------------ rotary positions
+
+def turn(x, positions, frequencies, amplitude=1.0, interleaved=False):
+    """Rows x [rows, heads, D] turned by positions [rows] in fp64, and the bound of what
+    the device may change: its angle is off by 2^-22 (a fraction of a turn in fp32 and
+    the sine's own error), sine, cosine, their products and the sum by 2^-22 of their
+    terms, and the result is rounded once to x's type."""
+    part = 2 * len(frequencies)
+    angle = torch.remainder(positions.double()[:, None] * frequencies[None].double(), 2 * math.pi)[:, None]
+    cos, sin = torch.cos(angle) * amplitude, torch.sin(angle) * amplitude
+    y = x.double().clone()
+    spread = torch.zeros_like(y)
+    first, second = (slice(0, part, 2), slice(1, part, 2)) if interleaved else (slice(0, part // 2), slice(part // 2, part))
+    a, b = x[..., first].double(), x[..., second].double()
+    y[..., first], y[..., second] = a * cos - b * sin, b * cos + a * sin
+    spread[..., first] = spread[..., second] = (a.abs() + b.abs()) * abs(amplitude)
+    half = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}[x.dtype]
+    floor = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}[x.dtype]
+    bound = y.abs() * half * (spread > 0) + spread * 2.0 ** -21 * (1 + half) + floor * (spread > 0)
+    return y, bound

@@ -72,6 +72,10 @@ SIGNATURES = {
     "prismkv_paged_attend": ([_PTR] * 2 + [_U64] * 4 + [_I32, _I32, _F64, _SZ], True, _I32),
     "prismkv_paged_evict_work_bytes": ([_I32, _I32, _I64], False, _SZ),
     "prismkv_paged_evict": ([_PTR] * 2 + [_U64] * 2 + [_I32] * 3 + [_SZ], True, _I32),
+    "prismkv_paged_append_rows": ([_PTR] * 2 + [_U64] * 6 + [_I64] * 7 + [_I32] * 3 + [_F64], True, _I32),
+    "prismkv_paged_read": ([_PTR] + [_U64] * 3 + [_I64], True, _I32),
+    "prismkv_paged_prompt_work_bytes": ([_I64] + [_I32] * 4 + [_I64, _I32], False, _SZ),
+    "prismkv_paged_prompt": ([_PTR] + [_U64] * 5 + [_I64, _I32, _F64, _SZ], True, _I32),
     # error handling of the bounded inter-workgroup waits
     "prismkv_set_spin_limit": ([_I32], False, _I32),
     "prismkv_get_spin_limit": ([], False, _I32),
@@ -85,7 +89,9 @@ class PagedCacheDesc(ctypes.Structure):
     """prismkv_paged_cache of include/prismkv_hip.h."""
     _fields_ = [(name, _U64) for name in ("k", "v", "table", "lengths", "seen", "scores", "positions", "err")] + \
                [(name, _I64) for name in ("pages", "page_stride", "head_stride", "slot_stride")] + \
-               [(name, _I32) for name in ("sequences", "kv_heads", "head_dim", "page_size", "max_pages", "dtype")]
+               [(name, _I32) for name in ("sequences", "kv_heads", "head_dim", "page_size", "max_pages", "dtype")] + \
+               [(name, _U64) for name in ("k_scales", "v_scales")] + \
+               [(name, _I64) for name in ("scale_page_stride", "scale_head_stride", "scale_slot_stride")]
 
 
 _loaded: dict[str, "Library"] = {}

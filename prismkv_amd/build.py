@@ -21,7 +21,8 @@ from pathlib import Path
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 INCLUDE = PACKAGE.parent / "include"
-SOURCES = ["route.hip", "union.hip", "attend.hip", "decode.hip", "update.hip", "paged.hip"]
+SOURCES = ["route.hip", "union.hip", "attend.hip", "decode.hip", "update.hip", "paged.hip", "paged4.hip",
+           "paged_rows.hip", "prompt.hip"]
 LIBRARY_NAME = "libprismkv_hip.so"
 ARCH = "gfx950"
 

@@ -4,25 +4,6 @@
 #include "attend_core.h"
 
 namespace prismkv {
-namespace {
-
-constexpr int kPT = 256;  // threads of the paged kernels but the selection
-// Error word: a slot within a sequence's length has no page of the cache; an append's
-// offsets do not cover its rows.
-constexpr unsigned kErrPages = 4u, kErrRows = 8u;
-
-// Element types of the C ABI (`dtype`).
-constexpr int kBf16 = 0, kFp16 = 1, kFp32 = 2;
-template <int DT>
-constexpr int kElem = DT == kFp32 ? 4 : 2;
-// P is held times 2^kBias: fp16 probabilities from 2^-29 of the maximum up stay
-// normal numbers (bf16 and fp32 have the exponents for them).
-template <int DT>
-constexpr int kBias = DT == kFp16 ? 15 : 0;
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // t / page_size of 0 <= t < 2^31 by one product (shift = 31 + ceil(log2 page_size),
 // mul = ceil(2^shift / page_size) < 2^32: exact over that range).
@@ -31,18 +12,6 @@ struct PageDiv {
   int shift;
   __device__ __forceinline__ int of(int t) const { return (int)(((unsigned long long)(unsigned)t * mul) >> shift); }
 };
-
-// Workgroups that the attention's rows are dealt to: one on each of the 256 CUs,
-// of 8 waves (two a SIMD, each with a tile in flight), or of 4 where a tile of
-// head_dim 256 takes the registers of two.  Two workgroups of 4 waves read as fast,
-// but leave twice the partial states to join (64K: 54.0 us against 47.8).
-constexpr int kUnits = 256;
-template <int D>
-constexpr int kAWaves = D == 256 ? 4 : 8;
-constexpr int kQuantum = 32;  // tokens that are dealt at a time
-// Quanta of a workgroup at least: a tile (32 tokens, fp32 16) for each wave.
-template <int DT, int D>
-constexpr int kLeast = DT == kFp32 ? kAWaves<D> / 2 : kAWaves<D>;
 
 struct PagedAttend {
   const void *q, *k, *v;
@@ -58,8 +27,57 @@ struct PagedAttend {
   PageDiv div;
   int sequences, kv_heads, group, tiles, page_size, max_pages, pages;
   float scale;  // log2(e) times the caller's
+  // pages in 4 bits: the scales' pages, their strides in bytes
+  const uint8_t *k_scales, *v_scales;
+  int64_t scale_page, scale_head;
+  unsigned scale_slot;
   bool many;    // kSoloPairs pairs or more
 };
+
+// The attention over pages in 4 bits (defined in paged4.hip).
+int attend_in_four(const PagedAttend& a, int dtype, int head_dim, int64_t units, hipStream_t stream);
+
+namespace {
+
+constexpr int kPT = 256;  // threads of the paged kernels but the selection
+// Error word: a slot within a sequence's length has no page of the cache; an append's
+// offsets do not cover its rows; the offsets of a prompt or a read do not cover its
+// rows; they ask for more rows than a sequence holds.
+constexpr unsigned kErrPages = 4u, kErrRows = 8u, kErrOffsets = 16u, kErrHeld = 32u;
+
+// Element types of the C ABI (`dtype`): of the rows that go in and out and, unless
+// kFour is added (pages in 4 bits), of the pages.
+constexpr int kBf16 = 0, kFp16 = 1, kFp32 = 2, kFour = 16;
+template <int DT>
+constexpr int kType = DT & 15;
+template <int DT>
+constexpr bool kInFour = DT >= kFour;
+template <int DT>
+constexpr int kElem = kType<DT> == kFp32 ? 4 : 2;
+// P is held times 2^kBias: fp16 probabilities from 2^-29 of the maximum up stay
+// normal numbers (bf16 and fp32 have the exponents for them).
+template <int DT>
+constexpr int kBias = kType<DT> == kFp16 ? 15 : 0;
+// ... and the sum of P times 2^kSumBias: fp16 pages in 4 bits are widened to half
+// their values (the largest, 65536, is no fp16 number), which halving the sum undoes.
+template <int DT>
+constexpr int kSumBias = kBias<DT> - (DT == (kFour | kFp16) ? 1 : 0);
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Workgroups that the attention's rows are dealt to: one on each of the 256 CUs,
+// of 8 waves (two a SIMD, each with a tile in flight), or of 4 where a tile of
+// head_dim 256 takes the registers of two.  Two workgroups of 4 waves read as fast,
+// but leave twice the partial states to join (64K: 54.0 us against 47.8).
+constexpr int kUnits = 256;
+template <int D>
+constexpr int kAWaves = D == 256 ? 4 : 8;
+constexpr int kQuantum = 32;  // tokens that are dealt at a time
+// Quanta of a workgroup at least: a tile (32 tokens, fp32 16) for each wave.
+template <int DT, int D>
+constexpr int kLeast = kType<DT> == kFp32 ? kAWaves<D> / 2 : kAWaves<D>;
 
 // 16 bytes that another workgroup wrote through (agent scope, as ld_dev).
 __device__ __forceinline__ float4 ld_dev4(__amdgpu_buffer_rsrc_t r, unsigned byte_offset) {
@@ -181,10 +199,10 @@ __device__ __forceinline__ PagedSpan<kL> find_span(const PagedAttend& a, int uni
   }
 }
 
-// log2 of a softmax's sum from its maximum and the sum held times 2^kBias.
+// log2 of a softmax's sum from its maximum and the sum held times 2^kSumBias.
 template <int DT>
 __device__ __forceinline__ float log_sum(float M, float den) {
-  return den == 0.f ? -INFINITY : M + (log2f(den) - kBias<DT>);
+  return den == 0.f ? -INFINITY : M + (log2f(den) - kSumBias<DT>);
 }
 
 // Writes output element i (query head i / D of the tile, dim i % D) from the
@@ -193,14 +211,14 @@ template <int DT, int D>
 __device__ __forceinline__ void finish(const PagedAttend& a, size_t head0, int i, float M, float den, float x) {
   const float y = den == 0.f ? 0.f : x / den;
   const size_t at = head0 * D + i;
-  if constexpr (DT == kBf16) reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(y);
-  else if constexpr (DT == kFp16) reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)y;
+  if constexpr (kType<DT> == kBf16) reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(y);
+  else if constexpr (kType<DT> == kFp16) reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)y;
   else reinterpret_cast<float*>(a.out)[at] = y;
   if (i % D == 0) {
     if (a.lse_out) a.lse_out[head0 + i / D] = log_sum<DT>(M, den) * 0.693147180559945309f;
     if (a.sums_work)
       a.sums_work[head0 + i / D] =
-          den == 0.f ? make_float2(0.f, 0.f) : make_float2(M, (float)(1 << kBias<DT>) / den);
+          den == 0.f ? make_float2(0.f, 0.f) : make_float2(M, (float)(1 << kSumBias<DT>) / den);
   }
 }
 
@@ -230,6 +248,9 @@ struct PagedEvict {
   int64_t page_bytes, head_bytes, slot_bytes, moves;
   PageDiv div;
   int sequences, kv_heads, log_pieces, page_size, max_pages, pages, slots, keep, recent, sinks, part, most_parts;
+  char *k_scales, *v_scales;  // of pages in 4 bits: a row's scale_bytes (else 0)
+  int64_t scale_page, scale_head, scale_slot;
+  int scale_bytes;
 };
 
 }  // namespace

@@ -7,660 +7,14 @@
 // table[b][t / page_size].  A table entry outside [0, pages) within a
 // sequence's length is reported through the cache's error word and never read
 // through.
-#include "paged.h"
+#include "paged_attend.h"
+#include "paged_host.h"
 
 #include <cfloat>
 
-#include "prismkv_hip.h"
 
 namespace prismkv {
 namespace {
-
-// ------------------------------------------------------------------ attention
-//
-// s_t = scale q.k_t, p_t = e^(s_t - m) / z, o = sum p_t v_t for the `group`
-// query heads of one KV head: every K and V row is read once for all of them
-// (2 bytes x 2 head_dim per 4 group head_dim flops), so the kernel is bound by
-// the reads.  One pass with the running maximum and sum (flash form).
-//
-// Split: the tokens of all pairs of a sequence and a KV head (with more than 16
-// query heads a tile of them) are dealt evenly to the workgroups, on the device,
-// where the lengths are; a workgroup's share may end one pair and begin others.
-// Each of its waves takes every 8th 32-token tile (fp32: 16 tokens) by itself: no
-// barrier and no LDS until the waves' states meet at a pair's end.  A pair of
-// several workgroups is joined from their states in the order of its tokens, by
-// the last to arrive or by a second launch, so the result does not depend on the
-// order of arrival.
-//
-// Measured (MI355X, launches after one another in a graph): 65792 tokens, 8 x 4
-// heads, bf16, 47.3 us = 5.7 TB/s; 32 sequences of 6.4K tokens 136 us = 6.2 TB/s
-// (a plain read of as much memory reaches 6.9); 16 x 8192 of head_dim 256 in fp32, 2
-// x 4 heads, 92 us = 5.9; of head_dim 64, 8 x 4 heads, 48 us = 5.6; 75 tokens 6.4 us.
-// About 6 us of a call are the launch and the chain lengths -> page -> rows, 3.7 more
-// the join (65792 tokens 43.7 us without it).
-
-// 16-bit types: P is a sum of terms of the type, each with a product of its own into
-// one accumulator: bf16 takes three, which hold all 24 bits of an fp32 p (with two,
-// outputs that cancel are off by 2^-17 of their terms; 65792 tokens, 8 x 4 heads take
-// as long with either), fp16 two, 22 bits.  Every term is positive wherever p is, so
-// that an infinite V is not multiplied by a term of 0: at least the type's least
-// number, which for fp16, with its bias, is 2^-39 of the maximum's weight.
-// The tile of one step as loaded.  16-bit (32 tokens, two 16-token blocks):
-// lane (j, q) holds row j of each block at dims 32c + 8q .. +8 (K, the A operand
-// of the 16x16x32 product) and of rows 4q + t (V) 16 bytes out of every 256 (8 of
-// head_dim 64's 128), so that the 16 lanes of a load cover whole rows.  Column
-// block n of the output takes element n of a lane, dim(n, j); the rows' pairs are
-// joined per dim with one byte permutation.
-// fp32 (16 tokens): K dims 16c + 4q .. +4 (four 16x16x4 products per load), V
-// the same with float columns.
-template <int DT, int D>
-struct Tile {
-  static constexpr int kBlocks = DT == kFp32 ? 1 : 2;
-  static constexpr int kTokens = 16 * kBlocks;
-  static constexpr int kKLoads = D * kElem<DT> / 64;        // 16-byte loads of a K row per lane
-  static constexpr int kVWords = D * kElem<DT> / 64;        // 32-bit words of a V row per lane
-  static constexpr int kVStep = kVWords < 4 ? 4 * kVWords : 16;  // bytes of a piece
-  static constexpr int kRun = kVStep / kElem<DT>;           // elements of a piece
-  static __device__ __forceinline__ int dim(int n, int j) { return n / kRun * (16 * kRun) + j * kRun + n % kRun; }
-  uint4 k[kBlocks][kKLoads];
-  unsigned v[kBlocks][4][kVWords];
-};
-
-template <int W>
-__device__ __forceinline__ void load_words(unsigned (&dst)[W], const char* p) {
-  if constexpr (W == 2) {
-    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
-    dst[0] = x.x;
-    dst[1] = x.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; i += 4) {
-      const uint4 x = load_nt16(p + 64 * i);
-      dst[i] = x.x;
-      dst[i + 1] = x.y;
-      dst[i + 2] = x.z;
-      dst[i + 3] = x.w;
-    }
-  }
-}
-
-template <int W>
-__device__ __forceinline__ void load_words_buf(unsigned (&dst)[W], __amdgpu_buffer_rsrc_t r, unsigned byte_offset) {
-  if constexpr (W == 2) {
-    const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, byte_offset, 0, 2);
-    dst[0] = x[0];
-    dst[1] = x[1];
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; i += 4) {
-      const uint4 x = load_nt16_buf(r, byte_offset + 64 * i);
-      dst[i] = x.x;
-      dst[i + 1] = x.y;
-      dst[i + 2] = x.z;
-      dst[i + 3] = x.w;
-    }
-  }
-}
-
-// Element N of two rows' words as a pair (low half from a).
-template <int N, int W>
-__device__ __forceinline__ unsigned pair16(const unsigned (&a)[W], const unsigned (&b)[W]) {
-  return __builtin_amdgcn_perm(b[N >> 1], a[N >> 1], (N & 1) ? 0x07060302u : 0x05040100u);
-}
-
-template <int DT>
-__device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (DT == kBf16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                   0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// p >= 0 as terms of the 16-bit type, each in the upper half of a word.  A NaN may be
-// lost here: the sum of the weights has it.
-template <int DT>
-constexpr int kTerms = DT == kBf16 ? 3 : 2;
-template <int DT>
-__device__ __forceinline__ void split16(float p, unsigned (&term)[kTerms<DT>]) {
-  if constexpr (DT == kBf16) {
-    // 8 bits each from the top, which is exact (as signed integers: a remainder
-    // below 0 is left behind a term that was raised)
-    const int least = p > 0.f ? 0x10000 : 0;
-    const int hi = max(__float_as_int(p) & (int)0xffff0000, least);
-    const float rest = p - __int_as_float(hi);
-    const int mid = max(__float_as_int(rest) & (int)0xffff0000, least);
-    term[0] = (unsigned)hi;
-    term[1] = (unsigned)mid;
-    term[2] = (unsigned)max(__float_as_int(rest - __int_as_float(mid)), least);
-  } else {
-    // the head rounded down, so that the remainder is positive
-    const float least = p > 0.f ? 0x1p-24f : 0.f, head = fmaxf(p, least);
-    const auto h = __builtin_amdgcn_cvt_pkrtz(0.f, head);  // {0, head}
-    const _Float16 l = (_Float16)fmaxf(head - (float)h[1], least);
-    term[0] = __builtin_bit_cast(unsigned, h);
-    term[1] = (unsigned)__builtin_bit_cast(unsigned short, l) << 16;
-  }
-}
-
-// The upper halves of two words (low half from a).
-__device__ __forceinline__ unsigned upper16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-
-template <int N, int DT, int D>
-__device__ __forceinline__ void pv_columns(f32x4 (&acc)[D / 16], const Tile<DT, D>& t,
-                                           const u32x4 (&p)[kTerms<DT>]) {
-  if constexpr (N < D / 16) {
-    const u32x4 vb = {pair16<N>(t.v[0][0], t.v[0][1]), pair16<N>(t.v[0][2], t.v[0][3]),
-                      pair16<N>(t.v[1][0], t.v[1][1]), pair16<N>(t.v[1][2], t.v[1][3])};
-#pragma unroll
-    for (int i = 0; i < kTerms<DT>; ++i) acc[N] = mfma32<DT>(p[i], vb, acc[N]);
-    pv_columns<N + 1, DT, D>(acc, t, p);
-  }
-}
-
-// 2^(scale s - m): one rounding of the difference.  m is a rounded product itself;
-// from 2^22 on, where its rounding is 1/8 and more (and at 2^32 takes all of the
-// exponent's range), the other products are rounded as it was, so that the largest
-// score's weight is 1.  m is finite or +infinity (no_less): where no score is above
-// -infinity, 0 serves.
-__device__ __forceinline__ float weight(float s, float scale, float m) {
-#pragma clang fp contract(off)
-  const float product = s * scale;
-  const float rounded = product - m;
-  return __builtin_amdgcn_exp2f(fabsf(m) < 0x1p22f ? fmaf(s, scale, -m) : rounded);
-}
-__device__ __forceinline__ float no_less(float m) { return m == -INFINITY ? 0.f : m; }
-
-// Factor of a state with maximum m under the joint maximum M >= m (no state: 0).
-__device__ __forceinline__ float rescale(float m, float M) {
-  return m == -INFINITY ? 0.f : m == M ? 1.f : exp2f(m - M);
-}
-
-// The joint maximum and sum of a pair's head g over its states, and the states'
-// factors in wt[c * stride] (LDS); by one wave.
-__device__ __forceinline__ float2 join_sums(const float* base, const PagedParts& parts, unsigned state_stride, int g,
-                                            float* wt, int stride) {
-  const int lane = threadIdx.x & 63;
-  float M = -INFINITY, den = 0.f;
-  for (int c0 = 0; c0 < parts.chunks; c0 += 64) {
-    const int c = c0 + lane;
-    const bool in = c < parts.chunks;
-    const float2 mz = ld_dev2(base + (in && c ? 2 * c : parts.odd) * state_stride + 2 * g);
-    const float m = in ? mz.x : -INFINITY;
-    const float nM = fmaxf(M, wave_max(m));
-    den = den * rescale(M, nM) + wave_sum(in ? rescale(m, nM) * mz.y : 0.f);
-    M = nM;
-    if (in && wt) wt[c * stride] = m;
-  }
-  if (wt)
-    for (int c = lane; c < parts.chunks; c += 64) wt[c * stride] = rescale(wt[c * stride], M);
-  return make_float2(M, den);
-}
-
-// Joins columns [col0, col0 + columns) (4 floats each of the [rows][D] output) of a
-// pair's states, by a workgroup of kThreads: the maxima and sums a wave per head,
-// while the first states' loads are in flight, then a thread per column and share
-// of the states, the shares added in LDS.
-template <int DT, int D, int kThreads>
-__device__ __forceinline__ void join_states(const PagedAttend& a, size_t head0, int rows, const PagedParts& parts, int col0,
-                                            int columns, float* lds) {
-  const int tid = threadIdx.x, w = tid >> 6;
-  float4* part = reinterpret_cast<float4*>(lds);  // [threads]
-  float* top = lds + 4 * kThreads;                // [16] joint maxima, [16] sums
-  float* wt = top + 32;                           // [chunks][rows] factors
-  const float* base = a.state + (size_t)2 * parts.unit * a.state_stride;
-  const __amdgpu_buffer_rsrc_t r = raw_buffer(base, 2 * parts.chunks * (int)a.state_stride * 4);
-  const int chunks = parts.chunks;
-  const int shares = max(kThreads / columns, 1), share = tid / columns;  // (columns > threads: in turns)
-  constexpr int kU = 8;
-  float4 x[kU];
-  auto load = [&](int c0, int col) {
-#pragma unroll
-    for (int e = 0; e < kU; ++e) {
-      const int c = min(c0 + e * shares, chunks - 1);
-      x[e] = ld_dev4(r, ((unsigned)(c ? 2 * c : parts.odd) * a.state_stride + 2 * rows + 4 * col) * 4);
-    }
-  };
-  int col = col0 + tid - share * columns;
-  load(share, col);
-  const int head = 4 * col0 / D, heads = (4 * (col0 + columns) - 1) / D + 1;  // of these columns
-  for (int i = head + w; i < heads; i += kThreads / 64) {
-    const float2 mz = join_sums(base, parts, a.state_stride, i, wt + i, rows);
-    if ((tid & 63) == 0) {
-      top[i] = mz.x;
-      top[16 + i] = mz.y;
-    }
-  }
-  __syncthreads();
-  while (true) {
-    const int g = 4 * col / D;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c0 = share; share < shares && c0 < chunks;) {
-#pragma unroll
-      for (int e = 0; e < kU; ++e) {
-        const int c = c0 + e * shares;
-        if (c < chunks) {
-          const float f = wt[c * rows + g];
-          sum.x = fmaf(f, x[e].x, sum.x);
-          sum.y = fmaf(f, x[e].y, sum.y);
-          sum.z = fmaf(f, x[e].z, sum.z);
-          sum.w = fmaf(f, x[e].w, sum.w);
-        }
-      }
-      c0 += kU * shares;
-      if (c0 < chunks) load(c0, col);
-    }
-    if (shares > 1) {  // (then all columns are in this turn)
-      part[tid] = sum;
-      __syncthreads();
-      for (int k = 1; share == 0 && k < shares; ++k) {
-        const float4 y = part[tid + k * columns];
-        sum.x += y.x;
-        sum.y += y.y;
-        sum.z += y.z;
-        sum.w += y.w;
-      }
-    }
-    if (share == 0) {
-      finish<DT, D>(a, head0, 4 * col, top[g], top[16 + g], sum.x);
-      finish<DT, D>(a, head0, 4 * col + 1, top[g], top[16 + g], sum.y);
-      finish<DT, D>(a, head0, 4 * col + 2, top[g], top[16 + g], sum.z);
-      finish<DT, D>(a, head0, 4 * col + 3, top[g], top[16 + g], sum.w);
-    }
-    col += kThreads;
-    if (shares > 1 || col >= col0 + columns) return;
-    load(share, col);
-  }
-}
-
-// Where a wave's tiles lie.  `ask` looks up the pages of the tile at t0, `move`
-// makes it the tile that is loaded.
-template <int DT, int D, bool kAligned>
-struct Rows;
-
-// Pages of whole 16-token blocks: a block's page is the same for all lanes, so it
-// is looked up through the scalar cache, beside the vector loads' order, and read
-// through a buffer resource of its own that ends with the last token: rows past
-// the end come back as zeros, a block past the end is not read at all, and a lane
-// has one fixed offset per row.
-template <int DT, int D>
-struct Rows<DT, D, true> {
-  typedef Tile<DT, D> T;
-  const PagedAttend& a;
-  const char *k, *v;
-  const int32_t* tab;
-  unsigned k_lane, v_lane[4];
-  int end;
-  int token[T::kBlocks], page[T::kBlocks];
-  __amdgpu_buffer_rsrc_t kr[T::kBlocks], vr[T::kBlocks];
-  bool bad = false;
-  __device__ __forceinline__ Rows(const PagedAttend& a, int b, int h, int end) : a(a), end(end) {
-    const unsigned lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4, slot = a.slot_units << 4;
-    k = reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes;
-    v = reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes;
-    tab = a.table + (size_t)b * a.max_pages;
-    k_lane = j * slot + 16 * q;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v_lane[r] = (4 * q + r) * slot + j * T::kVStep;
-  }
-  __device__ __forceinline__ void ask(int t0) {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) {
-      token[i] = t0 + 16 * i;
-      typedef const __attribute__((address_space(4))) int32_t* Uniform;
-      page[i] = *(Uniform)(uint64_t)(tab + __builtin_amdgcn_readfirstlane(a.div.of(min(token[i], end - 1))));
-    }
-  }
-  __device__ __forceinline__ void move() {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) {
-      const int rows = min(end - token[i], 16);
-      bad |= rows > 0 && (unsigned)page[i] >= (unsigned)a.pages;
-      const unsigned from = (unsigned)page[i] < (unsigned)a.pages ? (unsigned)page[i] : 0u;
-      const size_t at = ((size_t)from * a.page_units +
-                         (unsigned)(token[i] - a.div.of(token[i]) * a.page_size) * a.slot_units) << 4;
-      const int bytes = rows > 0 ? (int)((rows - 1) * (a.slot_units << 4)) + D * kElem<DT> : 0;
-      kr[i] = raw_buffer(k + at, bytes);
-      vr[i] = raw_buffer(v + at, bytes);
-    }
-  }
-  __device__ __forceinline__ void load_k(T& t) const {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int c = 0; c < T::kKLoads; ++c) t.k[i][c] = load_nt16_buf(kr[i], k_lane + 64 * c);
-  }
-  __device__ __forceinline__ void load_v(T& t) const {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) load_words_buf(t.v[i][r], vr[i], v_lane[r]);
-  }
-};
-
-// Any page size: each lane looks up the rows that it loads keys of, and takes the
-// values' rows from the lanes that have them.  Tokens past the end repeat the last.
-template <int DT, int D>
-struct Rows<DT, D, false> {
-  typedef Tile<DT, D> T;
-  const PagedAttend& a;
-  const char *k, *v;
-  const int32_t* tab;
-  int end, token[T::kBlocks], page[T::kBlocks];
-  unsigned row[T::kBlocks];  // 16-byte units
-  bool bad = false;
-  __device__ __forceinline__ Rows(const PagedAttend& a, int b, int h, int end) : a(a), end(end) {
-    const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
-    k = reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes + 16 * q;
-    v = reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes + j * T::kVStep;
-    tab = a.table + (size_t)b * a.max_pages;
-  }
-  __device__ __forceinline__ void ask(int t0) {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) {
-      token[i] = min(t0 + 16 * i + (int)(threadIdx.x & 15), end - 1);
-      page[i] = tab[a.div.of(token[i])];
-    }
-  }
-  __device__ __forceinline__ void move() {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) {
-      if ((unsigned)page[i] >= (unsigned)a.pages) {
-        bad = true;
-        page[i] = 0;
-      }
-      row[i] = (unsigned)page[i] * a.page_units +
-               (unsigned)(token[i] - a.div.of(token[i]) * a.page_size) * a.slot_units;
-    }
-  }
-  __device__ __forceinline__ void load_k(T& t) const {
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int c = 0; c < T::kKLoads; ++c) t.k[i][c] = load_nt16(k + ((size_t)row[i] << 4) + 64 * c);
-  }
-  __device__ __forceinline__ void load_v(T& t) const {
-    const int q = (threadIdx.x & 63) >> 4;
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) load_words(t.v[i][r], v + ((size_t)(unsigned)__shfl((int)row[i], 4 * q + r) << 4));
-  }
-};
-
-// `count` quanta of one pair from its quantum u.first on: this workgroup's state
-// of them, and the pair's output if it is the only or the last to come.
-template <int DT, int D, bool kAligned, bool kMany>
-__device__ __forceinline__ void attend_segment(const PagedAttend& a, const PagedSpan<kLeast<DT, D>>& u, int quanta, int count, float* lds) {
-  typedef Tile<DT, D> T;
-  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = u.hh / a.tiles, g0 = 16 * (u.hh - h * a.tiles);
-  const int rows = min(a.group - g0, 16);  // query heads of this tile
-  const int start = min(u.first * kQuantum, u.n), end = min(start + count * kQuantum, u.n);
-  // (a pair alone: all tiles are this wave's)
-  const bool alone = kMany && u.alone;
-  const int step = alone ? T::kTokens : kAWaves<D> * T::kTokens;
-
-  // Q^T: column j is head j (zero past the tile's heads)
-  u32x4 qop[T::kKLoads];
-  {
-    const char* qp = reinterpret_cast<const char*>(a.q) +
-                     (((size_t)u.b * a.kv_heads + h) * a.group + g0 + min(j, rows - 1)) * (D * kElem<DT>) + 16 * q;
-#pragma unroll
-    for (int c = 0; c < T::kKLoads; ++c) {
-      const uint4 x = *reinterpret_cast<const uint4*>(qp + 64 * c);
-      qop[c] = j < rows ? u32x4{x.x, x.y, x.z, x.w} : u32x4{0u, 0u, 0u, 0u};
-    }
-  }
-  f32x4 acc[D / 16];
-#pragma unroll
-  for (int n = 0; n < D / 16; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, z = 0.f;  // head j's running maximum (exp2 domain), this lane's share of its sum
-
-  float* logits = a.logits ? a.logits + (((size_t)u.b * a.kv_heads + h) * a.group + g0 + j) * a.logit_stride : nullptr;
-  Rows<DT, D, kAligned> rows_of(a, u.b, h, end);
-
-  // Loads run ahead without registers of their own: the next tile's keys are
-  // requested as soon as this one's are used up by the scores, its values after
-  // the products with this one's, and the pages of the tile after that in
-  // between (memory answers in order: whatever is waited for was asked first).
-  int t0 = start + (alone ? 0 : T::kTokens * w);
-  T t;
-  if (t0 < end) {
-    rows_of.ask(t0);
-    rows_of.move();
-    rows_of.load_k(t);
-    rows_of.ask(t0 + step);
-    rows_of.load_v(t);
-  }
-  // (the loads of the tile behind the last are issued too: on every path as many
-  // are in flight, so that the compiler's wait counts are exact)
-  for (; t0 < end; t0 += step) {
-    // scores: lane (j, q) gets tokens 16i + 4q + r of head j
-    float s[T::kBlocks][4];
-    float bm = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i) {
-      f32x4 d = {0.f, 0.f, 0.f, 0.f}, d2 = d;  // (fp32: two shorter chains, whose rounding errors are smaller)
-#pragma unroll
-      for (int c = 0; c < T::kKLoads; ++c) {
-        const u32x4 kw = {t.k[i][c].x, t.k[i][c].y, t.k[i][c].z, t.k[i][c].w};
-        const u32x4 qw = qop[c];
-        if constexpr (DT == kFp32) {
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e]), __uint_as_float(qw[e]), d, 0, 0, 0);
-            d2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[e + 1]), __uint_as_float(qw[e + 1]), d2, 0, 0,
-                                                      0);
-          }
-        } else {
-          d = mfma32<DT>(kw, qw, d);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[i][r] = DT == kFp32 ? d[r] + d2[r] : d[r];
-        bm = fmaxf(bm, t0 + 16 * i + 4 * q + r < end ? s[i][r] * a.scale : -INFINITY);
-      }
-    }
-    rows_of.move();
-    rows_of.load_k(t);
-    rows_of.ask(t0 + 2 * step);
-    bm = fmaxf(bm, xor16(bm));
-    bm = fmaxf(bm, xor32(bm));
-    if (__ballot(bm > m)) {
-      const float nm = fmaxf(m, bm);
-      const float alpha = m == nm ? 1.f : exp2_or_zero(m - nm);
-      m = nm;
-      z *= alpha;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float ah = __shfl(alpha, 4 * q + r);
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) acc[n][r] *= ah;
-      }
-    }
-    const float top = no_less(m);
-    float p[T::kBlocks][4];
-#pragma unroll
-    for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        p[i][r] = weight(s[i][r], a.scale, top);
-        if (t0 + 16 * i + 4 * q + r >= end) p[i][r] = 0.f;
-        if constexpr (kBias<DT> != 0) p[i][r] = ldexpf(p[i][r], kBias<DT>);
-        z += p[i][r];
-      }
-    if (!kAligned && t0 + T::kTokens > end) {  // rows past the end repeat the last one: 0 times its infinity must not be added
-#pragma unroll
-      for (int i = 0; i < T::kBlocks; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (t0 + 16 * i + 4 * q + r >= end) {
-#pragma unroll
-            for (int n = 0; n < T::kVWords; ++n) t.v[i][r][n] = 0u;
-          }
-    }
-    if constexpr (DT == kFp32) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n)
-          acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][r], __uint_as_float(t.v[0][r][n]), acc[n], 0, 0, 0);
-    } else {
-      unsigned term[8][kTerms<DT>];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) split16<DT>(p[i][r], term[4 * i + r]);
-      u32x4 pw[kTerms<DT>];
-#pragma unroll
-      for (int k = 0; k < kTerms<DT>; ++k)
-        pw[k] = u32x4{upper16(term[0][k], term[1][k]), upper16(term[2][k], term[3][k]), upper16(term[4][k], term[5][k]),
-                      upper16(term[6][k], term[7][k])};
-      pv_columns<0, DT, D>(acc, t, pw);
-    }
-    rows_of.load_v(t);
-    // behind the loads: memory answers stores in the same order, and what the next
-    // step waits for must not be behind them (16 sequences of 4099: 47.5 us before)
-    if (logits && j < rows) {
-#pragma unroll
-      for (int i = 0; i < T::kBlocks; ++i)
-        *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
-    }
-  }
-  if (__ballot(rows_of.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
-
-  z += xor16(z);
-  z += xor32(z);
-  const size_t head0 = ((size_t)u.b * a.kv_heads + h) * a.group + g0;  // this tile's first query head
-  if (alone) {  // lane (j, q) has dims dim(n, j) of heads 4q + r
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float M = __shfl(m, 4 * q + r), den = __shfl(z, 4 * q + r);
-      if (4 * q + r < rows) {
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) finish<DT, D>(a, head0, (4 * q + r) * D + T::dim(n, j), M, den, acc[n][r]);
-      }
-    }
-    return;
-  }
-  // the waves' states meet in LDS
-  float* sm = lds;  // [waves][16] maxima
-  float* sz = sm + 16 * kAWaves<D>;   // [waves][16] sums
-  float* sacc = sz + 16 * kAWaves<D>; // [waves][rows][D]
-  if (lane < 16) {
-    sm[16 * w + j] = m;
-    sz[16 * w + j] = z;
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (4 * q + r < rows) {
-      float* dst = sacc + ((size_t)w * rows + 4 * q + r) * D;
-#pragma unroll
-      for (int n = 0; n < D / 16; n += 4)  // (a piece is 4 or 8 elements)
-        *reinterpret_cast<float4*>(dst + T::dim(n, j)) = make_float4(acc[n][r], acc[n + 1][r], acc[n + 2][r], acc[n + 3][r]);
-    }
-  __syncthreads();
-  const int pair0 = u.at - u.first, unit = (int)blockIdx.x;
-  const bool whole = count == quanta;
-  float* state = a.state + (size_t)(2 * unit + (u.at != u.deal.begin(unit))) * a.state_stride;  // {max, sum}[rows], [rows][D]
-  for (int i = 2 * tid; i < rows * D; i += 128 * kAWaves<D>) {
-    const int g = i / D;
-    float M = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kAWaves<D>; ++k) M = fmaxf(M, sm[16 * k + g]);
-    float den = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-    for (int k = 0; k < kAWaves<D>; ++k) {
-      const float wt = rescale(sm[16 * k + g], M);
-      const float2 v = *reinterpret_cast<const float2*>(sacc + (size_t)k * rows * D + i);
-      den = fmaf(wt, sz[16 * k + g], den);
-      x = fmaf(wt, v.x, x);
-      y = fmaf(wt, v.y, y);
-    }
-    if (whole) {
-      finish<DT, D>(a, head0, i, M, den, x);
-      finish<DT, D>(a, head0, i + 1, M, den, y);
-    } else {
-      if (i % D == 0) st_dev2(state + 2 * g, M, den);
-      st_dev2(state + 2 * rows + i, x, y);
-    }
-  }
-  if (whole || !a.counters) return;
-
-  // the last workgroup of the pair joins the states
-  const PagedParts parts(u.deal, pair0, quanta);
-  int* last = reinterpret_cast<int*>(lds);
-  drain();
-  __syncthreads();
-  unsigned* counter = a.counters + (size_t)u.b * a.kv_heads * a.tiles + u.hh;
-  if (tid == 0) *last = inc_dev(counter) == (unsigned)(parts.chunks - 1);
-  __syncthreads();
-  const int is_last = *last;
-  __syncthreads();
-  if (!is_last) return;
-  if (tid == 0) st_dev(counter, 0u);
-  join_states<DT, D, 64 * kAWaves<D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
-}
-
-template <int DT, int D, bool kAligned, bool kMany>
-__global__ __launch_bounds__(64 * kAWaves<D>, kAWaves<D> / 4) void paged_attend_kernel(PagedAttend a) {
-  extern __shared__ float lds[];
-  constexpr int kL = kLeast<DT, D>;
-  PagedSpan<kL> u = find_span<kL, kMany>(a, blockIdx.x);
-  if constexpr (kMany) {
-    if (u.alone) {
-      const int heads = a.kv_heads * a.tiles;
-      u.first = 0;
-      for (int pair = blockIdx.x + gridDim.x * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); pair < a.sequences * heads;
-           pair += gridDim.x * kAWaves<D>) {
-        u.b = pair / heads;
-        u.hh = pair - u.b * heads;
-        u.n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[u.b]));
-        const int quanta = quanta_of<kL>(u.n);
-        attend_segment<DT, D, kAligned, kMany>(a, u, quanta, quanta, lds);
-      }
-      return;
-    }
-  }
-  while (u.at < u.end) {  // the pairs that this workgroup's share lies in
-    const int quanta = quanta_of<kL>(u.n);
-    const int count = min(quanta - u.first, u.end - u.at);
-    attend_segment<DT, D, kAligned, kMany>(a, u, quanta, count, lds);
-    u.at += count;
-    u.first = 0;
-    if (++u.hh == a.kv_heads * a.tiles) {
-      u.hh = 0;
-      u.n = ++u.b < a.sequences ? clamp_length(a, a.lengths[u.b]) : 0;
-    }
-    __syncthreads();  // the next pair's states go where these were
-  }
-}
-
-// Joins in a launch of their own: the states of a pair that are many and wide, over
-// several workgroups, kJoinColumns columns each.
-constexpr int kJoinColumns = 16;
-
-template <int DT, int D>
-__global__ __launch_bounds__(kPT) void paged_join_kernel(PagedAttend a) {
-  extern __shared__ float lds[];
-  const int b = blockIdx.z;
-  const int h = blockIdx.y / a.tiles, tile = blockIdx.y - h * a.tiles;
-  const int rows = min(a.group - 16 * tile, 16), col0 = blockIdx.x * kJoinColumns;
-  if (col0 >= rows * D / 4) return;
-  constexpr int kL = kLeast<DT, D>;
-  int longest = 0;
-  const PagedDeal<kL> deal{quanta_before<kL>(a, a.sequences, longest) * a.kv_heads * a.tiles};
-  if (pairs_alone(a, longest)) return;
-  const int from = quanta_before<kL>(a, b, longest), n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[b]));
-  const int quanta = quanta_of<kL>(n);
-  const PagedParts parts(deal, from * a.kv_heads * a.tiles + (int)blockIdx.y * quanta, quanta);
-  if (parts.chunks == 1) return;  // its workgroup has finished it
-  join_states<DT, D, kPT>(a, ((size_t)b * a.kv_heads + h) * a.group + 16 * tile, rows, parts, col0, kJoinColumns, lds);
-}
 
 // scores_out[t] = scores[t] + sum over the group's heads of its weight, from their
 // maxima and sums as the attention had them (a log-sum's rounding, 2^-24 of it, would
@@ -1004,6 +358,17 @@ __device__ __forceinline__ int write_moves(E each_key, const EvictCounts& mine, 
   return total;
 }
 
+// The scales (2, 4 or 8 bytes) of a moved row of pages in 4 bits.
+__device__ __forceinline__ void move_scales(const PagedEvict& a, char* pages, int h, int from_page, int src, int into_page,
+                                            int dst) {
+  const char* from = pages + (size_t)from_page * a.scale_page + (size_t)h * a.scale_head +
+                     (size_t)(src - a.div.of(src) * a.page_size) * a.scale_slot;
+  char* into = pages + (size_t)into_page * a.scale_page + (size_t)h * a.scale_head +
+               (size_t)(dst - a.div.of(dst) * a.page_size) * a.scale_slot;
+  for (int i = 0; i < a.scale_bytes; i += 2)
+    *reinterpret_cast<uint16_t*>(into + i) = *reinterpret_cast<const uint16_t*>(from + i);
+}
+
 // A move's rows of K and V, kRows of them in flight per thread; a row takes as many
 // lanes as it has 16-byte pieces.  Slots in srcs and dsts (`count` of them), this
 // workgroup's from its index on, every groups-th kRows * rows-at-a-time of them.
@@ -1014,7 +379,7 @@ __device__ __forceinline__ void move_rows(const PagedEvict& a, int b, int h, siz
   const int32_t* tab = a.table + (size_t)b * a.max_pages;
   for (int k1 = group * step * kRows; k1 < count; k1 += groups * step * kRows) {
     const int k0 = k1 + (threadIdx.x >> a.log_pieces);
-    int src[kRows], dst[kRows];
+    int src[kRows], dst[kRows], from_page[kRows], into_page[kRows];
     size_t to[kRows];
     bool in[kRows];
     uint4 kv[kRows], vv[kRows];
@@ -1036,6 +401,8 @@ __device__ __forceinline__ void move_rows(const PagedEvict& a, int b, int h, siz
         in[e] = false;
         from = into = 0;
       }
+      from_page[e] = from;
+      into_page[e] = into;
       const size_t f = (size_t)from * a.page_bytes + (size_t)(src[e] - ps * a.page_size) * a.slot_bytes +
                        (size_t)h * a.head_bytes + c;
       to[e] = (size_t)into * a.page_bytes + (size_t)(dst[e] - pd * a.page_size) * a.slot_bytes +
@@ -1050,6 +417,10 @@ __device__ __forceinline__ void move_rows(const PagedEvict& a, int b, int h, siz
         *reinterpret_cast<uint4*>(a.kp + to[e]) = kv[e];
         *reinterpret_cast<uint4*>(a.vp + to[e]) = vv[e];
         if (c == 0) {
+          if (a.scale_bytes) {
+            move_scales(a, a.k_scales, h, from_page[e], src[e], into_page[e], dst[e]);
+            move_scales(a, a.v_scales, h, from_page[e], src[e], into_page[e], dst[e]);
+          }
           a.scores_out[row * a.slots + dst[e]] = a.scores[row * a.slots + src[e]];
           a.positions_out[row * a.slots + dst[e]] = a.positions[row * a.slots + src[e]];
         }
@@ -1363,62 +734,6 @@ using namespace prismkv;
 
 namespace {
 
-PageDiv page_div(int page_size) {
-  int log = 0;
-  while ((1ll << log) < page_size) ++log;
-  const int shift = 31 + log;
-  return PageDiv{(unsigned)(((1ull << shift) + page_size - 1) / page_size), shift};
-}
-
-int element_bytes(int dtype) { return dtype == kFp32 ? 4 : 2; }
-
-// The second cache's lengths, tokens seen, scores and positions are all the first's or
-// lie apart from all of them: a launch reads the first's while it writes the second's.
-bool results_fit(const prismkv_paged_cache& c, const prismkv_paged_cache& to) {
-  if (to.lengths == c.lengths && to.seen == c.seen && to.scores == c.scores && to.positions == c.positions) return true;
-  const uint64_t few = 4ull * c.sequences, many = few * c.kv_heads * c.page_size * c.max_pages;
-  const uint64_t from[4] = {c.lengths, c.seen, c.scores, c.positions}, into[4] = {to.lengths, to.seen, to.scores, to.positions};
-  const uint64_t size[4] = {few, few, many, many};
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (from[i] && into[j] && from[i] < into[j] + size[j] && into[j] < from[i] + size[i]) return false;
-  return true;
-}
-
-// The cache and where its results go, checked alike by every entry point: rows,
-// heads and pages lie at 16-byte multiples, and a page's last row within 2^32
-// 16-byte units.  0, or the code to return.
-int check_cache(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, bool scored) {
-  if (!cache || !into) return kBadSize;
-  const prismkv_paged_cache& c = *cache;
-  const prismkv_paged_cache& to = *into;
-  if (c.dtype < kBf16 || c.dtype > kFp32) return kBadMode;
-  if (c.sequences < 1 || c.sequences > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.page_size < 1 ||
-      c.max_pages < 1 || c.pages < 1 || c.pages > INT32_MAX)
-    return kBadSize;
-  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return kBadSize;
-  const int64_t slots = (int64_t)c.page_size * c.max_pages;
-  if (slots > (1 << 30) || slots * c.sequences > INT32_MAX) return kBadSize;
-  const int64_t es = element_bytes(c.dtype), limit = 1ll << 36;  // bytes
-  if (c.page_stride < 0 || c.head_stride < 0 || c.slot_stride < c.head_dim) return kBadSize;
-  if (c.page_stride > limit || c.head_stride > limit || c.slot_stride > limit) return kBadSize;
-  if ((c.page_stride * es | c.head_stride * es | c.slot_stride * es) & 15) return kBadSize;
-  if (c.page_stride * es > limit / c.pages || c.slot_stride * es > limit / c.page_size) return kBadSize;
-  if ((c.pages - 1) * c.page_stride * es + (c.page_size - 1) * c.slot_stride * es >= limit) return kBadSize;
-  if (to.k != c.k || to.v != c.v || to.table != c.table || to.pages != c.pages || to.page_stride != c.page_stride ||
-      to.head_stride != c.head_stride || to.slot_stride != c.slot_stride || to.sequences != c.sequences ||
-      to.kv_heads != c.kv_heads || to.head_dim != c.head_dim || to.page_size != c.page_size ||
-      to.max_pages != c.max_pages || to.dtype != c.dtype)
-    return kBadSize;
-  if (!c.k || !c.v || !c.table || !c.lengths || !to.lengths || !c.err) return kBadSize;
-  if ((c.k | c.v) & 15 || c.err & 7 ||
-      (c.table | c.lengths | c.seen | c.scores | c.positions | to.lengths | to.seen | to.scores | to.positions) & 3)
-    return kBadSize;
-  const bool some = c.seen || c.scores || c.positions || to.seen || to.scores || to.positions;
-  const bool all = c.seen && c.scores && c.positions && to.seen && to.scores && to.positions;
-  return some != all || (scored && !all) || !results_fit(c, to) ? kBadSize : 0;
-}
-
 struct WorkLayout {
   size_t sums, state, logits, bytes;  // counters first
   unsigned state_stride;
@@ -1428,7 +743,7 @@ struct WorkLayout {
 WorkLayout attend_layout(int sequences, int kv_heads, int group, int head_dim, int64_t slots, bool weigh, int dtype) {
   WorkLayout w;
   const int64_t tiles = (group + 15) / 16, heads = (int64_t)kv_heads * tiles;
-  const int least = (dtype == kFp32 ? 1 : 2) * (head_dim == 256 ? kAWaves<256> : kAWaves<128>) / 2;
+  const int least = ((dtype & 15) == kFp32 ? 1 : 2) * (head_dim == 256 ? kAWaves<256> : kAWaves<128>) / 2;
   const int64_t workgroups = sequences * heads * ((slots + least * kQuantum - 1) / (least * kQuantum));  // of full tables
   w.quanta = workgroups * least;
   w.units = workgroups < kUnits ? workgroups : kUnits;
@@ -1463,58 +778,14 @@ EvictLayout evict_layout(int sequences, int kv_heads, int64_t slots) {
   return w;
 }
 
-template <int DT, int D, bool kAligned, bool kMany>
-int launch_attend_rows(const PagedAttend& a, int64_t units, int lds, hipStream_t stream) {
-  const auto kernel = paged_attend_kernel<DT, D, kAligned, kMany>;
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (e != hipSuccess) return (int)e;
-  }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(64 * kAWaves<D>), lds, stream, a);
-  return (int)hipGetLastError();
-}
-
-template <int DT, int D>
-int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
-  const int rows = a.group < 16 ? a.group : 16;
-  const int64_t longest = a.slots / (kLeast<DT, D> * kQuantum) + 2;
-  const int64_t most = kUnits / (a.kv_heads * a.tiles) + 2;  // (a sequence's pairs are alike)
-  const int chunks = (int)(longest < most ? longest : most);  // of one pair at most
-  // Where a pair's states may be many and wide a second launch joins them: 65536
-  // tokens of one KV head and 16 query heads (264K floats) 20.3 us, 44.9 by the last
-  // workgroup; of 8 KV heads and 4 (17K) 48.5 against 47.3.
-  const bool apart = (int64_t)chunks * rows * D > 49152;
-  const int merge = 32 * kAWaves<D> + kAWaves<D> * rows * D, sums = 32 + chunks * rows;
-  const int join = apart ? 0 : 256 * kAWaves<D> + sums;
-  const int lds = (merge > join ? merge : join) * (int)sizeof(float);
-  if (apart) a.counters = nullptr;
-  // a lane's offset within a block is 32 bits
-  const bool aligned = a.page_size % 16 == 0 && a.slot_units < (1u << 23);
-  a.many = (int64_t)a.sequences * a.kv_heads * a.tiles >= kSoloPairs;
-  const auto launch = aligned ? a.many ? launch_attend_rows<DT, D, true, true> : launch_attend_rows<DT, D, true, false>
-                              : a.many ? launch_attend_rows<DT, D, false, true> : launch_attend_rows<DT, D, false, false>;
-  const int rc = launch(a, units, lds, stream);
-  if (rc || !apart) return rc;
-  hipLaunchKernelGGL((paged_join_kernel<DT, D>), dim3((rows * D / 4 + kJoinColumns - 1) / kJoinColumns,
-                     a.kv_heads * a.tiles, a.sequences), dim3(kPT), (4 * kPT + sums) * (int)sizeof(float), stream, a);
-  return (int)hipGetLastError();
-}
-
-template <int DT>
-int launch_attend_dim(const PagedAttend& a, int head_dim, int64_t units, hipStream_t stream) {
-  if (head_dim == 64) return launch_attend<DT, 64>(a, units, stream);
-  if (head_dim == 128) return launch_attend<DT, 128>(a, units, stream);
-  return launch_attend<DT, 256>(a, units, stream);
-}
-
 }  // namespace
 
 extern "C" {
 
 size_t prismkv_paged_attend_work_bytes(int sequences, int kv_heads, int group, int head_dim, int64_t slots, int weigh,
                                        int dtype) {
-  if (dtype < kBf16 || dtype > kFp32 || sequences < 1 || kv_heads < 1 || group < 1 || head_dim < 1 || slots < 1) return 0;
+  const bool known = (dtype >= kBf16 && dtype <= kFp32) || dtype == (kFour | kBf16) || dtype == (kFour | kFp16);
+  if (!known || sequences < 1 || kv_heads < 1 || group < 1 || head_dim < 1 || slots < 1) return 0;
   const WorkLayout w = attend_layout(sequences, kv_heads, group, head_dim, slots, weigh != 0, dtype);
   return w.quanta > INT32_MAX ? 0 : w.bytes;  // (refused: quanta are counted in 32 bits)
 }
@@ -1527,12 +798,13 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   if (flags & ~3) return kBadMode;
   const prismkv_paged_cache& c = *cache;
   const double scale2 = scale * 1.4426950408889634;  // the exponents are powers of 2, in fp32
-  if (group < 1 || group > 1024 || !(scale2 >= -FLT_MAX && scale2 <= FLT_MAX)) return kBadSize;
+  const double most = c.dtype == (kFour | kFp16) ? FLT_MAX / 2 : FLT_MAX;
+  if (group < 1 || group > 1024 || !(scale2 >= -most && scale2 <= most)) return kBadSize;
   if (!q || !paged_work || !out || (q | paged_work) & 15 || lse & 3 || out & 3) return kBadSize;
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
   const WorkLayout w = attend_layout(c.sequences, c.kv_heads, group, c.head_dim, slots, weigh, c.dtype);
   if (work_bytes < w.bytes || w.quanta > INT32_MAX) return kBadSize;
-  const int es = element_bytes(c.dtype);
+  const int es = page_element_bytes(c.dtype);
   PagedAttend a{};
   a.q = reinterpret_cast<const void*>(q);
   a.k = reinterpret_cast<const void*>(c.k);
@@ -1566,11 +838,20 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   a.max_pages = c.max_pages;
   a.pages = (int)c.pages;
   a.scale = (float)scale2;
+  if (c.dtype >= kFour) {
+    a.k_scales = reinterpret_cast<const uint8_t*>(c.k_scales);
+    a.v_scales = reinterpret_cast<const uint8_t*>(c.v_scales);
+    a.scale_page = c.scale_page_stride;
+    a.scale_head = c.scale_head_stride;
+    a.scale_slot = (unsigned)c.scale_slot_stride;
+    if (c.dtype == (kFour | kFp16)) a.scale *= 2.f;  // (of keys at half their value)
+  }
   const hipStream_t s = (hipStream_t)stream;
   int rc;
   if (c.dtype == kBf16) rc = launch_attend_dim<kBf16>(a, c.head_dim, w.units, s);
   else if (c.dtype == kFp16) rc = launch_attend_dim<kFp16>(a, c.head_dim, w.units, s);
-  else rc = launch_attend_dim<kFp32>(a, c.head_dim, w.units, s);
+  else if (c.dtype == kFp32) rc = launch_attend_dim<kFp32>(a, c.head_dim, w.units, s);
+  else rc = attend_in_four(a, c.dtype, c.head_dim, w.units, s);
   if (rc || !weigh) return rc;
   const int64_t blocks = (slots + kPT - 1) / kPT;
   hipLaunchKernelGGL(paged_weigh_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024), c.kv_heads, c.sequences),
@@ -1582,6 +863,9 @@ int prismkv_paged_append(const prismkv_paged_cache* cache, const prismkv_paged_c
                          uint64_t offsets, int64_t rows, int64_t k_row_stride, int64_t k_head_stride,
                          int64_t v_row_stride, int64_t v_head_stride, uint64_t stream) {
   if (const int rc = check_cache(cache, into, false)) return rc;
+  if (cache->dtype >= kFour)
+    return prismkv_paged_append_rows(cache, into, k, v, 0, 0, offsets, 0, rows, k_row_stride, k_head_stride, v_row_stride,
+                                     v_head_stride, 0, 0, 0, 0, 0, 0., stream);
   const prismkv_paged_cache& c = *cache;
   if (rows < 0 || rows > INT32_MAX || (!offsets && rows != c.sequences)) return kBadSize;
   if (rows && (!k || !v)) return kBadSize;
@@ -1650,7 +934,7 @@ int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_ca
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
   const EvictLayout l = evict_layout(c.sequences, c.kv_heads, slots);
   if (work_bytes < l.bytes) return kBadSize;
-  const int es = element_bytes(c.dtype);
+  const int es = page_element_bytes(c.dtype);
   PagedEvict a{};
   a.kp = reinterpret_cast<char*>(c.k);
   a.vp = reinterpret_cast<char*>(c.v);
@@ -1681,7 +965,15 @@ int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_ca
   a.div = page_div(c.page_size);
   a.sequences = c.sequences;
   a.kv_heads = c.kv_heads;
-  while (16 << a.log_pieces < c.head_dim * es) ++a.log_pieces;
+  while (16 << a.log_pieces < page_row(c) * es) ++a.log_pieces;
+  if (c.dtype >= kFour) {
+    a.k_scales = reinterpret_cast<char*>(c.k_scales);
+    a.v_scales = reinterpret_cast<char*>(c.v_scales);
+    a.scale_page = c.scale_page_stride;
+    a.scale_head = c.scale_head_stride;
+    a.scale_slot = c.scale_slot_stride;
+    a.scale_bytes = c.head_dim / 32;
+  }
   a.page_size = c.page_size;
   a.max_pages = c.max_pages;
   a.pages = (int)c.pages;

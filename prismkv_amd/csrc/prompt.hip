@@ -1,0 +1,736 @@
+// Causal attention of a whole prompt, a chunk of one or a turn over the paged cache:
+// the queries of every sequence's last slots, packed, over all of its slots.
+//
+// Rows: the queries of the heads that share a KV head are the rows of one matrix,
+// m group of them for m tokens (row = token * group + head), so that few tokens of many
+// heads still fill a tile; row i of a sequence of n slots sees slots [0, n - m + i /
+// group].  4 head_dim flops for a row and a slot that it sees against 2 x 2 head_dim
+// bytes for a slot and 128 rows: the matrix products bound it, unless the rows are few.
+#include <cfloat>
+#include <type_traits>
+
+#include "paged_host.h"
+
+namespace prismkv {
+namespace {
+
+constexpr int kWaves = 4, kTileRows = 32 * kWaves, kThreads = 64 * kWaves;
+// Keys and values that are staged at a time.
+template <int DT, int D>
+constexpr int kTileTokens = kElem<DT> * D > 512 ? 32 : 64;
+// Waves of a SIMD, by the registers that products, queries and staged rows take.
+template <int DT, int D>
+constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
+// The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, nor
+// less than kLeastTiles tiles of keys.
+constexpr int kItemsLog = 9, kLeastTiles = 4;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct Prompt {
+  const char *q, *k, *v;
+  const uint8_t *ks, *vs;
+  const int32_t *table, *lengths, *offsets;
+  char* out;
+  float *lse, *state;
+  unsigned* err;
+  int64_t page_bytes, head_bytes, slot_bytes, scale_page, scale_head, scale_slot;
+  PageDiv div;
+  unsigned q_and, q_xor;  // the scale's sign, or a scale of 0, goes to the queries
+  float scale;            // log2(e) times the caller's magnitude
+  int rows, sequences, kv_heads, group, page_size, max_pages, pages, slots, states;
+};
+
+// New rows m from `first` of a sequence, its slots, and its tiles of rows and of keys.
+struct PromptRows {
+  int first, m, n, tiles, key_tiles;
+};
+
+template <int kTokens>
+__device__ __forceinline__ PromptRows prompt_rows(const Prompt& a, int b) {
+  PromptRows s{0, 0, 0, 0, 0};
+  if (b >= a.sequences) return s;
+  s.first = a.offsets ? min(max(a.offsets[b], 0), a.rows) : b;
+  const int to = a.offsets ? min(max(a.offsets[b + 1], 0), a.rows) : b + 1;
+  s.m = max(to - s.first, 0);
+  s.n = min(max(a.lengths[b], 0), a.slots);
+  s.tiles = (s.m * a.group + kTileRows - 1) / kTileRows;  // (rows * group < 2^30)
+  s.key_tiles = (s.n + kTokens - 1) / kTokens;
+  return s;
+}
+
+// Tiles of keys of a work item at most: every wave finds them, and its own item, by
+// itself from the lengths (two lane scans for every 64 sequences).
+template <int kTokens>
+__device__ __forceinline__ int item_tiles(const Prompt& a) {
+  uint64_t sum = 0;
+  for (int b = threadIdx.x & 63; b < a.sequences; b += 64) {
+    const PromptRows s = prompt_rows<kTokens>(a, b);
+    sum += (uint64_t)s.tiles * s.key_tiles;
+  }
+  const uint64_t low = wave_sum_i((int)(sum & 0xffffffu)), high = wave_sum_i((int)(sum >> 24));
+  const uint64_t share = (((high << 24) + low) * a.kv_heads >> kItemsLog) + 1;
+  return (int)(share < kLeastTiles ? kLeastTiles : share < (1u << 24) ? share : 1u << 24);
+}
+
+// Item `index` of the launch: a tile of rows of sequence b and KV head h, chunk `chunk`
+// of the `chunks` that its keys are cut into, `most` of which its longest tile has;
+// `state` counts the items of sequences that are cut.
+struct PromptItem {
+  PromptRows s;
+  int b, h, tile, chunk, most, state;
+};
+
+// The heads go round fastest: with 8 of them the workgroups of a head share an XCD's
+// L2, and what they read at a time is the same.  A sequence's last tiles, which see the
+// most, come first.
+template <int kTokens>
+__device__ __forceinline__ bool find_item(const Prompt& a, int per_item, int index, bool cut_tiles, PromptItem& it) {
+  int base = 0, cut = 0;
+  for (int b0 = 0; b0 < a.sequences; b0 += 64) {
+    const PromptRows s = prompt_rows<kTokens>(a, b0 + (threadIdx.x & 63));
+    const int most = max((s.key_tiles + per_item - 1) / per_item, 1);
+    // (cut_tiles: only those of sequences that are cut, one for all chunks of a tile)
+    const int states = most > 1 ? s.tiles * most * a.kv_heads : 0;
+    const int count = cut_tiles ? (most > 1 ? s.tiles * a.kv_heads : 0) : s.tiles * most * a.kv_heads;
+    const int upto = (int)wave_incl_scan((unsigned)count), total = __builtin_amdgcn_readlane(upto, 63);
+    const int states_upto = (int)wave_incl_scan((unsigned)states);
+    if (index - base < total) {
+      const int l = __ffsll((unsigned long long)__ballot(upto > index - base)) - 1;
+      it.s.first = __builtin_amdgcn_readlane(s.first, l);
+      it.s.m = __builtin_amdgcn_readlane(s.m, l);
+      it.s.n = __builtin_amdgcn_readlane(s.n, l);
+      it.s.tiles = __builtin_amdgcn_readlane(s.tiles, l);
+      it.s.key_tiles = __builtin_amdgcn_readlane(s.key_tiles, l);
+      it.most = __builtin_amdgcn_readlane(most, l);
+      it.b = b0 + l;
+      int at = index - base - __builtin_amdgcn_readlane(upto, l) + __builtin_amdgcn_readlane(count, l);
+      it.state = cut + __builtin_amdgcn_readlane(states_upto, l) - __builtin_amdgcn_readlane(states, l) + (cut_tiles ? 0 : at);
+      it.h = at % a.kv_heads;
+      at /= a.kv_heads;
+      it.chunk = cut_tiles ? 0 : at % it.most;
+      it.tile = it.s.tiles - 1 - (cut_tiles ? at : at / it.most);
+      return true;
+    }
+    base += total;
+    cut += __builtin_amdgcn_readlane(states_upto, 63);
+  }
+  return false;
+}
+
+// The chunks that a tile's keys are cut into evenly, and how many tiles of keys it sees.
+template <int kTokens>
+struct PromptCut {
+  int end, tiles, chunks, each;  // slots and tiles that its last row sees; tiles of a chunk
+  __device__ __forceinline__ PromptCut(const Prompt& a, const PromptItem& it, int per_item) {
+    const int last = (min((it.tile + 1) * kTileRows, it.s.m * a.group) - 1) / a.group;  // the tile's last token
+    end = max(it.s.n - it.s.m + last + 1, 0);
+    tiles = (end + kTokens - 1) / kTokens;
+    chunks = (tiles + per_item - 1) / per_item;
+    each = chunks ? (tiles + chunks - 1) / chunks : 0;
+    if (each) chunks = (tiles + each - 1) / each;
+  }
+};
+
+// Where chunk c (16 bytes) of row r lies in a staged tile of rows of kC chunks: moved
+// within the row so that neither 16 rows' same chunk (keys) nor two neighbouring chunks
+// of four rows (values, read transposed) meet in a bank.
+template <int kC>
+__device__ __forceinline__ int staged(int r, int c) {
+  const int f = kC == 8 ? (r & 2) | (r & 4) | ((r >> 3) & 1) : ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
+  return (r * kC + (c ^ f)) * 16;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma_rows(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (kType<DT> == kBf16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else if constexpr (kType<DT> == kFp16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+// Two probabilities as a word of the 16-bit type, rounded to nearest: half a step of
+// the type relative to each, which their product with V averages out to less than the
+// output's own rounding.  fp16 takes its least number for what is below it, so that an
+// infinite V is not multiplied by 0 (2^-39 of the largest weight, with the bias).
+template <int DT>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  if constexpr (kType<DT> == kBf16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, bf16x2{(__bf16)a, (__bf16)b});
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, f16x2{(_Float16)a, (_Float16)b});
+  }
+}
+
+// Whether any element of 16 bytes is an infinity or NaN.
+template <int DT>
+__device__ __forceinline__ bool any_special(u32x4 x) {
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (kType<DT> == kFp32) {
+      any |= (x[e] & 0x7f800000u) == 0x7f800000u;
+    } else {
+      constexpr unsigned kMask = kType<DT> == kBf16 ? 0x7f80u : 0x7c00u;
+      any |= (x[e] & kMask) == kMask || (x[e] >> 16 & kMask) == kMask;
+    }
+  }
+  return any;
+}
+
+// Eight codes as eight elements of the 16-bit type (for fp16 half of them, kSumBias).
+template <int DT>
+__device__ __forceinline__ u32x4 widen_eight(unsigned codes, unsigned byte) {
+  const unsigned e = kType<DT> == kFp16 ? max(byte, 1u) - 1u : byte;
+  const float scale = __uint_as_float(byte == 255u ? 0x7fc00000u : e << 23);
+  if constexpr (kType<DT> == kBf16)
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+  else
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
+}
+
+// A thread's part of a tile of keys and values on its way from the pages to LDS.
+template <int DT, int D>
+struct Stage {
+  static constexpr int kTokens = kTileTokens<DT, D>;
+  static constexpr int kC = D * kElem<DT> / 16;            // chunks of a row
+  static constexpr int kEach = kTokens * kC / kThreads;    // chunks of a thread
+  typedef typename std::conditional<kInFour<DT>, unsigned, u32x4>::type Word;
+  const Prompt& a;
+  const char *k, *v;
+  const uint8_t *ks, *vs;
+  const int32_t* tab;
+  int end, row, chunk;
+  bool bad = false;
+  int page[kEach];
+  Word kw[kEach], vw[kEach];
+  unsigned kb[kInFour<DT> ? kEach : 1], vb[kInFour<DT> ? kEach : 1];
+
+  __device__ __forceinline__ Stage(const Prompt& a, int b, int h, int end) : a(a), end(end) {
+    row = threadIdx.x / kC;
+    chunk = threadIdx.x % kC;
+    const int bytes = kInFour<DT> ? 4 : 16;  // of a chunk in the pages
+    k = a.k + (size_t)h * a.head_bytes + chunk * bytes;
+    v = a.v + (size_t)h * a.head_bytes + chunk * bytes;
+    if constexpr (kInFour<DT>) {
+      ks = a.ks + (size_t)h * a.scale_head + chunk / 4;
+      vs = a.vs + (size_t)h * a.scale_head + chunk / 4;
+    }
+    tab = a.table + (size_t)b * a.max_pages;
+  }
+  static __device__ __forceinline__ int step(int i) { return i * (kThreads / kC); }
+  __device__ __forceinline__ void ask(int t0) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) page[i] = tab[a.div.of(min(t0 + row + step(i), end - 1))];
+  }
+  // rows past the end stay 0
+  __device__ __forceinline__ void load(int t0) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int t = t0 + row + step(i);
+      kw[i] = Word{};
+      vw[i] = Word{};
+      if constexpr (kInFour<DT>) kb[i] = vb[i] = 0u;
+      if (t < end) {
+        bad |= (unsigned)page[i] >= (unsigned)a.pages;
+        const unsigned p = (unsigned)page[i] < (unsigned)a.pages ? (unsigned)page[i] : 0u;
+        const unsigned in = (unsigned)(t - a.div.of(t) * a.page_size);
+        const size_t at = (size_t)p * a.page_bytes + (size_t)in * a.slot_bytes;
+        kw[i] = *reinterpret_cast<const Word*>(k + at);
+        vw[i] = *reinterpret_cast<const Word*>(v + at);
+        if constexpr (kInFour<DT>) {
+          const size_t scale_at = (size_t)p * a.scale_page + (size_t)in * a.scale_slot;
+          kb[i] = ks[scale_at];
+          vb[i] = vs[scale_at];
+        }
+      }
+    }
+  }
+  // Writes the tile; whether a value is special (looked at only if asked for).
+  __device__ __forceinline__ bool store(char* keys, char* values, bool look) const {
+    bool special = false;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      u32x4 x, y;
+      if constexpr (kInFour<DT>) {
+        x = widen_eight<DT>(kw[i], kb[i]);
+        y = widen_eight<DT>(vw[i], vb[i]);
+      } else {
+        x = kw[i];
+        y = vw[i];
+      }
+      const int at = staged<kC>(row + step(i), chunk);
+      *reinterpret_cast<u32x4*>(keys + at) = x;
+      *reinterpret_cast<u32x4*>(values + at) = y;
+      if (look) special |= any_special<DT>(y);
+    }
+    return special;
+  }
+};
+
+// Four elements from LDS in 32 bits.
+template <int DT>
+__device__ __forceinline__ float4 four_of(const char* p) {
+  if constexpr (kType<DT> == kFp32) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    if constexpr (kType<DT> == kBf16) {
+      return make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
+    } else {
+      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+      const f16x4 h = __builtin_bit_cast(f16x4, w);
+      return make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+    }
+  }
+}
+
+// Writes four outputs of a row, and its log-sum.
+template <int DT, int D>
+__device__ __forceinline__ void put_four(const Prompt& a, size_t row_head, int dim, float den, float4 x) {
+  const float y[4] = {x.x / den, x.y / den, x.z / den, x.w / den};
+  float z[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = den == 0.f ? 0.f : y[e];
+  char* to = a.out + (row_head * D + dim) * kElem<DT>;
+  if constexpr (kType<DT> == kFp32) {
+    *reinterpret_cast<float4*>(to) = make_float4(z[0], z[1], z[2], z[3]);
+  } else {
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2<DT>(z[0], z[1]), pack2<DT>(z[2], z[3]));
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ float prompt_lse(float m, float den) {
+  return den == 0.f ? -INFINITY : (m + (log2f(den) - kSumBias<DT>)) * 0.693147180559945309f;
+}
+
+// Factor of a state with maximum m under the joint maximum M >= m (no state: 0).
+__device__ __forceinline__ float state_factor(float m, float M) {
+  return m == -INFINITY ? 0.f : m == M ? 1.f : exp2f(m - M);
+}
+
+// A state: maxima and sums [2][128], then the products [D / 4][128] of four dims.
+template <int D>
+constexpr int kStateFloats = kTileRows * (D + 2);
+
+// Scores are computed transposed, S^T = K Q^T, so that a lane has 16 (of 32 tokens)
+// scores of one row (lane & 31; the other half of the tokens with lane ^ 32): its maximum
+// and sum need one exchange a tile, its factors none, and its probabilities are the right
+// operand of O^T = V^T P^T as they stand, the tokens being summed in the order in which
+// they lie in registers (8 (r / 4) + 4 (lane / 32) + r % 4).  V^T comes out of LDS by
+// transposing reads.
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(Prompt a) {
+  constexpr int kTokens = kTileTokens<DT, D>, kT = kTokens / 32;
+  constexpr int kC = D * kElem<DT> / 16;  // 16-byte chunks of a row; half as many steps of the product (fp32: of four)
+  extern __shared__ char lds[];
+  char *keys = lds, *values = lds + kTokens * kC * 16;
+  if (blockIdx.x == 0 && a.offsets)
+    for (int b = threadIdx.x; b < a.sequences; b += kThreads) {
+      const int from = a.offsets[b], to = a.offsets[b + 1];
+      if (from > to || (b == 0 && from) || (b == a.sequences - 1 && to != a.rows))
+        report_error(a.err, error_host_slot(a.err), kErrOffsets);
+    }
+  const int per_item = item_tiles<kTokens>(a);
+  PromptItem it;
+  if (!find_item<kTokens>(a, per_item, blockIdx.x, false, it)) return;
+  const PromptCut<kTokens> cut(a, it, per_item);
+  if (it.chunk > 0 && it.chunk >= cut.chunks) return;
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rows = it.s.m * a.group - it.tile * kTileRows;  // of the tile and behind it
+  const int row = 32 * w + col;
+  const bool valid = row < rows;
+  const int of = it.tile * kTileRows + min(row, rows - 1), token = of / a.group;
+  const int before = it.s.n - it.s.m;
+  if (before < 0 && threadIdx.x == 0) report_error(a.err, error_host_slot(a.err), kErrHeld);
+  const int limit = valid ? before + token : -1;  // the last slot that the row sees
+  // the last slot that any row of the wave sees, and the first row's; the tile's first
+  const int wave_last = __builtin_amdgcn_readlane(32 * w < rows ? before + token : -1, 31);
+  const int wave_first = __builtin_amdgcn_readlane(limit, 0);
+  const int tile_first = before + it.tile * kTileRows / a.group;
+  const size_t row_head = (size_t)(it.s.first + token) * a.kv_heads * a.group + it.h * a.group + (of - token * a.group);
+
+  u32x4 q[kC / 2];
+  {
+    const char* from = a.q + row_head * (D * kElem<DT>) + 16 * half;
+#pragma unroll
+    for (int c = 0; c < kC / 2; ++c) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(from + 32 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[c][e] = (x[e] & a.q_and) ^ a.q_xor;
+    }
+  }
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  float m = -INFINITY, z = 0.f;  // the row's maximum (exp2 domain), this lane's share of its sum
+
+  const int from = it.chunk * cut.each, to = min(from + cut.each, cut.tiles);
+  Stage<DT, D> stage(a, it.b, it.h, cut.end);
+  if (from < to) {
+    stage.ask(from * kTokens);
+    stage.load(from * kTokens);
+    if (from + 1 < to) stage.ask((from + 1) * kTokens);
+  }
+  for (int t = from; t < to; ++t) {
+    const int t0 = t * kTokens;
+    // A tile that some row does not see all of: where a value there is an infinity or NaN,
+    // 0 times it must not reach that row.
+    const bool partly = t0 + kTokens - 1 > tile_first;
+    __syncthreads();  // the last tile has been read
+    bool special = stage.store(keys, values, partly);
+    if (t + 1 < to) {
+      stage.load(t0 + kTokens);
+      if (t + 2 < to) stage.ask(t0 + 2 * kTokens);
+    }
+    if (partly) special = __syncthreads_or(special);
+    else __syncthreads();
+    const bool seen = t0 <= wave_last;
+    f32x16 s[kT];
+    if (seen) {
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kC / 2; ++c)
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+          s[i] = mfma_rows<DT>(*reinterpret_cast<const u32x4*>(keys + staged<kC>(32 * i + col, 2 * c + half)), q[c], s[i]);
+      if (t0 + kTokens - 1 > wave_first) {
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (t0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 > limit) s[i][r] = -INFINITY;
+      }
+      float most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, s[i][r]);
+      most = fmaxf(most, xor32(most)) * a.scale;
+      if (__ballot(most > m)) {
+        const float nm = fmaxf(m, most);
+        const float alpha = state_factor(m, nm);
+        m = nm;
+        z *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+      }
+      const float top = m == -INFINITY ? 0.f : m;
+      const float least = kType<DT> == kFp16 ? 0x1p-24f : 0.f;
+      // From 2^22 on the maximum's own rounding is 1/8 and more (at 2^32 it takes all of
+      // the exponents' range): then the other products are rounded as it was.
+      if (__ballot(fabsf(m) >= 0x1p22f && m != -INFINITY)) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float product = s[i][r] * a.scale, x = product - top;
+            s[i][r] = __builtin_amdgcn_exp2f(x + (float)kBias<DT>);
+            z += s[i][r];
+            if (least > 0.f && x != -INFINITY) s[i][r] = fmaxf(s[i][r], least);
+          }
+      } else {
+        const float shift = (float)kBias<DT> - top;
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool none = s[i][r] == -INFINITY;
+            s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], a.scale, shift));
+            z += s[i][r];
+            if (least > 0.f && !none) s[i][r] = fmaxf(s[i][r], least);
+          }
+      }
+    }
+    if (partly && special) {  // (all threads alike)
+      __syncthreads();        // the keys have been read: the probabilities of 16 tokens at a time take their place
+      if (!seen) continue;
+      float* p = reinterpret_cast<float*>(keys) + 16 * 32 * w;
+#pragma unroll
+      for (int g = 0; g < 2 * kT; ++g) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) p[(8 * (r / 4) + 4 * half + r % 4) * 32 + col] = s[g / 2][8 * (g & 1) + r];
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll 1
+        for (int k = 0; k < 16; ++k) {
+          const int token_row = 16 * g + k;
+          const bool visible = t0 + token_row <= limit;
+          const float weight = p[k * 32 + col];
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int dim = 32 * d + 8 * j + 4 * half, byte = dim * kElem<DT>;
+              const float4 x = four_of<DT>(values + staged<kC>(token_row, byte >> 4) + (byte & 15));
+              acc[d][4 * j] = visible ? fmaf(weight, x.x, acc[d][4 * j]) : acc[d][4 * j];
+              acc[d][4 * j + 1] = visible ? fmaf(weight, x.y, acc[d][4 * j + 1]) : acc[d][4 * j + 1];
+              acc[d][4 * j + 2] = visible ? fmaf(weight, x.z, acc[d][4 * j + 2]) : acc[d][4 * j + 2];
+              acc[d][4 * j + 3] = visible ? fmaf(weight, x.w, acc[d][4 * j + 3]) : acc[d][4 * j + 3];
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_s_waitcnt(0);
+      }
+      continue;
+    }
+    if (!seen) continue;
+    if constexpr (kType<DT> == kFp32) {
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) {
+            const int at = staged<kC>(32 * i + 8 * (r / 4) + 4 * half + r % 4, 8 * d + col / 4) + 4 * (col & 3);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + at), s[i][r], acc[d], 0, 0, 0);
+          }
+    } else {
+      typedef __attribute__((address_space(3))) s16x4* Transposed;
+      const int in = lane & 15, side = lane >> 4 & 1;  // row in / 4 and piece in % 4 of 16 dims; which 16 dims
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const u32x4 p = {pack2<DT>(s[i][8 * u], s[i][8 * u + 1]), pack2<DT>(s[i][8 * u + 2], s[i][8 * u + 3]),
+                           pack2<DT>(s[i][8 * u + 4], s[i][8 * u + 5]), pack2<DT>(s[i][8 * u + 6], s[i][8 * u + 7])};
+          const int r = 32 * i + 16 * u + 4 * half + in / 4;
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) {
+            const int c = 4 * d + 2 * side + (in >> 1 & 1);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + staged<kC>(r, c) + 8 * (in & 1)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + staged<kC>(r + 8, c) + 8 * (in & 1)));
+            const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+            acc[d] = mfma_rows<DT>(u32x4{l.x, l.y, h.x, h.y}, p, acc[d]);
+          }
+        }
+    }
+  }
+  if (__ballot(stage.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
+
+  z += xor32(z);
+  if constexpr (kSumBias<DT> != kBias<DT>) z *= 0.5f;
+  if (!valid) return;
+  if (cut.chunks <= 1) {
+    if (a.lse && half == 0) a.lse[row_head] = prompt_lse<DT>(m, z);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        put_four<DT, D>(a, row_head, 32 * d + 8 * j + 4 * half, z,
+                        make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]));
+    return;
+  }
+  if (it.state >= a.states) return;  // (never, while the offsets ascend)
+  float* state = a.state + (size_t)it.state * kStateFloats<D>;
+  if (half == 0) {
+    state[row] = m;
+    state[kTileRows + row] = z;
+  }
+  float4* products = reinterpret_cast<float4*>(state + 2 * kTileRows);
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      products[(8 * d + 2 * j + half) * kTileRows + row] =
+          make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
+}
+
+// Joins the states of tiles whose keys were cut, in the order of their tokens: a
+// workgroup for kJoinDims dims of a tile, a thread for a row and four of them at a time.
+constexpr int kJoinDims = 16;
+
+template <int DT, int D>
+__global__ __launch_bounds__(kThreads) void prompt_join_kernel(Prompt a) {
+  constexpr int kTokens = kTileTokens<DT, D>;
+  const int per_item = item_tiles<kTokens>(a);
+  PromptItem it;
+  if (!find_item<kTokens>(a, per_item, blockIdx.x, true, it)) return;
+  const PromptCut<kTokens> cut(a, it, per_item);
+  if (cut.chunks <= 1) return;  // its workgroup has finished it
+  const int rows = min(it.s.m * a.group - it.tile * kTileRows, kTileRows);
+  const int row = threadIdx.x % kTileRows;
+  if (row >= rows) return;
+  // the states of chunk 0 and from chunk to chunk
+  const int first = it.state + (it.s.tiles - 1 - it.tile) * it.most * a.kv_heads + it.h;
+  if (first + (cut.chunks - 1) * a.kv_heads >= a.states) return;
+  const float* state = a.state + (size_t)first * kStateFloats<D> + row;
+  const size_t step = (size_t)a.kv_heads * kStateFloats<D>;
+  float M = -INFINITY, den = 0.f;
+  for (int c = 0; c < cut.chunks; ++c) M = fmaxf(M, state[c * step]);
+  const int quad0 = blockIdx.y * (kJoinDims / 4) + threadIdx.x / kTileRows;
+  constexpr int kQ = kJoinDims / 4 * kTileRows / kThreads;
+  float4 sum[kQ];
+#pragma unroll
+  for (int e = 0; e < kQ; ++e) sum[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = 0; c < cut.chunks; ++c) {
+    const float f = state_factor(state[c * step], M);
+    den = fmaf(f, state[c * step + kTileRows], den);
+#pragma unroll
+    for (int e = 0; e < kQ; ++e) {
+      const int quad = quad0 + e * (kThreads / kTileRows);
+      const float4 x = reinterpret_cast<const float4*>(state - row + c * step + 2 * kTileRows)[quad * kTileRows + row];
+      sum[e].x = fmaf(f, x.x, sum[e].x);
+      sum[e].y = fmaf(f, x.y, sum[e].y);
+      sum[e].z = fmaf(f, x.z, sum[e].z);
+      sum[e].w = fmaf(f, x.w, sum[e].w);
+    }
+  }
+  const int of = it.tile * kTileRows + row, token = of / a.group;
+  const size_t row_head = (size_t)(it.s.first + token) * a.kv_heads * a.group + it.h * a.group + (of - token * a.group);
+  if (a.lse && quad0 == 0) a.lse[row_head] = prompt_lse<DT>(M, den);
+#pragma unroll
+  for (int e = 0; e < kQ; ++e) put_four<DT, D>(a, row_head, 4 * (quad0 + e * (kThreads / kTileRows)), den, sum[e]);
+}
+
+// Work items, states and cut tiles of a launch at most.
+struct PromptLayout {
+  int64_t items, states, cut_tiles;
+  size_t bytes;
+};
+
+PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots, int dtype) {
+  PromptLayout l;
+  const int tokens = element_bytes(dtype) * head_dim > 512 ? 32 : 64;
+  const int64_t tiles = (rows * group) / kTileRows + (sequences < rows ? sequences : rows), key_tiles = (slots + tokens - 1) / tokens;
+  const int64_t all = 1ll << kItemsLog;
+  l.items = all + tiles * kv_heads;
+  // A sequence that is cut has most = ceil(x) <= 2x chunks a tile, x > 1 its share of
+  // an item: 2 all of them at most.
+  const int64_t full = tiles * kv_heads * ((key_tiles + kLeastTiles - 1) / kLeastTiles);
+  l.states = key_tiles <= kLeastTiles ? 0 : full < 2 * all ? full : 2 * all;
+  l.cut_tiles = key_tiles <= kLeastTiles ? 0 : tiles * kv_heads < all ? tiles * kv_heads : all;
+  l.bytes = (size_t)l.states * kTileRows * (head_dim + 2) * sizeof(float);
+  return l;
+}
+
+template <int DT, int D>
+int launch_prompt(const Prompt& a, const PromptLayout& l, hipStream_t stream) {
+  constexpr int lds = 2 * kTileTokens<DT, D> * D * kElem<DT>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_kernel<DT, D>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)l.items), dim3(kThreads), lds, stream, a);
+  if (const int rc = (int)hipGetLastError()) return rc;
+  if (!l.cut_tiles) return 0;
+  hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3((unsigned)l.cut_tiles, D / kJoinDims), dim3(kThreads), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <int DT>
+int launch_prompt_dim(const Prompt& a, int head_dim, const PromptLayout& l, hipStream_t stream) {
+  if (head_dim == 64) return launch_prompt<DT, 64>(a, l, stream);
+  if (head_dim == 128) return launch_prompt<DT, 128>(a, l, stream);
+  return launch_prompt<DT, 256>(a, l, stream);
+}
+
+bool prompt_fits(int64_t rows, int sequences, int kv_heads, int group) {
+  // (rows of a tile's index, items and states are counted in 32 bits)
+  return rows >= 0 && group >= 1 && group <= 1024 && rows <= (1 << 30) / group &&
+         (rows * group / kTileRows + sequences) * kv_heads < 1 << 30;
+}
+
+}  // namespace
+}  // namespace prismkv
+
+using namespace prismkv;
+
+extern "C" {
+
+size_t prismkv_paged_prompt_work_bytes(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots,
+                                       int dtype) {
+  const bool known = (dtype >= kBf16 && dtype <= kFp32) || dtype == (kFour | kBf16) || dtype == (kFour | kFp16);
+  if (!known || sequences < 1 || kv_heads < 1 || head_dim < 1 || slots < 1 || slots > 1 << 30 ||
+      !prompt_fits(rows, sequences, kv_heads, group))
+    return 0;
+  const size_t bytes = prompt_layout(rows, sequences, kv_heads, group, head_dim, slots, dtype).bytes;
+  return bytes < 16 ? 16 : bytes;
+}
+
+int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t offsets, uint64_t lse, uint64_t paged_work,
+                         uint64_t out, int64_t rows, int group, double scale, size_t work_bytes, uint64_t stream) {
+  if (const int rc = check_cache(cache, cache, false)) return rc;
+  const prismkv_paged_cache& c = *cache;
+  const double scale2 = scale * 1.4426950408889634;  // the exponents are powers of 2, in fp32
+  const double most = c.dtype == (kFour | kFp16) ? FLT_MAX / 2 : FLT_MAX;
+  if (!(scale2 >= -most && scale2 <= most) || !prompt_fits(rows, c.sequences, c.kv_heads, group)) return kBadSize;
+  if (!offsets && rows != c.sequences) return kBadSize;
+  if ((rows && (!q || !out || !paged_work)) || (q | out | paged_work) & 15 || (lse | offsets) & 3) return kBadSize;
+  const int64_t slots = (int64_t)c.page_size * c.max_pages;
+  const PromptLayout l = prompt_layout(rows, c.sequences, c.kv_heads, group, c.head_dim, slots, c.dtype);
+  if (work_bytes < l.bytes) return kBadSize;
+  Prompt a{};
+  a.q = reinterpret_cast<const char*>(q);
+  a.k = reinterpret_cast<const char*>(c.k);
+  a.v = reinterpret_cast<const char*>(c.v);
+  a.table = reinterpret_cast<const int32_t*>(c.table);
+  a.lengths = reinterpret_cast<const int32_t*>(c.lengths);
+  a.offsets = reinterpret_cast<const int32_t*>(offsets);
+  a.out = reinterpret_cast<char*>(out);
+  a.lse = reinterpret_cast<float*>(lse);
+  a.state = reinterpret_cast<float*>(paged_work);
+  a.err = reinterpret_cast<unsigned*>(c.err);
+  const int64_t es = page_element_bytes(c.dtype);
+  a.page_bytes = c.page_stride * es;
+  a.head_bytes = c.head_stride * es;
+  a.slot_bytes = c.slot_stride * es;
+  a.scale = (float)(scale2 < 0 ? -scale2 : scale2);
+  a.q_and = scale2 == 0 ? 0u : ~0u;
+  a.q_xor = !(scale2 < 0) ? 0u : element_bytes(c.dtype) == 4 ? 0x80000000u : 0x80008000u;
+  if (scale2 == 0) a.scale = 1.f;  // (of scores that are 0)
+  if (c.dtype >= kFour) {
+    a.ks = reinterpret_cast<const uint8_t*>(c.k_scales);
+    a.vs = reinterpret_cast<const uint8_t*>(c.v_scales);
+    a.scale_page = c.scale_page_stride;
+    a.scale_head = c.scale_head_stride;
+    a.scale_slot = c.scale_slot_stride;
+    if (c.dtype == (kFour | kFp16)) a.scale *= 2.f;  // (of keys at half their value)
+  }
+  a.div = page_div(c.page_size);
+  a.rows = (int)rows;
+  a.sequences = c.sequences;
+  a.kv_heads = c.kv_heads;
+  a.group = group;
+  a.page_size = c.page_size;
+  a.max_pages = c.max_pages;
+  a.pages = (int)c.pages;
+  a.slots = (int)slots;
+  a.states = (int)l.states;
+  const hipStream_t s = (hipStream_t)stream;
+  switch (c.dtype) {
+    case kBf16: return launch_prompt_dim<kBf16>(a, c.head_dim, l, s);
+    case kFp16: return launch_prompt_dim<kFp16>(a, c.head_dim, l, s);
+    case kFp32: return launch_prompt_dim<kFp32>(a, c.head_dim, l, s);
+    case kFour | kBf16: return launch_prompt_dim<kFour | kBf16>(a, c.head_dim, l, s);
+    default: return launch_prompt_dim<kFour | kFp16>(a, c.head_dim, l, s);
+  }
+}
+
+}  // extern "C"

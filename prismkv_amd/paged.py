@@ -1,11 +1,13 @@
 """Keys and values of several sequences in pages, for dense decoding beside
-the routed one: `PagedCache.append` writes new rows, `attend` runs one new
-query token of every sequence over its pages, and `evict` bounds a cache by
-accumulated attention weight.  No counterpart in the reference.
+the routed one: `PagedCache.append` writes new rows, turned by rotary positions if
+asked for, `attend` runs one new query token of every sequence over its pages,
+`attend_prompt` many, causally, `read` gives rows back, and `evict` bounds a cache
+by accumulated attention weight.  No counterpart in the reference.
 
 Any head layout with head_dim 64, 128 or 256 in bf16, fp16 or fp32, and up to 64
 GiB each of k and v pages (NotImplementedError otherwise); for inference, without
-gradients.  As for `Native8B`: validation happens on the host before
+gradients.  With storage "mxfp4" the pages hold bf16 or fp16 rows in 4 bits: e2m1
+numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6) times a power of two for every 32 dims.  As for `Native8B`: validation happens on the host before
 anything is enqueued (ValueError), calls go to the current stream of the
 cache's device, never synchronise and can be captured into a HIP graph after
 one eager call has made their workspaces; lengths and page table are read on
@@ -25,13 +27,18 @@ from collections import deque
 import torch
 
 from . import _lib
+from .rotary import Rotary
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 HEAD_DIMS = (64, 128, 256)
 MAX_SCALE = torch.finfo(torch.float32).max / 1.4426950408889634
-ERR_PAGES, ERR_ROWS = 4, 8  # codes of the error word, as the kernels write them
+STORAGES = (None, "mxfp4")
+IN_FOUR = 16  # added to the row type's code where the pages hold 4 bits
+ERR_PAGES, ERR_ROWS, ERR_OFFSETS, ERR_HELD = 4, 8, 16, 32  # codes of the error word, as the kernels write them
 ERROR_MESSAGES = {ERR_PAGES: "a slot below a sequence's length has no page",
-                  ERR_ROWS: "the offsets of an append did not ascend from 0 to its number of rows"}
+                  ERR_ROWS: "the offsets of an append did not ascend from 0 to its number of rows",
+                  ERR_OFFSETS: "the offsets of a prompt or a read did not ascend from 0 to its number of rows",
+                  ERR_HELD: "a prompt or a read asked for more rows than a sequence holds"}
 _SCORED = ("seen", "scores", "positions")
 
 
@@ -102,7 +109,10 @@ class PagedCache:
     """A cache of `sequences` sequences in `pages` pages of `page_size` slots;
     a sequence takes at most `max_pages` of them.
 
-    Tensors: k, v [pages, kv_heads, page_size, head_dim]; table i32
+    Tensors: k, v [pages, kv_heads, page_size, head_dim] (with storage "mxfp4" u8 [pages,
+    kv_heads, page_size, head_dim / 2], two codes a byte, the even dim in the lower half,
+    and k_scales, v_scales u8 [pages, kv_heads, page_size, head_dim / 32], the powers
+    of two plus 127, 255 for blocks that held an infinity or NaN); table i32
     [sequences, max_pages] (-1: no page); lengths i32 [sequences]; and, if
     `scored`, seen i32 [sequences] (tokens appended so far), scores f32 and
     positions i32 [sequences, kv_heads, max_pages * page_size] (each slot's
@@ -117,7 +127,7 @@ class PagedCache:
     changes; it is made anew when this cache has gone on by itself."""
 
     def __init__(self, sequences, pages, max_pages, *, page_size=64, kv_heads=8, head_dim=128, dtype=torch.bfloat16,
-                 scored=False, device="cuda", library=None, _err=None):
+                 scored=False, storage=None, device="cuda", library=None, _err=None):
         for value, what in ((sequences, "sequences"), (pages, "pages"), (max_pages, "max_pages"),
                             (page_size, "page_size"), (kv_heads, "kv_heads")):
             _check(int(value) >= 1, f"{what} must be positive")
@@ -125,48 +135,66 @@ class PagedCache:
         _check(device.type == "cuda", "native backend requires a device tensor")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        _native_types(int(head_dim), dtype)
-        shape = (int(pages), int(kv_heads), int(page_size), int(head_dim))
+        _native_types(int(head_dim), dtype, storage)
+        shape = (int(pages), int(kv_heads), int(page_size), int(head_dim) // (2 if storage else 1))
+        held = torch.uint8 if storage else dtype
         slots = int(max_pages) * int(page_size)
         _check_slots(int(sequences), slots)
-        if math.prod(shape) * dtype.itemsize > 1 << 36:
+        if math.prod(shape) * held.itemsize > 1 << 36:
             raise NotImplementedError("pages that span at most 64 GiB (of k, and of v)")
-        k = torch.zeros(shape, dtype=dtype, device=device)
-        v = torch.zeros(shape, dtype=dtype, device=device)
+        k = torch.zeros(shape, dtype=held, device=device)
+        v = torch.zeros(shape, dtype=held, device=device)
         table = torch.full((int(sequences), int(max_pages)), -1, dtype=torch.int32, device=device)
         lengths = torch.zeros(int(sequences), dtype=torch.int32, device=device)
         meta = {}
+        if storage:
+            meta = {name: torch.full(shape[:3] + (int(head_dim) // 32,), 2, dtype=torch.uint8, device=device)
+                    for name in ("k_scales", "v_scales")}
         if scored:
-            meta = dict(seen=torch.zeros_like(lengths),
+            meta.update(seen=torch.zeros_like(lengths),
                         scores=torch.zeros(int(sequences), int(kv_heads), slots, dtype=torch.float32, device=device),
                         positions=torch.zeros(int(sequences), int(kv_heads), slots, dtype=torch.int32, device=device))
-        self._setup(k, v, table, lengths, library=library, err=_err, **meta)
+        self._setup(k, v, table, lengths, dtype=dtype, library=library, err=_err, **meta)
         self._free = list(range(int(pages)))[::-1]
         self._pages = [[] for _ in range(int(sequences))]
 
     @classmethod
-    def from_tensors(cls, k, v, table, lengths, *, seen=None, scores=None, positions=None, library=None):
+    def from_tensors(cls, k, v, table, lengths, *, seen=None, scores=None, positions=None, k_scales=None, v_scales=None,
+                     dtype=None, library=None):
         """A cache over the caller's own tensors (pages of any strides of
         16-byte multiples, the same for k and v), whose page table the caller
         keeps: `reserve` and `release` are not offered.  seen, scores and
-        positions are given all or none."""
+        positions are given all or none.  Pages in 4 bits come with k_scales and
+        v_scales (strides of multiples of head_dim / 32, the same for both) and the
+        rows' dtype."""
         obj = cls.__new__(cls)
-        obj._setup(k, v, table, lengths, seen=seen, scores=scores, positions=positions, library=library)
+        obj._setup(k, v, table, lengths, seen=seen, scores=scores, positions=positions, k_scales=k_scales,
+                   v_scales=v_scales, dtype=dtype, library=library)
         return obj
 
-    def _setup(self, k, v, table, lengths, *, seen=None, scores=None, positions=None, library=None, err=None):
+    def _setup(self, k, v, table, lengths, *, seen=None, scores=None, positions=None, k_scales=None, v_scales=None,
+               dtype=None, library=None, err=None):
         _check(isinstance(k, torch.Tensor) and k.device.type == "cuda", "native backend requires a device tensor")
         _check(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device,
                "K and V pages [pages, kv_heads, page_size, head_dim] of one type required")
-        pages, kv_heads, page_size, head_dim = k.shape
-        _native_types(head_dim, k.dtype)
+        pages, kv_heads, page_size, row = k.shape
+        head_dim, scale_strides = row, (0, 0, 0)
+        storage = "mxfp4" if k.dtype == torch.uint8 else None
+        if storage:
+            head_dim = 2 * row
+            scale_strides = _check_scales(k, k_scales, v_scales)
+        else:
+            _check(k_scales is None and v_scales is None, "scales belong to pages in 4 bits (uint8)")
+            _check(dtype is None or dtype == k.dtype, "K and V pages of the rows' dtype required")
+            dtype = k.dtype
+        _native_types(head_dim, dtype, storage)
         _check(min(k.shape) >= 1, "K and V pages [pages, kv_heads, page_size, head_dim] of one type required")
         es = k.element_size()
         _check(k.stride() == v.stride() and k.stride(3) == 1, "K and V pages of equal strides and contiguous rows required")
         _check(not any(s * es % 16 for s in k.stride()[:3]) and not (k.data_ptr() | v.data_ptr()) % 16,
                "K/V rows must be 16-byte aligned")
-        _check(k.stride(2) >= head_dim and (pages == 1 or k.stride(0) >= head_dim) and
-               (kv_heads == 1 or k.stride(1) >= head_dim), "K/V rows must not overlap")
+        _check(k.stride(2) >= row and (pages == 1 or k.stride(0) >= row) and
+               (kv_heads == 1 or k.stride(1) >= row), "K/V rows must not overlap")
         if max(pages * k.stride(0), (pages - 1) * k.stride(0) + page_size * k.stride(2)) * es > 1 << 36:
             raise NotImplementedError("pages that span at most 64 GiB (of k, and of v)")
         _check(table.dim() == 2 and min(table.shape) >= 1, "an int32 page table [sequences, max_pages] required")
@@ -189,23 +217,26 @@ class PagedCache:
             raise RuntimeError(f"{self.lib.path.name} lacks entry points {self.lib.missing}; rebuild it")
         self._tensors = (k, v, table, lengths, seen, scores, positions)
         self.device = k.device
+        self.dtype, self.storage, self._scales = dtype, storage, (k_scales, v_scales)
         self._shape = (sequences, kv_heads, head_dim, page_size, max_pages)
         # the buffers that calls read and write besides the pages, as [from, to)
         self._spans = tuple((x.data_ptr(), x.data_ptr() + 4 * x.numel()) for x in self._tensors[3:] if x is not None)
         _check(not any(_overlap(x, y) for x, y in itertools.combinations(self._spans, 2)),
                "lengths, seen, scores and positions must not overlap")
         self._free = self._pages = None
-        self._attend_work, self._evict_work = {}, None
+        self._attend_work, self._evict_work, self._prompt_work, self._prompt_last = {}, None, {}, (None, None)
         self._err = _ErrorWord(self.lib, self.device) if err is None else err
         # what the C entries read of the cache; its tensors are fixed from here on
         pointers = [0 if x is None else x.data_ptr() for x in self._tensors]
         self._desc = _lib.PagedCacheDesc(*pointers, self._err.address, pages, *k.stride()[:3], *self._shape,
-                                         DTYPES[k.dtype])
+                                         DTYPES[dtype] + (IN_FOUR if storage else 0),
+                                         *(x.data_ptr() if storage else 0 for x in self._scales), *scale_strides)
         self._pointer = ctypes.c_void_p(ctypes.addressof(self._desc))
 
     # ------------------------------------------------------------ pages
 
     k, v, table, lengths, seen, scores, positions = (property(lambda self, i=i: self._tensors[i]) for i in range(7))
+    k_scales, v_scales = (property(lambda self, i=i: self._scales[i]) for i in range(2))
 
     @property
     def scored(self):
@@ -222,7 +253,8 @@ class PagedCache:
         taken back.  (Rows that `evict` moves are moved for both.)"""
         obj = PagedCache.__new__(PagedCache)
         meta = {name: getattr(self, name).clone() for name in _SCORED} if self.scored else {}
-        obj._setup(self.k, self.v, self.table, self.lengths.clone(), library=self.lib.path, err=self._err, **meta)
+        obj._setup(self.k, self.v, self.table, self.lengths.clone(), k_scales=self.k_scales, v_scales=self.v_scales,
+                   dtype=self.dtype, library=self.lib.path, err=self._err, **meta)
         return obj
 
     def reserve(self, tokens):
@@ -267,11 +299,15 @@ class PagedCache:
         counts = [min(len(held), int(max_pages)) for held in self._pages]
         _check(sum(counts) <= int(pages), "the sequences' pages do not fit")
         new = PagedCache(sequences, pages, max_pages, page_size=page_size, kv_heads=kv_heads, head_dim=head_dim,
-                         dtype=self.k.dtype, scored=self.scored, device=self.device, library=self.lib.path, _err=self._err)
+                         dtype=self.dtype, scored=self.scored, storage=self.storage, device=self.device,
+                         library=self.lib.path, _err=self._err)
         new.reserve([count * page_size for count in counts])
         for held, own, count in zip(self._pages, new._pages, counts):
             new.k[own] = self.k[held[:count]]
             new.v[own] = self.v[held[:count]]
+            if self.storage:
+                new.k_scales[own] = self.k_scales[held[:count]]
+                new.v_scales[own] = self.v_scales[held[:count]]
         new.lengths.copy_(self.lengths)
         if self.scored:
             slots = min(new.slots, self.slots)
@@ -323,7 +359,9 @@ class PagedCache:
         a, b = self._desc, into._desc
         if (a.k != b.k or a.v != b.v or a.table != b.table or a.pages != b.pages or a.page_stride != b.page_stride
                 or a.head_stride != b.head_stride or a.slot_stride != b.slot_stride or into._shape != self._shape
-                or a.dtype != b.dtype or (a.scores == 0) != (b.scores == 0)):
+                or a.dtype != b.dtype or (a.scores == 0) != (b.scores == 0) or a.k_scales != b.k_scales
+                or a.v_scales != b.v_scales or a.scale_page_stride != b.scale_page_stride
+                or a.scale_head_stride != b.scale_head_stride or a.scale_slot_stride != b.scale_slot_stride):
             raise ValueError("into must be a fork of this cache")
         # (what `fork` made has buffers of its own)
         if into._err is not self._err and into._spans != self._spans and any(
@@ -341,19 +379,25 @@ class PagedCache:
             work[:zero].zero_()
             return work
 
-    def append(self, k, v, offsets=None, *, into=None):
+    def append(self, k, v, offsets=None, *, q=None, rotary=None, into=None):
         """Writes new rows behind every sequence's: k and v [rows, kv_heads,
         head_dim] of the cache's type, one row per sequence, or with `offsets`
         (i32 [sequences + 1], ascending from 0) rows offsets[b] .. offsets[b +
         1] for sequence b.  Advances the lengths; of a scored cache also the
         tokens seen, the rows starting with score 0.  The slots need pages
-        (`reserve`); a row without one is dropped and reported."""
+        (`reserve`); a row without one is dropped and reported.
+
+        With `rotary`, a `Rotary`, the keys are turned by their positions on the way:
+        the slots that they take or, of a scored cache, the tokens seen before them
+        (eviction moves slots).  q [rows, heads, head_dim], the same tokens' queries,
+        comes back turned as a new contiguous tensor.  Turned rows are rounded to
+        their type, as if they had been turned before the call."""
         to = self if into is None else self._into(into)
         sequences, kv_heads, head_dim, _, _ = self._shape
         shape, ks, vs = k.shape, k.stride(), v.stride()
         if len(shape) != 3 or v.shape != shape or shape[1] != kv_heads or shape[2] != head_dim:
             raise ValueError(f"K and V rows [rows, {kv_heads}, {head_dim}] required")
-        dtype, device = self.k.dtype, self.device
+        dtype, device = self.dtype, self.device
         if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
             raise ValueError("K and V rows of the cache's type on its device required")
         rows, es = shape[0], k.element_size()
@@ -366,9 +410,53 @@ class PagedCache:
             _i32(offsets, (sequences + 1,), self.device, "offsets")
         elif rows != sequences:
             raise ValueError("one row per sequence, or offsets, required")
+        op = 0 if offsets is None else offsets.data_ptr()
+        if rotary is None:
+            _check(q is None, "q is turned by a rotary")
+            self.check_errors()
+            self._call("prismkv_paged_append", self._pointer, to._pointer, kp, vp, op, rows, ks[0], ks[1], vs[0], vs[1])
+            return None
+        _check(isinstance(rotary, Rotary) and rotary.head_dim == head_dim and rotary.device == device,
+               f"a Rotary of head_dim {head_dim} on the cache's device required")
+        out, heads, qs, qp, outp = None, 0, (0, 0), 0, 0
+        if q is not None:
+            shape, qs, qp = q.shape, q.stride(), q.data_ptr()
+            if (len(shape) != 3 or shape[0] != rows or shape[2] != head_dim or shape[1] < 1 or shape[1] % kv_heads
+                    or q.dtype != dtype or q.device != device):
+                raise ValueError(f"Q[{rows}, a multiple of {kv_heads} heads, {head_dim}] of the cache's type on its device "
+                                 "required")
+            if rows and (qs[2] != 1 or ((qs[0] | qs[1]) * es | qp) % 16):
+                raise ValueError("Q rows must be contiguous and 16-byte aligned")
+            heads = shape[1]
+            if heads > 1024 * kv_heads:
+                raise NotImplementedError("at most 1024 query heads per KV head")
+            out = torch.empty(shape, dtype=dtype, device=device)
+            outp = out.data_ptr()
         self.check_errors()
-        self._call("prismkv_paged_append", self._pointer, to._pointer, kp, vp,
-                   0 if offsets is None else offsets.data_ptr(), rows, ks[0], ks[1], vs[0], vs[1])
+        self._call("prismkv_paged_append_rows", self._pointer, to._pointer, kp, vp, qp, outp, op, rotary.turns.data_ptr(),
+                   rows, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], heads, rotary.rotary_dim, int(rotary.interleaved),
+                   rotary.amplitude)
+        return out
+
+    def read(self, offsets=None, *, rows=None):
+        """The keys and values of every sequence's last slot, or with `offsets` (i32
+        [sequences + 1], ascending from 0 to `rows`) of its last offsets[b + 1] -
+        offsets[b] ones, in the order of the slots: k and v [rows, kv_heads,
+        head_dim] of the cache's dtype (what 4 bits stand for is exact in it, but
+        for fp16's 65536, which becomes an infinity, and what is below its least number).
+        Rows that a sequence does not hold are 0 and reported."""
+        sequences, kv_heads, head_dim, _, _ = self._shape
+        if offsets is not None:
+            _i32(offsets, (sequences + 1,), self.device, "offsets")
+            _check(rows is not None, "offsets need the number of their rows")
+        rows = sequences if rows is None else int(rows)
+        _check(0 <= rows < 2 ** 31 and (offsets is not None or rows == sequences), "one row per sequence, or offsets, required")
+        k = torch.empty(rows, kv_heads, head_dim, dtype=self.dtype, device=self.device)
+        v = torch.empty_like(k)
+        self.check_errors()
+        self._call("prismkv_paged_read", self._pointer, 0 if offsets is None else offsets.data_ptr(), k.data_ptr(),
+                   v.data_ptr(), rows)
+        return k, v
 
     def attend(self, q, *, scale=None, accumulate=False, lse=None, into=None):
         """Softmax attention of q [sequences, heads, head_dim] (heads a
@@ -390,7 +478,7 @@ class PagedCache:
         if (len(shape) != 3 or shape[0] != sequences or shape[2] != head_dim or shape[1] < 1 or shape[1] % kv_heads
                 or not q.is_contiguous()):
             raise ValueError(f"contiguous Q[{sequences}, a multiple of {kv_heads} heads, {head_dim}] required")
-        if q.dtype != self.k.dtype or q.device != self.device:
+        if q.dtype != self.dtype or q.device != self.device:
             raise ValueError("Q of the cache's type on its device required")
         if q.data_ptr() % 16:
             raise ValueError("Q rows must be 16-byte aligned")
@@ -399,13 +487,17 @@ class PagedCache:
             raise NotImplementedError("at most 1024 query heads per KV head")
         if accumulate and self.scores is None:
             raise ValueError("accumulate needs a scored cache")
-        scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-        if not abs(scale) <= MAX_SCALE:
+        return group, self._check_scale(q, scale, lse, "sequences")
+
+    def _check_scale(self, q, scale, lse, rows):
+        scale = 1.0 / math.sqrt(self._shape[2]) if scale is None else float(scale)
+        # (fp16 rows are held in 4 bits at half their value, and the scale is doubled for it)
+        if not abs(scale) <= (MAX_SCALE / 2 if self.storage and self.dtype == torch.float16 else MAX_SCALE):
             raise ValueError("a scale that is finite in float32, as times log2(e), required")
         if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()
                                 or lse.device != self.device):
-            raise ValueError("lse must be a contiguous float32 [sequences, heads] on the cache's device")
-        return group, scale
+            raise ValueError(f"lse must be a contiguous float32 [{rows}, heads] on the cache's device")
+        return scale
 
     def _attend_workspace(self, group, accumulate):
         work = self._attend_work.get((group, accumulate))
@@ -428,18 +520,89 @@ class PagedCache:
                    work.data_ptr(), out.data_ptr(), group, flags + accumulate, scale, work.numel())
         return out
 
-    def __call__(self, q, k, v, *, scale=None, accumulate=False, lse=None, into=None):
+    def __call__(self, q, k, v, *, rotary=None, scale=None, accumulate=False, lse=None, into=None):
         """A decode step: `append` one row of k and v [sequences, kv_heads,
-        head_dim] to every sequence, then `attend`.  With `into` both results
-        go there, the new rows into the shared pages behind this cache's
-        lengths."""
+        head_dim] to every sequence, with `rotary` k and q turned, then `attend`.
+        With `into` both results go there, the new rows into the shared pages
+        behind this cache's lengths."""
         to = self if into is None else self._into(into)
         # nothing is appended for a query that is refused
         group, scale = self._check_q(q, scale, accumulate, lse)
         accumulate = bool(accumulate)
         work = self._attend_workspace(group, accumulate)
-        self.append(k, v, into=into)
-        return self._attend(q, group, scale, accumulate, lse, to, 2, work)
+        turned = self.append(k, v, q=q if rotary is not None else None, rotary=rotary, into=into)
+        return self._attend(q if turned is None else turned, group, scale, accumulate, lse, to, 2, work)
+
+    def attend_prompt(self, q, offsets=None, *, scale=None, lse=None):
+        """Causal softmax attention of many tokens of each sequence, all appended
+        before: q [rows, heads, head_dim] (heads a multiple of the cache's kv_heads;
+        consecutive heads share a KV head) packed by `offsets` (i32 [sequences + 1],
+        ascending from 0 to rows; None: one row each), the queries of every sequence's
+        last offsets[b + 1] - offsets[b] slots.  Each sees the slots up to its own, the
+        older ones among them: a prompt in chunks, or a turn after a history, is a call
+        each.  (After an `evict` of slots appended since, slots are no longer in the
+        order of their tokens.)  The output has q's shape and type; `lse`, an f32
+        [rows, heads] tensor, receives the logarithm of each softmax's sum.  More rows
+        than a sequence holds are reported, and those before its first slot are 0 and
+        -inf."""
+        group, scale = self._check_prompt(q, offsets, scale, lse)
+        return self._prompt(q, offsets, group, scale, lse, self._prompt_workspace(q.shape[0], group))
+
+    def _check_prompt(self, q, offsets, scale, lse, turned=False):
+        """The query heads per KV head, and the scale (turned: q comes contiguous)."""
+        sequences, kv_heads, head_dim, _, _ = self._shape
+        shape = q.shape
+        if (len(shape) != 3 or shape[2] != head_dim or shape[1] < 1 or shape[1] % kv_heads
+                or not (turned or q.is_contiguous())):
+            raise ValueError(f"contiguous Q[rows, a multiple of {kv_heads} heads, {head_dim}] required")
+        if q.dtype != self.dtype or q.device != self.device:
+            raise ValueError("Q of the cache's type on its device required")
+        if q.data_ptr() % 16:
+            raise ValueError("Q rows must be 16-byte aligned")
+        if offsets is not None:
+            _i32(offsets, (sequences + 1,), self.device, "offsets")
+        elif shape[0] != sequences:
+            raise ValueError("one row per sequence, or offsets, required")
+        group = shape[1] // kv_heads
+        if group > 1024:
+            raise NotImplementedError("at most 1024 query heads per KV head")
+        return group, self._check_scale(q, scale, lse, "rows")
+
+    def _prompt_workspace(self, rows, group):
+        key, work = self._prompt_last
+        if key != (rows, group):
+            sequences, kv_heads, head_dim, _, _ = self._shape
+            nbytes = self.lib.query("prismkv_paged_prompt_work_bytes", rows, sequences, kv_heads, group, head_dim, self.slots,
+                                    self._desc.dtype)
+            if not nbytes:
+                raise NotImplementedError("at most 2^30 rows of a prompt times the query heads of a KV head")
+            # sizes of powers of two, each kept: a captured graph goes on using its own
+            size = 1 << (nbytes - 1).bit_length()
+            work = self._prompt_work.get(size)
+            if work is None:
+                work = self._prompt_work[size] = self._workspace(size, 0)
+            self._prompt_last = (rows, group), work
+        return work
+
+    def _prompt(self, q, offsets, group, scale, lse, work):
+        self.check_errors()
+        out = torch.empty_like(q)
+        self._call("prismkv_paged_prompt", self._pointer, q.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+                   0 if lse is None else lse.data_ptr(), work.data_ptr(), out.data_ptr(), q.shape[0], group, scale,
+                   work.numel())
+        return out
+
+    def prompt(self, q, k, v, offsets=None, *, rotary=None, scale=None, lse=None, into=None):
+        """Prompts, or chunks of them: `append` rows of k and v, with `rotary` k and q
+        turned, then `attend_prompt`; arguments as theirs.  With `into` the lengths go
+        there, the new rows into the shared pages behind this cache's lengths."""
+        to = self if into is None else self._into(into)
+        # nothing is appended for a query that is refused
+        group, scale = self._check_prompt(q, offsets, scale, lse, rotary is not None)
+        _check(k.shape[0] == q.shape[0], "as many K and V rows as Q rows required")
+        work = to._prompt_workspace(q.shape[0], group)
+        turned = self.append(k, v, offsets, q=q if rotary is not None else None, rotary=rotary, into=into)
+        return to._prompt(q if turned is None else turned, offsets, group, scale, lse, work)
 
     def evict(self, keep, *, recent=0, sinks=0, into=None):
         """Cuts every sequence longer than `keep` slots (an int, or i32
@@ -473,9 +636,11 @@ class PagedCache:
         """Live tensors held here, by name (a fork's pages are its origin's)."""
         names = ("k", "v", "table", "lengths", "seen", "scores", "positions")
         held = {name: x for name, x in zip(names, self._tensors) if x is not None}
+        held.update((name, x) for name, x in zip(("k_scales", "v_scales"), self._scales) if x is not None)
         if self._evict_work is not None:
             held["evict_work"] = self._evict_work
         held.update((f"attend_work{key}", x) for key, x in self._attend_work.items())
+        held.update((f"prompt_work{key}", x) for key, x in self._prompt_work.items())
         return {name: x.numel() * x.element_size() for name, x in held.items()}
 
 
@@ -483,9 +648,29 @@ def _overlap(x, y):
     return x[0] < y[1] and y[0] < x[1]
 
 
-def _native_types(head_dim, dtype):
+def _native_types(head_dim, dtype, storage=None):
     if head_dim not in HEAD_DIMS or dtype not in DTYPES:
         raise NotImplementedError("the paged cache holds bf16, fp16 or fp32 rows of head_dim 64, 128 or 256")
+    _check(storage in STORAGES, f"storage must be one of {STORAGES}")
+    if storage and dtype == torch.float32:
+        raise NotImplementedError("the paged cache holds bf16 or fp16 rows in 4 bits")
+
+
+def _check_scales(k, k_scales, v_scales):
+    """The scales of pages in 4 bits: their strides of pages, heads and slots."""
+    shape = tuple(k.shape[:3]) + (k.shape[3] // 16,)
+    _check(all(isinstance(x, torch.Tensor) and x.dtype == torch.uint8 and tuple(x.shape) == shape and x.device == k.device
+               for x in (k_scales, v_scales)),
+           f"pages in 4 bits need k_scales and v_scales, uint8 {list(shape)} on their device")
+    strides, row = k_scales.stride(), max(shape[3], 1)
+    _check(strides == v_scales.stride() and strides[3] == 1, "scales of equal strides and contiguous rows required")
+    _check(not any(s % row for s in strides[:3]) and not (k_scales.data_ptr() | v_scales.data_ptr()) % row,
+           f"rows of scales must be {row}-byte aligned")
+    _check(strides[2] >= row and (shape[0] == 1 or strides[0] >= row) and (shape[1] == 1 or strides[1] >= row),
+           "rows of scales must not overlap")
+    if max(shape[0] * strides[0], shape[2] * strides[2]) > 1 << 36:
+        raise NotImplementedError("pages that span at most 64 GiB (of k, and of v)")
+    return strides[:3]
 
 
 def _check_slots(sequences, slots):
