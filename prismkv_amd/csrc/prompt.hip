@@ -17,7 +17,7 @@ namespace {
 constexpr int kWaves = 4, kTileRows = 32 * kWaves, kThreads = 64 * kWaves;
 // Keys and values that are staged at a time.
 template <int DT, int D>
-constexpr int kTileTokens = kElem<DT> * D > 512 ? 32 : 64;
+constexpr int kTileTokens = kElem<DT> * D > 256 ? 32 : 64;
 // Waves of a SIMD, by the registers that products, queries and staged rows take.
 template <int DT, int D>
 constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
@@ -35,7 +35,8 @@ struct Prompt {
   char* out;
   float *lse, *state;
   unsigned* err;
-  int64_t page_bytes, head_bytes, slot_bytes, scale_page, scale_head, scale_slot;
+  int64_t head_bytes, scale_page, scale_head, scale_slot;
+  unsigned page_units, slot_units;  // 16 bytes
   PageDiv div;
   unsigned q_and, q_xor;  // the scale's sign, or a scale of 0, goes to the queries
   float scale;            // log2(e) times the caller's magnitude
@@ -142,6 +143,38 @@ __device__ __forceinline__ int staged(int r, int c) {
   return (r * kC + (c ^ f)) * 16;
 }
 
+// The same places for what a lane reads in the main loop, as one address of the lane, a
+// constant to xor it with (few of them) and a constant offset: written out, as the
+// compiler does not take `staged` apart and keeps an address for every read.
+template <int kC>
+struct KeyAt {  // chunk 2c + half of row 32i + col
+  int lane;
+  __device__ __forceinline__ KeyAt(int col, int half) : lane(staged<kC>(col, half)) {}
+  __device__ __forceinline__ int of(int i, int c) const {
+    constexpr int kMask = kC == 8 ? 7 : 15;
+    return (lane ^ ((2 * c & kMask) << 4)) + ((2 * c & ~kMask) + 32 * i * kC) * 16;
+  }
+};
+template <int kC>
+struct ValueAt {  // chunk 4d + 2 side + (in >> 1 & 1) of row 32i + 16u + 8 hi + 4 half + in / 4, its in & 1 part
+  int lane;
+  __device__ __forceinline__ ValueAt(int l)
+      : lane(staged<kC>(4 * (l >> 5) + (l >> 2 & 3), 2 * (l >> 4 & 1) + (l >> 1 & 1)) + 8 * (l & 1)) {}
+  __device__ __forceinline__ int of(int i, int u, int hi, int d) const {
+    const int rows = (32 * i + 16 * u + 8 * hi) * kC * 16;
+    if constexpr (kC == 8) return (lane ^ ((4 * d ^ hi) << 4)) + rows;
+    else return (lane ^ (4 * (d & 1) << 4)) + rows + (8 * ((d >> 1 & 1) ^ hi) + 16 * (d >> 2)) * 16;
+  }
+};
+template <int kC>
+struct FloatAt {  // element 32d + col of row 32i + 8 (r / 4) + 4 half + r % 4, in fp32
+  int lane;
+  __device__ __forceinline__ FloatAt(int col, int half) : lane(staged<kC>(4 * half, col >> 2) + 4 * (col & 3)) {}
+  __device__ __forceinline__ int of(int i, int r, int d) const {
+    return (lane ^ ((r % 4) << 5)) + ((32 * i + 8 * (r / 4) + r % 4) * kC + 8 * ((d ^ (r / 4)) & 1) + 16 * (d >> 1)) * 16;
+  }
+};
+
 template <int DT>
 __device__ __forceinline__ f32x16 mfma_rows(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (kType<DT> == kBf16)
@@ -171,20 +204,21 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
   }
 }
 
-// Whether any element of 16 bytes is an infinity or NaN.
+// 16 bytes with 0 for each element that is an infinity or NaN; whether there was one.
 template <int DT>
-__device__ __forceinline__ bool any_special(u32x4 x) {
-  bool any = false;
+__device__ __forceinline__ u32x4 without_special(u32x4 x, bool& any) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
+    const unsigned w = x[e];
     if constexpr (kType<DT> == kFp32) {
-      any |= (x[e] & 0x7f800000u) == 0x7f800000u;
+      x[e] = (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
     } else {
       constexpr unsigned kMask = kType<DT> == kBf16 ? 0x7f80u : 0x7c00u;
-      any |= (x[e] & kMask) == kMask || (x[e] >> 16 & kMask) == kMask;
+      x[e] = ((w & kMask) == kMask ? 0u : w & 0xffffu) | ((w >> 16 & kMask) == kMask ? 0u : w & 0xffff0000u);
     }
+    any |= x[e] != w;
   }
-  return any;
+  return x;
 }
 
 // Eight codes as eight elements of the 16-bit type (for fp16 half of them, kSumBias).
@@ -204,7 +238,9 @@ __device__ __forceinline__ u32x4 widen_eight(unsigned codes, unsigned byte) {
                  __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
 }
 
-// A thread's part of a tile of keys and values on its way from the pages to LDS.
+// A thread's part of a tile of keys and values on its way from the pages to LDS.  Each
+// lane looks up one row's place, the tile ahead, and the rows' readers take it from
+// there.  Rows past the end repeat the last one: no row sees them.
 template <int DT, int D>
 struct Stage {
   static constexpr int kTokens = kTileTokens<DT, D>;
@@ -217,7 +253,7 @@ struct Stage {
   const int32_t* tab;
   int end, row, chunk;
   bool bad = false;
-  int page[kEach];
+  int page, token;  // of this lane's row
   Word kw[kEach], vw[kEach];
   unsigned kb[kInFour<DT> ? kEach : 1], vb[kInFour<DT> ? kEach : 1];
 
@@ -235,34 +271,30 @@ struct Stage {
   }
   static __device__ __forceinline__ int step(int i) { return i * (kThreads / kC); }
   __device__ __forceinline__ void ask(int t0) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) page[i] = tab[a.div.of(min(t0 + row + step(i), end - 1))];
+    token = min(t0 + (int)(threadIdx.x & (kTokens - 1)), end - 1);
+    page = tab[a.div.of(token)];
   }
-  // rows past the end stay 0
-  __device__ __forceinline__ void load(int t0) {
+  __device__ __forceinline__ void load() {
+    bad |= (unsigned)page >= (unsigned)a.pages;
+    const unsigned p = (unsigned)page < (unsigned)a.pages ? (unsigned)page : 0u;
+    const unsigned in = (unsigned)(token - a.div.of(token) * a.page_size);
+    const unsigned place = p * a.page_units + in * a.slot_units;  // of 16 bytes
+    uint64_t scale_place = 0;
+    if constexpr (kInFour<DT>) scale_place = (uint64_t)p * a.scale_page + (uint64_t)in * a.scale_slot;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int t = t0 + row + step(i);
-      kw[i] = Word{};
-      vw[i] = Word{};
-      if constexpr (kInFour<DT>) kb[i] = vb[i] = 0u;
-      if (t < end) {
-        bad |= (unsigned)page[i] >= (unsigned)a.pages;
-        const unsigned p = (unsigned)page[i] < (unsigned)a.pages ? (unsigned)page[i] : 0u;
-        const unsigned in = (unsigned)(t - a.div.of(t) * a.page_size);
-        const size_t at = (size_t)p * a.page_bytes + (size_t)in * a.slot_bytes;
-        kw[i] = *reinterpret_cast<const Word*>(k + at);
-        vw[i] = *reinterpret_cast<const Word*>(v + at);
-        if constexpr (kInFour<DT>) {
-          const size_t scale_at = (size_t)p * a.scale_page + (size_t)in * a.scale_slot;
-          kb[i] = ks[scale_at];
-          vb[i] = vs[scale_at];
-        }
+      const size_t at = (size_t)(unsigned)__shfl((int)place, row + step(i)) << 4;
+      kw[i] = *reinterpret_cast<const Word*>(k + at);
+      vw[i] = *reinterpret_cast<const Word*>(v + at);
+      if constexpr (kInFour<DT>) {
+        const size_t scale_at = (size_t)__shfl((unsigned long long)scale_place, row + step(i));
+        kb[i] = ks[scale_at];
+        vb[i] = vs[scale_at];
       }
     }
   }
-  // Writes the tile; whether a value is special (looked at only if asked for).
-  __device__ __forceinline__ bool store(char* keys, char* values, bool look) const {
+  // Writes the tile, `clean` without the values' infinities and NaN; whether there were any.
+  __device__ __forceinline__ bool store(char* keys, char* values, bool clean) const {
     bool special = false;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -274,10 +306,10 @@ struct Stage {
         x = kw[i];
         y = vw[i];
       }
+      if (clean) y = without_special<DT>(y, special);
       const int at = staged<kC>(row + step(i), chunk);
       *reinterpret_cast<u32x4*>(keys + at) = x;
       *reinterpret_cast<u32x4*>(values + at) = y;
-      if (look) special |= any_special<DT>(y);
     }
     return special;
   }
@@ -377,6 +409,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       for (int e = 0; e < 4; ++e) q[c][e] = (x[e] & a.q_and) ^ a.q_xor;
     }
   }
+  const KeyAt<kC> key_at(col, half);
   f32x16 acc[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -388,25 +421,25 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   Stage<DT, D> stage(a, it.b, it.h, cut.end);
   if (from < to) {
     stage.ask(from * kTokens);
-    stage.load(from * kTokens);
+    stage.load();
     if (from + 1 < to) stage.ask((from + 1) * kTokens);
   }
+  // In a tile that some row does not see all of, 0 times an infinity or NaN must not reach
+  // that row: such values are left out there, and added to the rows that see them at the end.
+  bool special = false;
   for (int t = from; t < to; ++t) {
     const int t0 = t * kTokens;
-    // A tile that some row does not see all of: where a value there is an infinity or NaN,
-    // 0 times it must not reach that row.
     const bool partly = t0 + kTokens - 1 > tile_first;
     __syncthreads();  // the last tile has been read
-    bool special = stage.store(keys, values, partly);
+    special |= stage.store(keys, values, partly);
     if (t + 1 < to) {
-      stage.load(t0 + kTokens);
+      stage.load();
       if (t + 2 < to) stage.ask(t0 + 2 * kTokens);
     }
-    if (partly) special = __syncthreads_or(special);
-    else __syncthreads();
-    const bool seen = t0 <= wave_last;
+    __syncthreads();
+    if (t0 > wave_last) continue;
     f32x16 s[kT];
-    if (seen) {
+    {
 #pragma unroll
       for (int i = 0; i < kT; ++i)
 #pragma unroll
@@ -415,7 +448,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       for (int c = 0; c < kC / 2; ++c)
 #pragma unroll
         for (int i = 0; i < kT; ++i)
-          s[i] = mfma_rows<DT>(*reinterpret_cast<const u32x4*>(keys + staged<kC>(32 * i + col, 2 * c + half)), q[c], s[i]);
+          s[i] = mfma_rows<DT>(*reinterpret_cast<const u32x4*>(keys + key_at.of(i, c)), q[c], s[i]);
       if (t0 + kTokens - 1 > wave_first) {
 #pragma unroll
         for (int i = 0; i < kT; ++i)
@@ -467,68 +500,56 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
           }
       }
     }
-    if (partly && special) {  // (all threads alike)
-      __syncthreads();        // the keys have been read: the probabilities of 16 tokens at a time take their place
-      if (!seen) continue;
-      float* p = reinterpret_cast<float*>(keys) + 16 * 32 * w;
-#pragma unroll
-      for (int g = 0; g < 2 * kT; ++g) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r) p[(8 * (r / 4) + 4 * half + r % 4) * 32 + col] = s[g / 2][8 * (g & 1) + r];
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_s_waitcnt(0);
-#pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          const int token_row = 16 * g + k;
-          const bool visible = t0 + token_row <= limit;
-          const float weight = p[k * 32 + col];
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int dim = 32 * d + 8 * j + 4 * half, byte = dim * kElem<DT>;
-              const float4 x = four_of<DT>(values + staged<kC>(token_row, byte >> 4) + (byte & 15));
-              acc[d][4 * j] = visible ? fmaf(weight, x.x, acc[d][4 * j]) : acc[d][4 * j];
-              acc[d][4 * j + 1] = visible ? fmaf(weight, x.y, acc[d][4 * j + 1]) : acc[d][4 * j + 1];
-              acc[d][4 * j + 2] = visible ? fmaf(weight, x.z, acc[d][4 * j + 2]) : acc[d][4 * j + 2];
-              acc[d][4 * j + 3] = visible ? fmaf(weight, x.w, acc[d][4 * j + 3]) : acc[d][4 * j + 3];
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_s_waitcnt(0);
-      }
-      continue;
-    }
-    if (!seen) continue;
     if constexpr (kType<DT> == kFp32) {
+      const FloatAt<kC> float_at(col, half);
 #pragma unroll
       for (int i = 0; i < kT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
 #pragma unroll
-          for (int d = 0; d < D / 32; ++d) {
-            const int at = staged<kC>(32 * i + 8 * (r / 4) + 4 * half + r % 4, 8 * d + col / 4) + 4 * (col & 3);
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + at), s[i][r], acc[d], 0, 0, 0);
-          }
+          for (int d = 0; d < D / 32; ++d)
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + float_at.of(i, r, d)), s[i][r],
+                                                          acc[d], 0, 0, 0);
     } else {
       typedef __attribute__((address_space(3))) s16x4* Transposed;
-      const int in = lane & 15, side = lane >> 4 & 1;  // row in / 4 and piece in % 4 of 16 dims; which 16 dims
+      const ValueAt<kC> value_at(lane);
 #pragma unroll
       for (int i = 0; i < kT; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const u32x4 p = {pack2<DT>(s[i][8 * u], s[i][8 * u + 1]), pack2<DT>(s[i][8 * u + 2], s[i][8 * u + 3]),
                            pack2<DT>(s[i][8 * u + 4], s[i][8 * u + 5]), pack2<DT>(s[i][8 * u + 6], s[i][8 * u + 7])};
-          const int r = 32 * i + 16 * u + 4 * half + in / 4;
 #pragma unroll
           for (int d = 0; d < D / 32; ++d) {
-            const int c = 4 * d + 2 * side + (in >> 1 & 1);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + staged<kC>(r, c) + 8 * (in & 1)));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + staged<kC>(r + 8, c) + 8 * (in & 1)));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 0, d)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 1, d)));
             const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
             acc[d] = mfma_rows<DT>(u32x4{l.x, l.y, h.x, h.y}, p, acc[d]);
           }
         }
+    }
+  }
+  if (__syncthreads_or(special)) {
+#pragma unroll 1
+    for (int t = max(from, (tile_first + 1) / kTokens); t < to; ++t) {
+      stage.ask(t * kTokens);
+      stage.load();
+      __syncthreads();
+      stage.store(keys, values, false);
+      __syncthreads();
+#pragma unroll 1
+      for (int k = 0; k < kTokens && t * kTokens + k <= limit; ++k)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int byte = (32 * d + 8 * j + 4 * half) * kElem<DT>;
+            const float4 x = four_of<DT>(values + staged<kC>(k, byte >> 4) + (byte & 15));
+            acc[d][4 * j] += fabsf(x.x) < INFINITY ? 0.f : x.x;
+            acc[d][4 * j + 1] += fabsf(x.y) < INFINITY ? 0.f : x.y;
+            acc[d][4 * j + 2] += fabsf(x.z) < INFINITY ? 0.f : x.z;
+            acc[d][4 * j + 3] += fabsf(x.w) < INFINITY ? 0.f : x.w;
+          }
     }
   }
   if (__ballot(stage.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
@@ -616,7 +637,7 @@ struct PromptLayout {
 
 PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots, int dtype) {
   PromptLayout l;
-  const int tokens = element_bytes(dtype) * head_dim > 512 ? 32 : 64;
+  const int tokens = element_bytes(dtype) * head_dim > 256 ? 32 : 64;
   const int64_t tiles = (rows * group) / kTileRows + (sequences < rows ? sequences : rows), key_tiles = (slots + tokens - 1) / tokens;
   const int64_t all = 1ll << kItemsLog;
   l.items = all + tiles * kv_heads;
@@ -698,9 +719,9 @@ int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t 
   a.state = reinterpret_cast<float*>(paged_work);
   a.err = reinterpret_cast<unsigned*>(c.err);
   const int64_t es = page_element_bytes(c.dtype);
-  a.page_bytes = c.page_stride * es;
+  a.page_units = (unsigned)(c.page_stride * es >> 4);
   a.head_bytes = c.head_stride * es;
-  a.slot_bytes = c.slot_stride * es;
+  a.slot_units = (unsigned)(c.slot_stride * es >> 4);
   a.scale = (float)(scale2 < 0 ? -scale2 : scale2);
   a.q_and = scale2 == 0 ? 0u : ~0u;
   a.q_xor = !(scale2 < 0) ? 0u : element_bytes(c.dtype) == 4 ? 0x80000000u : 0x80008000u;
