@@ -421,11 +421,11 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *            bytes) and
  *   k_scales, v_scales  u8 [pages][kv_heads][page_size][head_dim / 32], strides in
  *            bytes (multiples of head_dim / 32, as are the addresses): for every
- *            32 dims a byte s >= 2, the codes 0 .. 7 standing for 0, 0.5, 1, 1.5,
- *            2, 3, 4 and 6 times 2^(s - 127), 8 .. 15 for their negatives; all are
- *            NaN where s is 255.  A row is held with the smallest s >= 2 for which
- *            no value is above 7 times that (at most 252, and 255 for infinities and
- *            NaN) and the nearest codes, ties to even;
+ *            32 dims a byte s, in 2 .. 252 or of fp16 rows 104 .. 140, the codes
+ *            0 .. 7 standing for 0, 0.5, 1, 1.5, 2, 3, 4 and 6 times 2^(s - 127), 8 ..
+ *            15 for their negatives; all are NaN where s is 255.  A row is held with
+ *            the smallest s for which no value is above 7 times that (255 for
+ *            infinities and NaN) and the nearest codes, ties to even;
  *   table    i32 [sequences][max_pages]: the page of slots [i page_size,
  *            (i + 1) page_size) of a sequence; an entry outside [0, pages) is no
  *            page.  slots = max_pages * page_size <= 2^30, sequences * slots <

@@ -118,13 +118,14 @@ SIZES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 def hold(x):
     """Codes [..., D] (0 .. 15) and scale bytes [..., D / 32] of rows [..., D], by the
-    definition: the smallest power of two, at least 2^-125 and at most 2^125, for which no value
-    is above 7 times it; the nearest of the sizes, the even code on ties."""
+    definition: the smallest power of two, in 2^-125 .. 2^125 or for fp16 rows 2^-23 .. 2^13,
+    for which no value is above 7 times it; the nearest of the sizes, the even code on ties."""
     y = x.double().unflatten(-1, (-1, 32))
     amax = y.abs().amax(-1)
     special = ~torch.isfinite(amax)
-    e = torch.full(amax.shape, -125, dtype=torch.int32)
-    for power in range(-125, 125):
+    least, most = (-23, 13) if x.dtype == torch.float16 else (-125, 125)
+    e = torch.full(amax.shape, least, dtype=torch.int32)
+    for power in range(least, most):
         e[amax > 7 * 2.0 ** power] = power + 1
     unit = torch.pow(torch.tensor(2.0, dtype=torch.float64), e.double())[..., None]
     size = torch.nan_to_num(y.abs() / unit, nan=0.0, posinf=0.0)

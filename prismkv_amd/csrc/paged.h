@@ -26,8 +26,10 @@ struct PagedAttend {
   unsigned page_units, slot_units, state_stride;  // 16-byte units; floats per partial state
   PageDiv div;
   int sequences, kv_heads, group, tiles, page_size, max_pages, pages;
-  float scale;  // log2(e) times the caller's
-  // pages in 4 bits: the scales' pages, their strides in bytes
+  float scale;  // log2(e) times the caller's; in 4 bits its magnitude
+  // pages in 4 bits: the scales' pages, their strides in bytes; the sign of `scale`, or
+  // that it is 0, as bits of the queries
+  unsigned q_and, q_xor;
   const uint8_t *k_scales, *v_scales;
   int64_t scale_page, scale_head;
   unsigned scale_slot;
@@ -58,14 +60,33 @@ constexpr int kElem = kType<DT> == kFp32 ? 4 : 2;
 // normal numbers (bf16 and fp32 have the exponents for them).
 template <int DT>
 constexpr int kBias = kType<DT> == kFp16 ? 15 : 0;
-// ... and the sum of P times 2^kSumBias: fp16 pages in 4 bits are widened to half
-// their values (the largest, 65536, is no fp16 number), which halving the sum undoes.
+// Exponents of the scales in 4 bits, plus 127: those whose codes are all exact numbers
+// of the type, for fp16 2^-23 (of half of which its least number is) to 2^13 (6 times
+// which is its last), for bf16 what its normal numbers allow.
 template <int DT>
-constexpr int kSumBias = kBias<DT> - (DT == (kFour | kFp16) ? 1 : 0);
+constexpr int kLeastScale = kType<DT> == kFp16 ? 104 : 2;
+template <int DT>
+constexpr int kMostScale = kType<DT> == kFp16 ? 140 : 252;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// Eight codes, the lowest four bits first, times the scale as pairs of the 16-bit type
+// (NaN for an infinite scale, whose byte is 255).
+template <int DT>
+__device__ __forceinline__ u32x4 widen8(unsigned codes, float scale) {
+  if constexpr (kType<DT> == kBf16)
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+  else
+    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
+}
 
 // Workgroups that the attention's rows are dealt to: one on each of the 256 CUs,
 // of 8 waves (two a SIMD, each with a tile in flight), or of 4 where a tile of
@@ -75,9 +96,9 @@ constexpr int kUnits = 256;
 template <int D>
 constexpr int kAWaves = D == 256 ? 4 : 8;
 constexpr int kQuantum = 32;  // tokens that are dealt at a time
-// Quanta of a workgroup at least: a tile (32 tokens, fp32 16) for each wave.
+// Quanta of a workgroup at least: a tile (32 tokens, fp32 16, in 4 bits 64) for each wave.
 template <int DT, int D>
-constexpr int kLeast = kType<DT> == kFp32 ? kAWaves<D> / 2 : kAWaves<D>;
+constexpr int kLeast = kInFour<DT> ? 2 * kAWaves<D> : kType<DT> == kFp32 ? kAWaves<D> / 2 : kAWaves<D>;
 
 // 16 bytes that another workgroup wrote through (agent scope, as ld_dev).
 __device__ __forceinline__ float4 ld_dev4(__amdgpu_buffer_rsrc_t r, unsigned byte_offset) {
@@ -199,10 +220,10 @@ __device__ __forceinline__ PagedSpan<kL> find_span(const PagedAttend& a, int uni
   }
 }
 
-// log2 of a softmax's sum from its maximum and the sum held times 2^kSumBias.
+// log2 of a softmax's sum from its maximum and the sum held times 2^kBias.
 template <int DT>
 __device__ __forceinline__ float log_sum(float M, float den) {
-  return den == 0.f ? -INFINITY : M + (log2f(den) - kSumBias<DT>);
+  return den == 0.f ? -INFINITY : M + (log2f(den) - kBias<DT>);
 }
 
 // Writes output element i (query head i / D of the tile, dim i % D) from the
@@ -218,7 +239,7 @@ __device__ __forceinline__ void finish(const PagedAttend& a, size_t head0, int i
     if (a.lse_out) a.lse_out[head0 + i / D] = log_sum<DT>(M, den) * 0.693147180559945309f;
     if (a.sums_work)
       a.sums_work[head0 + i / D] =
-          den == 0.f ? make_float2(0.f, 0.f) : make_float2(M, (float)(1 << kSumBias<DT>) / den);
+          den == 0.f ? make_float2(0.f, 0.f) : make_float2(M, (float)(1 << kBias<DT>) / den);
   }
 }
 

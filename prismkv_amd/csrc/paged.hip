@@ -743,12 +743,12 @@ struct WorkLayout {
 WorkLayout attend_layout(int sequences, int kv_heads, int group, int head_dim, int64_t slots, bool weigh, int dtype) {
   WorkLayout w;
   const int64_t tiles = (group + 15) / 16, heads = (int64_t)kv_heads * tiles;
-  const int least = ((dtype & 15) == kFp32 ? 1 : 2) * (head_dim == 256 ? kAWaves<256> : kAWaves<128>) / 2;
+  const int least = (dtype >= kFour ? 4 : dtype == kFp32 ? 1 : 2) * (head_dim == 256 ? kAWaves<256> : kAWaves<128>) / 2;
   const int64_t workgroups = sequences * heads * ((slots + least * kQuantum - 1) / (least * kQuantum));  // of full tables
   w.quanta = workgroups * least;
   w.units = workgroups < kUnits ? workgroups : kUnits;
   w.state_stride = (unsigned)((group < 16 ? group : 16) * (head_dim + 2));
-  w.logit_stride = (slots + 31) & ~31ll;
+  w.logit_stride = (slots + 31) & ~31ll;  // (whole blocks of 16 are written)
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   w.sums = up((size_t)sequences * heads * sizeof(unsigned));
   w.state = w.sums + up((size_t)sequences * kv_heads * group * sizeof(float2));
@@ -798,8 +798,7 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
   if (flags & ~3) return kBadMode;
   const prismkv_paged_cache& c = *cache;
   const double scale2 = scale * 1.4426950408889634;  // the exponents are powers of 2, in fp32
-  const double most = c.dtype == (kFour | kFp16) ? FLT_MAX / 2 : FLT_MAX;
-  if (group < 1 || group > 1024 || !(scale2 >= -most && scale2 <= most)) return kBadSize;
+  if (group < 1 || group > 1024 || !(scale2 >= -FLT_MAX && scale2 <= FLT_MAX)) return kBadSize;
   if (!q || !paged_work || !out || (q | paged_work) & 15 || lse & 3 || out & 3) return kBadSize;
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
   const WorkLayout w = attend_layout(c.sequences, c.kv_heads, group, c.head_dim, slots, weigh, c.dtype);
@@ -844,7 +843,9 @@ int prismkv_paged_attend(const prismkv_paged_cache* cache, const prismkv_paged_c
     a.scale_page = c.scale_page_stride;
     a.scale_head = c.scale_head_stride;
     a.scale_slot = (unsigned)c.scale_slot_stride;
-    if (c.dtype == (kFour | kFp16)) a.scale *= 2.f;  // (of keys at half their value)
+    a.q_and = scale2 == 0 ? 0u : ~0u;
+    a.q_xor = scale2 < 0 ? 0x80008000u : 0u;
+    a.scale = scale2 == 0 ? 1.f : (float)(scale2 < 0 ? -scale2 : scale2);
   }
   const hipStream_t s = (hipStream_t)stream;
   int rc;

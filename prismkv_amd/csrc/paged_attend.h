@@ -101,28 +101,6 @@ __device__ __forceinline__ unsigned pair16(const unsigned (&a)[W], const unsigne
   return __builtin_amdgcn_perm(b[N >> 1], a[N >> 1], (N & 1) ? 0x07060302u : 0x05040100u);
 }
 
-// The factor that a scale byte stands for; for fp16 half of it (kSumBias).  Byte 255
-// makes NaN of all its codes.
-template <int DT>
-__device__ __forceinline__ float four_scale(unsigned byte) {
-  const unsigned e = kType<DT> == kFp16 ? max(byte, 1u) - 1u : byte;
-  return __uint_as_float(byte == 255u ? 0x7fc00000u : e << 23);
-}
-// Eight codes, the lowest four bits first, as pairs of the 16-bit type.
-template <int DT>
-__device__ __forceinline__ u32x4 widen8(unsigned codes, float scale) {
-  if constexpr (kType<DT> == kBf16)
-    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
-  else
-    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
-}
-
 template <int DT>
 __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (kType<DT> == kBf16)
@@ -160,6 +138,24 @@ __device__ __forceinline__ void split16(float p, unsigned (&term)[kTerms<DT>]) {
 
 // The upper halves of two words (low half from a).
 __device__ __forceinline__ unsigned upper16(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// Two of them as word w of each term's operand, where no V is infinite (in 4 bits): a
+// term may be 0.
+template <int DT>
+__device__ __forceinline__ void split_pair(float a, float b, u32x4 (&term)[kTerms<DT>], int w) {
+  if constexpr (kType<DT> == kBf16) {
+    const unsigned a0 = __float_as_uint(a) & 0xffff0000u, b0 = __float_as_uint(b) & 0xffff0000u;
+    const float ra = a - __uint_as_float(a0), rb = b - __uint_as_float(b0);
+    const unsigned a1 = __float_as_uint(ra) & 0xffff0000u, b1 = __float_as_uint(rb) & 0xffff0000u;
+    term[0][w] = upper16(a0, b0);
+    term[1][w] = upper16(a1, b1);
+    term[2][w] = upper16(__float_as_uint(ra - __uint_as_float(a1)), __float_as_uint(rb - __uint_as_float(b1)));
+  } else {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    term[0][w] = __builtin_bit_cast(unsigned, h);
+    term[1][w] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+  }
+}
 
 template <int N, int DT, int D, int W>
 __device__ __forceinline__ void pv_columns(f32x4 (&acc)[D / 16], const unsigned (&v)[2][4][W],
@@ -288,14 +284,15 @@ __device__ __forceinline__ void join_states(const PagedAttend& a, size_t head0, 
   }
 }
 
-// The tile over pages in 4 bits, as loaded: lane (j, q) holds row j of each block at
-// dims q D/4 .. + D/4 (K; step c of the product takes eight of them, and Q the same
-// dims) with the one or two scales of these, and of rows 4q + t (V) dims j D/16 ..
-// + D/16, which have one scale.  They are widened by the conversion instruction,
-// which multiplies by the scale, to exact numbers of the 16-bit type.
+// The tile over pages in 4 bits, as loaded (64 tokens, four 16-token blocks: half as
+// many leave too little in flight): lane (j, q) holds row j of each block at dims q D/4
+// .. + D/4 (K; step c of the product takes eight of them, and Q the same dims) with the
+// one or two scales of these, and of rows 4q + t (V) dims j D/16 .. + D/16, which have
+// one scale, a byte of the row's.  They are widened by the conversion instruction, which
+// multiplies by the scale, to exact numbers of the 16-bit type.
 template <int DT, int D>
 struct FourTile {
-  static constexpr int kBlocks = 2, kTokens = 32;
+  static constexpr int kBlocks = 4, kTokens = 64;
   static constexpr int kKLoads = D / 32;  // 32-bit words of a K row's codes per lane, and steps of the product
   static constexpr int kVWords = D / 32;  // 32-bit words of a V row per lane, widened
   static constexpr int kVCodes = D == 256 ? 2 : 1;
@@ -304,10 +301,9 @@ struct FourTile {
   unsigned v[kBlocks][4][kVCodes], vs[kBlocks][4];
 
   __device__ __forceinline__ u32x4 widen_k(int i, int c) const {
-    return widen8<DT>(k[i][c], four_scale<DT>(D == 256 ? c < 4 ? ks[i] & 255u : ks[i] >> 8 : ks[i]));
+    return widen8<DT>(k[i][c], __uint_as_float(D < 256 ? ks[i] << 23 : (ks[i] << (c < 4 ? 23 : 15)) & 0x7f800000u));
   }
-  __device__ __forceinline__ void widen_v(unsigned (&dst)[kVWords], int i, int r) const {
-    const float scale = four_scale<DT>(vs[i][r]);
+  __device__ __forceinline__ void widen_v(unsigned (&dst)[kVWords], int i, int r, float scale) const {
 #pragma unroll
     for (int w = 0; w < kVWords; w += 4) {
       const u32x4 x = widen8<DT>(v[i][r][w / 4], scale);
@@ -437,91 +433,110 @@ template <int DT, int D, bool kAligned>
 struct FourRows;
 
 template <int W>
-__device__ __forceinline__ void load_codes_buf(unsigned (&dst)[W], __amdgpu_buffer_rsrc_t r, unsigned byte_offset) {
+__device__ __forceinline__ void load_codes_buf(unsigned (&dst)[W], __amdgpu_buffer_rsrc_t r, unsigned lane, unsigned at) {
   if constexpr (W == 1) {
-    dst[0] = load_nt4_buf(r, byte_offset);
+    dst[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane, at, 2);
   } else if constexpr (W == 2) {
-    load_words_buf(dst, r, byte_offset);
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(r, lane, at, 2);
+    dst[0] = x[0];
+    dst[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
-      const uint4 x = load_nt16_buf(r, byte_offset + 4 * i);
-      dst[i] = x.x;
-      dst[i + 1] = x.y;
-      dst[i + 2] = x.z;
-      dst[i + 3] = x.w;
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, lane + 4 * i, at, 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[i + e] = x[e];
     }
   }
 }
 
+// Pages of whole 16-token blocks, of less than 4 GiB in all, so that a block is a scalar
+// offset into one buffer resource, and scales that follow one another from slot to slot,
+// so that a lane reads those of its four rows of V at once.  Blocks past the end repeat
+// the last one.
 template <int DT, int D>
 struct FourRows<DT, D, true> {
   typedef FourTile<DT, D> T;
+  static constexpr int kB = T::kBlocks, kScales = D / 32;  // bytes of a row's scales
   const PagedAttend& a;
-  const char *k, *v, *k_scales, *v_scales;
   const int32_t* tab;
-  unsigned k_lane, ks_lane, v_lane[4], vs_lane[4];
+  __amdgpu_buffer_rsrc_t k, v, k_scales, v_scales;
+  unsigned k_lane, ks_lane, v_lane[4], vs_lane, vs_turn;
   int end;
-  int token[2], page[2];
-  __amdgpu_buffer_rsrc_t kr[2], vr[2], ksr[2], vsr[2];
+  int token[kB], page[kB];
+  unsigned at[kB], scale_at[kB];
   bool bad = false;
   __device__ __forceinline__ FourRows(const PagedAttend& a, int b, int h, int end) : a(a), end(end) {
     const unsigned lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4, slot = a.slot_units << 4;
-    k = reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes;
-    v = reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes;
-    k_scales = reinterpret_cast<const char*>(a.k_scales) + (size_t)h * a.scale_head;
-    v_scales = reinterpret_cast<const char*>(a.v_scales) + (size_t)h * a.scale_head;
+    k = raw_buffer(reinterpret_cast<const char*>(a.k) + (size_t)h * a.head_bytes, -1);
+    v = raw_buffer(reinterpret_cast<const char*>(a.v) + (size_t)h * a.head_bytes, -1);
+    k_scales = raw_buffer(reinterpret_cast<const char*>(a.k_scales) + (size_t)h * a.scale_head, -1);
+    v_scales = raw_buffer(reinterpret_cast<const char*>(a.v_scales) + (size_t)h * a.scale_head, -1);
     tab = a.table + (size_t)b * a.max_pages;
     k_lane = j * slot + q * (D / 8);
-    ks_lane = j * a.scale_slot + q * D / 128;
+    ks_lane = j * kScales + q * D / 128;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      v_lane[r] = (4 * q + r) * slot + j * (D / 32);
-      vs_lane[r] = (4 * q + r) * a.scale_slot + j * D / 512;
-    }
+    for (int r = 0; r < 4; ++r) v_lane[r] = (4 * q + r) * slot + j * (D / 32);
+    vs_lane = 4 * q * kScales;
+    vs_turn = 8 * ((j * D / 512) & 3) - 23;  // (modulo 32: the byte goes to an exponent's place)
+    if constexpr (D == 256) vs_lane += j * D / 512 & 4;  // (of a row's eight scales the four that a lane's is one of)
   }
   __device__ __forceinline__ void ask(int t0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      token[i] = t0 + 16 * i;
+    for (int i = 0; i < kB; ++i) {
+      token[i] = min(t0 + 16 * i, (end - 1) & ~15);
       typedef const __attribute__((address_space(4))) int32_t* Uniform;
-      page[i] = *(Uniform)(uint64_t)(tab + __builtin_amdgcn_readfirstlane(a.div.of(min(token[i], end - 1))));
+      page[i] = *(Uniform)(uint64_t)(tab + __builtin_amdgcn_readfirstlane(a.div.of(token[i])));
     }
   }
   __device__ __forceinline__ void move() {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int rows = min(end - token[i], 16);
-      bad |= rows > 0 && (unsigned)page[i] >= (unsigned)a.pages;
+    for (int i = 0; i < kB; ++i) {
+      bad |= (unsigned)page[i] >= (unsigned)a.pages;
       const unsigned from = (unsigned)page[i] < (unsigned)a.pages ? (unsigned)page[i] : 0u;
       const unsigned in = (unsigned)(token[i] - a.div.of(token[i]) * a.page_size);
-      const size_t at = ((size_t)from * a.page_units + in * a.slot_units) << 4;
-      const size_t scale_at = (size_t)from * a.scale_page + (size_t)in * a.scale_slot;
-      const int bytes = rows > 0 ? (int)((rows - 1) * (a.slot_units << 4)) + D / 2 : 0;
-      const int scale_bytes = rows > 0 ? (int)((rows - 1) * a.scale_slot) + D / 32 : 0;
-      kr[i] = raw_buffer(k + at, bytes);
-      vr[i] = raw_buffer(v + at, bytes);
-      ksr[i] = raw_buffer(k_scales + scale_at, scale_bytes);
-      vsr[i] = raw_buffer(v_scales + scale_at, scale_bytes);
+      at[i] = (from * a.page_units + in * a.slot_units) << 4;
+      scale_at[i] = from * (unsigned)a.scale_page + in * kScales;
     }
   }
   __device__ __forceinline__ void load_k(T& t) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      load_codes_buf(t.k[i], kr[i], k_lane);
-      if constexpr (D == 256) t.ks[i] = __builtin_amdgcn_raw_buffer_load_b16(ksr[i], ks_lane, 0, 2);
-      else t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(ksr[i], ks_lane, 0, 2);
+    for (int i = 0; i < kB; ++i) {
+      load_codes_buf(t.k[i], k, k_lane, at[i]);
+      if constexpr (D == 256) t.ks[i] = __builtin_amdgcn_raw_buffer_load_b16(k_scales, ks_lane, scale_at[i], 2);
+      else t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(k_scales, ks_lane, scale_at[i], 2);
     }
   }
   __device__ __forceinline__ void load_v(T& t) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kB; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if constexpr (D == 64) t.v[i][r][0] = __builtin_amdgcn_raw_buffer_load_b16(vr[i], v_lane[r], 0, 2);
-        else load_codes_buf(t.v[i][r], vr[i], v_lane[r]);
-        t.vs[i][r] = __builtin_amdgcn_raw_buffer_load_b8(vsr[i], vs_lane[r], 0, 2);
+        if constexpr (D == 64) t.v[i][r][0] = __builtin_amdgcn_raw_buffer_load_b16(v, v_lane[r], at[i], 2);
+        else load_codes_buf(t.v[i][r], v, v_lane[r], at[i]);
       }
+      // four rows' scales; `scale` takes its byte of each
+      if constexpr (D == 64) {
+        unsigned x[2];
+        load_codes_buf(x, v_scales, vs_lane, scale_at[i]);
+        t.vs[i][0] = x[0];
+        t.vs[i][1] = x[1];
+      } else if constexpr (D == 128) {
+        load_codes_buf(t.vs[i], v_scales, vs_lane, scale_at[i]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          t.vs[i][r] = __builtin_amdgcn_raw_buffer_load_b32(v_scales, vs_lane + r * kScales, scale_at[i], 2);
+      }
+    }
+  }
+  __device__ __forceinline__ float scale(const T& t, int i, int r) const {
+    const unsigned x = t.vs[i][D == 64 ? r / 2 : r], turn = vs_turn + (D == 64 && r % 2 ? 16 : 0);
+    return __uint_as_float(__builtin_amdgcn_alignbit(x, x, turn) & 0x7f800000u);
+  }
+  __device__ __forceinline__ void no_scale(T& t, int i, int r) const {
+    if constexpr (D == 64) t.vs[i][r / 2] &= r % 2 ? 0xffffu : 0xffff0000u;
+    else t.vs[i][r] = 0u;
   }
 };
 
@@ -549,7 +564,7 @@ struct FourRows<DT, D, false> {
   const PagedAttend& a;
   const char *k, *v, *k_scales, *v_scales;
   const int32_t* tab;
-  int end, token[2], page[2], from[2], in[2];  // (`ask` is ahead of the loads of V)
+  int end, token[T::kBlocks], page[T::kBlocks], from[T::kBlocks], in[T::kBlocks];  // (`ask` is ahead of the loads of V)
   bool bad = false;
   __device__ __forceinline__ FourRows(const PagedAttend& a, int b, int h, int end) : a(a), end(end) {
     const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
@@ -561,14 +576,14 @@ struct FourRows<DT, D, false> {
   }
   __device__ __forceinline__ void ask(int t0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < T::kBlocks; ++i) {
       token[i] = min(t0 + 16 * i + (int)(threadIdx.x & 15), end - 1);
       page[i] = tab[a.div.of(token[i])];
     }
   }
   __device__ __forceinline__ void move() {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < T::kBlocks; ++i) {
       bad |= (unsigned)page[i] >= (unsigned)a.pages;
       from[i] = (unsigned)page[i] < (unsigned)a.pages ? page[i] : 0;
       in[i] = token[i] - a.div.of(token[i]) * a.page_size;
@@ -582,7 +597,7 @@ struct FourRows<DT, D, false> {
   }
   __device__ __forceinline__ void load_k(T& t) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < T::kBlocks; ++i) {
       load_codes(t.k[i], k + row(from[i], in[i]));
       const char* s = k_scales + scales(from[i], in[i]);
       t.ks[i] = D == 256 ? *reinterpret_cast<const uint16_t*>(s) : *reinterpret_cast<const uint8_t*>(s);
@@ -591,7 +606,7 @@ struct FourRows<DT, D, false> {
   __device__ __forceinline__ void load_v(T& t) const {
     const int q = (threadIdx.x & 63) >> 4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int p = __shfl(from[i], 4 * q + r), s = __shfl(in[i], 4 * q + r);
@@ -600,6 +615,8 @@ struct FourRows<DT, D, false> {
         t.vs[i][r] = *reinterpret_cast<const uint8_t*>(v_scales + scales(p, s));
       }
   }
+  __device__ __forceinline__ float scale(const T& t, int i, int r) const { return __uint_as_float(t.vs[i][r] << 23); }
+  __device__ __forceinline__ void no_scale(T& t, int i, int r) const { t.vs[i][r] = 0u; }
 };
 
 template <int DT, int D, bool kAligned, bool kFour>
@@ -638,6 +655,9 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
     for (int c = 0; c < T::kKLoads; ++c) {
       const uint4 x = *reinterpret_cast<const uint4*>(qp + (kInFour<DT> ? 16 : 64) * c);
       qop[c] = j < rows ? u32x4{x.x, x.y, x.z, x.w} : u32x4{0u, 0u, 0u, 0u};
+      if constexpr (kInFour<DT>)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qop[c][e] = (qop[c][e] & a.q_and) ^ a.q_xor;
     }
   }
   f32x4 acc[D / 16];
@@ -690,8 +710,24 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         s[i][r] = kType<DT> == kFp32 ? d[r] + d2[r] : d[r];
-        bm = fmaxf(bm, t0 + 16 * i + 4 * q + r < end ? s[i][r] * a.scale : -INFINITY);
+        if constexpr (!kInFour<DT>)
+          bm = fmaxf(bm, t0 + 16 * i + 4 * q + r < end ? s[i][r] * a.scale : -INFINITY);
       }
+    }
+    if constexpr (kInFour<DT>) {
+      // (in 4 bits the reads take less time than the instructions of a tile: what is the
+      // same for all of its tokens is branched over)
+      if (t0 + T::kTokens > end)
+#pragma unroll
+        for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t0 + 16 * i + 4 * q + r >= end) s[i][r] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bm = fmaxf(bm, s[i][r]);
+      bm *= a.scale;
     }
     rows_of.move();
     rows_of.load_k(t);
@@ -712,6 +748,24 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
     }
     const float top = no_less(m);
     float p[T::kBlocks][4];
+    if constexpr (kInFour<DT>) {
+      const float shift = (float)kBias<DT> - top;
+      if (__ballot(fabsf(top) >= 0x1p22f)) {  // (`weight`)
+#pragma unroll
+        for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[i][r] = ldexpf(weight(s[i][r], a.scale, top), kBias<DT>);
+      } else {
+#pragma unroll
+        for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], a.scale, shift));
+      }
+#pragma unroll
+      for (int i = 0; i < T::kBlocks; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z += p[i][r];
+    } else
 #pragma unroll
     for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
@@ -721,7 +775,7 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
         if constexpr (kBias<DT> != 0) p[i][r] = ldexpf(p[i][r], kBias<DT>);
         z += p[i][r];
       }
-    if (!kAligned && t0 + T::kTokens > end) {  // rows past the end repeat the last one: 0 times its infinity must not be added
+    if ((!kAligned || kInFour<DT>) && t0 + T::kTokens > end) {  // rows past the end repeat the last one: 0 times its infinity must not be added
 #pragma unroll
       for (int i = 0; i < T::kBlocks; ++i)
 #pragma unroll
@@ -729,7 +783,7 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
           if (t0 + 16 * i + 4 * q + r >= end) {
 #pragma unroll
             for (int n = 0; n < (int)(sizeof(t.v[i][r]) / sizeof(unsigned)); ++n) t.v[i][r][n] = 0u;
-            if constexpr (kInFour<DT>) t.vs[i][r] = 0u;
+            if constexpr (kInFour<DT>) rows_of.no_scale(t, i, r);
           }
     }
     if constexpr (kType<DT> == kFp32) {
@@ -739,25 +793,33 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
         for (int n = 0; n < D / 16; ++n)
           acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][r], __uint_as_float(t.v[0][r][n]), acc[n], 0, 0, 0);
     } else {
-      unsigned term[8][kTerms<DT>];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i0 = 0; i0 < T::kBlocks; i0 += 2) {
+        unsigned term[8][kTerms<DT>];
+        u32x4 pw[kTerms<DT>];
+        if constexpr (kInFour<DT>) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) split16<DT>(p[i][r], term[4 * i + r]);
-      u32x4 pw[kTerms<DT>];
+          for (int e = 0; e < 8; e += 2) split_pair<DT>(p[i0 + e / 4][e % 4], p[i0 + e / 4][e % 4 + 1], pw, e / 2);
+        } else {
 #pragma unroll
-      for (int k = 0; k < kTerms<DT>; ++k)
-        pw[k] = u32x4{upper16(term[0][k], term[1][k]), upper16(term[2][k], term[3][k]), upper16(term[4][k], term[5][k]),
-                      upper16(term[6][k], term[7][k])};
-      if constexpr (kInFour<DT>) {
-        unsigned v[2][4][T::kVWords];
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int r = 0; r < 4; ++r) split16<DT>(p[i0 + i][r], term[4 * i + r]);
+        }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) t.widen_v(v[i][r], i, r);
-        pv_columns<0, DT, D>(acc, v, pw);
-      } else {
-        pv_columns<0, DT, D>(acc, t.v, pw);
+        for (int k = 0; k < (kInFour<DT> ? 0 : kTerms<DT>); ++k)
+          pw[k] = u32x4{upper16(term[0][k], term[1][k]), upper16(term[2][k], term[3][k]), upper16(term[4][k], term[5][k]),
+                        upper16(term[6][k], term[7][k])};
+        if constexpr (kInFour<DT>) {
+          unsigned v[2][4][T::kVWords];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t.widen_v(v[i][r], i0 + i, r, rows_of.scale(t, i0 + i, r));
+          pv_columns<0, DT, D>(acc, v, pw);
+        } else {
+          pv_columns<0, DT, D>(acc, t.v, pw);
+        }
       }
     }
     rows_of.load_v(t);
@@ -765,15 +827,15 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
     // step waits for must not be behind them (16 sequences of 4099: 47.5 us before)
     if (logits && j < rows) {
 #pragma unroll
-      for (int i = 0; i < T::kBlocks; ++i)
-        *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+      for (int i = 0; i < T::kBlocks; ++i)  // (in 4 bits a tile may end in the next workgroup's share)
+        if (!kInFour<DT> || t0 + 16 * i < end)
+          *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
     }
   }
   if (__ballot(rows_of.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
 
   z += xor16(z);
   z += xor32(z);
-  if constexpr (kSumBias<DT> != kBias<DT>) z *= 0.5f;
   const size_t head0 = ((size_t)u.b * a.kv_heads + h) * a.group + g0;  // this tile's first query head
   if (alone) {  // lane (j, q) has dims dim(n, j) of heads 4q + r
 #pragma unroll
@@ -928,7 +990,11 @@ int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
   const int lds = (merge > join ? merge : join) * (int)sizeof(float);
   if (apart) a.counters = nullptr;
   // a lane's offset within a block is 32 bits
-  const bool aligned = a.page_size % 16 == 0 && a.slot_units < (1u << 23) && a.scale_slot < (1u << 27);
+  bool aligned = a.page_size % 16 == 0 && a.slot_units < (1u << 23);
+  if constexpr (kInFour<DT>)  // (FourRows)
+    aligned = aligned && a.scale_slot == D / 32 && ((uintptr_t)a.v_scales | a.scale_page | a.scale_head) % 4 == 0 &&
+              (uint64_t)a.page_units * a.pages + (uint64_t)a.slot_units * a.page_size < 1u << 28 &&
+              (uint64_t)a.scale_page * a.pages + (uint64_t)a.scale_slot * a.page_size < 1ull << 32;
   a.many = (int64_t)a.sequences * a.kv_heads * a.tiles >= kSoloPairs;
   const auto launch = aligned ? a.many ? launch_attend_rows<DT, D, true, true> : launch_attend_rows<DT, D, true, false>
                               : a.many ? launch_attend_rows<DT, D, false, true> : launch_attend_rows<DT, D, false, false>;

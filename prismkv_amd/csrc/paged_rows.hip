@@ -136,18 +136,22 @@ struct Eight {
 
 // The scale byte of 32 values by the bits of the largest magnitude: a NaN's or an
 // infinity's are the largest.  Above 1.75 of its power of two a value takes the next.
+template <int DT>
 __device__ __forceinline__ unsigned scale_byte(unsigned amax) {
-  return amax >= 0x7f800000u ? 255u : (unsigned)min(max((int)((amax + 0x1fffffu) >> 23) - 2, 2), 252);
+  return amax >= 0x7f800000u
+             ? 255u
+             : (unsigned)min(max((int)((amax + 0x1fffffu) >> 23) - 2, kLeastScale<DT>), kMostScale<DT>);
 }
 
 // Eight codes of eight of the 32 values, the others being with the neighbouring lanes.
+template <int DT>
 __device__ __forceinline__ unsigned codes8(const float (&f)[8], unsigned& byte) {
   unsigned amax = 0u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7fffffffu);
   amax = max(amax, __float_as_uint(xor1(__uint_as_float(amax))));
   amax = max(amax, __float_as_uint(xor2(__uint_as_float(amax))));
-  byte = scale_byte(amax);
+  byte = scale_byte<DT>(amax);
   const float scale = __uint_as_float(byte == 255u ? 0x3f800000u : byte << 23);
   unsigned c = 0u;
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], scale, 0);
@@ -233,7 +237,7 @@ __global__ __launch_bounds__(kPT) void paged_rows_kernel(PagedRows a) {
     }
     if constexpr (kInFour<DT>) {
       unsigned byte;
-      const unsigned codes = codes8(f, byte);
+      const unsigned codes = codes8<DT>(f, byte);
       if (kind == 0 || p.slot < 0) continue;
       *reinterpret_cast<unsigned*>((kind == 1 ? a.kp : a.vp) + p.at + (size_t)h * a.head_bytes + c / 2) = codes;
       if ((c & 31) == 0) (kind == 1 ? a.ks : a.vs)[p.scales + (size_t)h * a.scale_head + c / 32] = (uint8_t)byte;
@@ -316,7 +320,7 @@ __device__ __forceinline__ RowPlace read_place(const PagedRead& a, int64_t row) 
 
 template <int DT>
 __device__ __forceinline__ void widen_codes(unsigned codes, unsigned byte, float (&f)[8]) {
-  const float scale = __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
+  const float scale = __uint_as_float(byte << 23);  // (255: an infinity, which makes NaN of any code)
 #define PRISMKV_PAIR(i)                                                              \
   {                                                                                  \
     const auto x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, i);        \

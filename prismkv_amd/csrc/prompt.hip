@@ -221,23 +221,6 @@ __device__ __forceinline__ u32x4 without_special(u32x4 x, bool& any) {
   return x;
 }
 
-// Eight codes as eight elements of the 16-bit type (for fp16 half of them, kSumBias).
-template <int DT>
-__device__ __forceinline__ u32x4 widen_eight(unsigned codes, unsigned byte) {
-  const unsigned e = kType<DT> == kFp16 ? max(byte, 1u) - 1u : byte;
-  const float scale = __uint_as_float(byte == 255u ? 0x7fc00000u : e << 23);
-  if constexpr (kType<DT> == kBf16)
-    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
-  else
-    return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2)),
-                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3))};
-}
-
 // A thread's part of a tile of keys and values on its way from the pages to LDS.  Each
 // lane looks up one row's place, the tile ahead, and the rows' readers take it from
 // there.  Rows past the end repeat the last one: no row sees them.
@@ -300,8 +283,8 @@ struct Stage {
     for (int i = 0; i < kEach; ++i) {
       u32x4 x, y;
       if constexpr (kInFour<DT>) {
-        x = widen_eight<DT>(kw[i], kb[i]);
-        y = widen_eight<DT>(vw[i], vb[i]);
+        x = widen8<DT>(kw[i], __uint_as_float(kb[i] << 23));
+        y = widen8<DT>(vw[i], __uint_as_float(vb[i] << 23));
       } else {
         x = kw[i];
         y = vw[i];
@@ -349,7 +332,7 @@ __device__ __forceinline__ void put_four(const Prompt& a, size_t row_head, int d
 
 template <int DT>
 __device__ __forceinline__ float prompt_lse(float m, float den) {
-  return den == 0.f ? -INFINITY : (m + (log2f(den) - kSumBias<DT>)) * 0.693147180559945309f;
+  return den == 0.f ? -INFINITY : (m + (log2f(den) - kBias<DT>)) * 0.693147180559945309f;
 }
 
 // Factor of a state with maximum m under the joint maximum M >= m (no state: 0).
@@ -473,7 +456,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
           for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
       }
       const float top = m == -INFINITY ? 0.f : m;
-      const float least = kType<DT> == kFp16 ? 0x1p-24f : 0.f;
+      const float least = DT == kFp16 ? 0x1p-24f : 0.f;  // (in 4 bits no value is infinite)
       // From 2^22 on the maximum's own rounding is 1/8 and more (at 2^32 it takes all of
       // the exponents' range): then the other products are rounded as it was.
       if (__ballot(fabsf(m) >= 0x1p22f && m != -INFINITY)) {
@@ -555,7 +538,6 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   if (__ballot(stage.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
 
   z += xor32(z);
-  if constexpr (kSumBias<DT> != kBias<DT>) z *= 0.5f;
   if (!valid) return;
   if (cut.chunks <= 1) {
     if (a.lse && half == 0) a.lse[row_head] = prompt_lse<DT>(m, z);
@@ -700,8 +682,7 @@ int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t 
   if (const int rc = check_cache(cache, cache, false)) return rc;
   const prismkv_paged_cache& c = *cache;
   const double scale2 = scale * 1.4426950408889634;  // the exponents are powers of 2, in fp32
-  const double most = c.dtype == (kFour | kFp16) ? FLT_MAX / 2 : FLT_MAX;
-  if (!(scale2 >= -most && scale2 <= most) || !prompt_fits(rows, c.sequences, c.kv_heads, group)) return kBadSize;
+  if (!(scale2 >= -FLT_MAX && scale2 <= FLT_MAX) || !prompt_fits(rows, c.sequences, c.kv_heads, group)) return kBadSize;
   if (!offsets && rows != c.sequences) return kBadSize;
   if ((rows && (!q || !out || !paged_work)) || (q | out | paged_work) & 15 || (lse | offsets) & 3) return kBadSize;
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
@@ -732,7 +713,6 @@ int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t 
     a.scale_page = c.scale_page_stride;
     a.scale_head = c.scale_head_stride;
     a.scale_slot = c.scale_slot_stride;
-    if (c.dtype == (kFour | kFp16)) a.scale *= 2.f;  // (of keys at half their value)
   }
   a.div = page_div(c.page_size);
   a.rows = (int)rows;

@@ -7,7 +7,9 @@ by accumulated attention weight.  No counterpart in the reference.
 Any head layout with head_dim 64, 128 or 256 in bf16, fp16 or fp32, and up to 64
 GiB each of k and v pages (NotImplementedError otherwise); for inference, without
 gradients.  With storage "mxfp4" the pages hold bf16 or fp16 rows in 4 bits: e2m1
-numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6) times a power of two for every 32 dims.  As for `Native8B`: validation happens on the host before
+numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6) times a power of two for every 32 dims, the
+smallest for which none of them is above 7 (of fp16 rows 2^-23 to 2^13, so that what
+is above 6 times that is held as it).  As for `Native8B`: validation happens on the host before
 anything is enqueued (ValueError), calls go to the current stream of the
 cache's device, never synchronise and can be captured into a HIP graph after
 one eager call has made their workspaces; lengths and page table are read on
@@ -148,7 +150,7 @@ class PagedCache:
         lengths = torch.zeros(int(sequences), dtype=torch.int32, device=device)
         meta = {}
         if storage:
-            meta = {name: torch.full(shape[:3] + (int(head_dim) // 32,), 2, dtype=torch.uint8, device=device)
+            meta = {name: torch.full(shape[:3] + (int(head_dim) // 32,), 127, dtype=torch.uint8, device=device)
                     for name in ("k_scales", "v_scales")}
         if scored:
             meta.update(seen=torch.zeros_like(lengths),
@@ -442,9 +444,8 @@ class PagedCache:
         """The keys and values of every sequence's last slot, or with `offsets` (i32
         [sequences + 1], ascending from 0 to `rows`) of its last offsets[b + 1] -
         offsets[b] ones, in the order of the slots: k and v [rows, kv_heads,
-        head_dim] of the cache's dtype (what 4 bits stand for is exact in it, but
-        for fp16's 65536, which becomes an infinity, and what is below its least number).
-        Rows that a sequence does not hold are 0 and reported."""
+        head_dim] of the cache's dtype (what 4 bits stand for is exact in it).  Rows that a
+        sequence does not hold are 0 and reported."""
         sequences, kv_heads, head_dim, _, _ = self._shape
         if offsets is not None:
             _i32(offsets, (sequences + 1,), self.device, "offsets")
@@ -491,8 +492,7 @@ class PagedCache:
 
     def _check_scale(self, q, scale, lse, rows):
         scale = 1.0 / math.sqrt(self._shape[2]) if scale is None else float(scale)
-        # (fp16 rows are held in 4 bits at half their value, and the scale is doubled for it)
-        if not abs(scale) <= (MAX_SCALE / 2 if self.storage and self.dtype == torch.float16 else MAX_SCALE):
+        if not abs(scale) <= MAX_SCALE:
             raise ValueError("a scale that is finite in float32, as times log2(e), required")
         if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()
                                 or lse.device != self.device):
