@@ -743,7 +743,9 @@ struct WorkLayout {
 WorkLayout attend_layout(int sequences, int kv_heads, int group, int head_dim, int64_t slots, bool weigh, int dtype) {
   WorkLayout w;
   const int64_t tiles = (group + 15) / 16, heads = (int64_t)kv_heads * tiles;
-  const int least = (dtype >= kFour ? 4 : dtype == kFp32 ? 1 : 2) * (head_dim == 256 ? kAWaves<256> : kAWaves<128>) / 2;
+  const int least = dtype >= kFour     ? head_dim == 256 ? kLeast<kFour, 256> : kLeast<kFour, 128>
+                    : dtype == kFp32 ? head_dim == 256 ? kLeast<kFp32, 256> : kLeast<kFp32, 128>
+                                     : head_dim == 256 ? kLeast<kBf16, 256> : kLeast<kBf16, 128>;
   const int64_t workgroups = sequences * heads * ((slots + least * kQuantum - 1) / (least * kQuantum));  // of full tables
   w.quanta = workgroups * least;
   w.units = workgroups < kUnits ? workgroups : kUnits;

@@ -284,15 +284,16 @@ __device__ __forceinline__ void join_states(const PagedAttend& a, size_t head0, 
   }
 }
 
-// The tile over pages in 4 bits, as loaded (64 tokens, four 16-token blocks: half as
-// many leave too little in flight): lane (j, q) holds row j of each block at dims q D/4
+// The tile over pages in 4 bits, as loaded: lane (j, q) holds row j of each block at dims q D/4
 // .. + D/4 (K; step c of the product takes eight of them, and Q the same dims) with the
 // one or two scales of these, and of rows 4q + t (V) dims j D/16 .. + D/16, which have
 // one scale, a byte of the row's.  They are widened by the conversion instruction, which
-// multiplies by the scale, to exact numbers of the 16-bit type.
+// multiplies by the scale, to exact numbers of the 16-bit type.  (Tiles of 64 tokens, 12
+// or 16 waves, and V through LDS from 16-byte loads read no faster: 32 x 6.4K tokens of 8 x 4
+// heads 62, 57, 89 and 57 us against 56.)
 template <int DT, int D>
 struct FourTile {
-  static constexpr int kBlocks = 4, kTokens = 64;
+  static constexpr int kBlocks = 2, kTokens = 32;
   static constexpr int kKLoads = D / 32;  // 32-bit words of a K row's codes per lane, and steps of the product
   static constexpr int kVWords = D / 32;  // 32-bit words of a V row per lane, widened
   static constexpr int kVCodes = D == 256 ? 2 : 1;
@@ -643,7 +644,7 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   const int start = min(u.first * kQuantum, u.n), end = min(start + count * kQuantum, u.n);
   // (a pair alone: all tiles are this wave's)
   const bool alone = kMany && u.alone;
-  const int step = alone ? T::kTokens : kAWaves<D> * T::kTokens;
+  const int step = alone ? T::kTokens : kAWaves<DT, D> * T::kTokens;
 
   // Q^T: column j is head j (zero past the tile's heads)
   u32x4 qop[T::kKLoads];
@@ -850,8 +851,8 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   }
   // the waves' states meet in LDS
   float* sm = lds;  // [waves][16] maxima
-  float* sz = sm + 16 * kAWaves<D>;   // [waves][16] sums
-  float* sacc = sz + 16 * kAWaves<D>; // [waves][rows][D]
+  float* sz = sm + 16 * kAWaves<DT, D>;   // [waves][16] sums
+  float* sacc = sz + 16 * kAWaves<DT, D>; // [waves][rows][D]
   if (lane < 16) {
     sm[16 * w + j] = m;
     sz[16 * w + j] = z;
@@ -868,14 +869,14 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   const int pair0 = u.at - u.first, unit = (int)blockIdx.x;
   const bool whole = count == quanta;
   float* state = a.state + (size_t)(2 * unit + (u.at != u.deal.begin(unit))) * a.state_stride;  // {max, sum}[rows], [rows][D]
-  for (int i = 2 * tid; i < rows * D; i += 128 * kAWaves<D>) {
+  for (int i = 2 * tid; i < rows * D; i += 128 * kAWaves<DT, D>) {
     const int g = i / D;
     float M = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kAWaves<D>; ++k) M = fmaxf(M, sm[16 * k + g]);
+    for (int k = 0; k < kAWaves<DT, D>; ++k) M = fmaxf(M, sm[16 * k + g]);
     float den = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int k = 0; k < kAWaves<D>; ++k) {
+    for (int k = 0; k < kAWaves<DT, D>; ++k) {
       const float wt = rescale(sm[16 * k + g], M);
       const float2 v = *reinterpret_cast<const float2*>(sacc + (size_t)k * rows * D + i);
       den = fmaf(wt, sz[16 * k + g], den);
@@ -904,11 +905,11 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   __syncthreads();
   if (!is_last) return;
   if (tid == 0) st_dev(counter, 0u);
-  join_states<DT, D, 64 * kAWaves<D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
+  join_states<DT, D, 64 * kAWaves<DT, D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
 }
 
 template <int DT, int D, bool kAligned, bool kMany>
-__global__ __launch_bounds__(64 * kAWaves<D>, kAWaves<D> / 4) void paged_attend_kernel(PagedAttend a) {
+__global__ __launch_bounds__((64 * kAWaves<DT, D>), (kAWaves<DT, D> / 4)) void paged_attend_kernel(PagedAttend a) {
   extern __shared__ float lds[];
   constexpr int kL = kLeast<DT, D>;
   PagedSpan<kL> u = find_span<kL, kMany>(a, blockIdx.x);
@@ -917,7 +918,7 @@ __global__ __launch_bounds__(64 * kAWaves<D>, kAWaves<D> / 4) void paged_attend_
       const int heads = a.kv_heads * a.tiles;
       u.first = 0;
       for (int pair = blockIdx.x + gridDim.x * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); pair < a.sequences * heads;
-           pair += gridDim.x * kAWaves<D>) {
+           pair += gridDim.x * kAWaves<DT, D>) {
         u.b = pair / heads;
         u.hh = pair - u.b * heads;
         u.n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[u.b]));
@@ -971,7 +972,7 @@ int launch_attend_rows(const PagedAttend& a, int64_t units, int lds, hipStream_t
                                              hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(64 * kAWaves<D>), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(64 * kAWaves<DT, D>), lds, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -985,8 +986,8 @@ int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
   // tokens of one KV head and 16 query heads (264K floats) 20.3 us, 44.9 by the last
   // workgroup; of 8 KV heads and 4 (17K) 48.5 against 47.3.
   const bool apart = (int64_t)chunks * rows * D > 49152;
-  const int merge = 32 * kAWaves<D> + kAWaves<D> * rows * D, sums = 32 + chunks * rows;
-  const int join = apart ? 0 : 256 * kAWaves<D> + sums;
+  const int merge = 32 * kAWaves<DT, D> + kAWaves<DT, D> * rows * D, sums = 32 + chunks * rows;
+  const int join = apart ? 0 : 256 * kAWaves<DT, D> + sums;
   const int lds = (merge > join ? merge : join) * (int)sizeof(float);
   if (apart) a.counters = nullptr;
   // a lane's offset within a block is 32 bits
