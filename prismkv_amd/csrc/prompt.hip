@@ -20,7 +20,7 @@ template <int DT, int D>
 constexpr int kTileTokens = kElem<DT> * D > 256 ? 32 : 64;
 // Waves of a SIMD, by the registers that products, queries and staged rows take.
 template <int DT, int D>
-constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
+constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : kElem<DT> * D > 128 ? 2 : 3;
 // The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, nor
 // less than kLeastTiles tiles of keys.
 constexpr int kItemsLog = 9, kLeastTiles = 4;
@@ -221,32 +221,39 @@ __device__ __forceinline__ u32x4 without_special(u32x4 x, bool& any) {
   return x;
 }
 
-// A thread's part of a tile of keys and values on its way from the pages to LDS.  Each
-// lane looks up one row's place, the tile ahead, and the rows' readers take it from
+// A thread's part of the tiles of keys and values on their way from the pages to LDS: 16
+// bytes straight there, or from 4 bits through registers, where they are widened.  Each
+// lane looks up one row's place, two tiles ahead, and the rows' readers take it from
 // there.  Rows past the end repeat the last one: no row sees them.
 template <int DT, int D>
 struct Stage {
   static constexpr int kTokens = kTileTokens<DT, D>;
   static constexpr int kC = D * kElem<DT> / 16;            // chunks of a row
   static constexpr int kEach = kTokens * kC / kThreads;    // chunks of a thread
-  typedef typename std::conditional<kInFour<DT>, unsigned, u32x4>::type Word;
+  static constexpr int kRaw = kInFour<DT> ? kEach : 1;
+  typedef const __attribute__((address_space(1))) void* Global;
+  typedef __attribute__((address_space(3))) void* Local;
   const Prompt& a;
   const char *k, *v;
   const uint8_t *ks, *vs;
   const int32_t* tab;
   int end, row, chunk;
   bool bad = false;
-  int page, token;  // of this lane's row
-  Word kw[kEach], vw[kEach];
-  unsigned kb[kInFour<DT> ? kEach : 1], vb[kInFour<DT> ? kEach : 1];
+  int page, token;        // of this lane's row
+  // places (16-byte units) of the next tile of values and of the next one of keys, which
+  // is the tile behind it
+  unsigned v_at[kEach], k_at[kEach];
+  uint64_t v_scale_at[kRaw], k_scale_at[kRaw];
+  unsigned kw[kRaw], vw[kRaw], kb[kRaw], vb[kRaw];
 
   __device__ __forceinline__ Stage(const Prompt& a, int b, int h, int end) : a(a), end(end) {
     row = threadIdx.x / kC;
     chunk = threadIdx.x % kC;
-    const int bytes = kInFour<DT> ? 4 : 16;  // of a chunk in the pages
-    k = a.k + (size_t)h * a.head_bytes + chunk * bytes;
-    v = a.v + (size_t)h * a.head_bytes + chunk * bytes;
+    k = a.k + (size_t)h * a.head_bytes;
+    v = a.v + (size_t)h * a.head_bytes;
     if constexpr (kInFour<DT>) {
+      k += 4 * chunk;
+      v += 4 * chunk;
       ks = a.ks + (size_t)h * a.scale_head + chunk / 4;
       vs = a.vs + (size_t)h * a.scale_head + chunk / 4;
     }
@@ -257,42 +264,77 @@ struct Stage {
     token = min(t0 + (int)(threadIdx.x & (kTokens - 1)), end - 1);
     page = tab[a.div.of(token)];
   }
-  __device__ __forceinline__ void load() {
+  __device__ __forceinline__ void move() {
     bad |= (unsigned)page >= (unsigned)a.pages;
     const unsigned p = (unsigned)page < (unsigned)a.pages ? (unsigned)page : 0u;
     const unsigned in = (unsigned)(token - a.div.of(token) * a.page_size);
-    const unsigned place = p * a.page_units + in * a.slot_units;  // of 16 bytes
+    const unsigned place = p * a.page_units + in * a.slot_units;
     uint64_t scale_place = 0;
     if constexpr (kInFour<DT>) scale_place = (uint64_t)p * a.scale_page + (uint64_t)in * a.scale_slot;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const size_t at = (size_t)(unsigned)__shfl((int)place, row + step(i)) << 4;
-      kw[i] = *reinterpret_cast<const Word*>(k + at);
-      vw[i] = *reinterpret_cast<const Word*>(v + at);
+      v_at[i] = k_at[i];
+      k_at[i] = (unsigned)__shfl((int)place, row + step(i));
       if constexpr (kInFour<DT>) {
-        const size_t scale_at = (size_t)__shfl((unsigned long long)scale_place, row + step(i));
-        kb[i] = ks[scale_at];
-        vb[i] = vs[scale_at];
+        v_scale_at[i] = k_scale_at[i];
+        k_scale_at[i] = (uint64_t)__shfl((unsigned long long)scale_place, row + step(i));
       }
     }
   }
-  // Writes the tile, `clean` without the values' infinities and NaN; whether there were any.
-  __device__ __forceinline__ bool store(char* keys, char* values, bool clean) const {
+  // Which chunk of its row a lane reads: LDS takes the lanes' 16 bytes one after another.
+  __device__ __forceinline__ int source(int i) const {
+    return (staged<kC>(row + step(i), chunk) & (16 * kC - 1));
+  }
+  __device__ __forceinline__ void issue(const char* from, const unsigned (&at)[kEach], char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      __builtin_amdgcn_global_load_lds((Global)(from + ((size_t)at[i] << 4) + source(i)),
+                                       (Local)(tile + (64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + i * kThreads) * 16),
+                                       16, 0, 0);
+  }
+  __device__ __forceinline__ void issue_k(char* tile) {
+    if constexpr (kInFour<DT>) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        kw[i] = *reinterpret_cast<const unsigned*>(k + ((size_t)k_at[i] << 4));
+        kb[i] = ks[k_scale_at[i]];
+      }
+    } else {
+      issue(k, k_at, tile);
+    }
+  }
+  __device__ __forceinline__ void issue_v(char* tile) {
+    if constexpr (kInFour<DT>) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        vw[i] = *reinterpret_cast<const unsigned*>(v + ((size_t)v_at[i] << 4));
+        vb[i] = vs[v_scale_at[i]];
+      }
+    } else {
+      issue(v, v_at, tile);
+    }
+  }
+  __device__ __forceinline__ void finish(char* tile, const unsigned (&w)[kRaw], const unsigned (&b)[kRaw]) const {
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i)
+      *reinterpret_cast<u32x4*>(tile + staged<kC>(row + step(i), chunk)) = widen8<DT>(w[i], __uint_as_float(b[i] << 23));
+  }
+  __device__ __forceinline__ void finish_k(char* tile) const {
+    if constexpr (kInFour<DT>) finish(tile, kw, kb);
+  }
+  __device__ __forceinline__ void finish_v(char* tile) const {
+    if constexpr (kInFour<DT>) finish(tile, vw, vb);
+  }
+  // Takes the infinities and NaN out of a tile of values; whether there were any.
+  static __device__ __forceinline__ bool clean(char* tile) {
     bool special = false;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      u32x4 x, y;
-      if constexpr (kInFour<DT>) {
-        x = widen8<DT>(kw[i], __uint_as_float(kb[i] << 23));
-        y = widen8<DT>(vw[i], __uint_as_float(vb[i] << 23));
-      } else {
-        x = kw[i];
-        y = vw[i];
-      }
-      if (clean) y = without_special<DT>(y, special);
-      const int at = staged<kC>(row + step(i), chunk);
-      *reinterpret_cast<u32x4*>(keys + at) = x;
-      *reinterpret_cast<u32x4*>(values + at) = y;
+      u32x4* x = reinterpret_cast<u32x4*>(tile) + threadIdx.x + i * kThreads;
+      bool any = false;
+      const u32x4 y = without_special<DT>(*x, any);
+      if (any) *x = y;
+      special |= any;
     }
     return special;
   }
@@ -354,8 +396,8 @@ template <int DT, int D>
 __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(Prompt a) {
   constexpr int kTokens = kTileTokens<DT, D>, kT = kTokens / 32;
   constexpr int kC = D * kElem<DT> / 16;  // 16-byte chunks of a row; half as many steps of the product (fp32: of four)
-  extern __shared__ char lds[];
-  char *keys = lds, *values = lds + kTokens * kC * 16;
+  constexpr int kTile = kTokens * kC * 16;  // bytes
+  __shared__ __attribute__((aligned(16))) char keys0[kTile], keys1[kTile], values0[kTile], values1[kTile];
   if (blockIdx.x == 0 && a.offsets)
     for (int b = threadIdx.x; b < a.sequences; b += kThreads) {
       const int from = a.offsets[b], to = a.offsets[b + 1];
@@ -376,8 +418,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   const int before = it.s.n - it.s.m;
   if (before < 0 && threadIdx.x == 0) report_error(a.err, error_host_slot(a.err), kErrHeld);
   const int limit = valid ? before + token : -1;  // the last slot that the row sees
-  // the last slot that any row of the wave sees, and the first row's; the tile's first
-  const int wave_last = __builtin_amdgcn_readlane(32 * w < rows ? before + token : -1, 31);
+  // what the wave's first row sees, the tile's
   const int wave_first = __builtin_amdgcn_readlane(limit, 0);
   const int tile_first = before + it.tile * kTileRows / a.group;
   const size_t row_head = (size_t)(it.s.first + token) * a.kv_heads * a.group + it.h * a.group + (of - token * a.group);
@@ -402,43 +443,68 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
 
   const int from = it.chunk * cut.each, to = min(from + cut.each, cut.tiles);
   Stage<DT, D> stage(a, it.b, it.h, cut.end);
+  f32x16 s[kT];  // the scores of the tile at hand
+  auto scores = [&](f32x16 (&s)[kT], const char* keys) {
+#pragma unroll
+    for (int i = 0; i < kT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kC / 2; ++c)
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+        s[i] = mfma_rows<DT>(*reinterpret_cast<const u32x4*>(keys + key_at.of(i, c)), q[c], s[i]);
+  };
+  // -infinity where the tile's slots lie behind what the row sees
+  auto mask = [&](f32x16 (&s)[kT], int t0) {
+    if (t0 + kTokens - 1 <= wave_first) return;
+#pragma unroll
+    for (int i = 0; i < kT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (t0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 > limit) s[i][r] = -INFINITY;
+  };
+  const bool active = 32 * w < rows;
   if (from < to) {
     stage.ask(from * kTokens);
-    stage.load();
-    if (from + 1 < to) stage.ask((from + 1) * kTokens);
+    stage.move();
+    stage.issue_k(keys0);
+    stage.finish_k(keys0);
+    stage.ask(min(from + 1, to - 1) * kTokens);
+    stage.move();
+    stage.issue_v(values0);
+    stage.issue_k(keys1);
+    stage.finish_v(values0);
+    stage.finish_k(keys1);
+    stage.ask(min(from + 2, to - 1) * kTokens);
+    drain();
+    stage.move();
+    __syncthreads();
+    if (active) {
+      scores(s, keys0);
+      mask(s, from * kTokens);
+    }
+    __syncthreads();  // the first keys have been read
   }
+  // Step t has the scores of tile t, and in LDS its values and the next tile's keys: the
+  // next scores' products run beside this tile's exponentials, and the tile behind
+  // them is on its way.
   // In a tile that some row does not see all of, 0 times an infinity or NaN must not reach
   // that row: such values are left out there, and added to the rows that see them at the end.
   bool special = false;
-  for (int t = from; t < to; ++t) {
+  auto step = [&](int t, char* values, char* next_values, char* next_keys, char* later_keys) {
     const int t0 = t * kTokens;
-    const bool partly = t0 + kTokens - 1 > tile_first;
-    __syncthreads();  // the last tile has been read
-    special |= stage.store(keys, values, partly);
-    if (t + 1 < to) {
-      stage.load();
-      if (t + 2 < to) stage.ask(t0 + 2 * kTokens);
+    if (t0 + kTokens - 1 > tile_first) {
+      special |= stage.clean(values);
+      __syncthreads();
     }
-    __syncthreads();
-    if (t0 > wave_last) continue;
-    f32x16 s[kT];
-    {
-#pragma unroll
-      for (int i = 0; i < kT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
-#pragma unroll
-      for (int c = 0; c < kC / 2; ++c)
-#pragma unroll
-        for (int i = 0; i < kT; ++i)
-          s[i] = mfma_rows<DT>(*reinterpret_cast<const u32x4*>(keys + key_at.of(i, c)), q[c], s[i]);
-      if (t0 + kTokens - 1 > wave_first) {
-#pragma unroll
-        for (int i = 0; i < kT; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (t0 + 32 * i + 8 * (r / 4) + 4 * half + r % 4 > limit) s[i][r] = -INFINITY;
-      }
+    if (t + 1 < to) {
+      stage.issue_v(next_values);
+      stage.issue_k(later_keys);  // (the last one again, behind the last)
+      stage.ask(min(t + 3, to - 1) * kTokens);
+    }
+    if (active) {
+      f32x16 next[kT];
       float most = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kT; ++i)
@@ -455,8 +521,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
       }
-      const float top = m == -INFINITY ? 0.f : m;
-      const float least = DT == kFp16 ? 0x1p-24f : 0.f;  // (in 4 bits no value is infinite)
+      float scale = a.scale, shift = m == -INFINITY ? (float)kBias<DT> : (float)kBias<DT> - m;
       // From 2^22 on the maximum's own rounding is 1/8 and more (at 2^32 it takes all of
       // the exponents' range): then the other products are rounded as it was.
       if (__ballot(fabsf(m) >= 0x1p22f && m != -INFINITY)) {
@@ -465,60 +530,77 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
         for (int i = 0; i < kT; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float product = s[i][r] * a.scale, x = product - top;
-            s[i][r] = __builtin_amdgcn_exp2f(x + (float)kBias<DT>);
-            z += s[i][r];
-            if (least > 0.f && x != -INFINITY) s[i][r] = fmaxf(s[i][r], least);
+            const float product = s[i][r] * a.scale;
+            s[i][r] = product - (m == -INFINITY ? 0.f : m);
           }
-      } else {
-        const float shift = (float)kBias<DT> - top;
+        scale = 1.f;
+        shift = (float)kBias<DT>;
+      }
+      scores(next, next_keys);  // (of no tile, behind the last)
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, shift));
+          z += s[i][r];
+          // (2^-24, or 0 for 0; in 4 bits no value is infinite)
+          if constexpr (DT == kFp16) s[i][r] = fmaxf(s[i][r], fminf(s[i][r] * 0x1p126f, 0x1p-24f));
+        }
+      if constexpr (kType<DT> == kFp32) {
+        const FloatAt<kC> float_at(col, half);
 #pragma unroll
         for (int i = 0; i < kT; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool none = s[i][r] == -INFINITY;
-            s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], a.scale, shift));
-            z += s[i][r];
-            if (least > 0.f && !none) s[i][r] = fmaxf(s[i][r], least);
+          for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + float_at.of(i, r, d)), s[i][r],
+                                                            acc[d], 0, 0, 0);
+      } else {
+        typedef __attribute__((address_space(3))) s16x4* Transposed;
+        const ValueAt<kC> value_at(lane);
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const u32x4 p = {pack2<DT>(s[i][8 * u], s[i][8 * u + 1]), pack2<DT>(s[i][8 * u + 2], s[i][8 * u + 3]),
+                             pack2<DT>(s[i][8 * u + 4], s[i][8 * u + 5]), pack2<DT>(s[i][8 * u + 6], s[i][8 * u + 7])};
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) {
+              const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 0, d)));
+              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 1, d)));
+              const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+              acc[d] = mfma_rows<DT>(u32x4{l.x, l.y, h.x, h.y}, p, acc[d]);
+            }
           }
       }
+#pragma unroll
+      for (int i = 0; i < kT; ++i) s[i] = next[i];
+      if (t + 1 < to) mask(s, t0 + kTokens);
     }
-    if constexpr (kType<DT> == kFp32) {
-      const FloatAt<kC> float_at(col, half);
-#pragma unroll
-      for (int i = 0; i < kT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d)
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + float_at.of(i, r, d)), s[i][r],
-                                                          acc[d], 0, 0, 0);
-    } else {
-      typedef __attribute__((address_space(3))) s16x4* Transposed;
-      const ValueAt<kC> value_at(lane);
-#pragma unroll
-      for (int i = 0; i < kT; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const u32x4 p = {pack2<DT>(s[i][8 * u], s[i][8 * u + 1]), pack2<DT>(s[i][8 * u + 2], s[i][8 * u + 3]),
-                           pack2<DT>(s[i][8 * u + 4], s[i][8 * u + 5]), pack2<DT>(s[i][8 * u + 6], s[i][8 * u + 7])};
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d) {
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 0, d)));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 1, d)));
-            const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
-            acc[d] = mfma_rows<DT>(u32x4{l.x, l.y, h.x, h.y}, p, acc[d]);
-          }
-        }
-    }
+    stage.finish_v(next_values);
+    stage.finish_k(later_keys);
+    drain();
+    stage.move();
+    __syncthreads();
+  };
+  // (each tile has its own array, and the two steps are written out, so that the compiler
+  // sees that what is on its way does not meet what is read)
+  for (int t = from; t < to; t += 2) {
+    step(t, values0, values1, keys1, keys0);
+    if (t + 1 < to) step(t + 1, values1, values0, keys0, keys1);
   }
   if (__syncthreads_or(special)) {
 #pragma unroll 1
     for (int t = max(from, (tile_first + 1) / kTokens); t < to; ++t) {
+      char* values = values0;
       stage.ask(t * kTokens);
-      stage.load();
+      stage.move();
+      stage.move();
       __syncthreads();
-      stage.store(keys, values, false);
+      stage.issue_v(values);
+      stage.finish_v(values);
+      drain();
       __syncthreads();
 #pragma unroll 1
       for (int k = 0; k < kTokens && t * kTokens + k <= limit; ++k)
@@ -565,50 +647,75 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
 }
 
 // Joins the states of tiles whose keys were cut, in the order of their tokens: a
-// workgroup for kJoinDims dims of a tile, a thread for a row and four of them at a time.
-constexpr int kJoinDims = 16;
+// workgroup for kJoinRows rows of a tile, a thread for a row and four dims.  The factors
+// are found by as many lanes as there are chunks, and kU states are in flight a thread.
+constexpr int kJoinRows = 8;
 
 template <int DT, int D>
-__global__ __launch_bounds__(kThreads) void prompt_join_kernel(Prompt a) {
-  constexpr int kTokens = kTileTokens<DT, D>;
+__global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a) {
+  constexpr int kTokens = kTileTokens<DT, D>, kLanes = D / 4, kU = 8;
+  __shared__ float factors[kLanes][kJoinRows], parts[kLanes][kJoinRows];
   const int per_item = item_tiles<kTokens>(a);
   PromptItem it;
   if (!find_item<kTokens>(a, per_item, blockIdx.x, true, it)) return;
   const PromptCut<kTokens> cut(a, it, per_item);
-  if (cut.chunks <= 1) return;  // its workgroup has finished it
-  const int rows = min(it.s.m * a.group - it.tile * kTileRows, kTileRows);
-  const int row = threadIdx.x % kTileRows;
-  if (row >= rows) return;
+  const int rows = it.s.m * a.group - it.tile * kTileRows, row0 = blockIdx.y * kJoinRows;
+  if (cut.chunks <= 1 || row0 >= rows) return;  // (a tile of one chunk its workgroup has finished)
   // the states of chunk 0 and from chunk to chunk
   const int first = it.state + (it.s.tiles - 1 - it.tile) * it.most * a.kv_heads + it.h;
-  if (first + (cut.chunks - 1) * a.kv_heads >= a.states) return;
-  const float* state = a.state + (size_t)first * kStateFloats<D> + row;
+  if (first + (cut.chunks - 1) * a.kv_heads >= a.states) return;  // (never, while the offsets ascend)
+  const float* state = a.state + (size_t)first * kStateFloats<D>;
   const size_t step = (size_t)a.kv_heads * kStateFloats<D>;
+  const int row = threadIdx.x % kJoinRows, quad = threadIdx.x / kJoinRows;
+  const bool valid = row0 + row < rows;
+  // (rows behind the tile's have no state: a row that has is read in their place)
+  const float* own = state + row0 + (valid ? row : 0);
+  const float4* products = reinterpret_cast<const float4*>(state + 2 * kTileRows) + quad * kTileRows + row0 + (valid ? row : 0);
   float M = -INFINITY, den = 0.f;
-  for (int c = 0; c < cut.chunks; ++c) M = fmaxf(M, state[c * step]);
-  const int quad0 = blockIdx.y * (kJoinDims / 4) + threadIdx.x / kTileRows;
-  constexpr int kQ = kJoinDims / 4 * kTileRows / kThreads;
-  float4 sum[kQ];
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 < cut.chunks; c0 += kLanes) {
+    const int count = min(cut.chunks - c0, kLanes);
+    float4 x[kU];
+    auto load = [&](int c) {
 #pragma unroll
-  for (int e = 0; e < kQ; ++e) sum[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = 0; c < cut.chunks; ++c) {
-    const float f = state_factor(state[c * step], M);
-    den = fmaf(f, state[c * step + kTileRows], den);
+      for (int e = 0; e < kU; ++e)
+        x[e] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(products) + (size_t)(c0 + min(c + e, count - 1)) * step);
+    };
+    load(0);
+    // the joint maximum so far and what it makes of what was joined before
+    __syncthreads();
+    factors[quad][row] = quad < count ? own[(c0 + quad) * step] : -INFINITY;
+    const float z = quad < count ? own[(c0 + quad) * step + kTileRows] : 0.f;
+    __syncthreads();
+    float nm = M;
+    for (int c = 0; c < count; ++c) nm = fmaxf(nm, factors[c][row]);
+    const float before = state_factor(M, nm), f = state_factor(factors[quad][row], nm);
+    M = nm;
+    __syncthreads();
+    factors[quad][row] = f;
+    den *= before;
+    sum = make_float4(sum.x * before, sum.y * before, sum.z * before, sum.w * before);
+    parts[quad][row] = f * z;
+    __syncthreads();
+    for (int c = 0; c < count; ++c) den += parts[c][row];
+    for (int c = 0; c < count; c += kU) {
 #pragma unroll
-    for (int e = 0; e < kQ; ++e) {
-      const int quad = quad0 + e * (kThreads / kTileRows);
-      const float4 x = reinterpret_cast<const float4*>(state - row + c * step + 2 * kTileRows)[quad * kTileRows + row];
-      sum[e].x = fmaf(f, x.x, sum[e].x);
-      sum[e].y = fmaf(f, x.y, sum[e].y);
-      sum[e].z = fmaf(f, x.z, sum[e].z);
-      sum[e].w = fmaf(f, x.w, sum[e].w);
+      for (int e = 0; e < kU; ++e)
+        if (c + e < count) {
+          const float g = factors[c + e][row];
+          sum.x = fmaf(g, x[e].x, sum.x);
+          sum.y = fmaf(g, x[e].y, sum.y);
+          sum.z = fmaf(g, x[e].z, sum.z);
+          sum.w = fmaf(g, x[e].w, sum.w);
+        }
+      if (c + kU < count) load(c + kU);
     }
   }
-  const int of = it.tile * kTileRows + row, token = of / a.group;
+  if (!valid) return;
+  const int of = it.tile * kTileRows + row0 + row, token = of / a.group;
   const size_t row_head = (size_t)(it.s.first + token) * a.kv_heads * a.group + it.h * a.group + (of - token * a.group);
-  if (a.lse && quad0 == 0) a.lse[row_head] = prompt_lse<DT>(M, den);
-#pragma unroll
-  for (int e = 0; e < kQ; ++e) put_four<DT, D>(a, row_head, 4 * (quad0 + e * (kThreads / kTileRows)), den, sum[e]);
+  if (a.lse && quad == 0) a.lse[row_head] = prompt_lse<DT>(M, den);
+  put_four<DT, D>(a, row_head, 4 * quad, den, sum);
 }
 
 // Work items, states and cut tiles of a launch at most.
@@ -634,16 +741,11 @@ PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group,
 
 template <int DT, int D>
 int launch_prompt(const Prompt& a, const PromptLayout& l, hipStream_t stream) {
-  constexpr int lds = 2 * kTileTokens<DT, D> * D * kElem<DT>;
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_kernel<DT, D>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return (int)e;
-  }
-  hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)l.items), dim3(kThreads), lds, stream, a);
+  hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)l.items), dim3(kThreads), 0, stream, a);
   if (const int rc = (int)hipGetLastError()) return rc;
   if (!l.cut_tiles) return 0;
-  hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3((unsigned)l.cut_tiles, D / kJoinDims), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3((unsigned)l.cut_tiles, kTileRows / kJoinRows),
+                     dim3(kJoinRows * D / 4), 0, stream, a);
   return (int)hipGetLastError();
 }
 
