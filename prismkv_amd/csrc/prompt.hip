@@ -20,7 +20,7 @@ template <int DT, int D>
 constexpr int kTileTokens = kElem<DT> * D > 256 ? 32 : 64;
 // Waves of a SIMD, by the registers that products, queries and staged rows take.
 template <int DT, int D>
-constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : kElem<DT> * D > 128 ? 2 : 3;
+constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
 // The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, nor
 // less than kLeastTiles tiles of keys.
 constexpr int kItemsLog = 9, kLeastTiles = 4;
@@ -480,10 +480,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
     drain();
     stage.move();
     __syncthreads();
-    if (active) {
-      scores(s, keys0);
-      mask(s, from * kTokens);
-    }
+    if (active) scores(s, keys0);
     __syncthreads();  // the first keys have been read
   }
   // Step t has the scores of tile t, and in LDS its values and the next tile's keys: the
@@ -504,6 +501,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       stage.ask(min(t + 3, to - 1) * kTokens);
     }
     if (active) {
+      mask(s, t0);
       f32x16 next[kT];
       float most = -INFINITY;
 #pragma unroll
@@ -536,17 +534,23 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
         scale = 1.f;
         shift = (float)kBias<DT>;
       }
-      scores(next, next_keys);  // (of no tile, behind the last)
-#pragma unroll
-      for (int i = 0; i < kT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], scale, shift));
-          z += s[i][r];
-          // (2^-24, or 0 for 0; in 4 bits no value is infinite)
-          if constexpr (DT == kFp16) s[i][r] = fmaxf(s[i][r], fminf(s[i][r] * 0x1p126f, 0x1p-24f));
+      // 2^(..), in place
+      auto exponential = [&](int e) {
+        float x = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], scale, shift));
+        // (2^-24, or 0 for 0; in 4 bits no value is infinite.  NaN is left to the sum)
+        if constexpr (DT == kFp16) {
+          z += x;
+          x = __builtin_amdgcn_fmed3f(x, x * 0x1p126f, 0x1p-24f);
         }
+        s[e / 16][e % 16] = x;
+      };
       if constexpr (kType<DT> == kFp32) {
+        scores(next, next_keys);  // (of no tile, behind the last)
+#pragma unroll
+        for (int e = 0; e < 16 * kT; ++e) {
+          exponential(e);
+          z += s[e / 16][e % 16];
+        }
         const FloatAt<kC> float_at(col, half);
 #pragma unroll
         for (int i = 0; i < kT; ++i)
@@ -557,26 +561,64 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
               acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + float_at.of(i, r, d)), s[i][r],
                                                             acc[d], 0, 0, 0);
       } else {
+        // The order of the instructions is this one (the compiler's own has LDS read right
+        // before the products that wait for it): the reads are kAhead products ahead, and
+        // the exponentials between the first products, the sum between the others.
+        constexpr int kSteps = kC / 2, kPer = 16 * kT / kSteps, kAhead = 3;
+        constexpr int kCols = D / 32, kPv = 2 * kT * kCols;
         typedef __attribute__((address_space(3))) s16x4* Transposed;
         const ValueAt<kC> value_at(lane);
+        u32x4 kf[kAhead][kT], vf[kAhead + 1], p;
+        auto read_k = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < kT; ++i) kf[c % kAhead][i] = *reinterpret_cast<const u32x4*>(next_keys + key_at.of(i, c));
+        };
+        auto read_v = [&](int j) {
+          const int i = j / (2 * kCols), u = j / kCols % 2, d = j % kCols;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 0, d)));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 1, d)));
+          const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+          vf[j % (kAhead + 1)] = u32x4{l.x, l.y, h.x, h.y};
+        };
+        auto pack = [&](int g) {
+          const f32x16& x = s[g / 2];
+          const int o = 8 * (g & 1);
+          p = u32x4{pack2<DT>(x[o], x[o + 1]), pack2<DT>(x[o + 2], x[o + 3]), pack2<DT>(x[o + 4], x[o + 5]),
+                    pack2<DT>(x[o + 6], x[o + 7])};
+        };
 #pragma unroll
         for (int i = 0; i < kT; ++i)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const u32x4 p = {pack2<DT>(s[i][8 * u], s[i][8 * u + 1]), pack2<DT>(s[i][8 * u + 2], s[i][8 * u + 3]),
-                             pack2<DT>(s[i][8 * u + 4], s[i][8 * u + 5]), pack2<DT>(s[i][8 * u + 6], s[i][8 * u + 7])};
+          for (int r = 0; r < 16; ++r) next[i][r] = 0.f;
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-              const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 0, d)));
-              const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 1, d)));
-              const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
-              acc[d] = mfma_rows<DT>(u32x4{l.x, l.y, h.x, h.y}, p, acc[d]);
-            }
+        for (int c = 0; c < kAhead - 1; ++c) read_k(c);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+          if (c + kAhead - 1 < kSteps) read_k(c + kAhead - 1);
+          else read_v(c + kAhead - 1 - kSteps);
+#pragma unroll
+          for (int i = 0; i < kT; ++i) next[i] = mfma_rows<DT>(kf[c % kAhead][i], q[c], next[i]);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) exponential(c * kPer + e);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        read_v(kAhead - 1);
+#pragma unroll
+        for (int j = 0; j < kPv; ++j) {
+          if (j % kCols == 0) pack(j / kCols);
+          if (j + kAhead < kPv) read_v(j + kAhead);
+          acc[j % kCols] = mfma_rows<DT>(vf[j % (kAhead + 1)], p, acc[j % kCols]);
+#pragma unroll
+          for (int e = 0; e < 8 / kCols; ++e) {
+            const int at = j / kCols * 8 + j % kCols * (8 / kCols) + e;
+            if constexpr (DT != kFp16) z += s[at / 16][at % 16];
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
 #pragma unroll
       for (int i = 0; i < kT; ++i) s[i] = next[i];
-      if (t + 1 < to) mask(s, t0 + kTokens);
     }
     stage.finish_v(next_values);
     stage.finish_k(later_keys);
