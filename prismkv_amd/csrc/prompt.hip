@@ -21,9 +21,13 @@ constexpr int kTileTokens = kElem<DT> * D > 256 ? 32 : 64;
 // Waves of a SIMD, by the registers that products, queries and staged rows take.
 template <int DT, int D>
 constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
-// The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, nor
-// less than kLeastTiles tiles of keys.
-constexpr int kItemsLog = 9, kLeastTiles = 4;
+// The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, but
+// no item is less than kLeastTiles tiles of keys.  Twice as many items are slower (2048
+// rows of 8 x 4 heads 92 us against 60, 48 rows over 65000 slots 116 against 94).  A sequence
+// is cut only where that saves its longest tile more tiles of keys than the states and
+// their join take: kCutSaves and one for every kCutTiles tiles of rows (16 rows over 1016
+// slots cut 16 us, whole 28; 1500 rows cut 61, whole 45; 64 x 64 rows over 2000 slots each 73 and 61).
+constexpr int kItemsLog = 9, kLeastTiles = 4, kCutSaves = 4, kCutTiles = 16;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -61,18 +65,27 @@ __device__ __forceinline__ PromptRows prompt_rows(const Prompt& a, int b) {
   return s;
 }
 
-// Tiles of keys of a work item at most: every wave finds them, and its own item, by
-// itself from the lengths (two lane scans for every 64 sequences).
+// Tiles of keys of a work item at most, and of a sequence that is not cut: every wave
+// finds them, and its own item, by itself from the lengths (two lane scans for every 64
+// sequences).
+struct PromptPlan {
+  int per_item, whole;
+};
+
 template <int kTokens>
-__device__ __forceinline__ int item_tiles(const Prompt& a) {
+__device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
   uint64_t sum = 0;
+  int tiles = 0;
   for (int b = threadIdx.x & 63; b < a.sequences; b += 64) {
     const PromptRows s = prompt_rows<kTokens>(a, b);
     sum += (uint64_t)s.tiles * s.key_tiles;
+    tiles += s.tiles;
   }
   const uint64_t low = wave_sum_i((int)(sum & 0xffffffu)), high = wave_sum_i((int)(sum >> 24));
   const uint64_t share = (((high << 24) + low) * a.kv_heads >> kItemsLog) + 1;
-  return (int)(share < kLeastTiles ? kLeastTiles : share < (1u << 24) ? share : 1u << 24);
+  const int per_item = (int)(share < kLeastTiles ? kLeastTiles : share < (1u << 24) ? share : 1u << 24);
+  // (tiles * kv_heads < 2^30, key tiles of a sequence < 2^26)
+  return PromptPlan{per_item, a.states ? per_item + kCutSaves + wave_sum_i(tiles) * a.kv_heads / kCutTiles : INT32_MAX};
 }
 
 // Item `index` of the launch: a tile of rows of sequence b and KV head h, chunk `chunk`
@@ -87,18 +100,18 @@ struct PromptItem {
 // L2, and what they read at a time is the same.  A sequence's last tiles, which see the
 // most, come first.
 template <int kTokens>
-__device__ __forceinline__ bool find_item(const Prompt& a, int per_item, int index, bool cut_tiles, PromptItem& it) {
+__device__ __forceinline__ bool find_item(const Prompt& a, const PromptPlan& plan, int index, bool cut_tiles, PromptItem& it) {
   int base = 0, cut = 0;
   for (int b0 = 0; b0 < a.sequences; b0 += 64) {
     const PromptRows s = prompt_rows<kTokens>(a, b0 + (threadIdx.x & 63));
-    const int most = max((s.key_tiles + per_item - 1) / per_item, 1);
+    const int most = s.key_tiles > plan.whole ? (s.key_tiles + plan.per_item - 1) / plan.per_item : 1;
     // (cut_tiles: only those of sequences that are cut, one for all chunks of a tile)
     const int states = most > 1 ? s.tiles * most * a.kv_heads : 0;
     const int count = cut_tiles ? (most > 1 ? s.tiles * a.kv_heads : 0) : s.tiles * most * a.kv_heads;
     const int upto = (int)wave_incl_scan((unsigned)count), total = __builtin_amdgcn_readlane(upto, 63);
     const int states_upto = (int)wave_incl_scan((unsigned)states);
     if (index - base < total) {
-      const int l = __ffsll((unsigned long long)__ballot(upto > index - base)) - 1;
+      const int l = max(__ffsll((unsigned long long)__ballot(upto > index - base)) - 1, 0);
       it.s.first = __builtin_amdgcn_readlane(s.first, l);
       it.s.m = __builtin_amdgcn_readlane(s.m, l);
       it.s.n = __builtin_amdgcn_readlane(s.n, l);
@@ -107,6 +120,7 @@ __device__ __forceinline__ bool find_item(const Prompt& a, int per_item, int ind
       it.most = __builtin_amdgcn_readlane(most, l);
       it.b = b0 + l;
       int at = index - base - __builtin_amdgcn_readlane(upto, l) + __builtin_amdgcn_readlane(count, l);
+      if ((unsigned)at >= (unsigned)__builtin_amdgcn_readlane(count, l)) return false;  // (offsets that do not ascend)
       it.state = cut + __builtin_amdgcn_readlane(states_upto, l) - __builtin_amdgcn_readlane(states, l) + (cut_tiles ? 0 : at);
       it.h = at % a.kv_heads;
       at /= a.kv_heads;
@@ -124,11 +138,11 @@ __device__ __forceinline__ bool find_item(const Prompt& a, int per_item, int ind
 template <int kTokens>
 struct PromptCut {
   int end, tiles, chunks, each;  // slots and tiles that its last row sees; tiles of a chunk
-  __device__ __forceinline__ PromptCut(const Prompt& a, const PromptItem& it, int per_item) {
+  __device__ __forceinline__ PromptCut(const Prompt& a, const PromptItem& it, const PromptPlan& plan) {
     const int last = (min((it.tile + 1) * kTileRows, it.s.m * a.group) - 1) / a.group;  // the tile's last token
     end = max(it.s.n - it.s.m + last + 1, 0);
     tiles = (end + kTokens - 1) / kTokens;
-    chunks = (tiles + per_item - 1) / per_item;
+    chunks = it.most > 1 ? (tiles + plan.per_item - 1) / plan.per_item : tiles > 0;
     each = chunks ? (tiles + chunks - 1) / chunks : 0;
     if (each) chunks = (tiles + each - 1) / each;
   }
@@ -360,7 +374,10 @@ __device__ __forceinline__ float4 four_of(const char* p) {
 // Writes four outputs of a row, and its log-sum.
 template <int DT, int D>
 __device__ __forceinline__ void put_four(const Prompt& a, size_t row_head, int dim, float den, float4 x) {
-  const float y[4] = {x.x / den, x.y / den, x.z / den, x.w / den};
+  // (16-bit types: one division, and a rounding more that theirs hides)
+  const float inverse = 1.f / den;
+  const float y[4] = {kType<DT> == kFp32 ? x.x / den : x.x * inverse, kType<DT> == kFp32 ? x.y / den : x.y * inverse,
+                      kType<DT> == kFp32 ? x.z / den : x.z * inverse, kType<DT> == kFp32 ? x.w / den : x.w * inverse};
   float z[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) z[e] = den == 0.f ? 0.f : y[e];
@@ -404,10 +421,10 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       if (from > to || (b == 0 && from) || (b == a.sequences - 1 && to != a.rows))
         report_error(a.err, error_host_slot(a.err), kErrOffsets);
     }
-  const int per_item = item_tiles<kTokens>(a);
+  const PromptPlan plan = prompt_plan<kTokens>(a);
   PromptItem it;
-  if (!find_item<kTokens>(a, per_item, blockIdx.x, false, it)) return;
-  const PromptCut<kTokens> cut(a, it, per_item);
+  if (!find_item<kTokens>(a, plan, blockIdx.x, false, it)) return;
+  const PromptCut<kTokens> cut(a, it, plan);
   if (it.chunk > 0 && it.chunk >= cut.chunks) return;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -544,35 +561,58 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
         }
         s[e / 16][e % 16] = x;
       };
+      // The order of the instructions is this one (the compiler's own has LDS read right
+      // before the products that wait for it): the reads are kAhead products ahead, and
+      // the exponentials between the first products, the sum between the others.  (The
+      // next scores are of no tile, behind the last.)
+      constexpr int kSteps = kC / 2, kAhead = 3;
+      u32x4 kf[kAhead][kT];
+      auto read_k = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < kT; ++i) kf[c % kAhead][i] = *reinterpret_cast<const u32x4*>(next_keys + key_at.of(i, c));
+      };
+#pragma unroll
+      for (int i = 0; i < kT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) next[i][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kAhead - 1; ++c) read_k(c);
+      __builtin_amdgcn_sched_barrier(0);
+      auto score_step = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < kT; ++i) next[i] = mfma_rows<DT>(kf[c % kAhead][i], q[c], next[i]);
+#pragma unroll
+        for (int e = c * 16 * kT / kSteps; e < (c + 1) * 16 * kT / kSteps; ++e) exponential(e);
+        __builtin_amdgcn_sched_barrier(0);
+      };
       if constexpr (kType<DT> == kFp32) {
-        scores(next, next_keys);  // (of no tile, behind the last)
-#pragma unroll
-        for (int e = 0; e < 16 * kT; ++e) {
-          exponential(e);
-          z += s[e / 16][e % 16];
-        }
         const FloatAt<kC> float_at(col, half);
+        constexpr int kCols = D / 32, kPv = 16 * kT * kCols, kVAhead = 6;
+        float vf[kVAhead + 1];
+        auto read_v = [&](int j) {
+          vf[j % (kVAhead + 1)] =
+              *reinterpret_cast<const float*>(values + float_at.of(j / (16 * kCols), j / kCols % 16, j % kCols));
+        };
 #pragma unroll
-        for (int i = 0; i < kT; ++i)
+        for (int c = 0; c < kSteps; ++c) {
+          if (c + kAhead - 1 < kSteps) read_k(c + kAhead - 1);
+          score_step(c);
+        }
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
+        for (int j = 0; j < kVAhead; ++j) read_v(j);
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d)
-              acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(values + float_at.of(i, r, d)), s[i][r],
-                                                            acc[d], 0, 0, 0);
+        for (int j = 0; j < kPv; ++j) {
+          if (j + kVAhead < kPv) read_v(j + kVAhead);
+          const float p = s[j / (16 * kCols)][j / kCols % 16];
+          acc[j % kCols] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[j % (kVAhead + 1)], p, acc[j % kCols], 0, 0, 0);
+          if (j % kCols == 0) z += p;
+          __builtin_amdgcn_sched_barrier(0);
+        }
       } else {
-        // The order of the instructions is this one (the compiler's own has LDS read right
-        // before the products that wait for it): the reads are kAhead products ahead, and
-        // the exponentials between the first products, the sum between the others.
-        constexpr int kSteps = kC / 2, kPer = 16 * kT / kSteps, kAhead = 3;
         constexpr int kCols = D / 32, kPv = 2 * kT * kCols;
         typedef __attribute__((address_space(3))) s16x4* Transposed;
         const ValueAt<kC> value_at(lane);
-        u32x4 kf[kAhead][kT], vf[kAhead + 1], p;
-        auto read_k = [&](int c) {
-#pragma unroll
-          for (int i = 0; i < kT; ++i) kf[c % kAhead][i] = *reinterpret_cast<const u32x4*>(next_keys + key_at.of(i, c));
-        };
+        u32x4 vf[kAhead + 1], p;
         auto read_v = [&](int j) {
           const int i = j / (2 * kCols), u = j / kCols % 2, d = j % kCols;
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Transposed)(values + value_at.of(i, u, 0, d)));
@@ -587,21 +627,10 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
                     pack2<DT>(x[o + 6], x[o + 7])};
         };
 #pragma unroll
-        for (int i = 0; i < kT; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) next[i][r] = 0.f;
-#pragma unroll
-        for (int c = 0; c < kAhead - 1; ++c) read_k(c);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           if (c + kAhead - 1 < kSteps) read_k(c + kAhead - 1);
           else read_v(c + kAhead - 1 - kSteps);
-#pragma unroll
-          for (int i = 0; i < kT; ++i) next[i] = mfma_rows<DT>(kf[c % kAhead][i], q[c], next[i]);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) exponential(c * kPer + e);
-          __builtin_amdgcn_sched_barrier(0);
+          score_step(c);
         }
         read_v(kAhead - 1);
 #pragma unroll
@@ -697,10 +726,10 @@ template <int DT, int D>
 __global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a) {
   constexpr int kTokens = kTileTokens<DT, D>, kLanes = D / 4, kU = 8;
   __shared__ float factors[kLanes][kJoinRows], parts[kLanes][kJoinRows];
-  const int per_item = item_tiles<kTokens>(a);
+  const PromptPlan plan = prompt_plan<kTokens>(a);
   PromptItem it;
-  if (!find_item<kTokens>(a, per_item, blockIdx.x, true, it)) return;
-  const PromptCut<kTokens> cut(a, it, per_item);
+  if (!find_item<kTokens>(a, plan, blockIdx.x, true, it)) return;
+  const PromptCut<kTokens> cut(a, it, plan);
   const int rows = it.s.m * a.group - it.tile * kTileRows, row0 = blockIdx.y * kJoinRows;
   if (cut.chunks <= 1 || row0 >= rows) return;  // (a tile of one chunk its workgroup has finished)
   // the states of chunk 0 and from chunk to chunk
@@ -775,8 +804,11 @@ PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group,
   // A sequence that is cut has most = ceil(x) <= 2x chunks a tile, x > 1 its share of
   // an item: 2 all of them at most.
   const int64_t full = tiles * kv_heads * ((key_tiles + kLeastTiles - 1) / kLeastTiles);
-  l.states = key_tiles <= kLeastTiles ? 0 : full < 2 * all ? full : 2 * all;
-  l.cut_tiles = key_tiles <= kLeastTiles ? 0 : tiles * kv_heads < all ? tiles * kv_heads : all;
+  // Never cut: few slots; one sequence whose tiles are as many as the items are to be.
+  const bool whole = key_tiles <= kLeastTiles + kCutSaves ||
+                     (sequences == 1 && (rows * group + kTileRows - 1) / kTileRows * kv_heads >= all);
+  l.states = whole ? 0 : full < 2 * all ? full : 2 * all;
+  l.cut_tiles = whole ? 0 : tiles * kv_heads < all ? tiles * kv_heads : all;
   l.bytes = (size_t)l.states * kTileRows * (head_dim + 2) * sizeof(float);
   return l;
 }

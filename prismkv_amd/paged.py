@@ -24,6 +24,7 @@ import ctypes
 import itertools
 import math
 import threading
+import weakref
 from collections import deque
 
 import torch
@@ -48,6 +49,11 @@ _SCORED = ("seen", "scores", "positions")
 # call's 7.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+# torch.cuda.current_device() without its check that CUDA has been initialised, which a
+# cache's tensors have done: 0.7 us of a call.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _check(cond, what):
@@ -226,6 +232,7 @@ class PagedCache:
         _check(not any(_overlap(x, y) for x, y in itertools.combinations(self._spans, 2)),
                "lengths, seen, scores and positions must not overlap")
         self._free = self._pages = None
+        self._checked = None  # the cache that was last found to be a fork of this one
         self._attend_work, self._evict_work, self._prompt_work, self._prompt_last = {}, None, {}, (None, None)
         self._err = _ErrorWord(self.lib, self.device) if err is None else err
         # what the C entries read of the cache; its tensors are fixed from here on
@@ -347,7 +354,7 @@ class PagedCache:
 
     def _call(self, name, *args):
         index = self.device.index
-        if torch.cuda.current_device() == index:
+        if _current_device() == index:
             self.lib.call(name, *args, stream=_raw_stream(index))
         else:
             with torch.cuda.device(index):
@@ -356,6 +363,8 @@ class PagedCache:
     def _into(self, into):
         if into is None or into is self:
             return self
+        if self._checked is not None and self._checked() is into:  # (the tensors of a cache are fixed)
+            return into
         if not isinstance(into, PagedCache) or into.device != self.device:
             raise ValueError("into must be a fork of this cache")
         a, b = self._desc, into._desc
@@ -369,6 +378,7 @@ class PagedCache:
         if into._err is not self._err and into._spans != self._spans and any(
                 _overlap(x, y) for x in self._spans for y in into._spans):
             raise ValueError("into's lengths, seen, scores and positions must be all of this cache's or overlap none")
+        self._checked = weakref.ref(into)
         return into
 
     def _workspace(self, nbytes, zero):
