@@ -27,8 +27,8 @@ step then appends its token, attends to what is held and adds the step's
 weights to the scores, and a cache that has grown by `evict_every` tokens is
 cut again: the `cache_recent` newest and `cache_sinks` first tokens stay, then
 the highest scores.  Any number of KV and query heads with head_dim 64, 128 or 256;
-encoders are not used.  (The model's own cache object still grows; it is not
-read.)
+encoders are not used.  `cache_storage` "mxfp4" holds the cache in 4 bits, of bf16
+and fp16 models.  (The model's own cache object still grows; it is not read.)
 
 Records keep the reference's per-(layer, group) fields, including the
 `detailed_records` ones (old_unique, old_raw, generated_indexed_unique,
@@ -54,7 +54,7 @@ from dataclasses import dataclass
 import torch
 
 from .native8b import DIM, FEATURES, GROUPS, HEADS, MAX_BLOCK, Native8B
-from .paged import DTYPES, HEAD_DIMS, PagedCache
+from .paged import DTYPES, HEAD_DIMS, STORAGES, PagedCache
 from .weights import Encoder, layer_tables  # noqa: F401  (Encoder re-exported: reference name)
 
 BACKEND = "prismkv_native"
@@ -234,7 +234,7 @@ class _BoundedLayer:
         most = max(min(prefix, session.cache_budget), 1) + session.evict_every + 1
         pages = -(-max(prefix, most) // PAGE)
         cache = PagedCache(1, pages, pages, page_size=PAGE, kv_heads=kv_heads, head_dim=head_dim, dtype=K.dtype,
-                           scored=True, device=K.device, library=session.library)
+                           scored=True, storage=session.cache_storage, device=K.device, library=session.library)
         cache.reserve(prefix)
         ends = torch.tensor([0, prefix], dtype=torch.int32, device=K.device)
         cache.append(K[:, :prefix].transpose(0, 1), V[:, :prefix].transpose(0, 1), ends)
@@ -283,13 +283,15 @@ class HFNative:
 
     def __init__(self, model, encoders, *, mode="sparse", router="moments", selected_buckets=16, unique_cap=None,
                  update_interval=4096, detailed_records=False, capacity_step=8192, library=None,
-                 cache_budget=4096, cache_recent=512, cache_sinks=4, evict_every=64, observe=32):
+                 cache_budget=4096, cache_recent=512, cache_sinks=4, evict_every=64, observe=32, cache_storage=None):
         # the reference's policy checks (hf_reference.py:77-84), then the native limits
         if mode not in ("sparse", "all_read", "evict"):
             raise ValueError("mode must be sparse, all_read or evict")
         if mode == "evict" and (cache_budget < 1 or evict_every < 1 or min(cache_recent, cache_sinks, observe) < 0
                                 or cache_recent + cache_sinks > cache_budget):
             raise ValueError("a positive cache budget that holds the recent and first tokens required")
+        if cache_storage not in STORAGES or (cache_storage and mode != "evict"):
+            raise ValueError(f"cache_storage must be one of {STORAGES}, and is mode evict's")
         if router not in ("moments", "q_activation") or selected_buckets <= 0:
             raise ValueError("unsupported router/bucket count")
         if unique_cap is not None and not 0 <= unique_cap <= 1:
@@ -313,6 +315,7 @@ class HFNative:
         self.update_interval, self.force_prefill = update_interval, False
         self.cache_budget, self.cache_recent, self.cache_sinks = int(cache_budget), int(cache_recent), int(cache_sinks)
         self.evict_every, self.observe = int(evict_every), int(observe)
+        self.cache_storage = cache_storage
         self.detailed_records = detailed_records
         self.capacity_step, self.library = int(capacity_step), library
         self._hooked = hooked
@@ -454,6 +457,8 @@ class HFNative:
         if q.shape[-1] not in HEAD_DIMS or q.dtype not in DTYPES or q.device.type != "cuda":
             raise NotImplementedError("the paged cache holds bf16, fp16 or fp32 rows of head_dim 64, 128 or 256 on the "
                                       "device")
+        if self.cache_storage and q.dtype == torch.float32:
+            raise NotImplementedError("the paged cache holds bf16 or fp16 rows in 4 bits")
         if K.stride(-1) != 1 or V.stride(-1) != 1:
             K, V = K.contiguous(), V.contiguous()
         prefix, op = self.prefix_lengths[layer], self.ops.get(layer)
