@@ -286,7 +286,7 @@ struct PagedRead {
   int sequences, kv_heads, page_size, max_pages, pages, slots;
 };
 
-// The place of a row (slot -1: none); reports what is wrong with it.
+// The place of a row (slot -1: none); reports a slot or a page that there is not.
 __device__ __forceinline__ RowPlace read_place(const PagedRead& a, int64_t row) {
   RowPlace p{0, 0, 0, 0, -1, 0};
   int64_t back = 1;  // from the sequence's end
@@ -295,10 +295,7 @@ __device__ __forceinline__ RowPlace read_place(const PagedRead& a, int64_t row) 
   } else {
     p.b = sequence_of(a.offsets, a.sequences, row);
     const int from = a.offsets[p.b], to = a.offsets[p.b + 1];
-    if (row < from || row >= to || (p.b == a.sequences - 1 && to != a.rows)) {
-      report_error(a.err, error_host_slot(a.err), kErrOffsets);
-      if (row < from || row >= to) return p;  // a row of no sequence
-    }
+    if (row < from || row >= to) return p;  // a row of no sequence
     back = to - row;
   }
   const int64_t slot = min(max(a.lengths[p.b], 0), a.slots) - back;
@@ -339,6 +336,12 @@ __global__ __launch_bounds__(kPT) void paged_read_kernel(PagedRead a) {
   const int64_t row0 = a.first_row + (int64_t)blockIdx.x * kRowsEach;
   const int rows = (int)min((int64_t)kRowsEach, a.rows - row0);
   if (tid < rows) places[tid] = read_place(a, row0 + tid);
+  if (row0 == 0 && a.offsets)
+    for (int b = tid; b < a.sequences; b += kPT) {
+      const int from = a.offsets[b], to = a.offsets[b + 1];
+      if (from > to || (b == 0 && from) || (b == a.sequences - 1 && to != a.rows))
+        report_error(a.err, error_host_slot(a.err), kErrOffsets);
+    }
   __syncthreads();
   const int per_row = a.kv_heads * kC, items = rows * per_row;
   for (int i = tid; i < items; i += kPT) {

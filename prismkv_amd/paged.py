@@ -482,12 +482,12 @@ class PagedCache:
         accumulate = bool(accumulate)
         return self._attend(q, group, scale, accumulate, lse, to, 0, self._attend_workspace(group, accumulate))
 
-    def _check_q(self, q, scale, accumulate, lse):
-        """The query heads per KV head, and the scale."""
+    def _check_q(self, q, scale, accumulate, lse, turned=False):
+        """The query heads per KV head, and the scale (turned: q comes contiguous)."""
         sequences, kv_heads, head_dim, _, _ = self._shape
         shape = q.shape
         if (len(shape) != 3 or shape[0] != sequences or shape[2] != head_dim or shape[1] < 1 or shape[1] % kv_heads
-                or not q.is_contiguous()):
+                or not (turned or q.is_contiguous())):
             raise ValueError(f"contiguous Q[{sequences}, a multiple of {kv_heads} heads, {head_dim}] required")
         if q.dtype != self.dtype or q.device != self.device:
             raise ValueError("Q of the cache's type on its device required")
@@ -537,7 +537,7 @@ class PagedCache:
         behind this cache's lengths."""
         to = self if into is None else self._into(into)
         # nothing is appended for a query that is refused
-        group, scale = self._check_q(q, scale, accumulate, lse)
+        group, scale = self._check_q(q, scale, accumulate, lse, rotary is not None)
         accumulate = bool(accumulate)
         work = self._attend_workspace(group, accumulate)
         turned = self.append(k, v, q=q if rotary is not None else None, rotary=rotary, into=into)
