@@ -420,7 +420,8 @@ int prismkv_attend_f32(uint64_t q, uint64_t k, uint64_t v, uint64_t ids, uint64_
  *            of codes (the even dim in the lower half of a byte; strides in
  *            bytes) and
  *   k_scales, v_scales  u8 [pages][kv_heads][page_size][head_dim / 32], strides in
- *            bytes (multiples of head_dim / 32, as are the addresses): for every
+ *            bytes (multiples of head_dim / 32, as are the addresses; all of a
+ *            head within 2^33 bytes): for every
  *            32 dims a byte s, in 2 .. 252 or of fp16 rows 104 .. 140, the codes
  *            0 .. 7 standing for 0, 0.5, 1, 1.5, 2, 3, 4 and 6 times 2^(s - 127), 8 ..
  *            15 for their negatives; all are NaN where s is 255.  A row is held with

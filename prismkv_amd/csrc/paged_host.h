@@ -70,7 +70,9 @@ inline int check_cache(const prismkv_paged_cache* cache, const prismkv_paged_cac
         to.scale_head_stride != c.scale_head_stride || to.scale_slot_stride != c.scale_slot_stride)
       return kBadSize;
     if (c.scale_page_stride < 0 || c.scale_head_stride < 0 || c.scale_slot_stride < row) return kBadSize;
-    if (c.scale_page_stride > limit / c.pages || c.scale_head_stride > limit || c.scale_slot_stride > limit / c.page_size)
+    const int64_t most = 1ll << 33;  // (a row's place is counted in 32 bits)
+    if (c.scale_page_stride > most / c.pages || c.scale_head_stride > most || c.scale_slot_stride > most / c.page_size ||
+        (c.pages - 1) * c.scale_page_stride + (c.page_size - 1) * c.scale_slot_stride >= most)
       return kBadSize;
     if ((c.scale_page_stride | c.scale_head_stride | c.scale_slot_stride) % row) return kBadSize;
   }

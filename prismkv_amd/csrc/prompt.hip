@@ -39,8 +39,9 @@ struct Prompt {
   char* out;
   float *lse, *state;
   unsigned* err;
-  int64_t head_bytes, scale_page, scale_head, scale_slot;
-  unsigned page_units, slot_units;  // 16 bytes
+  int64_t head_bytes, scale_head;
+  unsigned page_units, slot_units;              // 16 bytes
+  unsigned scale_page_units, scale_slot_units;  // head_dim / 32 bytes
   PageDiv div;
   unsigned q_and, q_xor;  // the scale's sign, or a scale of 0, goes to the queries
   float scale;            // log2(e) times the caller's magnitude
@@ -257,7 +258,7 @@ struct Stage {
   // places (16-byte units) of the next tile of values and of the next one of keys, which
   // is the tile behind it
   unsigned v_at[kEach], k_at[kEach];
-  uint64_t v_scale_at[kRaw], k_scale_at[kRaw];
+  unsigned v_scale_at[kRaw], k_scale_at[kRaw];
   unsigned kw[kRaw], vw[kRaw], kb[kRaw], vb[kRaw];
 
   __device__ __forceinline__ Stage(const Prompt& a, int b, int h, int end) : a(a), end(end) {
@@ -283,15 +284,14 @@ struct Stage {
     const unsigned p = (unsigned)page < (unsigned)a.pages ? (unsigned)page : 0u;
     const unsigned in = (unsigned)(token - a.div.of(token) * a.page_size);
     const unsigned place = p * a.page_units + in * a.slot_units;
-    uint64_t scale_place = 0;
-    if constexpr (kInFour<DT>) scale_place = (uint64_t)p * a.scale_page + (uint64_t)in * a.scale_slot;
+    const unsigned scale_place = p * a.scale_page_units + in * a.scale_slot_units;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       v_at[i] = k_at[i];
       k_at[i] = (unsigned)__shfl((int)place, row + step(i));
       if constexpr (kInFour<DT>) {
         v_scale_at[i] = k_scale_at[i];
-        k_scale_at[i] = (uint64_t)__shfl((unsigned long long)scale_place, row + step(i));
+        k_scale_at[i] = (unsigned)__shfl((int)scale_place, row + step(i));
       }
     }
   }
@@ -311,7 +311,7 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         kw[i] = *reinterpret_cast<const unsigned*>(k + ((size_t)k_at[i] << 4));
-        kb[i] = ks[k_scale_at[i]];
+        kb[i] = ks[(size_t)k_scale_at[i] * (D / 32)];
       }
     } else {
       issue(k, k_at, tile);
@@ -322,7 +322,7 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
         vw[i] = *reinterpret_cast<const unsigned*>(v + ((size_t)v_at[i] << 4));
-        vb[i] = vs[v_scale_at[i]];
+        vb[i] = vs[(size_t)v_scale_at[i] * (D / 32)];
       }
     } else {
       issue(v, v_at, tile);
@@ -886,9 +886,9 @@ int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t 
   if (c.dtype >= kFour) {
     a.ks = reinterpret_cast<const uint8_t*>(c.k_scales);
     a.vs = reinterpret_cast<const uint8_t*>(c.v_scales);
-    a.scale_page = c.scale_page_stride;
+    a.scale_page_units = (unsigned)(c.scale_page_stride / (c.head_dim / 32));
     a.scale_head = c.scale_head_stride;
-    a.scale_slot = c.scale_slot_stride;
+    a.scale_slot_units = (unsigned)(c.scale_slot_stride / (c.head_dim / 32));
   }
   a.div = page_div(c.page_size);
   a.rows = (int)rows;

@@ -678,8 +678,8 @@ def _check_scales(k, k_scales, v_scales):
            f"rows of scales must be {row}-byte aligned")
     _check(strides[2] >= row and (shape[0] == 1 or strides[0] >= row) and (shape[1] == 1 or strides[1] >= row),
            "rows of scales must not overlap")
-    if max(shape[0] * strides[0], shape[2] * strides[2]) > 1 << 36:
-        raise NotImplementedError("pages that span at most 64 GiB (of k, and of v)")
+    if max(shape[0] * strides[0], shape[2] * strides[2], (shape[0] - 1) * strides[0] + shape[2] * strides[2]) > 1 << 33:
+        raise NotImplementedError("scales that span at most 8 GiB (of k, and of v)")
     return strides[:3]
 
 
