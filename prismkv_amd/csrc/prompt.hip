@@ -29,6 +29,12 @@ constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
 // slots cut 16 us, whole 28; 1500 rows cut 61, whole 45; 64 x 64 rows over 2000 slots each 73 and 61).
 constexpr int kItemsLog = 9, kLeastTiles = 4, kCutSaves = 4, kCutTiles = 16;
 
+// By how much (in powers of 2) a row's largest score may pass the maximum that its weights
+// are taken from before what was summed so far is multiplied anew: nearly every tile raises
+// one of a wave's 32 rows' a little.  fp16 has no room above its bias.
+template <int DT>
+constexpr float kLead = kType<DT> == kFp16 ? 0.f : 8.f;
+
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -526,7 +532,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, s[i][r]);
       most = fmaxf(most, xor32(most)) * a.scale;
-      if (__ballot(most > m)) {
+      if (__ballot(most > m + kLead<DT>)) {
         const float nm = fmaxf(m, most);
         const float alpha = state_factor(m, nm);
         m = nm;
