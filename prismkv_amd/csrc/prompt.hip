@@ -51,7 +51,7 @@ struct Prompt {
   PageDiv div;
   unsigned q_and, q_xor;  // the scale's sign, or a scale of 0, goes to the queries
   float scale;            // log2(e) times the caller's magnitude
-  int rows, sequences, kv_heads, group, page_size, max_pages, pages, slots, states;
+  int rows, sequences, kv_heads, group, page_size, max_pages, pages, slots, states, cut_tiles;
 };
 
 // New rows m from `first` of a sequence, its slots, and its tiles of rows and of keys.
@@ -733,66 +733,67 @@ __global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a)
   constexpr int kTokens = kTileTokens<DT, D>, kLanes = D / 4, kU = 8;
   __shared__ float factors[kLanes][kJoinRows], parts[kLanes][kJoinRows];
   const PromptPlan plan = prompt_plan<kTokens>(a);
+  const int row0 = blockIdx.y * kJoinRows, row = threadIdx.x % kJoinRows, quad = threadIdx.x / kJoinRows;
   PromptItem it;
-  if (!find_item<kTokens>(a, plan, blockIdx.x, true, it)) return;
-  const PromptCut<kTokens> cut(a, it, plan);
-  const int rows = it.s.m * a.group - it.tile * kTileRows, row0 = blockIdx.y * kJoinRows;
-  if (cut.chunks <= 1 || row0 >= rows) return;  // (a tile of one chunk its workgroup has finished)
-  // the states of chunk 0 and from chunk to chunk
-  const int first = it.state + (it.s.tiles - 1 - it.tile) * it.most * a.kv_heads + it.h;
-  if (first + (cut.chunks - 1) * a.kv_heads >= a.states) return;  // (never, while the offsets ascend)
-  const float* state = a.state + (size_t)first * kStateFloats<D>;
-  const size_t step = (size_t)a.kv_heads * kStateFloats<D>;
-  const int row = threadIdx.x % kJoinRows, quad = threadIdx.x / kJoinRows;
-  const bool valid = row0 + row < rows;
-  // (rows behind the tile's have no state: a row that has is read in their place)
-  const float* own = state + row0 + (valid ? row : 0);
-  const float4* products = reinterpret_cast<const float4*>(state + 2 * kTileRows) + quad * kTileRows + row0 + (valid ? row : 0);
-  float M = -INFINITY, den = 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = 0; c0 < cut.chunks; c0 += kLanes) {
-    const int count = min(cut.chunks - c0, kLanes);
-    float4 x[kU];
-    auto load = [&](int c) {
+  for (int tile = blockIdx.x; tile < a.cut_tiles && find_item<kTokens>(a, plan, tile, true, it); tile += gridDim.x) {
+    const PromptCut<kTokens> cut(a, it, plan);
+    const int rows = it.s.m * a.group - it.tile * kTileRows;
+    if (cut.chunks <= 1 || row0 >= rows) continue;  // (a tile of one chunk its workgroup has finished)
+    // the states of chunk 0 and from chunk to chunk
+    const int first = it.state + (it.s.tiles - 1 - it.tile) * it.most * a.kv_heads + it.h;
+    if (first + (cut.chunks - 1) * a.kv_heads >= a.states) continue;  // (never, while the offsets ascend)
+    const float* state = a.state + (size_t)first * kStateFloats<D>;
+    const size_t step = (size_t)a.kv_heads * kStateFloats<D>;
+    const bool valid = row0 + row < rows;
+    // (rows behind the tile's have no state: one that has is read in their place)
+    const float* own = state + row0 + (valid ? row : 0);
+    const float* products = state + 2 * kTileRows + 4 * (quad * kTileRows + row0 + (valid ? row : 0));
+    float M = -INFINITY, den = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c0 = 0; c0 < cut.chunks; c0 += kLanes) {
+      const int count = min(cut.chunks - c0, kLanes);
+      float4 x[kU];
+      auto load = [&](int c) {
 #pragma unroll
-      for (int e = 0; e < kU; ++e)
-        x[e] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(products) + (size_t)(c0 + min(c + e, count - 1)) * step);
-    };
-    load(0);
-    // the joint maximum so far and what it makes of what was joined before
-    __syncthreads();
-    factors[quad][row] = quad < count ? own[(c0 + quad) * step] : -INFINITY;
-    const float z = quad < count ? own[(c0 + quad) * step + kTileRows] : 0.f;
-    __syncthreads();
-    float nm = M;
-    for (int c = 0; c < count; ++c) nm = fmaxf(nm, factors[c][row]);
-    const float before = state_factor(M, nm), f = state_factor(factors[quad][row], nm);
-    M = nm;
-    __syncthreads();
-    factors[quad][row] = f;
-    den *= before;
-    sum = make_float4(sum.x * before, sum.y * before, sum.z * before, sum.w * before);
-    parts[quad][row] = f * z;
-    __syncthreads();
-    for (int c = 0; c < count; ++c) den += parts[c][row];
-    for (int c = 0; c < count; c += kU) {
+        for (int e = 0; e < kU; ++e) x[e] = *reinterpret_cast<const float4*>(products + (size_t)(c0 + min(c + e, count - 1)) * step);
+      };
+      load(0);
+      // the joint maximum so far and what it makes of what was joined before
+      __syncthreads();
+      factors[quad][row] = quad < count ? own[(c0 + quad) * step] : -INFINITY;
+      const float z = quad < count ? own[(c0 + quad) * step + kTileRows] : 0.f;
+      __syncthreads();
+      float nm = M;
+      for (int c = 0; c < count; ++c) nm = fmaxf(nm, factors[c][row]);
+      const float before = state_factor(M, nm), f = state_factor(factors[quad][row], nm);
+      M = nm;
+      __syncthreads();
+      factors[quad][row] = f;
+      parts[quad][row] = f * z;
+      den *= before;
+      sum = make_float4(sum.x * before, sum.y * before, sum.z * before, sum.w * before);
+      __syncthreads();
+      for (int c = 0; c < count; ++c) den += parts[c][row];
+      for (int c = 0; c < count; c += kU) {
 #pragma unroll
-      for (int e = 0; e < kU; ++e)
-        if (c + e < count) {
-          const float g = factors[c + e][row];
-          sum.x = fmaf(g, x[e].x, sum.x);
-          sum.y = fmaf(g, x[e].y, sum.y);
-          sum.z = fmaf(g, x[e].z, sum.z);
-          sum.w = fmaf(g, x[e].w, sum.w);
-        }
-      if (c + kU < count) load(c + kU);
+        for (int e = 0; e < kU; ++e)
+          if (c + e < count) {
+            const float g = factors[c + e][row];
+            sum.x = fmaf(g, x[e].x, sum.x);
+            sum.y = fmaf(g, x[e].y, sum.y);
+            sum.z = fmaf(g, x[e].z, sum.z);
+            sum.w = fmaf(g, x[e].w, sum.w);
+          }
+        if (c + kU < count) load(c + kU);
+      }
+    }
+    if (valid) {
+      const int of = it.tile * kTileRows + row0 + row, token = of / a.group;
+      const size_t row_head = (size_t)(it.s.first + token) * a.kv_heads * a.group + it.h * a.group + (of - token * a.group);
+      if (a.lse && quad == 0) a.lse[row_head] = prompt_lse<DT>(M, den);
+      put_four<DT, D>(a, row_head, 4 * quad, den, sum);
     }
   }
-  if (!valid) return;
-  const int of = it.tile * kTileRows + row0 + row, token = of / a.group;
-  const size_t row_head = (size_t)(it.s.first + token) * a.kv_heads * a.group + it.h * a.group + (of - token * a.group);
-  if (a.lse && quad == 0) a.lse[row_head] = prompt_lse<DT>(M, den);
-  put_four<DT, D>(a, row_head, 4 * quad, den, sum);
 }
 
 // Work items, states and cut tiles of a launch at most.
@@ -824,7 +825,10 @@ int launch_prompt(const Prompt& a, const PromptLayout& l, hipStream_t stream) {
   hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)l.items), dim3(kThreads), 0, stream, a);
   if (const int rc = (int)hipGetLastError()) return rc;
   if (!l.cut_tiles) return 0;
-  hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3((unsigned)l.cut_tiles, kTileRows / kJoinRows),
+  // (few workgroups, each of every 64th tile: most launches find little to join; with one
+  // for each tile that might be cut 1000 rows took 34 us, so 31)
+  const unsigned tiles = (unsigned)(l.cut_tiles < 64 ? l.cut_tiles : 64);
+  hipLaunchKernelGGL((prompt_join_kernel<DT, D>), dim3(tiles, kTileRows / kJoinRows),
                      dim3(kJoinRows * D / 4), 0, stream, a);
   return (int)hipGetLastError();
 }
@@ -905,7 +909,7 @@ int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t 
   a.max_pages = c.max_pages;
   a.pages = (int)c.pages;
   a.slots = (int)slots;
-  a.states = (int)l.states;
+  a.states = (int)l.states, a.cut_tiles = (int)l.cut_tiles;
   const hipStream_t s = (hipStream_t)stream;
   switch (c.dtype) {
     case kBf16: return launch_prompt_dim<kBf16>(a, c.head_dim, l, s);
