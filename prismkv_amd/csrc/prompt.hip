@@ -708,7 +708,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
                         make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]));
     return;
   }
-  if (it.state >= a.states) return;  // (never, while the offsets ascend)
+  if ((unsigned)it.state >= (unsigned)a.states) return;  // (never, while the offsets ascend)
   float* state = a.state + (size_t)it.state * kStateFloats<D>;
   if (half == 0) {
     state[row] = m;
@@ -741,7 +741,8 @@ __global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a)
     if (cut.chunks <= 1 || row0 >= rows) continue;  // (a tile of one chunk its workgroup has finished)
     // the states of chunk 0 and from chunk to chunk
     const int first = it.state + (it.s.tiles - 1 - it.tile) * it.most * a.kv_heads + it.h;
-    if (first + (cut.chunks - 1) * a.kv_heads >= a.states) continue;  // (never, while the offsets ascend)
+    if ((unsigned)first >= (unsigned)a.states || (int64_t)(cut.chunks - 1) * a.kv_heads >= a.states - first)
+      continue;  // (never, while the offsets ascend)
     const float* state = a.state + (size_t)first * kStateFloats<D>;
     const size_t step = (size_t)a.kv_heads * kStateFloats<D>;
     const bool valid = row0 + row < rows;
@@ -807,13 +808,13 @@ PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group,
   const int tokens = element_bytes(dtype) * head_dim > 256 ? 32 : 64;
   const int64_t tiles = (rows * group) / kTileRows + (sequences < rows ? sequences : rows), key_tiles = (slots + tokens - 1) / tokens;
   const int64_t all = 1ll << kItemsLog;
-  l.items = all + tiles * kv_heads;
   // A sequence that is cut has most = ceil(x) <= 2x chunks a tile, x > 1 its share of
   // an item: 2 all of them at most.
   const int64_t full = tiles * kv_heads * ((key_tiles + kLeastTiles - 1) / kLeastTiles);
   // Never cut: few slots; one sequence whose tiles are as many as the items are to be.
   const bool whole = key_tiles <= kLeastTiles + kCutSaves ||
                      (sequences == 1 && (rows * group + kTileRows - 1) / kTileRows * kv_heads >= all);
+  l.items = (whole ? 0 : all) + tiles * kv_heads;
   l.states = whole ? 0 : full < 2 * all ? full : 2 * all;
   l.cut_tiles = whole ? 0 : tiles * kv_heads < all ? tiles * kv_heads : all;
   l.bytes = (size_t)l.states * kTileRows * (head_dim + 2) * sizeof(float);
@@ -822,7 +823,7 @@ PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group,
 
 template <int DT, int D>
 int launch_prompt(const Prompt& a, const PromptLayout& l, hipStream_t stream) {
-  hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)l.items), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)(l.items ? l.items : 1)), dim3(kThreads), 0, stream, a);
   if (const int rc = (int)hipGetLastError()) return rc;
   if (!l.cut_tiles) return 0;
   // (few workgroups, each of every 64th tile: most launches find little to join; with one
