@@ -81,6 +81,7 @@ struct PromptPlan {
 
 template <int kTokens>
 __device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
+  if (!a.states) return PromptPlan{1, INT32_MAX};  // (nothing is cut)
   uint64_t sum = 0;
   int tiles = 0;
   for (int b = threadIdx.x & 63; b < a.sequences; b += 64) {
@@ -92,7 +93,7 @@ __device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
   const uint64_t share = (((high << 24) + low) * a.kv_heads >> kItemsLog) + 1;
   const int per_item = (int)(share < kLeastTiles ? kLeastTiles : share < (1u << 24) ? share : 1u << 24);
   // (tiles * kv_heads < 2^30, key tiles of a sequence < 2^26)
-  return PromptPlan{per_item, a.states ? per_item + kCutSaves + wave_sum_i(tiles) * a.kv_heads / kCutTiles : INT32_MAX};
+  return PromptPlan{per_item, per_item + kCutSaves + wave_sum_i(tiles) * a.kv_heads / kCutTiles};
 }
 
 // Item `index` of the launch: a tile of rows of sequence b and KV head h, chunk `chunk`
@@ -490,11 +491,15 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   const bool active = 32 * w < rows;
   if (from < to) {
     stage.ask(from * kTokens);
+    const int first_page = stage.page, first_token = stage.token;
+    stage.ask(min(from + 1, to - 1) * kTokens);
+    const int second_page = stage.page, second_token = stage.token;
+    stage.page = first_page, stage.token = first_token;
     stage.move();
     stage.issue_k(keys0);
-    stage.finish_k(keys0);
-    stage.ask(min(from + 1, to - 1) * kTokens);
+    stage.page = second_page, stage.token = second_token;
     stage.move();
+    stage.finish_k(keys0);
     stage.issue_v(values0);
     stage.issue_k(keys1);
     stage.finish_v(values0);
