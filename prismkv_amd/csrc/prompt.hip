@@ -35,6 +35,8 @@ constexpr int kItemsLog = 9, kLeastTiles = 4, kCutSaves = 4, kCutTiles = 16;
 template <int DT>
 constexpr float kLead = kType<DT> == kFp16 ? 0.f : 8.f;
 
+constexpr int kRawBuffer = 0x27000;  // a buffer resource's last word: 32-bit data, no swizzle
+
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -247,12 +249,18 @@ __device__ __forceinline__ u32x4 without_special(u32x4 x, bool& any) {
 // bytes straight there, or from 4 bits through registers, where they are widened.  Each
 // lane looks up one row's place, two tiles ahead, and the rows' readers take it from
 // there.  Rows past the end repeat the last one: no row sees them.
-template <int DT, int D>
+//
+// kGroups: the 64 / kC rows that a wave loads at once always lie in one page.  Then their
+// place is one scalar, and a buffer load from it has a lane's offset alone.  (Beside the
+// vector work that this saves: while a global load to LDS is on its way the compiler lets
+// no read of LDS pass another, and waits for all of them.)
+template <int DT, int D, bool kGroups>
 struct Stage {
   static constexpr int kTokens = kTileTokens<DT, D>;
   static constexpr int kC = D * kElem<DT> / 16;            // chunks of a row
   static constexpr int kEach = kTokens * kC / kThreads;    // chunks of a thread
   static constexpr int kRaw = kInFour<DT> ? kEach : 1;
+  static constexpr int kRows = 64 / kC;                    // rows of a wave's load
   typedef const __attribute__((address_space(1))) void* Global;
   typedef __attribute__((address_space(3))) void* Local;
   const Prompt& a;
@@ -284,6 +292,7 @@ struct Stage {
   static __device__ __forceinline__ int step(int i) { return i * (kThreads / kC); }
   __device__ __forceinline__ void ask(int t0) {
     token = min(t0 + (int)(threadIdx.x & (kTokens - 1)), end - 1);
+    if constexpr (kGroups) token &= -kRows;  // (the page has the rows behind the end that are loaded too)
     page = tab[a.div.of(token)];
   }
   __device__ __forceinline__ void move() {
@@ -295,7 +304,10 @@ struct Stage {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       v_at[i] = k_at[i];
-      k_at[i] = (unsigned)__shfl((int)place, row + step(i));
+      if constexpr (kGroups)
+        k_at[i] = (unsigned)__builtin_amdgcn_readlane((int)place, kRows * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + step(i));
+      else
+        k_at[i] = (unsigned)__shfl((int)place, row + step(i));
       if constexpr (kInFour<DT>) {
         v_scale_at[i] = k_scale_at[i];
         k_scale_at[i] = (unsigned)__shfl((int)scale_place, row + step(i));
@@ -308,10 +320,15 @@ struct Stage {
   }
   __device__ __forceinline__ void issue(const char* from, const unsigned (&at)[kEach], char* tile) const {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      __builtin_amdgcn_global_load_lds((Global)(from + ((size_t)at[i] << 4) + source(i)),
-                                       (Local)(tile + (64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + i * kThreads) * 16),
-                                       16, 0, 0);
+    for (int i = 0; i < kEach; ++i) {
+      const Local to = (Local)(tile + (64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + i * kThreads) * 16);
+      if constexpr (kGroups) {
+        const auto rows = __builtin_amdgcn_make_buffer_rsrc((void*)(from + ((size_t)at[i] << 4)), 0, -1, kRawBuffer);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, to, 16, (row & (kRows - 1)) * (int)(a.slot_units << 4) + source(i), 0, 0, 0);
+      } else {
+        __builtin_amdgcn_global_load_lds((Global)(from + ((size_t)at[i] << 4) + source(i)), to, 16, 0, 0);
+      }
+    }
   }
   __device__ __forceinline__ void issue_k(char* tile) {
     if constexpr (kInFour<DT>) {
@@ -416,7 +433,7 @@ constexpr int kStateFloats = kTileRows * (D + 2);
 // operand of O^T = V^T P^T as they stand, the tokens being summed in the order in which
 // they lie in registers (8 (r / 4) + 4 (lane / 32) + r % 4).  V^T comes out of LDS by
 // transposing reads.
-template <int DT, int D>
+template <int DT, int D, bool kGroups>
 __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(Prompt a) {
   constexpr int kTokens = kTileTokens<DT, D>, kT = kTokens / 32;
   constexpr int kC = D * kElem<DT> / 16;  // 16-byte chunks of a row; half as many steps of the product (fp32: of four)
@@ -466,7 +483,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   float m = -INFINITY, z = 0.f;  // the row's maximum (exp2 domain), this lane's share of its sum
 
   const int from = it.chunk * cut.each, to = min(from + cut.each, cut.tiles);
-  Stage<DT, D> stage(a, it.b, it.h, cut.end);
+  Stage<DT, D, kGroups> stage(a, it.b, it.h, cut.end);
   f32x16 s[kT];  // the scores of the tile at hand
   auto scores = [&](f32x16 (&s)[kT], const char* keys) {
 #pragma unroll
@@ -828,7 +845,11 @@ PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group,
 
 template <int DT, int D>
 int launch_prompt(const Prompt& a, const PromptLayout& l, hipStream_t stream) {
-  hipLaunchKernelGGL((prompt_kernel<DT, D>), dim3((unsigned)(l.items ? l.items : 1)), dim3(kThreads), 0, stream, a);
+  constexpr int kRow = D * kElem<DT>, kRows = 1024 / kRow;  // of a wave's load
+  auto kernel = prompt_kernel<DT, D, !kInFour<DT> && kRows == 1>;
+  if constexpr (!kInFour<DT> && kRows > 1)
+    if (a.page_size % kRows == 0 && a.slot_units <= (INT32_MAX / 16 - 64) / (kRows - 1)) kernel = prompt_kernel<DT, D, true>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(l.items ? l.items : 1)), dim3(kThreads), 0, stream, a);
   if (const int rc = (int)hipGetLastError()) return rc;
   if (!l.cut_tiles) return 0;
   // (few workgroups, each of every 64th tile: most launches find little to join; with one
