@@ -18,16 +18,22 @@ constexpr int kWaves = 4, kTileRows = 32 * kWaves, kThreads = 64 * kWaves;
 // Keys and values that are staged at a time.
 template <int DT, int D>
 constexpr int kTileTokens = kElem<DT> * D > 256 ? 32 : 64;
-// Waves of a SIMD, by the registers that products, queries and staged rows take.
+// Waves of a SIMD, by the registers that products, queries and staged rows take.  (Three
+// for head_dim 64 in 16 bits; the widening from 4 bits has no room for that: 2000 rows over
+// 4000 slots 87 us, with two 82.)
 template <int DT, int D>
-constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : 2;
+constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : kElem<DT> * D == 128 && !kInFour<DT> ? 3 : 2;
 // The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, but
 // no item is less than kLeastTiles tiles of keys.  Twice as many items are slower (2048
 // rows of 8 x 4 heads 92 us against 60, 48 rows over 65000 slots 116 against 94).  A sequence
 // is cut only where that saves its longest tile more tiles of keys than the states and
-// their join take: kCutSaves and one for every kCutTiles tiles of rows (16 rows over 1016
-// slots cut 16 us, whole 28; 1500 rows cut 61, whole 45; 64 x 64 rows over 2000 slots each 73 and 61).
-constexpr int kItemsLog = 9, kLeastTiles = 4, kCutSaves = 4, kCutTiles = 16;
+// their join take: cut_saves and one for every cut_tiles tiles of rows (16 rows over 1016
+// slots cut 16 us, whole 28; 1500 rows cut 61, whole 45; 64 x 64 rows over 2000 slots each 73
+// and 61).  A tile of fp32 takes longer (300 rows cut 38 us, whole 56; 1000 rows of head_dim 64
+// cut 88, whole 80).
+constexpr int kItemsLog = 9, kLeastTiles = 4;
+constexpr int cut_saves(int dtype) { return (dtype & 15) == kFp32 ? 2 : 4; }
+constexpr int cut_tiles(int dtype) { return (dtype & 15) == kFp32 ? 24 : 16; }
 
 // By how much (in powers of 2) a row's largest score may pass the maximum that its weights
 // are taken from before what was summed so far is multiplied anew: nearly every tile raises
@@ -81,7 +87,7 @@ struct PromptPlan {
   int per_item, whole;
 };
 
-template <int kTokens>
+template <int DT, int kTokens>
 __device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
   if (!a.states) return PromptPlan{1, INT32_MAX};  // (nothing is cut)
   uint64_t sum = 0;
@@ -95,7 +101,7 @@ __device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
   const uint64_t share = (((high << 24) + low) * a.kv_heads >> kItemsLog) + 1;
   const int per_item = (int)(share < kLeastTiles ? kLeastTiles : share < (1u << 24) ? share : 1u << 24);
   // (tiles * kv_heads < 2^30, key tiles of a sequence < 2^26)
-  return PromptPlan{per_item, per_item + kCutSaves + wave_sum_i(tiles) * a.kv_heads / kCutTiles};
+  return PromptPlan{per_item, per_item + cut_saves(DT) + wave_sum_i(tiles) * a.kv_heads / cut_tiles(DT)};
 }
 
 // Item `index` of the launch: a tile of rows of sequence b and KV head h, chunk `chunk`
@@ -190,12 +196,13 @@ struct ValueAt {  // chunk 4d + 2 side + (in >> 1 & 1) of row 32i + 16u + 8 hi +
     else return (lane ^ (4 * (d & 1) << 4)) + rows + (8 * ((d >> 1 & 1) ^ hi) + 16 * (d >> 2)) * 16;
   }
 };
-template <int kC>
-struct FloatAt {  // element 32d + col of row 32i + 8 (r / 4) + 4 half + r % 4, in fp32
+template <int kC, int kVec>
+struct FloatsAt {  // fp32 elements 32 kVec g + kVec col .. of row 32i + 8 (r / 4) + 4 half + r % 4
   int lane;
-  __device__ __forceinline__ FloatAt(int col, int half) : lane(staged<kC>(4 * half, col >> 2) + 4 * (col & 3)) {}
-  __device__ __forceinline__ int of(int i, int r, int d) const {
-    return (lane ^ ((r % 4) << 5)) + ((32 * i + 8 * (r / 4) + r % 4) * kC + 8 * ((d ^ (r / 4)) & 1) + 16 * (d >> 1)) * 16;
+  __device__ __forceinline__ FloatsAt(int col, int half)
+      : lane(staged<kC>(4 * half, col * kVec / 4) + 4 * (col * kVec & 3)) {}
+  __device__ __forceinline__ int of(int i, int r, int g) const {
+    return (lane ^ ((r % 4 << 1 | (r / 4 & 1) << 3) << 4)) + ((32 * i + 8 * (r / 4) + r % 4) * kC + 8 * kVec * g) * 16;
   }
 };
 
@@ -252,8 +259,9 @@ __device__ __forceinline__ u32x4 without_special(u32x4 x, bool& any) {
 //
 // kGroups: the 64 / kC rows that a wave loads at once always lie in one page.  Then their
 // place is one scalar, and a buffer load from it has a lane's offset alone.  (Beside the
-// vector work that this saves: while a global load to LDS is on its way the compiler lets
-// no read of LDS pass another, and waits for all of them.)
+// vector work that this saves: while a global load to LDS is on its way the compiler waits
+// for all reads of LDS at once.  4000 rows over pages of 64 slots 148 us, of 31 slots 156;
+// of head_dim 256 359 and 411.)
 template <int DT, int D, bool kGroups>
 struct Stage {
   static constexpr int kTokens = kTileTokens<DT, D>;
@@ -318,9 +326,9 @@ struct Stage {
   __device__ __forceinline__ int source(int i) const {
     return (staged<kC>(row + step(i), chunk) & (16 * kC - 1));
   }
-  __device__ __forceinline__ void issue(const char* from, const unsigned (&at)[kEach], char* tile) const {
+  __device__ __forceinline__ void issue(const char* from, const unsigned (&at)[kEach], char* tile, int i0 = 0, int i1 = kEach) const {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = i0; i < i1; ++i) {
       const Local to = (Local)(tile + (64 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + i * kThreads) * 16);
       if constexpr (kGroups) {
         const auto rows = __builtin_amdgcn_make_buffer_rsrc((void*)(from + ((size_t)at[i] << 4)), 0, -1, kRawBuffer);
@@ -438,6 +446,10 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   constexpr int kTokens = kTileTokens<DT, D>, kT = kTokens / 32;
   constexpr int kC = D * kElem<DT> / 16;  // 16-byte chunks of a row; half as many steps of the product (fp32: of four)
   constexpr int kTile = kTokens * kC * 16;  // bytes
+  // Whether the next tiles' loads are issued between the products (fp32 prompts 1190 us, so
+  // 1159; 16384 rows of head_dim 128 2052 and 2012) or before them (head_dim 64 97 and 91;
+  // 256 366 and 360).
+  constexpr bool kLate = kGroups && (kType<DT> == kFp32 || D == 128);
   __shared__ __attribute__((aligned(16))) char keys0[kTile], keys1[kTile], values0[kTile], values1[kTile];
   if (blockIdx.x == 0 && a.offsets)
     for (int b = threadIdx.x; b < a.sequences; b += kThreads) {
@@ -445,7 +457,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       if (from > to || (b == 0 && from) || (b == a.sequences - 1 && to != a.rows))
         report_error(a.err, error_host_slot(a.err), kErrOffsets);
     }
-  const PromptPlan plan = prompt_plan<kTokens>(a);
+  const PromptPlan plan = prompt_plan<DT, kTokens>(a);
   PromptItem it;
   if (!find_item<kTokens>(a, plan, blockIdx.x, false, it)) return;
   const PromptCut<kTokens> cut(a, it, plan);
@@ -480,6 +492,26 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  // A lane's sums, four neighbouring dims at a time: row i of product d is dim 32d + i or,
+  // in fp32, 32 kVec (d / kVec) + kVec i + d % kVec.
+  constexpr int kVec = D >= 128 ? 4 : 2;
+  struct Place {
+    int d, r;
+  };
+  auto place = [](int n, int e) {
+    if constexpr (kType<DT> != kFp32) return Place{n / 4, n % 4 * 4 + e};
+    else if constexpr (kVec == 4) return Place{n / 16 * 4 + e, n % 16};
+    else return Place{e % 2, 2 * n + e / 2};
+  };
+  auto four = [&](int n) {
+    const Place x = place(n, 0), y = place(n, 1), u = place(n, 2), w = place(n, 3);
+    return make_float4(acc[x.d][x.r], acc[y.d][y.r], acc[u.d][u.r], acc[w.d][w.r]);
+  };
+  auto four_dim = [&](int n) {
+    if constexpr (kType<DT> != kFp32) return 8 * n + 4 * half;
+    else if constexpr (kVec == 4) return n / 16 * 128 + 4 * (8 * (n % 16 / 4) + 4 * half + n % 4);
+    else return 2 * (8 * (n / 2) + 4 * half + 2 * (n % 2));
+  };
   float m = -INFINITY, z = 0.f;  // the row's maximum (exp2 domain), this lane's share of its sum
 
   const int from = it.chunk * cut.each, to = min(from + cut.each, cut.tiles);
@@ -540,10 +572,15 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       special |= stage.clean(values);
       __syncthreads();
     }
-    if (t + 1 < to) {
+    if (!kLate && t + 1 < to) {
       stage.issue_v(next_values);
       stage.issue_k(later_keys);  // (the last one again, behind the last)
       stage.ask(min(t + 3, to - 1) * kTokens);
+    }
+    if (kLate) stage.ask(min(t + 3, to - 1) * kTokens);
+    if (kLate && !active) {
+      stage.issue_v(next_values);
+      stage.issue_k(later_keys);
     }
     if (active) {
       mask(s, t0);
@@ -593,7 +630,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       // before the products that wait for it): the reads are kAhead products ahead, and
       // the exponentials between the first products, the sum between the others.  (The
       // next scores are of no tile, behind the last.)
-      constexpr int kSteps = kC / 2, kAhead = 3;
+      constexpr int kSteps = kC / 2, kAhead = kC == 8 ? 2 : 3;  // (4000 rows of head_dim 64 with 3: 98 us, 2: 92)
       u32x4 kf[kAhead][kT];
       auto read_k = [&](int c) {
 #pragma unroll
@@ -611,15 +648,33 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
         for (int i = 0; i < kT; ++i) next[i] = mfma_rows<DT>(kf[c % kAhead][i], q[c], next[i]);
 #pragma unroll
         for (int e = c * 16 * kT / kSteps; e < (c + 1) * 16 * kT / kSteps; ++e) exponential(e);
+        if constexpr (kLate) {
+          constexpr int kE = Stage<DT, D, kGroups>::kEach;
+          constexpr int kPer = (2 * kE + kSteps - 1) / kSteps;
+#pragma unroll
+          for (int x = c * kPer; x < (c + 1) * kPer; ++x) {
+            if (x < kE) stage.issue(stage.v, stage.v_at, next_values, x, x + 1);
+            else if (x < 2 * kE) stage.issue(stage.k, stage.k_at, later_keys, x - kE, x - kE + 1);
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       };
       if constexpr (kType<DT> == kFp32) {
-        const FloatAt<kC> float_at(col, half);
-        constexpr int kCols = D / 32, kPv = 16 * kT * kCols, kVAhead = 6;
-        float vf[kVAhead + 1];
+        // A lane reads kVec dims at once, each for a product of its own (one dim at a time a
+        // product takes 87 cycles, not 64: 4097 rows of head_dim 256 1163 us, so 1033)
+        const FloatsAt<kC, kVec> floats_at(col, half);
+        constexpr int kOf = D / (32 * kVec), kReads = 16 * kT * kOf, kVAhead = 2;
+        float vf[kVAhead + 1][kVec];
         auto read_v = [&](int j) {
-          vf[j % (kVAhead + 1)] =
-              *reinterpret_cast<const float*>(values + float_at.of(j / (16 * kCols), j / kCols % 16, j % kCols));
+          const char* from = values + floats_at.of(j / (16 * kOf), j / kOf % 16, j % kOf);
+          if constexpr (kVec == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(from);
+            vf[j % (kVAhead + 1)][0] = x.x, vf[j % (kVAhead + 1)][1] = x.y;
+            vf[j % (kVAhead + 1)][2] = x.z, vf[j % (kVAhead + 1)][3] = x.w;
+          } else {
+            const float2 x = *reinterpret_cast<const float2*>(from);
+            vf[j % (kVAhead + 1)][0] = x.x, vf[j % (kVAhead + 1)][1] = x.y;
+          }
         };
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
@@ -629,11 +684,14 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
 #pragma unroll
         for (int j = 0; j < kVAhead; ++j) read_v(j);
 #pragma unroll
-        for (int j = 0; j < kPv; ++j) {
-          if (j + kVAhead < kPv) read_v(j + kVAhead);
-          const float p = s[j / (16 * kCols)][j / kCols % 16];
-          acc[j % kCols] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[j % (kVAhead + 1)], p, acc[j % kCols], 0, 0, 0);
-          if (j % kCols == 0) z += p;
+        for (int j = 0; j < kReads; ++j) {
+          if (j + kVAhead < kReads) read_v(j + kVAhead);
+          const float p = s[j / (16 * kOf)][j / kOf % 16];
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            acc[j % kOf * kVec + e] =
+                __builtin_amdgcn_mfma_f32_32x32x2f32(vf[j % (kVAhead + 1)][e], p, acc[j % kOf * kVec + e], 0, 0, 0);
+          if (j % kOf == 0) z += p;
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
@@ -704,16 +762,13 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
 #pragma unroll 1
       for (int k = 0; k < kTokens && t * kTokens + k <= limit; ++k)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+        for (int n = 0; n < D / 8; ++n) {
+          const int byte = four_dim(n) * kElem<DT>;
+          const float4 x = four_of<DT>(values + staged<kC>(k, byte >> 4) + (byte & 15));
+          const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int byte = (32 * d + 8 * j + 4 * half) * kElem<DT>;
-            const float4 x = four_of<DT>(values + staged<kC>(k, byte >> 4) + (byte & 15));
-            acc[d][4 * j] += fabsf(x.x) < INFINITY ? 0.f : x.x;
-            acc[d][4 * j + 1] += fabsf(x.y) < INFINITY ? 0.f : x.y;
-            acc[d][4 * j + 2] += fabsf(x.z) < INFINITY ? 0.f : x.z;
-            acc[d][4 * j + 3] += fabsf(x.w) < INFINITY ? 0.f : x.w;
-          }
+          for (int e = 0; e < 4; ++e) acc[place(n, e).d][place(n, e).r] += fabsf(y[e]) < INFINITY ? 0.f : y[e];
+        }
     }
   }
   if (__ballot(stage.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
@@ -723,11 +778,8 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   if (cut.chunks <= 1) {
     if (a.lse && half == 0) a.lse[row_head] = prompt_lse<DT>(m, z);
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        put_four<DT, D>(a, row_head, 32 * d + 8 * j + 4 * half, z,
-                        make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]));
+    for (int n = 0; n < D / 8; ++n)
+      put_four<DT, D>(a, row_head, four_dim(n), z, four(n));
     return;
   }
   if ((unsigned)it.state >= (unsigned)a.states) return;  // (never, while the offsets ascend)
@@ -738,11 +790,8 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   }
   float4* products = reinterpret_cast<float4*>(state + 2 * kTileRows);
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      products[(8 * d + 2 * j + half) * kTileRows + row] =
-          make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
+  for (int n = 0; n < D / 8; ++n)
+    products[four_dim(n) / 4 * kTileRows + row] = four(n);
 }
 
 // Joins the states of tiles whose keys were cut, in the order of their tokens: a
@@ -754,7 +803,7 @@ template <int DT, int D>
 __global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a) {
   constexpr int kTokens = kTileTokens<DT, D>, kLanes = D / 4, kU = 8;
   __shared__ float factors[kLanes][kJoinRows], parts[kLanes][kJoinRows];
-  const PromptPlan plan = prompt_plan<kTokens>(a);
+  const PromptPlan plan = prompt_plan<DT, kTokens>(a);
   const int row0 = blockIdx.y * kJoinRows, row = threadIdx.x % kJoinRows, quad = threadIdx.x / kJoinRows;
   PromptItem it;
   for (int tile = blockIdx.x; tile < a.cut_tiles && find_item<kTokens>(a, plan, tile, true, it); tile += gridDim.x) {
@@ -834,7 +883,7 @@ PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group,
   // an item: 2 all of them at most.
   const int64_t full = tiles * kv_heads * ((key_tiles + kLeastTiles - 1) / kLeastTiles);
   // Never cut: few slots; one sequence whose tiles are as many as the items are to be.
-  const bool whole = key_tiles <= kLeastTiles + kCutSaves ||
+  const bool whole = key_tiles <= kLeastTiles + cut_saves(dtype) ||
                      (sequences == 1 && (rows * group + kTileRows - 1) / kTileRows * kv_heads >= all);
   l.items = (whole ? 0 : all) + tiles * kv_heads;
   l.states = whole ? 0 : full < 2 * all ? full : 2 * all;
