@@ -146,3 +146,30 @@ def test_a_prompt_of_one_row_each_is_attend():
         out = cache.attend_prompt(q.cuda())
         check_prompt(q, host, [5, 77, 3000], [1, 1, 1], out)
         check_prompt(q, host, [5, 77, 3000], [1, 1, 1], cache.attend(q.cuda()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lengths,new", [([230, 61], [90, 61]), ([1300], [10])])
+def test_pages_of_every_size_give_the_same(lengths, new, dim, dtype):
+    """Rows that a wave loads at once lie in one page or in several: no result tells."""
+    gen = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(sum(lengths), 2, dim, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(sum(new), 6, dim, generator=gen).to(dtype).cuda()
+    v[lengths[0] - 4, 0, 5] = math.inf
+    v[lengths[0] - 6, 1, dim - 1] = math.nan
+    k[lengths[0] - 2, 1, 7] = math.nan
+    want = None
+    for page in (64, 1, 2, 5, 12, 24):
+        cache = PagedCache(len(lengths), sum(-(-n // page) for n in lengths) + 3, -(-max(lengths) // page), page_size=page,
+                           kv_heads=2, head_dim=dim, dtype=dtype)
+        for x in (cache.k, cache.v):
+            x.fill_(math.nan)
+        cache.reserve(lengths)
+        cache.append(k.cuda(), v.cuda(), ends(lengths))
+        lse = torch.empty(sum(new), 6, device="cuda")
+        got = cache.attend_prompt(q, ends(new), lse=lse), lse
+        cache.check_errors()
+        want = got if want is None else want
+        torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True, msg=f"pages of {page}")
+    assert want[0].isnan().any() and not want[0].isnan().all()
