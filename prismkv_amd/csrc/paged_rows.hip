@@ -14,10 +14,15 @@ namespace {
 // each: the angles' sines are computed once for a row (in LDS) and used by all of its
 // heads.  The angle is an integer, 2^-64 of a turn: position times turns[j] modulo 2^64
 // is exact for any position, where a product in fp32 is off by 0.06 radians at 10^6.
+// Measured: 20011 rows of 32 + 8 + 8 heads of 64 in fp16, 47.4 us = 5.2 TB/s of what is
+// read and written; one row for each of 128 sequences, 32 + 8 + 8 heads of 128, 5.6 us, most
+// of it the launch and the chain lengths -> page -> store.
 //
 // In 4 bits 32 dims share a scale: a thread has 8 dims, so the largest of four
 // neighbouring lanes' is the block's, and the conversion instruction divides, rounds
-// (ties to even) and saturates.
+// (ties to even) and saturates.  Measured: 20011 rows of 8 heads of 128, k and v, 29.2 us =
+// 3.6 TB/s; bound by the latency of a row's reads.  Four items' loads in flight for a thread
+// were slower (with a read of all after it 54 us against 51; turned 58 against 47).
 
 constexpr int kRowsEach = 8;   // packed rows of a workgroup
 constexpr int64_t kLaunchRows = 1 << 26;  // (a launch has fewer than 2^32 threads: 2^27 rows)
@@ -273,7 +278,8 @@ __global__ __launch_bounds__(kPT) void paged_rows_advance_kernel(PagedRows a) {
 // ------------------------------------------------------------------ read
 
 // The rows of the sequences' last slots, widened from 4 bits (exactly) or copied: bound
-// by reading and writing them; a thread has 8 dims of a row's key and value.
+// by reading and writing them; a thread has 8 dims of a row's key and value.  Measured: 20011
+// rows of 8 heads of 128 out of 4 bits 19.4 us = 5.3 TB/s.
 struct PagedRead {
   const char *kp, *vp;
   const uint8_t *ks, *vs;
