@@ -633,8 +633,10 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       // The order of the instructions is this one (the compiler's own has LDS read right
       // before the products that wait for it): the reads are kAhead products ahead, and
       // the exponentials between the first products, the sum between the others.  (The
-      // next scores are of no tile, behind the last.)
-      constexpr int kSteps = kC / 2, kAhead = kC == 8 ? 2 : 3;  // (4000 rows of head_dim 64 with 3: 98 us, 2: 92)
+      // next scores are of no tile, behind the last.  kAhead: by the registers that are left;
+      // 4000 rows of head_dim 64 98 us with 3, 92 with 2, of 128 2047 and 2070 for 16384, over
+      // 4-bit pages 939 and 932 for 6007 rows.)
+      constexpr int kSteps = kC / 2, kAhead = kC == 8 || (kInFour<DT> && D == 128) ? 2 : 3;
       u32x4 kf[kAhead][kT];
       auto read_k = [&](int c) {
 #pragma unroll
