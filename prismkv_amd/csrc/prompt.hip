@@ -8,8 +8,8 @@
 // bytes for a slot and 128 rows: the matrix products bound it, unless the rows are few.
 // Measured: 16384 rows of 8 x 4 heads of 128 in bf16 2092 us = 1.05 PFLOP/s (a product of
 // 8192^3 reaches 1.12); 48 rows over 65048 slots 89 us = 574 TFLOP/s and 3.0 TB/s; fp16,
-// head_dim 64, 9 ragged sequences of 1.0K rows 150 us = 511; fp32, head_dim 256, 4097 rows
-// 1035 us = 96 (of 153); over 4-bit pages 6007 rows over 5 x 9K slots 953 us = 912.
+// head_dim 64, 9 ragged sequences of 1.0K rows 147 us = 524; fp32, head_dim 256, 4097 rows
+// 1035 us = 96 (of 153); over 4-bit pages 6007 rows over 5 x 9K slots 926 us = 939.
 #include <cfloat>
 #include <type_traits>
 
