@@ -85,7 +85,11 @@ def prompt(q, k, v, new, dtype=None, scale=None):
 
     As for `attend`, and P is rounded once to q's type (half a step, `half`, of
     each weight; fp16 weights below 2^-29 of the largest, and at least 2^-39 of
-    it, by 2^-39 more), which fp32 is not."""
+    it, by 2^-39 more), which fp32 is not.  A row is divided by the sum of what was not
+    rounded but for its largest weight (in fp16 that is a power of two): with p_t
+    (1 + e_t) in place of p_t the output is off by the sum of p_t e_t v_t, of which the
+    largest's is p_k e_k (v_k - out), over 1 + p_k e_k.  k is any slot whose score the
+    device may find the largest, and none where scores pass 2^22."""
     m, heads, D = q.shape
     H, n = k.shape[0], k.shape[1]
     scale = 1 / math.sqrt(D) if scale is None else scale
@@ -103,8 +107,16 @@ def prompt(q, k, v, new, dtype=None, scale=None):
         p[torch.isinf(lse[:, g])] = 0
         out[:, g] = p @ vd
         rel = 2 * delta + 2.0 ** -20 + n * 2.0 ** -24
-        rounded, least = (0, 0) if dtype == torch.float32 else (half, 2.0 ** -38 if dtype == torch.float16 else 0)
-        lost = (p @ vd.abs()) * (rel[:, None] + rounded) + least * p.amax(-1)[:, None] * ((~later).double() @ vd.abs())
+        lost = (p @ vd.abs()) * rel[:, None]
+        if dtype != torch.float32:
+            rounded = p @ vd.abs()
+            for i in range(m):
+                if p[i].amax() > 0 and s[i].amax().abs() < 2.0 ** 21:
+                    best = s[i] >= s[i].amax() - 2 * delta[i]
+                    rounded[i] += (p[i, best, None] * ((vd[best] - out[i, g]).abs() - vd[best].abs())).amax(0)
+            lost += rounded * half / (1 - half)
+        if dtype == torch.float16:
+            lost += 2.0 ** -38 * p.amax(-1)[:, None] * ((~later).double() @ vd.abs())
         floor = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}[dtype]
         bound[:, g] = out[:, g].abs() * half + lost * (1 + half) + floor
         lse_bound[:, g] = delta + 2.0 ** -20 + n * 2.0 ** -24 + lse[:, g].abs() * 2.0 ** -22

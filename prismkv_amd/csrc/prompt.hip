@@ -225,9 +225,12 @@ __device__ __forceinline__ f32x16 mfma_rows(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // Two probabilities as a word of the 16-bit type, rounded to nearest: half a step of
-// the type relative to each, which their product with V averages out to less than the
-// output's own rounding.  fp16 takes its least number for what is below it, so that an
-// infinite V is not multiplied by 0 (2^-39 of the largest weight, with the bias).
+// the type relative to each, where two or three terms would take as many products with V
+// again (`attend` has them).  Over many slots of normal V that is 0.0016 of the output in
+// bf16, whose own rounding is 0.0017 (fp16 0.00015 and 0.00021).  The row's sum is of what
+// was not rounded, but for its largest weight (share_largest).  fp16 takes its least number
+// for what is below it, so that an infinite V is not multiplied by 0 (2^-39 of the largest
+// weight, with the bias).
 template <int DT>
 __device__ __forceinline__ unsigned pack2(float a, float b) {
   if constexpr (kType<DT> == kBf16) {
@@ -435,6 +438,25 @@ __device__ __forceinline__ float state_factor(float m, float M) {
   return m == -INFINITY ? 0.f : m == M ? 1.f : exp2f(m - M);
 }
 
+// Whether the largest weight of a row is rounded: not where it is 1 (2^kBias).
+template <int DT>
+constexpr bool kShared = kType<DT> == kBf16;
+
+// What the sums of a row are multiplied by before they are divided by its sum z: that with
+// its largest weight as V was multiplied by it, so that a slot that outweighs all others
+// comes back as its V (without, off by up to 2^-8, the same for every dim).  `top` is that
+// slot's score and `at` the maximum that its weight was taken from, `m` the last one.  (The
+// sum of all rounded weights, by two-element products of the words, is little better, 0.0014
+// for 0.0016 above, and takes longer: 16384 rows 2155 us against 2040.  From 2^22 on a
+// maximum's weights are taken otherwise, of scores that are off by 1/4 and more.)
+template <int DT>
+__device__ __forceinline__ float share_largest(float top, float at, float m, float scale, float z) {
+  const float p = __builtin_amdgcn_exp2f(fmaf(top, scale, (float)kBias<DT> - at));
+  const float error = __uint_as_float(pack2<DT>(p, 0.f) << 16) / p - 1.f;
+  const float sum = z + error * __builtin_amdgcn_exp2f(fmaf(top, scale, (float)kBias<DT> - m));
+  return fabsf(at) < 0x1p22f ? z / sum : 1.f;
+}
+
 // A state: maxima and sums [2][128], then the products [D / 4][128] of four dims.
 template <int D>
 constexpr int kStateFloats = kTileRows * (D + 2);
@@ -516,7 +538,9 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
     else if constexpr (kVec == 4) return n / 16 * 128 + 4 * (8 * (n % 16 / 4) + 4 * half + n % 4);
     else return 2 * (8 * (n / 2) + 4 * half + 2 * (n % 2));
   };
-  float m = -INFINITY, z = 0.f;  // the row's maximum (exp2 domain), this lane's share of its sum
+  // The maximum (exp2 domain) that the row's weights are taken from, this lane's share of
+  // its sum; its largest score, and the maximum that this one's weight was taken from.
+  float m = -INFINITY, z = 0.f, top = -INFINITY, top_at = -INFINITY;
 
   const int from = it.chunk * cut.each, to = min(from + cut.each, cut.tiles);
   Stage<DT, D, kGroups> stage(a, it.b, it.h, cut.end);
@@ -594,7 +618,8 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       for (int i = 0; i < kT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) most = fmaxf(most, s[i][r]);
-      most = fmaxf(most, xor32(most)) * a.scale;
+      const float peak = fmaxf(most, xor32(most));
+      most = peak * a.scale;
       if (__ballot(most > m + kLead<DT>)) {
         const float nm = fmaxf(m, most);
         const float alpha = state_factor(m, nm);
@@ -604,6 +629,10 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
+      }
+      if constexpr (kShared<DT>) {
+        top_at = peak > top ? m : top_at;
+        top = fmaxf(top, peak);
       }
       float scale = a.scale, shift = m == -INFINITY ? (float)kBias<DT> : (float)kBias<DT> - m;
       // From 2^22 on the maximum's own rounding is 1/8 and more (at 2^32 it takes all of
@@ -780,6 +809,13 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   if (__ballot(stage.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
 
   z += xor32(z);
+  if constexpr (kShared<DT>) {
+    const float share = share_largest<DT>(top, top_at, m, a.scale, z);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= share;
+  }
   if (!valid) return;
   if (cut.chunks <= 1) {
     if (a.lse && half == 0) a.lse[row_head] = prompt_lse<DT>(m, z);
