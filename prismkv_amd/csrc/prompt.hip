@@ -910,6 +910,11 @@ __global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a)
   }
 }
 
+// Tiles of rows of one KV head at most, however the rows are dealt to the sequences.
+int64_t most_tiles(int64_t rows, int sequences, int group) {
+  return rows * group / kTileRows + (sequences < rows ? sequences : rows);
+}
+
 // Work items, states and cut tiles of a launch at most.
 struct PromptLayout {
   int64_t items, states, cut_tiles;
@@ -919,7 +924,7 @@ struct PromptLayout {
 PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots, int dtype) {
   PromptLayout l;
   const int tokens = element_bytes(dtype) * head_dim > 256 ? 32 : 64;
-  const int64_t tiles = (rows * group) / kTileRows + (sequences < rows ? sequences : rows), key_tiles = (slots + tokens - 1) / tokens;
+  const int64_t tiles = most_tiles(rows, sequences, group), key_tiles = (slots + tokens - 1) / tokens;
   const int64_t all = 1ll << kItemsLog;
   // A sequence that is cut has most = ceil(x) <= 2x chunks a tile, x > 1 its share of
   // an item: 2 all of them at most.
@@ -958,10 +963,10 @@ int launch_prompt_dim(const Prompt& a, int head_dim, const PromptLayout& l, hipS
   return launch_prompt<DT, 256>(a, l, stream);
 }
 
+// Rows times the group are counted in 32 bits, and a launch has fewer than 2^32 threads.
 bool prompt_fits(int64_t rows, int sequences, int kv_heads, int group) {
-  // (rows of a tile's index, items and states are counted in 32 bits)
   return rows >= 0 && group >= 1 && group <= 1024 && rows <= (1 << 30) / group &&
-         (rows * group / kTileRows + sequences) * kv_heads < 1 << 30;
+         most_tiles(rows, sequences, group) * kv_heads + (1 << kItemsLog) < (1ll << 32) / kThreads;
 }
 
 }  // namespace

@@ -585,7 +585,8 @@ class PagedCache:
             nbytes = self.lib.query("prismkv_paged_prompt_work_bytes", rows, sequences, kv_heads, group, head_dim, self.slots,
                                     self._desc.dtype)
             if not nbytes:
-                raise NotImplementedError("at most 2^30 rows of a prompt times the query heads of a KV head")
+                raise NotImplementedError("at most 2^30 rows of a prompt times the query heads of a KV head, and less than 2^24 "
+                                          "blocks of 128 of them (of every KV head; one more for each sequence)")
             # sizes of powers of two, each kept: a captured graph goes on using its own
             size = 1 << (nbytes - 1).bit_length()
             work = self._prompt_work.get(size)

@@ -105,6 +105,25 @@ def test_refused_prompts(lib):  # noqa: F811
         assert query(*bad) == 0, bad
 
 
+def test_prompts_of_more_blocks_than_a_launch_holds(lib):  # noqa: F811
+    """Workgroups of 256 threads, of which a launch has fewer than 2^32: 512 for what is cut,
+    and one for each KV head, 128 rows of one and sequence that has some."""
+    def need(rows, sequences, kv_heads, group):
+        return lib.query("prismkv_paged_prompt_work_bytes", rows, sequences, kv_heads, group, 64, 16, 0)
+
+    most = 2 ** 24 - 512
+    assert need(65535, 65535, 250, 1) and need(65535, 65535, 257, 1) == 0
+    many = desc(sequences=65535, kv_heads=257, max_pages=1)
+    assert prompt(lib, many, count=65535, group=1) == -1
+    assert passes(prompt(lib, desc(sequences=65535, kv_heads=250, max_pages=1), count=65535, group=1))
+    for kv_heads, group in ((8, 4), (16, 1), (3, 7)):
+        rows = ((most - 1) // kv_heads - 1) * 128 // group
+        assert (rows * group // 128 + 1) * kv_heads < most and need(rows, 1, kv_heads, group)
+        rows = (-(-most // kv_heads) - 1) * 128 // group + 128
+        assert need(rows, 1, kv_heads, group) == 0
+    assert need(5, 65535, 65535, 1)  # (no more tiles than rows)
+
+
 def test_the_descriptor_mirrors_the_header():
     import re
     from pathlib import Path
