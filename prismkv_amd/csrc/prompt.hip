@@ -14,31 +14,20 @@
 #include <type_traits>
 
 #include "paged_host.h"
+#include "prompt_plan.h"
 
 namespace prismkv {
 namespace {
 
-constexpr int kWaves = 4, kTileRows = 32 * kWaves, kThreads = 64 * kWaves;
+constexpr int kWaves = kTileRows / 32, kThreads = 64 * kWaves;
 // Keys and values that are staged at a time.
 template <int DT, int D>
-constexpr int kTileTokens = kElem<DT> * D > 256 ? 32 : 64;
+constexpr int kTileTokens = tile_tokens(kElem<DT> * D);
 // Waves of a SIMD, by the registers that products, queries and staged rows take.  (Three
 // for head_dim 64 in 16 bits; the widening from 4 bits has no room for that: 2000 rows over
 // 4000 slots 87 us, with two 82.)
 template <int DT, int D>
 constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : kElem<DT> * D == 128 && !kInFour<DT> ? 3 : 2;
-// The work of all tiles is cut so that no item is more than 1 / 2^kItemsLog of it, but
-// no item is less than kLeastTiles tiles of keys.  Twice as many items are slower (2048
-// rows of 8 x 4 heads 92 us against 60, 48 rows over 65000 slots 116 against 94).  A sequence
-// is cut only where that saves its longest tile more tiles of keys than the states and
-// their join take: cut_saves and one for every cut_tiles tiles of rows (16 rows over 1016
-// slots cut 16 us, whole 28; 1500 rows cut 61, whole 45; 64 x 64 rows over 2000 slots each 73
-// and 61).  A tile of fp32 takes longer (300 rows cut 38 us, whole 56; 1000 rows of head_dim 64
-// cut 88, whole 80).
-constexpr int kItemsLog = 9, kLeastTiles = 4;
-constexpr int cut_saves(int dtype) { return (dtype & 15) == kFp32 ? 2 : 4; }
-constexpr int cut_tiles(int dtype) { return (dtype & 15) == kFp32 ? 24 : 16; }
-
 // By how much (in powers of 2) a row's largest score may pass the maximum that its weights
 // are taken from before what was summed so far is multiplied anew: nearly every tile raises
 // one of a wave's 32 rows' a little.  fp16 has no room above its bias.
@@ -84,13 +73,8 @@ __device__ __forceinline__ PromptRows prompt_rows(const Prompt& a, int b) {
   return s;
 }
 
-// Tiles of keys of a work item at most, and of a sequence that is not cut: every wave
-// finds them, and its own item, by itself from the lengths (two lane scans for every 64
-// sequences).
-struct PromptPlan {
-  int per_item, whole;
-};
-
+// Every wave finds the plan, and its own item, by itself from the lengths (two lane scans
+// for every 64 sequences).
 template <int DT, int kTokens>
 __device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
   if (!a.states) return PromptPlan{1, INT32_MAX};  // (nothing is cut)
@@ -102,10 +86,7 @@ __device__ __forceinline__ PromptPlan prompt_plan(const Prompt& a) {
     tiles += s.tiles;
   }
   const uint64_t low = wave_sum_i((int)(sum & 0xffffffu)), high = wave_sum_i((int)(sum >> 24));
-  const uint64_t share = (((high << 24) + low) * a.kv_heads >> kItemsLog) + 1;
-  const int per_item = (int)(share < kLeastTiles ? kLeastTiles : share < (1u << 24) ? share : 1u << 24);
-  // (tiles * kv_heads < 2^30, key tiles of a sequence < 2^26)
-  return PromptPlan{per_item, per_item + cut_saves(DT) + wave_sum_i(tiles) * a.kv_heads / cut_tiles(DT)};
+  return prompt_cuts(((high << 24) + low) * a.kv_heads, wave_sum_i(tiles) * a.kv_heads, kType<DT> == kFp32);
 }
 
 // Item `index` of the launch: a tile of rows of sequence b and KV head h, chunk `chunk`
@@ -124,7 +105,7 @@ __device__ __forceinline__ bool find_item(const Prompt& a, const PromptPlan& pla
   int base = 0, cut = 0;
   for (int b0 = 0; b0 < a.sequences; b0 += 64) {
     const PromptRows s = prompt_rows<kTokens>(a, b0 + (threadIdx.x & 63));
-    const int most = s.key_tiles > plan.whole ? (s.key_tiles + plan.per_item - 1) / plan.per_item : 1;
+    const int most = plan.chunks(s.key_tiles);
     // (cut_tiles: only those of sequences that are cut, one for all chunks of a tile)
     const int states = most > 1 ? s.tiles * most * a.kv_heads : 0;
     const int count = cut_tiles ? (most > 1 ? s.tiles * a.kv_heads : 0) : s.tiles * most * a.kv_heads;
@@ -910,35 +891,6 @@ __global__ __launch_bounds__(kJoinRows* D / 4) void prompt_join_kernel(Prompt a)
   }
 }
 
-// Tiles of rows of one KV head at most, however the rows are dealt to the sequences.
-int64_t most_tiles(int64_t rows, int sequences, int group) {
-  return rows * group / kTileRows + (sequences < rows ? sequences : rows);
-}
-
-// Work items, states and cut tiles of a launch at most.
-struct PromptLayout {
-  int64_t items, states, cut_tiles;
-  size_t bytes;
-};
-
-PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots, int dtype) {
-  PromptLayout l;
-  const int tokens = element_bytes(dtype) * head_dim > 256 ? 32 : 64;
-  const int64_t tiles = most_tiles(rows, sequences, group), key_tiles = (slots + tokens - 1) / tokens;
-  const int64_t all = 1ll << kItemsLog;
-  // A sequence that is cut has most = ceil(x) <= 2x chunks a tile, x > 1 its share of
-  // an item: 2 all of them at most.
-  const int64_t full = tiles * kv_heads * ((key_tiles + kLeastTiles - 1) / kLeastTiles);
-  // Never cut: few slots; one sequence whose tiles are as many as the items are to be.
-  const bool whole = key_tiles <= kLeastTiles + cut_saves(dtype) ||
-                     (sequences == 1 && (rows * group + kTileRows - 1) / kTileRows * kv_heads >= all);
-  l.items = (whole ? 0 : all) + tiles * kv_heads;
-  l.states = whole ? 0 : full < 2 * all ? full : 2 * all;
-  l.cut_tiles = whole ? 0 : tiles * kv_heads < all ? tiles * kv_heads : all;
-  l.bytes = (size_t)l.states * kTileRows * (head_dim + 2) * sizeof(float);
-  return l;
-}
-
 template <int DT, int D>
 int launch_prompt(const Prompt& a, const PromptLayout& l, hipStream_t stream) {
   constexpr int kRow = D * kElem<DT>, kRows = 1024 / kRow;  // of a wave's load
@@ -982,7 +934,8 @@ size_t prismkv_paged_prompt_work_bytes(int64_t rows, int sequences, int kv_heads
   if (!known || sequences < 1 || kv_heads < 1 || head_dim < 1 || slots < 1 || slots > 1 << 30 ||
       !prompt_fits(rows, sequences, kv_heads, group))
     return 0;
-  const size_t bytes = prompt_layout(rows, sequences, kv_heads, group, head_dim, slots, dtype).bytes;
+  const size_t bytes = prompt_layout(rows, sequences, kv_heads, group, head_dim, slots, element_bytes(dtype) * head_dim,
+                                     (dtype & 15) == kFp32).bytes;
   return bytes < 16 ? 16 : bytes;
 }
 
@@ -995,7 +948,8 @@ int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t 
   if (!offsets && rows != c.sequences) return kBadSize;
   if ((rows && (!q || !out || !paged_work)) || (q | out | paged_work) & 15 || (lse | offsets) & 3) return kBadSize;
   const int64_t slots = (int64_t)c.page_size * c.max_pages;
-  const PromptLayout l = prompt_layout(rows, c.sequences, c.kv_heads, group, c.head_dim, slots, c.dtype);
+  const PromptLayout l = prompt_layout(rows, c.sequences, c.kv_heads, group, c.head_dim, slots,
+                                       element_bytes(c.dtype) * c.head_dim, (c.dtype & 15) == kFp32);
   if (work_bytes < l.bytes) return kBadSize;
   Prompt a{};
   a.q = reinterpret_cast<const char*>(q);
