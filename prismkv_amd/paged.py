@@ -611,7 +611,7 @@ class PagedCache:
         # nothing is appended for a query that is refused
         group, scale = self._check_prompt(q, offsets, scale, lse, rotary is not None)
         _check(k.shape[0] == q.shape[0], "as many K and V rows as Q rows required")
-        work = to._prompt_workspace(q.shape[0], group)
+        work = self._prompt_workspace(q.shape[0], group)  # (forks are many: this cache's, as a step's)
         turned = self.append(k, v, offsets, q=q if rotary is not None else None, rotary=rotary, into=into)
         return to._prompt(q if turned is None else turned, offsets, group, scale, lse, work)
 
