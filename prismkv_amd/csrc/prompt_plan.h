@@ -54,7 +54,7 @@ inline int64_t most_tiles(int64_t rows, int sequences, int group) {
   return rows * group / kTileRows + (sequences < rows ? sequences : rows);
 }
 
-// Work items, states and cut tiles of a launch at most.
+// Work items, states and cut tiles of a launch at most; bytes of the states.
 struct PromptLayout {
   int64_t items, states, cut_tiles;
   size_t bytes;
@@ -73,7 +73,9 @@ inline PromptLayout prompt_layout(int64_t rows, int sequences, int kv_heads, int
   const bool whole = key_tiles <= kLeastTiles + cut_saves(fp32) ||
                      (sequences == 1 && (rows * group + kTileRows - 1) / kTileRows * kv_heads >= all);
   l.items = (whole ? 0 : all) + tiles * kv_heads;
-  l.states = whole ? 0 : full < 2 * all ? full : 2 * all;
+  // (powers of two, so that workspaces are of few sizes)
+  l.states = whole || full < 1 ? 0 : 1;
+  while (l.states && l.states < full && l.states < 2 * all) l.states *= 2;
   l.cut_tiles = whole ? 0 : tiles * kv_heads < all ? tiles * kv_heads : all;
   l.bytes = (size_t)l.states * kTileRows * (head_dim + 2) * sizeof(float);
   return l;

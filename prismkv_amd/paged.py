@@ -587,8 +587,9 @@ class PagedCache:
             if not nbytes:
                 raise NotImplementedError("at most 2^30 rows of a prompt times the query heads of a KV head, and less than 2^24 "
                                           "blocks of 128 of them (of every KV head; one more for each sequence)")
-            # sizes of powers of two, each kept: a captured graph goes on using its own
-            size = 1 << (nbytes - 1).bit_length()
+            # states in powers of two; each kept, as a captured graph goes on using its own,
+            # and the least that is large enough taken
+            size = min((x for x in self._prompt_work if x >= nbytes), default=nbytes)
             work = self._prompt_work.get(size)
             if work is None:
                 work = self._prompt_work[size] = self._workspace(size, 0)
