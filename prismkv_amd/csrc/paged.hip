@@ -372,7 +372,9 @@ __device__ __forceinline__ void move_scales(const PagedEvict& a, char* pages, in
 // A move's rows of K and V, kRows of them in flight per thread; a row takes as many
 // lanes as it has 16-byte pieces.  Slots in srcs and dsts (`count` of them), this
 // workgroup's from its index on, every groups-th kRows * rows-at-a-time of them.
-template <int kThreads, int kRows>
+// kFourBits: with their scales (a kernel of its own: as a branch it took 9 more registers
+// and spilled 12 scalar ones of the selection over 16-bit pages, 10.6 -> 10.9 us for a cut of 64).
+template <int kThreads, int kRows, bool kFourBits>
 __device__ __forceinline__ void move_rows(const PagedEvict& a, int b, int h, size_t row, const int32_t* srcs,
                                           const int32_t* dsts, int count, int group, int groups) {
   const int c = (threadIdx.x & ((1 << a.log_pieces) - 1)) << 4, step = kThreads >> a.log_pieces;
@@ -417,7 +419,7 @@ __device__ __forceinline__ void move_rows(const PagedEvict& a, int b, int h, siz
         *reinterpret_cast<uint4*>(a.kp + to[e]) = kv[e];
         *reinterpret_cast<uint4*>(a.vp + to[e]) = vv[e];
         if (c == 0) {
-          if (a.scale_bytes) {
+          if constexpr (kFourBits) {
             move_scales(a, a.k_scales, h, from_page[e], src[e], into_page[e], dst[e]);
             move_scales(a, a.v_scales, h, from_page[e], src[e], into_page[e], dst[e]);
           }
@@ -451,6 +453,7 @@ __device__ __forceinline__ void evict_lengths(const PagedEvict& a, const EvictRo
 // 75 in parts).
 constexpr int kLongRow = 16384, kManyRows = 64;
 
+template <bool kFourBits>
 __global__ __launch_bounds__(kET) void paged_select_kernel(PagedEvict a) {
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -507,7 +510,7 @@ __global__ __launch_bounds__(kET) void paged_select_kernel(PagedEvict a) {
   if (tid == 0) a.count[r.row] = total <= kFew ? 0 : total;
   if (total <= kFew) __syncthreads();  // (the fork's copies of what stays come before the moves')
   evict_lengths(a, r, b, a.kv_heads);
-  if (total <= kFew) move_rows<kET, 4>(a, b, h, r.row, few[0], few[1], total, 0, 1);
+  if (total <= kFew) move_rows<kET, 4, kFourBits>(a, b, h, r.row, few[0], few[1], total, 0, 1);
 }
 
 // Longer rows take one launch per pass, a part of a row per workgroup: a.part slots,
@@ -721,10 +724,12 @@ __global__ __launch_bounds__(kET) void paged_pick_kernel(PagedEvict a) {
 // thread: fewer workgroups, and 1 to 4 us more).
 constexpr int kMoveRows = 2;
 
+template <bool kFourBits>
 __global__ __launch_bounds__(kPT) void paged_move_kernel(PagedEvict a) {
   const int h = blockIdx.y, b = blockIdx.z;
   const size_t row = (size_t)b * a.kv_heads + h;
-  move_rows<kPT, kMoveRows>(a, b, h, row, a.src + row * a.moves, a.dst + row * a.moves, a.count[row], blockIdx.x, gridDim.x);
+  move_rows<kPT, kMoveRows, kFourBits>(a, b, h, row, a.src + row * a.moves, a.dst + row * a.moves, a.count[row], blockIdx.x,
+                                       gridDim.x);
 }
 
 }  // namespace
@@ -988,15 +993,17 @@ int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_ca
   int64_t most = slots / 2;  // moves of a row
   if (!keeps) most = keep < slots - keep ? keep : slots > keep ? slots - keep : 0;
   if (most > slots / 2) most = slots / 2;
+  const auto select = c.dtype >= kFour ? paged_select_kernel<true> : paged_select_kernel<false>;
+  const auto move = c.dtype >= kFour ? paged_move_kernel<true> : paged_move_kernel<false>;
   int rc;
   if (!l.parts) {
     const int lds = (int)((slots + 64 * kEWaves - 1) / (64 * kEWaves)) * 64 * kEWaves * (int)sizeof(unsigned);
     if (lds > 32 * 1024) {  // (beside the static 27 KB)
-      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_select_kernel),
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(select),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, 2 * kLongRow * (int)sizeof(unsigned));
       if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(paged_select_kernel, dim3(c.kv_heads, c.sequences), dim3(kET), lds, s, a);
+    hipLaunchKernelGGL(select, dim3(c.kv_heads, c.sequences), dim3(kET), lds, s, a);
     rc = (int)hipGetLastError();
     if (rc || most <= kFew) return rc;
   } else {
@@ -1011,7 +1018,7 @@ int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_ca
   const int64_t blocks = (most + (kPT >> a.log_pieces) * kMoveRows - 1) / ((kPT >> a.log_pieces) * kMoveRows);
   const int64_t room = 4096 / ((int64_t)c.sequences * c.kv_heads) + 1;  // workgroups of a row where there are many rows
   const int64_t grid = blocks < 1 ? 1 : blocks < room ? blocks : room;
-  hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)grid, c.kv_heads, c.sequences), dim3(kPT), 0, s, a);
+  hipLaunchKernelGGL(move, dim3((unsigned)grid, c.kv_heads, c.sequences), dim3(kPT), 0, s, a);
   return (int)hipGetLastError();
 }
 
