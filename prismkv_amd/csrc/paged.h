@@ -93,12 +93,12 @@ __device__ __forceinline__ u32x4 widen8(unsigned codes, float scale) {
 // head_dim 256 takes the registers of two.  Two workgroups of 4 waves read as fast,
 // but leave twice the partial states to join (64K: 54.0 us against 47.8).
 constexpr int kUnits = 256;
-template <int DT, int D>
+template <int D>
 constexpr int kAWaves = D == 256 ? 4 : 8;
 constexpr int kQuantum = 32;  // tokens that are dealt at a time
 // Quanta of a workgroup at least: a tile (32 tokens, fp32 16) for each wave.
 template <int DT, int D>
-constexpr int kLeast = kType<DT> == kFp32 ? kAWaves<DT, D> / 2 : kAWaves<DT, D>;
+constexpr int kLeast = kType<DT> == kFp32 ? kAWaves<D> / 2 : kAWaves<D>;
 
 // 16 bytes that another workgroup wrote through (agent scope, as ld_dev).
 __device__ __forceinline__ float4 ld_dev4(__amdgpu_buffer_rsrc_t r, unsigned byte_offset) {

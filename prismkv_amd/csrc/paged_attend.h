@@ -637,6 +637,7 @@ template <int DT, int D, bool kAligned, bool kMany>
 __device__ __forceinline__ void attend_segment(const PagedAttend& a, const PagedSpan<kLeast<DT, D>>& u, int quanta, int count, float* lds) {
   typedef Pages<DT, D, kAligned, kInFour<DT>> P;
   typedef typename P::T T;
+  static_assert(kQuantum % T::kTokens == 0, "no tile ends in the next workgroup's share");
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, q = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = u.hh / a.tiles, g0 = 16 * (u.hh - h * a.tiles);
@@ -644,7 +645,7 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   const int start = min(u.first * kQuantum, u.n), end = min(start + count * kQuantum, u.n);
   // (a pair alone: all tiles are this wave's)
   const bool alone = kMany && u.alone;
-  const int step = alone ? T::kTokens : kAWaves<DT, D> * T::kTokens;
+  const int step = alone ? T::kTokens : kAWaves<D> * T::kTokens;
 
   // Q^T: column j is head j (zero past the tile's heads)
   u32x4 qop[T::kKLoads];
@@ -794,33 +795,27 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
         for (int n = 0; n < D / 16; ++n)
           acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][r], __uint_as_float(t.v[0][r][n]), acc[n], 0, 0, 0);
     } else {
+      unsigned term[8][kTerms<DT>];
+      u32x4 pw[kTerms<DT>];
+      if constexpr (kInFour<DT>) {
 #pragma unroll
-      for (int i0 = 0; i0 < T::kBlocks; i0 += 2) {
-        unsigned term[8][kTerms<DT>];
-        u32x4 pw[kTerms<DT>];
-        if constexpr (kInFour<DT>) {
+        for (int e = 0; e < 8; e += 2) split_pair<DT>(p[e / 4][e % 4], p[e / 4][e % 4 + 1], pw, e / 2);
+        unsigned v[2][4][T::kVWords];
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) split_pair<DT>(p[i0 + e / 4][e % 4], p[i0 + e / 4][e % 4 + 1], pw, e / 2);
-        } else {
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int r = 0; r < 4; ++r) t.widen_v(v[i][r], i, r, rows_of.scale(t, i, r));
+        pv_columns<0, DT, D>(acc, v, pw);
+      } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) split16<DT>(p[i0 + i][r], term[4 * i + r]);
-        }
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = 0; k < (kInFour<DT> ? 0 : kTerms<DT>); ++k)
+          for (int r = 0; r < 4; ++r) split16<DT>(p[i][r], term[4 * i + r]);
+#pragma unroll
+        for (int k = 0; k < kTerms<DT>; ++k)
           pw[k] = u32x4{upper16(term[0][k], term[1][k]), upper16(term[2][k], term[3][k]), upper16(term[4][k], term[5][k]),
                         upper16(term[6][k], term[7][k])};
-        if constexpr (kInFour<DT>) {
-          unsigned v[2][4][T::kVWords];
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t.widen_v(v[i][r], i0 + i, r, rows_of.scale(t, i0 + i, r));
-          pv_columns<0, DT, D>(acc, v, pw);
-        } else {
-          pv_columns<0, DT, D>(acc, t.v, pw);
-        }
+        pv_columns<0, DT, D>(acc, t.v, pw);
       }
     }
     rows_of.load_v(t);
@@ -828,9 +823,8 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
     // step waits for must not be behind them (16 sequences of 4099: 47.5 us before)
     if (logits && j < rows) {
 #pragma unroll
-      for (int i = 0; i < T::kBlocks; ++i)  // (in 4 bits a tile may end in the next workgroup's share)
-        if (!kInFour<DT> || t0 + 16 * i < end)
-          *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+      for (int i = 0; i < T::kBlocks; ++i)
+        *reinterpret_cast<float4*>(logits + t0 + 16 * i + 4 * q) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
     }
   }
   if (__ballot(rows_of.bad) && lane == 0) report_error(a.err, error_host_slot(a.err), kErrPages);
@@ -851,8 +845,8 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   }
   // the waves' states meet in LDS
   float* sm = lds;  // [waves][16] maxima
-  float* sz = sm + 16 * kAWaves<DT, D>;   // [waves][16] sums
-  float* sacc = sz + 16 * kAWaves<DT, D>; // [waves][rows][D]
+  float* sz = sm + 16 * kAWaves<D>;   // [waves][16] sums
+  float* sacc = sz + 16 * kAWaves<D>; // [waves][rows][D]
   if (lane < 16) {
     sm[16 * w + j] = m;
     sz[16 * w + j] = z;
@@ -869,14 +863,14 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   const int pair0 = u.at - u.first, unit = (int)blockIdx.x;
   const bool whole = count == quanta;
   float* state = a.state + (size_t)(2 * unit + (u.at != u.deal.begin(unit))) * a.state_stride;  // {max, sum}[rows], [rows][D]
-  for (int i = 2 * tid; i < rows * D; i += 128 * kAWaves<DT, D>) {
+  for (int i = 2 * tid; i < rows * D; i += 128 * kAWaves<D>) {
     const int g = i / D;
     float M = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < kAWaves<DT, D>; ++k) M = fmaxf(M, sm[16 * k + g]);
+    for (int k = 0; k < kAWaves<D>; ++k) M = fmaxf(M, sm[16 * k + g]);
     float den = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int k = 0; k < kAWaves<DT, D>; ++k) {
+    for (int k = 0; k < kAWaves<D>; ++k) {
       const float wt = rescale(sm[16 * k + g], M);
       const float2 v = *reinterpret_cast<const float2*>(sacc + (size_t)k * rows * D + i);
       den = fmaf(wt, sz[16 * k + g], den);
@@ -905,11 +899,11 @@ __device__ __forceinline__ void attend_segment(const PagedAttend& a, const Paged
   __syncthreads();
   if (!is_last) return;
   if (tid == 0) st_dev(counter, 0u);
-  join_states<DT, D, 64 * kAWaves<DT, D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
+  join_states<DT, D, 64 * kAWaves<D>>(a, head0, rows, parts, 0, rows * D / 4, lds);
 }
 
 template <int DT, int D, bool kAligned, bool kMany>
-__global__ __launch_bounds__((64 * kAWaves<DT, D>), (kAWaves<DT, D> / 4)) void paged_attend_kernel(PagedAttend a) {
+__global__ __launch_bounds__((64 * kAWaves<D>), (kAWaves<D> / 4)) void paged_attend_kernel(PagedAttend a) {
   extern __shared__ float lds[];
   constexpr int kL = kLeast<DT, D>;
   PagedSpan<kL> u = find_span<kL, kMany>(a, blockIdx.x);
@@ -918,7 +912,7 @@ __global__ __launch_bounds__((64 * kAWaves<DT, D>), (kAWaves<DT, D> / 4)) void p
       const int heads = a.kv_heads * a.tiles;
       u.first = 0;
       for (int pair = blockIdx.x + gridDim.x * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); pair < a.sequences * heads;
-           pair += gridDim.x * kAWaves<DT, D>) {
+           pair += gridDim.x * kAWaves<D>) {
         u.b = pair / heads;
         u.hh = pair - u.b * heads;
         u.n = __builtin_amdgcn_readfirstlane(clamp_length(a, a.lengths[u.b]));
@@ -972,7 +966,7 @@ int launch_attend_rows(const PagedAttend& a, int64_t units, int lds, hipStream_t
                                              hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(64 * kAWaves<DT, D>), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3(64 * kAWaves<D>), lds, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -986,8 +980,8 @@ int launch_attend(PagedAttend a, int64_t units, hipStream_t stream) {
   // tokens of one KV head and 16 query heads (264K floats) 20.3 us, 44.9 by the last
   // workgroup; of 8 KV heads and 4 (17K) 48.5 against 47.3.
   const bool apart = (int64_t)chunks * rows * D > 49152;
-  const int merge = 32 * kAWaves<DT, D> + kAWaves<DT, D> * rows * D, sums = 32 + chunks * rows;
-  const int join = apart ? 0 : 256 * kAWaves<DT, D> + sums;
+  const int merge = 32 * kAWaves<D> + kAWaves<D> * rows * D, sums = 32 + chunks * rows;
+  const int join = apart ? 0 : 256 * kAWaves<D> + sums;
   const int lds = (merge > join ? merge : join) * (int)sizeof(float);
   if (apart) a.counters = nullptr;
   // a lane's offset within a block is 32 bits
