@@ -23,7 +23,9 @@ def attend(q, k_pages, v_pages, table, lengths, scale=None):
     2 delta (its own and the denominator's) and the exponentials' and the
     sums' own steps, 2^-20 + n 2^-24.  bf16 multiplies V with P as three terms,
     which is exact, fp16 as two, 2^-22 and, as each is 2^-39 of the largest weight
-    at least, 2^-38 |v| a slot."""
+    at least, 2^-38 |v| a slot.  A weight below 2^-126 of the largest is below fp32's
+    least normal number, and may be 0, and so may its product with V: 2^-126 (1 + |v|) a
+    slot, over a sum of 1 at least, and the same again for the sum's share."""
     B, heads, D = q.shape
     H = k_pages.shape[1]
     scale = 1 / math.sqrt(D) if scale is None else scale
@@ -51,7 +53,7 @@ def attend(q, k_pages, v_pages, table, lengths, scale=None):
         # (a subnormal output is off by half of the type's smallest step)
         floor = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}[q.dtype]
         lost = spread * (rel[:, None] + split) + least * (p.amax(-1)[:, None, None] * v.abs()).sum(1)
-        out_bound = out.abs() * eps + lost * (1 + eps) + floor
+        out_bound = out.abs() * eps + lost * (1 + eps) + floor + 2.0 ** -125 * (1 + v.abs()).sum(1)
         group = heads // H
         weights = p.view(H, group, n).sum(1)
         weights_bound = (p * rel[:, None]).view(H, group, n).sum(1) + weights * (group + 2) * 2.0 ** -24
@@ -118,7 +120,8 @@ def prompt(q, k, v, new, dtype=None, scale=None):
         if dtype == torch.float16:
             lost += 2.0 ** -38 * p.amax(-1)[:, None] * ((~later).double() @ vd.abs())
         floor = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}[dtype]
-        bound[:, g] = out[:, g].abs() * half + lost * (1 + half) + floor
+        # (below fp32's least normal number: as for `attend`)
+        bound[:, g] = out[:, g].abs() * half + lost * (1 + half) + floor + 2.0 ** -125 * (1 + vd.abs()).sum(0)
         lse_bound[:, g] = delta + 2.0 ** -20 + n * 2.0 ** -24 + lse[:, g].abs() * 2.0 ** -22
     return (out, lse), (bound, lse_bound)
 
