@@ -47,8 +47,11 @@ class Rotary:
         _check(base > 0 and math.isfinite(base), "a positive base required")
         self.base, self.interleaved = base, bool(interleaved)
         pairs = range(self.rotary_dim // 2)
-        frequencies, self.amplitude = _scaled([base ** (-2.0 * j / self.rotary_dim) for j in pairs], scaling, base,
-                                              self.rotary_dim)
+        try:
+            frequencies, self.amplitude = _scaled([base ** (-2.0 * j / self.rotary_dim) for j in pairs], scaling, base,
+                                                  self.rotary_dim)
+        except OverflowError:
+            raise ValueError("a base and scaling of which float64 holds the numbers required") from None
         _check(all(math.isfinite(f) for f in frequencies), "frequencies that are finite required")
         _check(math.isfinite(self.amplitude) and abs(self.amplitude) <= torch.finfo(torch.float32).max,
                "an attention factor that is finite in float32 required")
