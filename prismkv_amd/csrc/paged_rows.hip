@@ -397,12 +397,13 @@ int launch_rows(PagedRows a, hipStream_t stream) {
 
 template <int DT, int D>
 int launch_read(PagedRead a, hipStream_t stream) {
-  for (; a.first_row < a.rows; a.first_row += kLaunchRows) {
+  do {  // (once for no rows, whose offsets are looked at too)
     const int64_t more = a.rows - a.first_row < kLaunchRows ? a.rows - a.first_row : kLaunchRows;
-    hipLaunchKernelGGL((paged_read_kernel<DT, D>), dim3((unsigned)((more + kRowsEach - 1) / kRowsEach)), dim3(kPT), 0,
-                       stream, a);
+    const unsigned groups = (unsigned)((more + kRowsEach - 1) / kRowsEach);
+    hipLaunchKernelGGL((paged_read_kernel<DT, D>), dim3(groups ? groups : 1), dim3(kPT), 0, stream, a);
     if (const int rc = (int)hipGetLastError()) return rc;
-  }
+    a.first_row += kLaunchRows;
+  } while (a.first_row < a.rows);
   return 0;
 }
 
