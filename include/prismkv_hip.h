@@ -502,9 +502,10 @@ int prismkv_paged_evict(const prismkv_paged_cache* cache, const prismkv_paged_ca
  * and y of a pair become x cos - y sin and y cos + x sin, times `amplitude`, of the angle
  * p turns[j] / 2^64 of a full turn; pair j is dims j and j + rotary_dim / 2, or with
  * `interleaved` 2j and 2j + 1, of the first rotary_dim (a multiple of 16, up to
- * head_dim) dims; turns is u64 [rotary_dim / 2].  The turned q goes to q_out, contiguous;
- * strides of q as of k and v.  q may be 0 (heads 0).  turns 0: nothing is turned, and q
- * is 0.  Turned rows are rounded to their type before they are held in 4 bits. */
+ * head_dim) dims; turns is u64 [rotary_dim / 2].  The turned q goes to q_out, contiguous,
+ * which overlaps none of the rows; strides of q as of k and v.  q may be 0 (heads 0).
+ * turns 0: nothing is turned, and q is 0.  Turned rows are rounded to their type before
+ * they are held in 4 bits. */
 int prismkv_paged_append_rows(const prismkv_paged_cache* cache, const prismkv_paged_cache* into, uint64_t k, uint64_t v,
                               uint64_t q, uint64_t q_out, uint64_t offsets, uint64_t turns, int64_t rows,
                               int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
@@ -520,8 +521,9 @@ int prismkv_paged_read(const prismkv_paged_cache* cache, uint64_t offsets, uint6
 /* Causal attention of the last m = offsets[b + 1] - offsets[b] slots' queries of every
  * sequence (q [rows][kv_heads * group][head_dim], packed; offsets as above) over its
  * slots: row i sees slots t <= lengths[b] - m + i; out as q, 0 where there is none; lse
- * f32 [rows][kv_heads * group] (or 0) as for prismkv_paged_attend.  The workspace
- * needs no preparation. */
+ * f32 [rows][kv_heads * group] (or 0) as for prismkv_paged_attend.  rows * group <= 2^30,
+ * and (rows * group / 128 + min(rows, sequences)) * kv_heads + 512 < 2^24 workgroups (0
+ * bytes, and -1, otherwise).  The workspace needs no preparation. */
 size_t prismkv_paged_prompt_work_bytes(int64_t rows, int sequences, int kv_heads, int group, int head_dim, int64_t slots,
                                        int dtype);
 int prismkv_paged_prompt(const prismkv_paged_cache* cache, uint64_t q, uint64_t offsets, uint64_t lse, uint64_t paged_work,

@@ -6,10 +6,12 @@
 // heads still fill a tile; row i of a sequence of n slots sees slots [0, n - m + i /
 // group].  4 head_dim flops for a row and a slot that it sees against 2 x 2 head_dim
 // bytes for a slot and 128 rows: the matrix products bound it, unless the rows are few.
-// Measured: 16384 rows of 8 x 4 heads of 128 in bf16 2092 us = 1.05 PFLOP/s (a product of
-// 8192^3 reaches 1.12); 48 rows over 65048 slots 89 us = 574 TFLOP/s and 3.0 TB/s; fp16,
-// head_dim 64, 9 ragged sequences of 1.0K rows 147 us = 524; fp32, head_dim 256, 4097 rows
-// 1035 us = 96 (of 153); over 4-bit pages 6007 rows over 5 x 9K slots 926 us = 939.
+// Measured: 16384 rows of 8 x 4 heads of 128 in bf16 2114 us = 1.04 PFLOP/s (a product of
+// 8192^3 reaches 1.12); 48 rows over 65048 slots 91 us = 562 TFLOP/s and 2.9 TB/s; fp16,
+// head_dim 64, 9 ragged sequences of 1.0K rows 149 us = 516; fp32, head_dim 256, 4097 rows
+// 1043 us = 96 (of 153); over 4-bit pages 6007 rows over 5 x 9K slots 953 us = 912.  (The
+// clock goes with the power and the card: the same kernel takes 2040 to 2120 us for the
+// first, and figures are to be compared with those beside them.)
 #include <cfloat>
 #include <type_traits>
 
@@ -25,7 +27,7 @@ template <int DT, int D>
 constexpr int kTileTokens = tile_tokens(kElem<DT> * D);
 // Waves of a SIMD, by the registers that products, queries and staged rows take.  (Three
 // for head_dim 64 in 16 bits; the widening from 4 bits has no room for that: 2000 rows over
-// 4000 slots 87 us, with two 82.)
+// 4000 slots 87 us, with two 84.)
 template <int DT, int D>
 constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : kElem<DT> * D == 128 && !kInFour<DT> ? 3 : 2;
 // By how much (in powers of 2) a row's largest score may pass the maximum that its weights
@@ -248,8 +250,8 @@ __device__ __forceinline__ u32x4 without_special(u32x4 x, bool& any) {
 // kGroups: the 64 / kC rows that a wave loads at once always lie in one page.  Then their
 // place is one scalar, and a buffer load from it has a lane's offset alone.  (Beside the
 // vector work that this saves: while a global load to LDS is on its way the compiler waits
-// for all reads of LDS at once.  4000 rows over pages of 64 slots 148 us, of 31 slots 156;
-// of head_dim 256 359 and 411.)
+// for all reads of LDS at once.  4000 rows over pages of 64 slots 150 us, of 31 slots 157;
+// of head_dim 256 371 and 427.)
 template <int DT, int D, bool kGroups>
 struct Stage {
   static constexpr int kTokens = kTileTokens<DT, D>;
@@ -428,8 +430,8 @@ constexpr bool kShared = kType<DT> == kBf16;
 // comes back as its V (without, off by up to 2^-8, the same for every dim).  `top` is that
 // slot's score and `at` the maximum that its weight was taken from, `m` the last one.  (The
 // sum of all rounded weights, by two-element products of the words, is little better, 0.0014
-// for 0.0016 above, and takes longer: 16384 rows 2155 us against 2040.  From 2^22 on a
-// maximum's weights are taken otherwise, of scores that are off by 1/4 and more.)
+// for 0.0016 above, and makes 16384 rows take 6% longer, where this makes it 0.6.  From 2^22
+// on a maximum's weights are taken otherwise, of scores that are off by 1/4 and more.)
 template <int DT>
 __device__ __forceinline__ float share_largest(float top, float at, float m, float scale, float z) {
   const float p = __builtin_amdgcn_exp2f(fmaf(top, scale, (float)kBias<DT> - at));
@@ -453,9 +455,9 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
   constexpr int kTokens = kTileTokens<DT, D>, kT = kTokens / 32;
   constexpr int kC = D * kElem<DT> / 16;  // 16-byte chunks of a row; half as many steps of the product (fp32: of four)
   constexpr int kTile = kTokens * kC * 16;  // bytes
-  // Whether the next tiles' loads are issued between the products (fp32 prompts 1190 us, so
-  // 1159; 16384 rows of head_dim 128 2052 and 2012) or before them (head_dim 64 97 and 91;
-  // 256 366 and 360).
+  // Whether the next tiles' loads are issued between the products (4097 fp32 rows 1037 us,
+  // before them 1070; 16384 rows of head_dim 128 2121 and 2146) or before them (4000 rows of
+  // head_dim 256 in fp16 500, between them 511; in bf16 368 and 363; of 64 no difference).
   constexpr bool kLate = kGroups && (kType<DT> == kFp32 || D == 128);
   __shared__ __attribute__((aligned(16))) char keys0[kTile], keys1[kTile], values0[kTile], values1[kTile];
   if (blockIdx.x == 0 && a.offsets)
@@ -644,8 +646,8 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       // before the products that wait for it): the reads are kAhead products ahead, and
       // the exponentials between the first products, the sum between the others.  (The
       // next scores are of no tile, behind the last.  kAhead: by the registers that are left;
-      // 4000 rows of head_dim 64 98 us with 3, 92 with 2, of 128 2047 and 2070 for 16384, over
-      // 4-bit pages 939 and 932 for 6007 rows.)
+      // 4000 rows of head_dim 64 99 us with 3, 92 with 2, of 256 370 and 417, of 128 the same,
+      // over 4-bit pages 995 and 953 for 6007 rows.)
       constexpr int kSteps = kC / 2, kAhead = kC == 8 || (kInFour<DT> && D == 128) ? 2 : 3;
       u32x4 kf[kAhead][kT];
       auto read_k = [&](int c) {
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(kThreads, (kOccupancy<DT, D>)) void prompt_kernel(P
       };
       if constexpr (kType<DT> == kFp32) {
         // A lane reads kVec dims at once, each for a product of its own (one dim at a time a
-        // product takes 87 cycles, not 64: 4097 rows of head_dim 256 1163 us, so 1033)
+        // product takes 87 cycles, not 64: 4097 rows of head_dim 256 then took 1163 us, so 1033)
         const FloatsAt<kC, kVec> floats_at(col, half);
         constexpr int kOf = D / (32 * kVec), kReads = 16 * kT * kOf, kVAhead = 2;
         float vf[kVAhead + 1][kVec];

@@ -551,10 +551,10 @@ class PagedCache:
         last offsets[b + 1] - offsets[b] slots.  Each sees the slots up to its own, the
         older ones among them: a prompt in chunks, or a turn after a history, is a call
         each.  (After an `evict` of slots appended since, slots are no longer in the
-        order of their tokens.)  The output has q's shape and type; `lse`, an f32
-        [rows, heads] tensor, receives the logarithm of each softmax's sum.  More rows
-        than a sequence holds are reported, and those before its first slot are 0 and
-        -inf."""
+        order of their tokens.)  Scores are not added to.  The output has q's shape and type,
+        of weights rounded once to it; `lse`, an f32 [rows, heads] tensor, receives the
+        logarithm of each softmax's sum.  More rows than a sequence holds are reported, and
+        those before its first slot are 0 and -inf."""
         group, scale = self._check_prompt(q, offsets, scale, lse)
         return self._prompt(q, offsets, group, scale, lse, self._prompt_workspace(q.shape[0], group))
 
