@@ -30,6 +30,7 @@ constexpr int kTileTokens = tile_tokens(kElem<DT> * D);
 // 4000 slots 87 us, with two 84.)
 template <int DT, int D>
 constexpr int kOccupancy = kElem<DT> * D > 256 ? 1 : kElem<DT> * D == 128 && !kInFour<DT> ? 3 : 2;
+
 // By how much (in powers of 2) a row's largest score may pass the maximum that its weights
 // are taken from before what was summed so far is multiplied anew: nearly every tile raises
 // one of a wave's 32 rows' a little.  fp16 has no room above its bias.
